@@ -33,6 +33,9 @@ extern "C" {
 #define GG_TYPE_F32 0u
 #define GG_TYPE_F16 1u
 #define GG_TYPE_Q8_0 8u
+/* further types of the kernel-level entry points (ggml's numbers) */
+#define GG_TYPE_BF16 30u
+#define GG_TYPE_MXFP4 39u
 
 /* attention modes: 0 = reference (src/ as shipped: one RoPE theta, full
  * attention on every layer, types.ts:32-33, shaders.ts:229-325);
@@ -277,6 +280,65 @@ int gg_select_logits(const float* logits, int32_t n, const uint32_t* seen_bitmap
 int gg_select_logits_noalloc(const float* logits, int32_t n, const uint32_t* seen_bitmap,
                              const gg_sample* s, double u, void* topk_out, int32_t* out_token,
                              void* stream);
+
+/* ---- MXFP4 matrices -------------------------------------------------------
+ * 4-bit rows: every 32 consecutive values of a row are elements 0, .5, 1, 1.5,
+ * 2, 3, 4, 6 with a sign times one power of two. No counterpart in the
+ * reference (its weights are Q8_0, 34 bytes per 32 values; these take 17).
+ * A packed matrix is a device buffer of gg_mxfp4_packed_size(rows, k) bytes,
+ * 16-byte aligned; any rows from 1 to 2^30 and k from 1 to 2^20 (a last block
+ * of fewer than 32 values is filled with zeros, 0 is returned outside).
+ * All pointers are device pointers of the current device, which must be the
+ * stream's too; elements are aligned to their size. The calls only queue
+ * kernels on the stream and may be captured into a HIP graph. */
+size_t gg_mxfp4_packed_size(int64_t rows, int64_t k);
+
+/* rows x k values (GG_TYPE_F32 / F16 / BF16, rows ld >= k elements apart) ->
+ * packed MXFP4. With a the largest magnitude of a block, its power of two is
+ * 2^(floor(log2 a) - 2), at least 2^-127; values are rounded to the nearest
+ * element, ties to even, magnitudes above 6 to 6. A block that holds an
+ * infinity or a NaN stands for 32 NaN. */
+int gg_mxfp4_quantize(const void* src, uint32_t type, int64_t rows, int64_t k, int64_t ld, void* packed,
+                      void* stream);
+
+/* The values that a packed matrix stands for, f32, rows ld >= k apart. */
+int gg_mxfp4_dequant(const void* packed, float* out, int64_t rows, int64_t k, int64_t ld, void* stream);
+
+/* y[m][rows] = x[m][k] W[rows][k]^T with W packed, sums in f32, rounded once to
+ * y_type (GG_TYPE_F32 / F16 / BF16). x_type GG_TYPE_MXFP4: x is packed too (m
+ * rows; ldx is not read). GG_TYPE_F32 / F16 / BF16: rows of x ldx >= k apart;
+ * of every 32-block of x, relative to its largest magnitude, 2^-24 is kept for
+ * f32 x and y, 2^-19 for 16-bit x and f32 y, 2^-19 for f16 y (2^-14 from
+ * bf16 x), 2^-14 for bf16 y, finer than the result's rounding. A row of x
+ * with an infinity or a NaN gives NaN. Rows of y are ldy >= rows apart; what
+ * lies between them is left alone. y overlaps neither operand.
+ * workspace: gg_mxfp4_linear_workspace_size() device bytes, 16-byte aligned
+ * (NULL where that is 0), used until the call's kernels have run: calls that
+ * may overlap, and captured graphs, need one each. */
+size_t gg_mxfp4_linear_workspace_size(uint32_t x_type, int64_t m, int64_t rows, int64_t k);
+int gg_mxfp4_linear(const void* w, const void* x, uint32_t x_type, int64_t ldx, void* y, uint32_t y_type, int64_t ldy,
+                    int64_t m, int64_t rows, int64_t k, void* workspace, void* stream);
+
+/* ---- scoring ---------------------------------------------------------------
+ * Log probabilities over rows of logits: rows x n (GG_TYPE_F32 / F16 / BF16),
+ * ld >= n elements apart, n from 1 to 2^30. Each output may be NULL:
+ *   lse[row]          ln sum e^z
+ *   entropy[row]      -sum p ln p, in nats
+ *   id_logprobs       [rows][n_ids]: z[ids] - lse; 0 for the id -1 (no token),
+ *                     NaN for any other id outside [0, n)
+ *   top_ids, top_logprobs  [rows][top_n], top_n from 0 to 64: the largest
+ *                     logits in descending order, equal ones by ascending id;
+ *                     NaN and -inf are never among them, slots without one
+ *                     hold id -1 and -inf
+ * Logits of -inf have probability 0. A row of nothing else has lse and log
+ * probabilities -inf and entropy 0; a row with a NaN or +inf has NaN for every
+ * value. Sums are f32. No counterpart in the reference. Same rules for
+ * pointers, streams and the workspace (gg_score_workspace_size bytes) as
+ * gg_mxfp4_linear. */
+size_t gg_score_workspace_size(int64_t rows, int32_t n, int32_t top_n);
+int gg_score_logits(const void* logits, uint32_t type, int64_t rows, int32_t n, int64_t ld, const int32_t* ids,
+                    int32_t n_ids, float* id_logprobs, float* lse, float* entropy, int32_t top_n, int32_t* top_ids,
+                    float* top_logprobs, void* workspace, void* stream);
 
 #ifdef __cplusplus
 }

@@ -427,4 +427,109 @@ inline PrefillPlan prefill_plan(int window, int start, int M) {
   return best;
 }
 
+// ---- MXFP4 matrices and products (gg_mxfp4.hip), scoring (gg_score.hip) -----
+enum ElemType { ELEM_F32 = 0, ELEM_F16 = 1, ELEM_BF16 = 2 };
+
+// MXFP4: 32 consecutive values of a row are 4-bit elements (sign, e2m1: 0, .5,
+// 1, 1.5, 2, 3, 4, 6) times one power of two, 2^(byte - 127) (byte 255: NaN).
+// Device layout of a rows x k matrix, in the operand order of the 64-deep
+// MX matrix instruction: tiles of 32 rows x 64 k are 1024 bytes, lane
+// 32 b + r holding the 16 bytes (element i in nibble i) of block b (k 32 b ..)
+// of row r; tile (row group R, k group t) at (R kt + t) 1024. The scale bytes
+// follow: four k groups share 256 bytes, byte t % 4 of lane's dword at
+// (R ks + t / 4) 256. Rows and k are filled with zero codes and scale byte 0.
+struct Mx4Layout {
+  int64_t rt;   // row groups of 32
+  int kt, ks;   // k groups of 64, and of 256
+  __host__ __device__ size_t codes() const { return (size_t)rt * kt * 1024; }
+  __host__ __device__ size_t bytes() const { return codes() + (size_t)rt * ks * 256; }
+};
+constexpr int kMx4MaxK = 1 << 20;
+__host__ __device__ inline Mx4Layout mx4_layout(int64_t rows, int64_t k) {
+  const int kt = (int)((k + 63) / 64);
+  return Mx4Layout{(rows + 31) / 32, kt, (kt + 3) / 4};
+}
+
+// Activations of a product as P parts: with 2^e the power of two at or below
+// the largest magnitude of a 32-block, x / 2^e = sum_p d_p 2^(-3 - 5 p) + r,
+// d_p whole numbers in [-16, 16], |r| <= 2^(-4 - 5 (P - 1)). d_p / 8 is an
+// e2m3 (6-bit) value, exactly, so part p is a 6-bit MX block of scale
+// 2^(e - 5 p) and the matrix instruction multiplies it by the 4-bit weights
+// without another rounding. Parts by what the result can show: a bf16 result
+// keeps 8 bits and takes 3 parts (2^-14 of the block's maximum), an f16
+// result 11 and takes 4 (3 from bf16, whose own 8 bits they hold), an f32
+// result takes 5 from f32 (2^-24: as f32 itself) and 4 (2^-19) from 16-bit
+// types, whose values they hold down to 2^-8 of the block's maximum.
+__host__ __device__ inline int mx_parts(int x_elem, int y_elem) {
+  if (y_elem == ELEM_BF16) return 3;
+  if (y_elem == ELEM_F16) return x_elem == ELEM_BF16 ? 3 : 4;
+  return x_elem == ELEM_F32 ? 5 : 4;
+}
+constexpr int kMxMaxParts = 5;
+constexpr int kMxPartBytes = 1536;   // 32 rows x 64 k of one part: 16 bytes a lane, then 8 bytes a lane
+// Workspace of m x k activations in parts: [row group][k group][part][1536],
+// then the scale bytes of part 0 as in Mx4Layout.
+inline size_t mx_parts_bytes(int64_t m, int64_t k, int parts) {
+  const Mx4Layout L = mx4_layout(m, k);
+  return (size_t)L.rt * L.kt * parts * kMxPartBytes + (size_t)L.rt * L.ks * 256;
+}
+
+struct Mx4LinearArgs {
+  const uint8_t* w;      // packed weights
+  int64_t n;             // output features
+  int k, kt, ks;
+  int64_t wrt;           // row groups of w
+  const void* x;         // rows of x_elem (few rows), packed MXFP4, or parts
+  int64_t ldx;
+  int x_elem;
+  int64_t m, xrt;
+  void* y;
+  int64_t ldy;
+  int y_elem;
+  int parts;
+  int y_vec;             // 4 consecutive outputs may be stored at once
+};
+constexpr int kMxGemvCols = 16;
+inline size_t mx_gemv_lds(int cols, int k) { return (size_t)((k + 127) / 128 * 4) * (24 + 1) * cols; }
+// A product with m rows and `parts` parts takes the few-row kernel, which has
+// a column of the matrix instruction for each part of each row.
+inline bool mx_gemv_fits(int64_t m, int parts, int64_t k) {
+  return m * parts <= kMxGemvCols && mx_gemv_lds((int)m * parts, (int)k) <= 52 * 1024;
+}
+int launch_mx4_quantize(int elem, const void* src, int64_t rows, int64_t k, int64_t ld, uint8_t* dst, void* stream);
+int launch_mx4_dequant(const uint8_t* src, float* out, int64_t rows, int64_t k, int64_t ld, void* stream);
+int launch_mx_split(int elem, const void* src, int64_t rows, int64_t k, int64_t ld, int parts, uint8_t* dst,
+                    void* stream);
+int launch_mx4_gemv(const Mx4LinearArgs& a, void* stream);
+int launch_mx4_gemm(const Mx4LinearArgs& a, bool x_mx4, void* stream);
+
+constexpr int kScoreMaxTop = 64;       // best alternatives of a row at most
+constexpr int kScoreMaxChunks = 256;   // blocks that share a row at most
+struct ScoreArgs {
+  const void* z;
+  long long ld, rows;
+  int n;
+  int nch, per;          // chunks of a row, each `per` 16-byte units of its address range
+  const int32_t* ids;    // [rows][n_ids]
+  int n_ids;
+  float *lp, *lse, *entropy;
+  int top;
+  int32_t* top_ids;
+  float* top_lp;
+  float* part;           // [rows][nch][4]
+  uint64_t* keys;        // [rows][nch][top]
+};
+constexpr int kScoreTile = 8192;       // elements a block takes at a time
+// Chunks of a row: about 1024 blocks in all, each of whole tiles. The first
+// tile may start up to 7 elements early (16-byte units of the address range).
+inline void score_plan(long long rows, int n, int* nch, int* tiles_per) {
+  const int tiles = (int)(((long long)n + 7 + kScoreTile - 1) / kScoreTile);
+  long long c = (1024 + rows - 1) / rows;
+  if (c > tiles) c = tiles;
+  if (c > kScoreMaxChunks) c = kScoreMaxChunks;
+  *tiles_per = (int)((tiles + c - 1) / c);
+  *nch = (tiles + *tiles_per - 1) / *tiles_per;
+}
+int launch_score(int elem, const ScoreArgs& a, void* stream);
+
 }  // namespace gg

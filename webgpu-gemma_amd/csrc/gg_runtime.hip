@@ -1756,3 +1756,138 @@ int gg_select_logits_noalloc(const float* logits, int32_t n, const uint32_t* see
 }
 
 }  // extern "C"
+
+// ---- MXFP4 matrices and scoring ---------------------------------------------
+
+namespace {
+
+// Element type of a kernel-level operand, -1 for others.
+int elem_of(uint32_t type) {
+  switch (type) {
+    case GG_TYPE_F32: return ELEM_F32;
+    case GG_TYPE_F16: return ELEM_F16;
+    case GG_TYPE_BF16: return ELEM_BF16;
+  }
+  return -1;
+}
+size_t elem_size(int elem) { return elem == ELEM_F32 ? 4 : 2; }
+
+// The stream belongs to the current device (the null stream always does).
+bool stream_here(void* stream) {
+  if (!stream) return true;
+  hipDevice_t of = 0;
+  int cur = 0;
+  if (hipStreamGetDevice((hipStream_t)stream, &of) != hipSuccess || hipGetDevice(&cur) != hipSuccess) {
+    (void)hipGetLastError();
+    return false;
+  }
+  return (int)of == cur;
+}
+
+bool aligned_to(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
+bool mx4_shape(int64_t rows, int64_t k) { return rows > 0 && rows <= (1LL << 30) && k > 0 && k <= kMx4MaxK; }
+
+}  // namespace
+
+extern "C" {
+
+size_t gg_mxfp4_packed_size(int64_t rows, int64_t k) { return mx4_shape(rows, k) ? mx4_layout(rows, k).bytes() : 0; }
+
+int gg_mxfp4_quantize(const void* src, uint32_t type, int64_t rows, int64_t k, int64_t ld, void* packed,
+                      void* stream) {
+  const int e = elem_of(type);
+  if (!src || !packed || e < 0 || !mx4_shape(rows, k) || ld < k || !aligned_to(src, elem_size(e)) ||
+      !aligned_to(packed, 16) || !stream_here(stream))
+    return GG_ERR_INVALID;
+  return launch_mx4_quantize(e, src, rows, k, ld, (uint8_t*)packed, stream) ? GG_ERR_HIP : GG_OK;
+}
+
+int gg_mxfp4_dequant(const void* packed, float* out, int64_t rows, int64_t k, int64_t ld, void* stream) {
+  if (!packed || !out || !mx4_shape(rows, k) || ld < k || !aligned_to(packed, 16) || !aligned_to(out, 4) ||
+      !stream_here(stream))
+    return GG_ERR_INVALID;
+  return launch_mx4_dequant((const uint8_t*)packed, out, rows, k, ld, stream) ? GG_ERR_HIP : GG_OK;
+}
+
+// The size holds for every y_type: the most parts that one takes.
+size_t gg_mxfp4_linear_workspace_size(uint32_t x_type, int64_t m, int64_t rows, int64_t k) {
+  const int e = elem_of(x_type);
+  if (e < 0 || !mx4_shape(m, k) || !mx4_shape(rows, k)) return 0;
+  const int parts = mx_parts(e, ELEM_F32);
+  return mx_gemv_fits(m, parts, k) ? 0 : mx_parts_bytes(m, k, parts);
+}
+
+int gg_mxfp4_linear(const void* w, const void* x, uint32_t x_type, int64_t ldx, void* y, uint32_t y_type, int64_t ldy,
+                    int64_t m, int64_t rows, int64_t k, void* workspace, void* stream) {
+  const bool x4 = x_type == GG_TYPE_MXFP4;
+  const int xe = elem_of(x_type), ye = elem_of(y_type);
+  if (!w || !x || !y || (xe < 0 && !x4) || ye < 0 || !mx4_shape(m, k) || !mx4_shape(rows, k) || ldy < rows ||
+      (!x4 && ldx < k) || !aligned_to(w, 16) || !aligned_to(x, x4 ? 16 : elem_size(xe)) ||
+      !aligned_to(y, elem_size(ye)) || !stream_here(stream))
+    return GG_ERR_INVALID;
+  const Mx4Layout lw = mx4_layout(rows, k), lx = mx4_layout(m, k);
+  Mx4LinearArgs a{};
+  a.w = (const uint8_t*)w;
+  a.n = rows;
+  a.k = (int)k;
+  a.kt = lw.kt;
+  a.ks = lw.ks;
+  a.wrt = lw.rt;
+  a.x = x;
+  a.ldx = ldx;
+  a.x_elem = xe;
+  a.m = m;
+  a.xrt = lx.rt;
+  a.y = y;
+  a.ldy = ldy;
+  a.y_elem = ye;
+  a.y_vec = aligned_to(y, 4 * elem_size(ye)) && ldy % 4 == 0;
+  a.parts = x4 ? 1 : mx_parts(xe, ye);
+  if (!x4) {
+    if (mx_gemv_fits(m, a.parts, k)) return launch_mx4_gemv(a, stream) ? GG_ERR_HIP : GG_OK;
+    if (!workspace || !aligned_to(workspace, 16)) return GG_ERR_INVALID;
+    if (launch_mx_split(xe, x, m, k, ldx, a.parts, (uint8_t*)workspace, stream)) return GG_ERR_HIP;
+    a.x = workspace;
+  }
+  return launch_mx4_gemm(a, x4, stream) ? GG_ERR_HIP : GG_OK;
+}
+
+size_t gg_score_workspace_size(int64_t rows, int32_t n, int32_t top_n) {
+  if (rows <= 0 || rows > (1LL << 30) || n <= 0 || n > (1 << 30) || top_n < 0 || top_n > kScoreMaxTop) return 0;
+  int nch, per;
+  score_plan(rows, n, &nch, &per);
+  return nch == 1 ? 0 : (size_t)rows * nch * (16 + 8 * (size_t)top_n);
+}
+
+int gg_score_logits(const void* logits, uint32_t type, int64_t rows, int32_t n, int64_t ld, const int32_t* ids,
+                    int32_t n_ids, float* id_logprobs, float* lse, float* entropy, int32_t top_n, int32_t* top_ids,
+                    float* top_logprobs, void* workspace, void* stream) {
+  const int e = elem_of(type);
+  if (!logits || e < 0 || rows <= 0 || rows > (1LL << 30) || n <= 0 || n > (1 << 30) || ld < n || n_ids < 0 ||
+      (n_ids > 0 && (!ids || !id_logprobs)) || top_n < 0 || top_n > kScoreMaxTop ||
+      !aligned_to(logits, elem_size(e)) || !stream_here(stream))
+    return GG_ERR_INVALID;
+  const size_t ws = gg_score_workspace_size(rows, n, top_n);
+  if (ws && (!workspace || !aligned_to(workspace, 16))) return GG_ERR_INVALID;
+  ScoreArgs a{};
+  a.z = logits;
+  a.ld = ld;
+  a.rows = rows;
+  a.n = n;
+  int tiles;
+  score_plan(rows, n, &a.nch, &tiles);
+  a.per = tiles * (int)(kScoreTile * elem_size(e) / 16);
+  a.ids = ids;
+  a.n_ids = n_ids;
+  a.lp = id_logprobs;
+  a.lse = lse;
+  a.entropy = entropy;
+  a.top = top_n;
+  a.top_ids = top_ids;
+  a.top_lp = top_logprobs;
+  a.part = (float*)workspace;
+  a.keys = (uint64_t*)((char*)workspace + (size_t)rows * a.nch * 16);
+  return launch_score(e, a, stream) ? GG_ERR_HIP : GG_OK;
+}
+
+}  // extern "C"

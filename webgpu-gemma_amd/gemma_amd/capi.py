@@ -25,6 +25,8 @@ GG_ERR_OOM = -6
 GG_TYPE_F32 = 0
 GG_TYPE_F16 = 1
 GG_TYPE_Q8_0 = 8
+GG_TYPE_BF16 = 30
+GG_TYPE_MXFP4 = 39
 
 GG_ATTN_REFERENCE = 0
 GG_ATTN_GEMMA3 = 1
@@ -84,6 +86,7 @@ class GGError(RuntimeError):
 _LIB = None
 
 _P = ctypes.c_void_p
+_I64 = ctypes.c_int64
 _SIGS = {
     "gg_create": (_P, [ctypes.POINTER(GGConfig)]),
     "gg_upload_tensor": (ctypes.c_int, [_P, ctypes.c_char_p, ctypes.c_uint32, ctypes.POINTER(ctypes.c_uint64),
@@ -118,6 +121,15 @@ _SIGS = {
                                         ctypes.POINTER(ctypes.c_int32), _P]),
     "gg_select_logits_noalloc": (ctypes.c_int, [_P, ctypes.c_int32, _P, ctypes.POINTER(GGSample), ctypes.c_double,
                                                 _P, ctypes.POINTER(ctypes.c_int32), _P]),
+    "gg_mxfp4_packed_size": (ctypes.c_size_t, [_I64, _I64]),
+    "gg_mxfp4_quantize": (ctypes.c_int, [_P, ctypes.c_uint32, _I64, _I64, _I64, _P, _P]),
+    "gg_mxfp4_dequant": (ctypes.c_int, [_P, _P, _I64, _I64, _I64, _P]),
+    "gg_mxfp4_linear_workspace_size": (ctypes.c_size_t, [ctypes.c_uint32, _I64, _I64, _I64]),
+    "gg_mxfp4_linear": (ctypes.c_int, [_P, _P, ctypes.c_uint32, _I64, _P, ctypes.c_uint32, _I64, _I64, _I64, _I64,
+                                       _P, _P]),
+    "gg_score_workspace_size": (ctypes.c_size_t, [_I64, ctypes.c_int32, ctypes.c_int32]),
+    "gg_score_logits": (ctypes.c_int, [_P, ctypes.c_uint32, _I64, ctypes.c_int32, _I64, _P, ctypes.c_int32, _P, _P, _P,
+                                       ctypes.c_int32, _P, _P, _P, _P]),
 }
 
 
@@ -330,3 +342,42 @@ def select_logits_noalloc(logits_ptr: int, n: int, seen_ptr: int | None, tempera
     _check(None, lib().gg_select_logits_noalloc(logits_ptr, n, seen_ptr or None, ctypes.byref(s), float(u),
                                                 topk_ptr or None, ctypes.byref(out), _stream_ptr(stream)))
     return out.value
+
+
+def mxfp4_packed_size(rows: int, k: int) -> int:
+    return int(lib().gg_mxfp4_packed_size(rows, k))
+
+
+def mxfp4_quantize(src_ptr: int, ggml_type: int, rows: int, k: int, ld: int, packed_ptr: int, stream=None):
+    """Rows of f32 / f16 / bf16 -> packed MXFP4."""
+    _check(None, lib().gg_mxfp4_quantize(src_ptr, ggml_type, rows, k, ld, packed_ptr, _stream_ptr(stream)))
+
+
+def mxfp4_dequant(packed_ptr: int, out_ptr: int, rows: int, k: int, ld: int, stream=None):
+    _check(None, lib().gg_mxfp4_dequant(packed_ptr, out_ptr, rows, k, ld, _stream_ptr(stream)))
+
+
+def mxfp4_linear_workspace_size(x_type: int, m: int, rows: int, k: int) -> int:
+    return int(lib().gg_mxfp4_linear_workspace_size(x_type, m, rows, k))
+
+
+def mxfp4_linear(w_ptr: int, x_ptr: int, x_type: int, ldx: int, y_ptr: int, y_type: int, ldy: int, m: int, rows: int,
+                 k: int, ws_ptr: int | None = None, stream=None):
+    """y[m][rows] = x[m][k] W[rows][k]^T, W packed MXFP4, x f32 / f16 / bf16 rows or packed MXFP4."""
+    _check(None, lib().gg_mxfp4_linear(w_ptr, x_ptr, x_type, ldx, y_ptr, y_type, ldy, m, rows, k, ws_ptr or None,
+                                       _stream_ptr(stream)))
+
+
+def score_workspace_size(rows: int, n: int, top_n: int) -> int:
+    return int(lib().gg_score_workspace_size(rows, n, top_n))
+
+
+def score_logits(logits_ptr: int, ggml_type: int, rows: int, n: int, ld: int, ids_ptr: int | None, n_ids: int,
+                 id_logprobs_ptr: int | None, lse_ptr: int | None, entropy_ptr: int | None, top_n: int = 0,
+                 top_ids_ptr: int | None = None, top_logprobs_ptr: int | None = None, ws_ptr: int | None = None,
+                 stream=None):
+    """Log probabilities of given ids, log-sum-exp, entropy and the best alternatives of rows of logits."""
+    _check(None, lib().gg_score_logits(logits_ptr, ggml_type, rows, n, ld, ids_ptr or None, n_ids,
+                                       id_logprobs_ptr or None, lse_ptr or None, entropy_ptr or None, top_n,
+                                       top_ids_ptr or None, top_logprobs_ptr or None, ws_ptr or None,
+                                       _stream_ptr(stream)))
