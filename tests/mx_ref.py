@@ -38,7 +38,7 @@ def parts(x_type, y_type):
         return 3
     if y_type == "f16":
         return 3 if x_type == "bf16" else 4
-    return 5 if x_type == "f32" else 4
+    return 5
 
 
 def product_bound(x, w, y, x_type, y_type):

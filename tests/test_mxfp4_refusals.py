@@ -26,11 +26,13 @@ def test_packed_sizes():
 
 def test_workspace_sizes():
     ws = capi.mxfp4_linear_workspace_size
-    assert ws(MX, 1000, 1000, 1000) == 0
-    assert ws(F32, 1, 1152, 6912) == 0 and ws(F32, 3, 1536, 1152) == 0
-    assert ws(F32, 4, 1536, 1152) == 18 * 5 * 1536 + 5 * 256
-    assert ws(BF16, 64, 1536, 1152) == 2 * (18 * 4 * 1536 + 5 * 256)
+    assert ws(F32, 1, 1152, 6912) == 0 and ws(F32, 3, 1536, 1152) == 0     # few rows: none
+    parts = 64 * (18 + 7) * 5 * 48 + 2 * 5 * 256                           # at least the parts of x
+    assert ws(F32, 64, 1536, 1152) >= parts - 7 * 5 * 1536
+    assert ws(MX, 4096, 8192, 8192) == 0                                    # enough blocks: no slices of k
+    assert ws(MX, 16, 64, 1 << 20) > 0
     assert ws(capi.GG_TYPE_Q8_0, 64, 1536, 1152) == 0 and ws(F32, 0, 1, 1) == 0
+    assert ws(F32, 1 << 30, 1 << 30, 1 << 20) > 1 << 50                     # no overflow
     assert capi.score_workspace_size(1 << 20, 1000, 5) == 0     # one block a row
     assert capi.score_workspace_size(1, 262144, 20) > 0
     assert capi.score_workspace_size(0, 1000, 5) == 0 and capi.score_workspace_size(1, 0, 5) == 0

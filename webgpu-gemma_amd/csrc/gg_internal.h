@@ -456,22 +456,26 @@ __host__ __device__ inline Mx4Layout mx4_layout(int64_t rows, int64_t k) {
 // e2m3 (6-bit) value, exactly, so part p is a 6-bit MX block of scale
 // 2^(e - 5 p) and the matrix instruction multiplies it by the 4-bit weights
 // without another rounding. Parts by what the result can show: a bf16 result
-// keeps 8 bits and takes 3 parts (2^-14 of the block's maximum), an f16
-// result 11 and takes 4 (3 from bf16, whose own 8 bits they hold), an f32
-// result takes 5 from f32 (2^-24: as f32 itself) and 4 (2^-19) from 16-bit
-// types, whose values they hold down to 2^-8 of the block's maximum.
+// keeps 8 bits and takes 3 parts (2^-14 of the block's maximum), an f16 result
+// 11 and takes 4 (3 from bf16, whose own 8 bits they hold), an f32 result takes
+// 5 (2^-24, as f32 itself; 4 parts of 16-bit inputs with outliers in a block
+// left errors of 1.5e-6 where f32 products of the same inputs leave 2e-8).
 __host__ __device__ inline int mx_parts(int x_elem, int y_elem) {
   if (y_elem == ELEM_BF16) return 3;
   if (y_elem == ELEM_F16) return x_elem == ELEM_BF16 ? 3 : 4;
-  return x_elem == ELEM_F32 ? 5 : 4;
+  return 5;
 }
 constexpr int kMxMaxParts = 5;
 constexpr int kMxPartBytes = 1536;   // 32 rows x 64 k of one part: 16 bytes a lane, then 8 bytes a lane
-// Workspace of m x k activations in parts: [row group][k group][part][1536],
-// then the scale bytes of part 0 as in Mx4Layout.
+constexpr int kMxPadGroups = 7;      // row groups that a block of a product may read past the last
+// Workspace of m x k activations in parts: [k group][row group][part][1536]
+// and the padding, then the scale bytes of part 0 as in Mx4Layout.
+__host__ __device__ inline size_t mx_codes_bytes(int64_t rt, int kt, int parts) {
+  return ((size_t)rt * kt + kMxPadGroups) * parts * kMxPartBytes;
+}
 inline size_t mx_parts_bytes(int64_t m, int64_t k, int parts) {
   const Mx4Layout L = mx4_layout(m, k);
-  return (size_t)L.rt * L.kt * parts * kMxPartBytes + (size_t)L.rt * L.ks * 256;
+  return mx_codes_bytes(L.rt, L.kt, parts) + (size_t)L.rt * L.ks * 256;
 }
 
 struct Mx4LinearArgs {
@@ -487,21 +491,79 @@ struct Mx4LinearArgs {
   int64_t ldy;
   int y_elem;
   int parts;
-  int y_vec;             // 4 consecutive outputs may be stored at once
+  int y_vec;             // rows of y are 16-byte aligned
+  int kslices;           // k slices of the many-row kernel; above 1 they leave
+  float* partial;        // f32 sums [kslices][m][ldp] that k_mx4_join adds
+  int64_t ldp;
 };
-constexpr int kMxGemvCols = 16;
-inline size_t mx_gemv_lds(int cols, int k) { return (size_t)((k + 127) / 128 * 4) * (24 + 1) * cols; }
-// A product with m rows and `parts` parts takes the few-row kernel, which has
-// a column of the matrix instruction for each part of each row.
+// A product with m rows and `parts` parts takes the few-row kernel when it has
+// a column of its matrix instructions for each part of each row, and LDS holds
+// them (32 bytes of each 32-block's part) and the sums.
+constexpr int kMxGemvCols = 64, kMxGemvWaves = 8;
+__host__ __device__ constexpr size_t mx_gemv_sums(int col_tiles) {   // f32 [wave][16][16 col_tiles + 1]
+  return (size_t)kMxGemvWaves * 16 * (16 * col_tiles + 1) * 4;
+}
+inline size_t mx_gemv_lds(int cols, int k) {
+  return mx_gemv_sums((cols + 15) / 16) + (size_t)((k + 127) / 128 * 4) * cols * 32;
+}
 inline bool mx_gemv_fits(int64_t m, int parts, int64_t k) {
-  return m * parts <= kMxGemvCols && mx_gemv_lds((int)m * parts, (int)k) <= 52 * 1024;
+  return m * parts <= kMxGemvCols && mx_gemv_lds((int)m * parts, (int)k) <= 160 * 1024;
+}
+// Tiles of the many-row kernel (features x rows) and slices of k.
+enum Mx4TileId { MT_256x256, MT_256x64, MT_128x64, MT_128x32, MT_COUNT };
+struct Mx4Tile {
+  int bn, bm;
+  // us: a 64-deep step of a block alone on a CU (with parts: + for each), its
+  // start and end; the same for each block when the CUs are full
+  float lat, lat_part, lat_end, thr, thr_part, thr_end;
+};
+// Least-squares fits of 11,000 timings (240 products of 1 to 4096 rows, 64 to
+// 262144 features and k of 64 to 8192, each tile, 1 to 16 slices): 11% rms for
+// parts, 8% for packed x; the choice costs 1.8% and 3.5% over the best of all.
+constexpr Mx4Tile kMx4PartTiles[MT_COUNT] = {{256, 256, .15f, .05f, 2.f, .006f, .326f, 12.1f},
+                                             {256, 64, .127f, .094f, 4.6f, .052f, .097f, 3.1f},
+                                             {},
+                                             {128, 32, .222f, .005f, 1.3f, .078f, .020f, 1.4f}};
+constexpr Mx4Tile kMx4PackedTiles[MT_COUNT] = {{256, 256, .205f, 0.f, 2.4f, .432f, 0.f, 8.1f},
+                                               {},
+                                               {128, 64, .114f, 0.f, 1.6f, .097f, 0.f, 1.2f},
+                                               {128, 32, .040f, 0.f, .95f, .065f, 0.f, 1.1f}};
+constexpr int kMx4MaxSlices = 16;
+constexpr int64_t kMx4MaxSums = 1 << 24;   // f32 sums that slices may leave
+struct Mx4Plan { int tile, slices; };
+inline Mx4Plan mx4_plan(bool packed, int parts, int64_t m, int64_t n, int64_t k) {
+  const Mx4Tile* tiles = packed ? kMx4PackedTiles : kMx4PartTiles;
+  const int kt = (int)((k + 63) / 64), ks = (kt + 3) / 4;
+  Mx4Plan best{-1, 1};
+  double best_cost = 0.0;
+  for (int t = 0; t < MT_COUNT; ++t) {
+    const Mx4Tile& T = tiles[t];
+    if (!T.bn) continue;
+    const double blocks = (double)((n + T.bn - 1) / T.bn) * (double)((m + T.bm - 1) / T.bm);
+    for (int s = 1; s <= kMx4MaxSlices && s <= ks; s += s < 4 ? 1 : s < 8 ? 2 : 4) {
+      if (s > 1 && (m > 65535 || (int64_t)s * m > kMx4MaxSums / ((n + 3) / 4 * 4))) break;
+      const int slice = 4 * ((ks + s - 1) / s), steps = kt < slice ? kt : slice;
+      const double alone = steps * (T.lat + T.lat_part * parts) + T.lat_end;
+      const double full = steps * (T.thr + T.thr_part * parts) + T.thr_end;
+      const double rounds = (double)(int64_t)((blocks * s + 255) / 256) * full;
+      const double cost = (alone > rounds ? alone : rounds) + (s > 1 ? 2.9 + 0.6e-6 * s * m * n : 0.0);
+      if (best.tile < 0 || cost < best_cost) {
+        best_cost = cost;
+        best = {t, s};
+      }
+    }
+  }
+  return best;
+}
+inline size_t mx4_sums_bytes(const Mx4Plan& p, int64_t m, int64_t n) {
+  return p.slices > 1 ? (size_t)p.slices * m * ((n + 3) / 4 * 4) * 4 : 0;
 }
 int launch_mx4_quantize(int elem, const void* src, int64_t rows, int64_t k, int64_t ld, uint8_t* dst, void* stream);
 int launch_mx4_dequant(const uint8_t* src, float* out, int64_t rows, int64_t k, int64_t ld, void* stream);
 int launch_mx_split(int elem, const void* src, int64_t rows, int64_t k, int64_t ld, int parts, uint8_t* dst,
                     void* stream);
 int launch_mx4_gemv(const Mx4LinearArgs& a, void* stream);
-int launch_mx4_gemm(const Mx4LinearArgs& a, bool x_mx4, void* stream);
+int launch_mx4_gemm(const Mx4LinearArgs& a, bool packed, int tile, void* stream);
 
 constexpr int kScoreMaxTop = 64;       // best alternatives of a row at most
 constexpr int kScoreMaxChunks = 256;   // blocks that share a row at most

@@ -146,78 +146,88 @@ __global__ __launch_bounds__(256) void k_mx4_dequant(const uint8_t* __restrict__
 // Activations in parts (mx_parts). A block of 32 with largest magnitude in
 // [2^e, 2^(e+1)): scale byte e + 127, at least 21 so that every part's is at
 // least 1, 255 when the block holds an Inf or a NaN (its row's results are
-// NaN). part_round: u to the nearest multiple of 1/8 for |u| <= 2.
+// NaN). Part p of u = x / 2^e is what is left of u rounded to a multiple of
+// 2^(-3 - 5 p), to nearest: |u| <= 2 before part 0, 2^(-4 - 5 p) after part p.
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ float part_round(float u) { return (u + 1572864.0f) - 1572864.0f; }   // 1.5 2^20: ulp 1/8
+
+// 32 values, even elements in a, odd ones in b, over scale -> their e2m3 codes,
+// element i at bit 6 i. The instruction writes its result while it still reads
+// its operands, so the result must not share their registers: that is asked
+// for here, since the builtin's result was placed over the scale (and the
+// elements behind the first two were divided by something else).
+__device__ __forceinline__ u32x6 to_fp6(const f32x16& a, const f32x16& b, float scale) {
+  u32x6 z;
+  asm("v_cvt_scalef32_2xpk16_fp6_f32 %0, %1, %2, %3\n\ts_nop 1" : "=&v"(z) : "v"(a), "v"(b), "v"(scale));
+  return z;
+}
+
+constexpr float kPartMagic = 1572864.0f;   // 1.5 2^20, whose last bit is 1/8: adding and subtracting it rounds to 1/8
 __device__ __forceinline__ int parts_byte(uint32_t amax_bits) {
   const int ex = (int)(amax_bits >> 23);
   return max(ex, 1 + 5 * (kMxMaxParts - 1));
 }
 
-// 32 rows x 256 k of a row-major matrix -> parts; thread tid owns the 32-block
-// of lane tid % 64 of tile tid / 64.
-template <class T, bool VEC>
-__global__ __launch_bounds__(256) void k_mx_split(const T* __restrict__ src, int64_t rows, int64_t k, int64_t ld,
-                                                  int parts, uint8_t* __restrict__ dst, Mx4Layout L) {
-  constexpr int kPitch = 257;   // a thread reads its row's block: 32 rows x 2 blocks fall on 64 banks
-  __shared__ float xs[32 * kPitch];
-  __shared__ __align__(4) uint8_t scales[256];
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-  const int64_t R = blockIdx.x;
-  const int g = blockIdx.y;
-  const int64_t c = (int64_t)g * 256 + 4 * lane;
-  float v[8][4];
+// A 32-block of x in a thread: its elements, even and odd ones apart as the
+// conversion takes them, and the parts one after the other.
+struct Block32 {
+  f32x16 ev, od;
+  float magic, unit;
+  template <class T, bool VEC>
+  __device__ __forceinline__ void load(const T* row, int64_t c, int64_t k) {
+    float v[8][4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int64_t r = R * 32 + wv * 8 + i;
-    if (r < rows) {
-      load4<T, VEC>(src + r * ld, c, k, v[i]);
-    } else {
-      v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0.f;
+    for (int i = 0; i < 8; ++i) load4<T, VEC>(row, c + 4 * i, k, v[i]);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      ev[i] = v[i / 2][2 * (i & 1)];
+      od[i] = v[i / 2][2 * (i & 1) + 1];
     }
   }
+  // the scale byte; the elements become x / 2^e
+  __device__ __forceinline__ int scale() {
+    uint32_t a = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 16; ++i)
+      a = max(a, max(__float_as_uint(ev[i]) & 0x7fffffffu, __float_as_uint(od[i]) & 0x7fffffffu));
+    const int byte = parts_byte(a);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) xs[(wv * 8 + i) * kPitch + 4 * lane + j] = v[i][j];
-  __syncthreads();
-  const float* x = xs + (lane & 31) * kPitch + 64 * wv + 32 * (lane >> 5);
-  f32x16 ev, od;   // even and odd elements: the conversion interleaves its operands
-  uint32_t a = 0;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    ev[i] = x[2 * i];
-    od[i] = x[2 * i + 1];
-    a = max(a, max(__float_as_uint(ev[i]) & 0x7fffffffu, __float_as_uint(od[i]) & 0x7fffffffu));
+    for (int i = 0; i < 16; ++i) {
+      ev[i] = ldexpf(ev[i], 127 - byte);
+      od[i] = ldexpf(od[i], 127 - byte);
+    }
+    return byte;
   }
-  const int byte = parts_byte(a);
-  scales[4 * lane + wv] = (uint8_t)byte;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    ev[i] = ldexpf(ev[i], 127 - byte);
-    od[i] = ldexpf(od[i], 127 - byte);
-  }
-  const int t = g * 4 + wv;
-  uint8_t* out = dst + ((size_t)R * L.kt + t) * parts * kMxPartBytes;
-  for (int p = 0; p < parts; ++p) {
+  __device__ __forceinline__ u32x6 part(bool first) {
+    magic = first ? kPartMagic : magic * 0.03125f;
+    unit = first ? 1.f : unit * 0.03125f;
     f32x16 qe, qo;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      qe[i] = part_round(ev[i]);
-      qo[i] = part_round(od[i]);
-      ev[i] = (ev[i] - qe[i]) * 32.0f;
-      od[i] = (od[i] - qo[i]) * 32.0f;
+      qe[i] = (ev[i] + magic) - magic;
+      qo[i] = (od[i] + magic) - magic;
+      ev[i] -= qe[i];
+      od[i] -= qo[i];
     }
-    const u32x6 z = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(qe, qo, 1.0f);
-    if (t < L.kt) {
-      *(u32x4*)(out + p * kMxPartBytes + 16 * lane) = u32x4{z[0], z[1], z[2], z[3]};
-      *(u32x2*)(out + p * kMxPartBytes + 1024 + 8 * lane) = u32x2{z[4], z[5]};
-    }
+    return to_fp6(qe, qo, unit);
   }
-  __syncthreads();
-  if (wv == 0)
-    *(uint32_t*)(dst + (size_t)L.rt * L.kt * parts * kMxPartBytes + ((size_t)R * L.ks + g) * 256 + 4 * lane) =
-        *(const uint32_t*)(scales + 4 * lane);
+};
+
+// A wave takes 32 rows x 64 k, a thread one 32-block of them.
+template <class T, bool VEC>
+__global__ __launch_bounds__(64) void k_mx_split(const T* __restrict__ src, int64_t rows, int64_t k, int64_t ld,
+                                                 int parts, uint8_t* __restrict__ dst, Mx4Layout L) {
+  const int lane = threadIdx.x;
+  const int64_t R = blockIdx.x, r = R * 32 + (lane & 31);
+  const int t = blockIdx.y;
+  Block32 v;
+  v.load<T, VEC>(src + min(r, rows - 1) * ld, (int64_t)t * 64 + 32 * (lane >> 5), r < rows ? k : 0);
+  dst[mx_codes_bytes(L.rt, L.kt, parts) + ((size_t)R * L.ks + (t >> 2)) * 256 + 4 * lane + (t & 3)] = (uint8_t)v.scale();
+  uint8_t* out = dst + ((size_t)t * L.rt + R) * parts * kMxPartBytes;
+  for (int p = 0; p < parts; ++p, out += kMxPartBytes) {
+    const u32x6 z = v.part(p == 0);
+    *(u32x4*)(out + 16 * lane) = u32x4{z[0], z[1], z[2], z[3]};
+    *(u32x2*)(out + 1024 + 8 * lane) = u32x2{z[4], z[5]};
+  }
 }
 
 template <class T>
@@ -228,124 +238,328 @@ __device__ __forceinline__ void store_elem(int elem, void* y, int64_t i, float v
   else store_y<__bf16>(y, i, v);
 }
 
-// ---------------------------------------------------------------------------
-// Few rows: m x parts <= 16 columns of the 16 x 16 x 128 matrix instruction,
-// column r parts + p holding part p of row r, so that one instruction
-// multiplies 16 weight rows x 128 k by every part at once and the sum over
-// the parts is taken once, at the end, in f32. The parts are made in LDS by
-// every block (k x m values), the weights go from memory to registers.
-// A wave takes 16 weight rows; `kw` waves share their k.
-// Bound by the read of the weights (17/32 byte each).
-// ---------------------------------------------------------------------------
-template <class T>
-__device__ void gemv_parts(const Mx4LinearArgs& a, int nb, int cols, uint8_t* xs, uint8_t* sc) {
-  // eight lanes to a 32-block, four elements each
-  const T* x = (const T*)a.x;
-  const int tid = threadIdx.x, P = a.parts, unit = tid & 7;
-  const int items = (int)a.m * nb;
-  for (int it = tid >> 3; it < items; it += blockDim.x >> 3) {
-    const int r = it / nb, kb = it - r * nb;
-    const int64_t c = (int64_t)kb * 32 + 4 * unit;
-    float v[4];
-    load4<T, false>(x + r * a.ldx, c, a.k, v);
-    uint32_t mx = 0;
+// A wave's 32 rows x F results from LDS (row pitch P floats) to y: 16 bytes a
+// lane where `vec` (rows of y 16-byte aligned) and all of them exist, else an
+// element a lane; either way the lanes go along the rows.
+template <class T, int F, int P>
+__device__ __forceinline__ void store_tile_t(T* y, int64_t ldy, int64_t row0, int64_t f0, int64_t m, int64_t n, int vec,
+                                             const float* tile, int lane) {
+  constexpr int V = 16 / sizeof(T);
+  typedef T vec_t __attribute__((ext_vector_type(V)));
+  if (vec && f0 + F <= n) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) mx = max(mx, __float_as_uint(v[j]) & 0x7fffffffu);
-    mx = max(mx, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)mx, 0xB1, 0xf, 0xf, false));
-    mx = max(mx, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)mx, 0x4E, 0xf, 0xf, false));
-    mx = max(mx, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)mx, 0x141, 0xf, 0xf, false));
-    const int byte = parts_byte(mx);
-    float u[4];
+    for (int i = 0; i < 32 * F / (64 * V); ++i) {
+      const int c = (i * 64 + lane) * V, r = c / F, f = c % F;
+      vec_t o;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) u[j] = ldexpf(v[j], 127 - byte);
-    for (int p = 0; p < P; ++p) {
-      uint32_t w = 0;
+      for (int q = 0; q < V / 4; ++q) {
+        const f32x4 t = *(const f32x4*)(tile + r * P + f + 4 * q);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float q = part_round(u[j]);
-        // e2m3 code of d / 8, d = 0..16, is d itself; bit 5 is the sign
-        const uint32_t code = (uint32_t)fabsf(q * 8.0f) | (q < 0.f ? 32u : 0u);
-        w |= (code & 63u) << (6 * j);
-        u[j] = (u[j] - q) * 32.0f;
+        for (int e = 0; e < 4; ++e) o[4 * q + e] = (T)t[e];
       }
-      uint8_t* d = xs + ((size_t)kb * cols + r * P + p) * 24 + 3 * unit;
-      d[0] = (uint8_t)w;
-      d[1] = (uint8_t)(w >> 8);
-      d[2] = (uint8_t)(w >> 16);
-      if (unit == 0) sc[kb * cols + r * P + p] = (uint8_t)(byte == 255 ? 255 : byte - 5 * p);
+      if (row0 + r < m) *(vec_t*)(y + (row0 + r) * ldy + f0 + f) = o;
+    }
+  } else {
+#pragma unroll 4
+    for (int i = 0; i < 32 * F / 64; ++i) {
+      const int c = i * 64 + lane, r = c / F, f = c % F;
+      if (row0 + r < m && f0 + f < n) y[(row0 + r) * ldy + f0 + f] = (T)tile[r * P + f];
     }
   }
 }
+template <int F, int P>
+__device__ __forceinline__ void store_tile(int elem, void* y, int64_t ldy, int64_t row0, int64_t f0, int64_t m, int64_t n,
+                                           int vec, const float* tile, int lane) {
+  if (elem == ELEM_F32) store_tile_t<float, F, P>((float*)y, ldy, row0, f0, m, n, vec, tile, lane);
+  else if (elem == ELEM_F16) store_tile_t<_Float16, F, P>((_Float16*)y, ldy, row0, f0, m, n, vec, tile, lane);
+  else store_tile_t<__bf16, F, P>((__bf16*)y, ldy, row0, f0, m, n, vec, tile, lane);
+}
 
-constexpr int kGemvWaves = 8;
-__global__ __launch_bounds__(64 * kGemvWaves) void k_mx4_gemv(Mx4LinearArgs a, int kw) {
-  extern __shared__ uint8_t lds[];
-  __shared__ float red[kGemvWaves][16][17];
+// ---------------------------------------------------------------------------
+// Few rows: m x parts columns in NC tiles of the 16 x 16 x 128 matrix
+// instruction, column r parts + p holding part p of row r, so that one
+// instruction multiplies 16 weight rows x 128 k by 16 of them at once; the sum
+// over the parts is taken once, at the end, in f32. One block a CU makes the
+// parts in its LDS (one launch, no workspace) and goes over its share of the
+// weights, which travel from memory to registers, kGemvAhead KB ahead in each
+// wave. A wave takes 16 weight rows; `kw` waves of a block share their k.
+// Bound by the read of the weights (17/32 byte each); a small product by its
+// chain of x, parts, weights, sums.
+// ---------------------------------------------------------------------------
+constexpr int kGemvAhead = 8;
+constexpr int kGemvRec = 32;         // bytes of a 32-block's part: 24 of elements, the scale byte, 7 unused
+
+template <class T, int NC>
+__global__ __launch_bounds__(64 * kMxGemvWaves) void k_mx4_gemv(Mx4LinearArgs a, int kw) {
+  constexpr int RP = 16 * NC + 1;
+  extern __shared__ f32x4 gemv_lds[];
+  float* red = (float*)gemv_lds;                                       // the waves' sums
+  uint8_t* rec = (uint8_t*)gemv_lds + mx_gemv_sums(NC);                // the parts
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int nb = (a.k + 127) / 128 * 4, cols = (int)a.m * a.parts;
-  uint8_t* xs = lds;
-  uint8_t* sc = lds + (size_t)nb * cols * 24;
-  if (a.x_elem == ELEM_F32) gemv_parts<float>(a, nb, cols, xs, sc);
-  else if (a.x_elem == ELEM_F16) gemv_parts<_Float16>(a, nb, cols, xs, sc);
-  else gemv_parts<__bf16>(a, nb, cols, xs, sc);
-  __syncthreads();
-  const int gb = kGemvWaves / kw, slot = wv / kw, kz = wv % kw;
-  const int steps = nb / 4, s0 = steps * kz / kw, s1 = steps * (kz + 1) / kw;
-  const int g = lane >> 4, c16 = lane & 15, col = min(c16, cols - 1);
+  const int nb = (a.k + 127) / 128 * 4, P = a.parts, cols = (int)a.m * P;
+  const int gb = kMxGemvWaves / kw, slot = wv / kw, kz = wv % kw;
+  const int steps = nb / 4, ns = (steps + kw - 1) / kw, s0 = kz * ns;   // this wave's steps [s0, s0 + ns), as far as they exist
+  const int g = lane >> 4, c16 = lane & 15;
   const int64_t groups = (a.n + 15) / 16;
   const uint8_t* wsc = a.w + (size_t)a.wrt * a.kt * 1024;
-  for (int64_t base = (int64_t)blockIdx.x * gb; base < groups; base += (int64_t)gridDim.x * gb) {
-    const int64_t q = min(base + slot, groups - 1), R = q >> 1;
+  const int kt = a.kt, ks = a.ks;
+
+  // the ring of weights in flight: (group, step) pairs in the order of use
+  u32x4 wr[kGemvAhead];
+  int wsr[kGemvAhead];
+  int64_t lbase = (int64_t)blockIdx.x * gb;
+  int ls = 0;
+  auto issue = [&](int r) __attribute__((always_inline)) {
+    // reads past the end repeat the last row group or k group: past the k
+    // groups x is zero (the last step's second tile) or the step is not used
+    const int64_t q = min(lbase + slot, groups - 1), R = q >> 1;
     const int in = 32 * (g & 1) + 16 * (int)(q & 1) + c16;
-    f32x4 acc{0.f, 0.f, 0.f, 0.f};
-    for (int s = s0; s < s1; ++s) {
-      // the last step's second tile may lie past the matrix: its x is zero,
-      // the tile read instead is the last one
-      const int t = min(2 * s + (g >> 1), a.kt - 1);
-      const u32x4 w4 = *(const u32x4*)(a.w + ((size_t)R * a.kt + t) * 1024 + 16 * in);
-      const int ws = wsc[((size_t)R * a.ks + (t >> 2)) * 256 + 4 * in + (t & 3)];
-      const uint8_t* xp = xs + ((size_t)(4 * s + g) * cols + col) * 24;
-      const u32x2 x0 = *(const u32x2*)xp, x1 = *(const u32x2*)(xp + 8), x2 = *(const u32x2*)(xp + 16);
-      const int xsv = sc[(4 * s + g) * cols + col];
-      const i32x8 wa = {(int)w4[0], (int)w4[1], (int)w4[2], (int)w4[3], 0, 0, 0, 0};
-      const i32x8 xb = {(int)x0[0], (int)x0[1], (int)x1[0], (int)x1[1], (int)x2[0], (int)x2[1], 0, 0};
-      acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wa, xb, acc, kFp4, kFp6, 0, ws, 0, xsv);
+    const int t = min(2 * (s0 + ls) + (g >> 1), kt - 1);
+    wr[r] = __builtin_nontemporal_load((const u32x4*)(a.w + ((size_t)R * kt + t) * 1024 + 16 * in));
+    wsr[r] = wsc[((size_t)R * ks + (t >> 2)) * 256 + 4 * in + (t & 3)];
+    if (++ls == ns) {
+      ls = 0;
+      lbase += (int64_t)gridDim.x * gb;
     }
-    __syncthreads();
+  };
+
+  // The parts: four lanes to a 32-block, eight elements each, the low 48 bits
+  // of a conversion. Loads return in order, so x is asked for before the
+  // weights are.
+  {
+    const T* x = (const T*)a.x;
+    const int items = (int)a.m * nb, unit = lane & 3;
+    const bool vec = ((uintptr_t)x % (4 * sizeof(T))) == 0 && a.ldx % 4 == 0;
+    f32x16 qe, qo;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) red[wv][4 * g + r][c16] = acc[r];
-    __syncthreads();
-    for (int i = tid; i < gb * 16 * (int)a.m; i += 64 * kGemvWaves) {
-      const int row = i % 16, sl = (i / 16) % gb, mr = i / (16 * gb);
-      const int64_t nrow = (base + sl) * 16 + row;
-      if (nrow >= a.n) continue;
-      float v = 0.f;
-      for (int p = a.parts - 1; p >= 0; --p)
-        for (int z = 0; z < kw; ++z) v += red[sl * kw + z][row][mr * a.parts + p];
-      store_elem(a.y_elem, a.y, mr * a.ldy + nrow, v);
+    for (int j = 4; j < 16; ++j) qe[j] = qo[j] = 0.f;
+    for (int i0 = 0; i0 < items; i0 += kMxGemvWaves * 16) {
+      const int it = i0 + (tid >> 2), ic = min(it, items - 1), r = ic / nb, kb = ic - r * nb;
+      const int64_t c = (int64_t)kb * 32 + 8 * unit;
+      float u[2][4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (vec) load4<T, true>(x + r * a.ldx, c + 4 * h, a.k, u[h]);
+        else load4<T, false>(x + r * a.ldx, c + 4 * h, a.k, u[h]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (i0 == 0) {
+#pragma unroll
+        for (int q = 0; q < kGemvAhead; ++q) issue(q);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      uint32_t mx = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) mx = max(mx, __float_as_uint(u[j >> 2][j & 3]) & 0x7fffffffu);
+      mx = max(mx, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)mx, 0xB1, 0xf, 0xf, false));
+      mx = max(mx, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)mx, 0x4E, 0xf, 0xf, false));
+      const int byte = parts_byte(mx);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) u[j >> 2][j & 3] = ldexpf(u[j >> 2][j & 3], 127 - byte);
+      float magic = kPartMagic, scale = 1.f;
+      uint8_t* d = rec + ((size_t)kb * cols + r * P) * kGemvRec;
+      for (int p = 0; p < P; ++p) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float &e = u[j >> 1][2 * (j & 1)], &o = u[j >> 1][2 * (j & 1) + 1];
+          qe[j] = (e + magic) - magic;
+          qo[j] = (o + magic) - magic;
+          e -= qe[j];
+          o -= qo[j];
+        }
+        const u32x6 z = to_fp6(qe, qo, scale);
+        // two lanes' 48 bits are three dwords: the first lane's low one, its
+        // high half with its neighbour's low half, the neighbour's rest
+        const uint32_t nz = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)z[0], 0xB1, 0xf, 0xf, false);
+        uint32_t* dw = (uint32_t*)(d + 12 * (unit >> 1));
+        if (it < items) {
+          dw[2 * (unit & 1)] = unit & 1 ? (z[0] >> 16) | (z[1] << 16) : z[0];
+          if ((unit & 1) == 0) dw[1] = (z[1] & 0xffffu) | (nz << 16);
+          else if (unit == 3) *(uint32_t*)(d + 24) = byte == 255 ? 255 : byte - 5 * p;
+        }
+        d += kGemvRec;
+        magic *= 0.03125f;
+        scale *= 0.03125f;
+      }
+    }
+  }
+  __syncthreads();
+  const int64_t iters = (groups + (int64_t)gridDim.x * gb - 1) / ((int64_t)gridDim.x * gb);
+  const int64_t total = iters * ns;
+  const uint8_t* xr[NC];   // this lane's records of the wave's next step
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+    xr[c] = rec + ((size_t)(4 * s0 + g) * cols + min(16 * c + c16, cols - 1)) * kGemvRec;
+  f32x4 acc[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+  int64_t base = (int64_t)blockIdx.x * gb;
+  int s = 0;
+  for (int64_t i = 0; i < total; i += kGemvAhead) {
+#pragma unroll
+    for (int r = 0; r < kGemvAhead; ++r) {
+      if (i + r >= total) break;
+      if (s0 + s < steps) {
+        const i32x8 wa = {(int)wr[r][0], (int)wr[r][1], (int)wr[r][2], (int)wr[r][3], 0, 0, 0, 0};
+        u32x4 x0[NC], x1[NC];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          x0[c] = *(const u32x4*)(xr[c] + (size_t)s * 4 * cols * kGemvRec);
+          x1[c] = *(const u32x4*)(xr[c] + (size_t)s * 4 * cols * kGemvRec + 16);
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const i32x8 xb = {(int)x0[c][0], (int)x0[c][1], (int)x0[c][2], (int)x0[c][3], (int)x1[c][0], (int)x1[c][1], 0, 0};
+          acc[c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wa, xb, acc[c], kFp4, kFp6, 0, wsr[r], 0, (int)x1[c][2]);
+        }
+      }
+      issue(r);
+      if (++s < ns) continue;
+      // the row groups' sums over the parts and over the waves that share them
+      s = 0;
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          red[(wv * 16 + 4 * g + e) * RP + 16 * c + c16] = acc[c][e];
+          acc[c][e] = 0.f;
+        }
+      __syncthreads();
+      // kw lanes an output, each the parts of one wave
+      const int outs = gb * 16 * (int)a.m, z = tid & (kw - 1);
+      for (int o0 = 0; o0 < outs; o0 += 64 * kMxGemvWaves / kw) {
+        const int o = o0 + tid / kw, oc = min(o, outs - 1);
+        const int row = oc & 15, sl = (oc >> 4) & (gb - 1), mr = oc / (16 * gb);
+        const float* q = red + ((sl * kw + z) * 16 + row) * RP + mr * P;
+        float t[kMxMaxParts], v = 0.f;
+#pragma unroll
+        for (int p = 0; p < kMxMaxParts; ++p) t[p] = q[min(p, P - 1)];
+#pragma unroll
+        for (int p = kMxMaxParts - 1; p >= 0; --p) v += p < P ? t[p] : 0.f;
+        if (kw >= 2) v += dpp_mov<0xB1>(v);
+        if (kw >= 4) v += dpp_mov<0x4E>(v);
+        if (kw >= 8) v += dpp_mov<0x141>(v);
+        const int64_t nrow = (base + sl) * 16 + row;
+        if (z == 0 && o < outs && nrow < a.n) store_elem(a.y_elem, a.y, mr * a.ldy + nrow, v);
+      }
+      __syncthreads();
+      base += (int64_t)gridDim.x * gb;
     }
   }
 }
 
 // ---------------------------------------------------------------------------
 // Many rows: 32 x 32 x 64 matrix instructions, weights as the first operand
-// (rows of the result), x as the second. A wave computes NF x MF tiles; the
-// operands come from memory in operand order.
+// (rows of the result), x as the second; a block computes BN features of BM
+// rows over one slice of k, a wave NF x MF instruction tiles of it.
+// The operands lie in memory in operand order, so a stage (ST groups of 64 k)
+// goes to LDS as it is, by DMA, 1 KB an instruction, NS - 1 stages ahead of
+// the one that is multiplied; one barrier a stage. With more than two stages
+// every wave starts the same number of copies (CPW) in every stage, so that
+// the number in flight tells which stage has arrived.
 // ---------------------------------------------------------------------------
-template <bool X4, int NF, int MF, int WN, int WM>
-__global__ __launch_bounds__(64 * WN * WM) void k_mx4_gemm(Mx4LinearArgs a, int nbn, int nbm) {
+template <int P, bool X4, int NF, int MF, int WN, int WM, int ST, int NS>
+struct GemmShape {
+  static constexpr int BN = 32 * NF * WN, BM = 32 * MF * WM, NW = WN * WM;
+  static constexpr int XG = X4 ? 1024 : P * kMxPartBytes;      // bytes of a row group's x per k group
+  static constexpr int WU = BN / 32 * ST;                      // DMA units of a stage's weights,
+  static constexpr int XB = BM / 32 * XG;                      // bytes of a k group's x,
+  static constexpr int XQ = (XB + 1023) / 1024, XU = XQ * ST;  // units of it and of a stage's,
+  static constexpr int GN = (BN + BM) / 32, SU = (GN + 3) / 4; // and of the row groups' scale dwords
+  static constexpr int CPW = (WU + NW - 1) / NW + (XU + NW - 1) / NW + (SU + NW - 1) / NW;
+  static_assert(ST == 4 || ST == 2 || ST == 1, "a stage lies within four k groups, whose scale bytes are one dword");
+  static_assert(NS >= 2 && NS <= 4, "scale dwords of two groups are held");
+  static_assert(BM / 32 <= kMxPadGroups + 1 || X4, "the parts are padded for the last block");
+  static_assert((NS - 2) * CPW < 64, "what a wave can wait for");
+};
+
+// One DMA instruction: lane l's 16 bytes at src go to dst + 16 l. Inline asm,
+// because the compiler would wait for every DMA in flight before any LDS read;
+// the waits before the barrier that precedes the readers are written out.
+__device__ __forceinline__ void dma16(const uint8_t* src, uint32_t dst) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(
+                   __builtin_amdgcn_readfirstlane(dst)),
+               "v"(src)
+               : "memory", "m0");
+}
+template <int N>
+__device__ __forceinline__ void wait_copies() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
+template <int P, bool X4, int NF, int MF, int WN, int WM, int ST, int NS, int OCC>
+__global__ __launch_bounds__(64 * WN * WM, OCC) void k_mx4_gemm(Mx4LinearArgs a, int nbn, int nbm) {
+  typedef GemmShape<P, X4, NF, MF, WN, WM, ST, NS> S;
+  __shared__ __align__(1024) uint8_t stage[NS][(S::WU + S::XU) * 1024];
+  __shared__ __align__(1024) uint8_t sstage[2][S::SU * 1024];
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wn = wv % WN, wm = wv / WN;
-  const int64_t bn = blockIdx.x % nbn, bm = blockIdx.x / nbn;
-  const int P = a.parts;
-  int64_t rn[NF], rm[MF];
-#pragma unroll
-  for (int i = 0; i < NF; ++i) rn[i] = min((bn * WN + wn) * NF + i, a.wrt - 1);
-#pragma unroll
-  for (int j = 0; j < MF; ++j) rm[j] = min((bm * WM + wm) * MF + j, a.xrt - 1);
+  // Tile order: the blocks with one value of blockIdx % 8 share an XCD and its
+  // L2; they take a contiguous range of an order with the k slices slowest,
+  // then groups of 4 tile rows, the rows fastest.
+  constexpr int GROUP = 4;
+  const int G = gridDim.x, xcd = blockIdx.x & 7;
+  const int LL = xcd * (G >> 3) + min(xcd, G & 7) + (blockIdx.x >> 3);
+  const int kz = LL / (nbn * nbm), L = LL - kz * (nbn * nbm);
+  const int fm = L / (GROUP * nbn) * GROUP, gm = min(nbm - fm, GROUP), Lp = L % (GROUP * nbn);
+  const int64_t bm = fm + Lp % gm, bn = Lp / gm;
+  const int t_lo = 4 * (int)((int64_t)a.ks * kz / a.kslices), t_hi = min(4 * (int)((int64_t)a.ks * (kz + 1) / a.kslices), a.kt);
   const uint8_t* x = (const uint8_t*)a.x;
   const uint8_t* wsc = a.w + (size_t)a.wrt * a.kt * 1024;
-  const uint8_t* xsc = x + (size_t)a.xrt * a.kt * (X4 ? 1024 : P * kMxPartBytes);
+  const uint8_t* xsc = x + (X4 ? (size_t)a.xrt * a.kt * 1024 : mx_codes_bytes(a.xrt, a.kt, P));
+  const int64_t rn0 = bn * (S::BN / 32), rm0 = bm * (S::BM / 32);   // first row groups
+  const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)&stage[0][0];
+  const uint32_t slds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)&sstage[0][0];
+  // The lanes' sources at k group 0. Row groups and k groups past the matrix
+  // read its last ones, parts past the last row group what follows them; their
+  // results are not stored, their x is not multiplied.
+  constexpr int NWC = (S::WU + S::NW - 1) / S::NW, NXC = (S::XU + S::NW - 1) / S::NW, NSC = (S::SU + S::NW - 1) / S::NW;
+  const uint8_t *wsrc[NWC], *xsrc[NXC], *ssrc[NSC];
+  const int kt = a.kt, ks = a.ks;
+  const int64_t wlast = a.wrt - 1, xlast = a.xrt - 1;
+  const size_t xstep = X4 ? 1024 : (size_t)a.xrt * S::XG;
+#pragma unroll
+  for (int i = 0; i < NWC; ++i) {
+    const int u = min(i * S::NW + wv, S::WU - 1);
+    wsrc[i] = a.w + (size_t)min(rn0 + u / ST, wlast) * kt * 1024 + 16 * lane;
+  }
+#pragma unroll
+  for (int i = 0; i < NXC; ++i) {
+    const int u = min(i * S::NW + wv, S::XU - 1);
+    if constexpr (X4) xsrc[i] = x + (size_t)min(rm0 + u / ST, xlast) * kt * 1024 + 16 * lane;
+    // the block's row groups of one k group lie one after the other
+    else xsrc[i] = x + (size_t)rm0 * S::XG + min(u % S::XQ * 1024 + 16 * lane, S::XB - 16);
+  }
+#pragma unroll
+  for (int i = 0; i < NSC; ++i) {
+    // 16 lanes a row group's 256 bytes of scales
+    const int gi = min(4 * min(i * S::NW + wv, S::SU - 1) + (lane >> 4), S::GN - 1);
+    ssrc[i] = (gi < S::BN / 32 ? wsc + (size_t)min(rn0 + gi, wlast) * ks * 256
+                               : xsc + (size_t)min(rm0 + gi - S::BN / 32, xlast) * ks * 256) + 16 * (lane & 15);
+  }
+  // With two stages a wave waits for all its copies, and nothing is copied
+  // twice. With more their number has to be the same in every stage: units and
+  // scales of the four k groups are fetched again where there are none left.
+  constexpr bool ONCE = NS == 2;
+  auto copy = [&](int t, int buf) __attribute__((always_inline)) {
+    const uint32_t dst = lds + buf * ((S::WU + S::XU) * 1024);
+#pragma unroll
+    for (int i = 0; i < NWC; ++i) {
+      const int u = min(i * S::NW + wv, S::WU - 1);
+      if (!ONCE || S::WU % S::NW == 0 || i * S::NW + wv < S::WU)
+        dma16(wsrc[i] + (size_t)(ST == 1 ? t : min(t + u % ST, kt - 1)) * 1024, dst + 1024 * u);
+    }
+#pragma unroll
+    for (int i = 0; i < NXC; ++i) {
+      const int u = min(i * S::NW + wv, S::XU - 1), q = X4 ? u % ST : u / S::XQ;
+      if (!ONCE || S::XU % S::NW == 0 || i * S::NW + wv < S::XU)
+        dma16(xsrc[i] + (size_t)(ST == 1 ? t : min(t + q, kt - 1)) * xstep, dst + 1024 * (S::WU + u));
+    }
+    if (ONCE && ST < 4 && (t & 3) != 0) return;
+#pragma unroll
+    for (int i = 0; i < NSC; ++i) {
+      const int u = min(i * S::NW + wv, S::SU - 1);
+      if (!ONCE || i * S::NW + wv < S::SU) dma16(ssrc[i] + (t >> 2) * 256, slds + ((t >> 2) & 1) * (S::SU * 1024) + u * 1024);
+    }
+  };
   f32x16 acc[NF][MF];
 #pragma unroll
   for (int i = 0; i < NF; ++i)
@@ -353,52 +567,115 @@ __global__ __launch_bounds__(64 * WN * WM) void k_mx4_gemm(Mx4LinearArgs a, int 
     for (int j = 0; j < MF; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-  for (int t = 0; t < a.kt; ++t) {
-    i32x8 w[NF];
-    int ws[NF], xs[MF];
 #pragma unroll
-    for (int i = 0; i < NF; ++i) {
-      const u32x4 q = *(const u32x4*)(a.w + ((size_t)rn[i] * a.kt + t) * 1024 + 16 * lane);
-      w[i] = i32x8{(int)q[0], (int)q[1], (int)q[2], (int)q[3], 0, 0, 0, 0};
-      ws[i] = wsc[((size_t)rn[i] * a.ks + (t >> 2)) * 256 + 4 * lane + (t & 3)];
-    }
+  for (int i = 0; i < NS - 1; ++i)
+    if (t_lo + i * ST < t_hi) copy(t_lo + i * ST, i);
+  int buf = 0, fill = NS - 1;
+  for (int t = t_lo; t < t_hi; t += ST) {
+    // the copies that may stay in flight: those of the NS - 2 stages behind
+    // this one, as far as there are any
+    if (NS == 2) wait_copies<0>();
+    else if (t + (NS - 2) * ST < t_hi) wait_copies<(NS - 2) * S::CPW>();
+    else if (NS == 4 && t + ST < t_hi) wait_copies<S::CPW>();
+    else wait_copies<0>();
+    __syncthreads();   // the stage has arrived for every wave, and every wave has read the one before
+    if (t + (NS - 1) * ST < t_hi) copy(t + (NS - 1) * ST, fill);
+    fill = fill + 1 == NS ? 0 : fill + 1;
+    const uint8_t* ws = stage[buf] + 16 * lane;
+    const uint8_t* xs = ws + S::WU * 1024;
+    buf = buf + 1 == NS ? 0 : buf + 1;
+    const uint32_t* sd = (const uint32_t*)sstage[(t >> 2) & 1] + lane;
+    int wd[NF], xd[MF];   // scale dwords: byte t % 4 is this k group's
 #pragma unroll
-    for (int j = 0; j < MF; ++j) xs[j] = xsc[((size_t)rm[j] * a.ks + (t >> 2)) * 256 + 4 * lane + (t & 3)];
-    for (int p = 0; p < P; ++p) {
+    for (int i = 0; i < NF; ++i) wd[i] = sd[(wn * NF + i) * 64];
 #pragma unroll
-      for (int j = 0; j < MF; ++j) {
-        i32x8 b;
-        if constexpr (X4) {
-          const u32x4 q = *(const u32x4*)(x + ((size_t)rm[j] * a.kt + t) * 1024 + 16 * lane);
-          b = i32x8{(int)q[0], (int)q[1], (int)q[2], (int)q[3], 0, 0, 0, 0};
-        } else {
-          const uint8_t* xp = x + (((size_t)rm[j] * a.kt + t) * P + p) * kMxPartBytes;
-          const u32x4 q = *(const u32x4*)(xp + 16 * lane);
-          const u32x2 h = *(const u32x2*)(xp + 1024 + 8 * lane);
-          b = i32x8{(int)q[0], (int)q[1], (int)q[2], (int)q[3], (int)h[0], (int)h[1], 0, 0};
+    for (int j = 0; j < MF; ++j) xd[j] = sd[(S::BN / 32 + wm * MF + j) * 64];
+#pragma unroll
+    for (int q = 0; q < ST; ++q) {
+      if (ST > 1 && t + q >= t_hi) break;
+      i32x8 w[NF];
+#pragma unroll
+      for (int i = 0; i < NF; ++i) {
+        const u32x4 v = *(const u32x4*)(ws + ((wn * NF + i) * ST + q) * 1024);
+        w[i] = i32x8{(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0};
+      }
+      const int sh = 8 * ((t & 3) + q);
+      int wsv[NF], xsv[MF];
+#pragma unroll
+      for (int i = 0; i < NF; ++i) wsv[i] = (uint32_t)wd[i] >> sh;
+#pragma unroll
+      for (int j = 0; j < MF; ++j) xsv[j] = ((uint32_t)xd[j] >> sh) & 255;
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+#pragma unroll
+        for (int j = 0; j < MF; ++j) {
+          i32x8 b;
+          if constexpr (X4) {
+            const u32x4 v = *(const u32x4*)(xs + ((wm * MF + j) * ST + q) * 1024);
+            b = i32x8{(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0};
+          } else {
+            const uint8_t* xp = xs + q * (S::XQ * 1024) + ((wm * MF + j) * P + p) * kMxPartBytes;
+            const u32x4 v = *(const u32x4*)xp;
+            const u32x2 h = *(const u32x2*)(xp + 1024 - 8 * lane);
+            b = i32x8{(int)v[0], (int)v[1], (int)v[2], (int)v[3], (int)h[0], (int)h[1], 0, 0};
+          }
+          // a NaN scale (255) stays one in part 0; the later parts' scales are 5 less each
+          const int sx = xsv[j] - 5 * p;
+#pragma unroll
+          for (int i = 0; i < NF; ++i)
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w[i], b, acc[i][j], kFp4, X4 ? kFp4 : kFp6, 0,
+                                                                        wsv[i], 0, sx);
         }
-        const int s = xs[j] == 255 ? 255 : xs[j] - 5 * p;
-#pragma unroll
-        for (int i = 0; i < NF; ++i)
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w[i], b, acc[i][j], kFp4, X4 ? kFp4 : kFp6, 0,
-                                                                      ws[i], 0, s);
       }
     }
   }
-  // lane: result column lane % 32 (a row of y); elements 4 e .. 4 e + 3 are
-  // features 8 e + 4 (lane / 32) ..
+  // A lane holds elements 4 e .. 4 e + 3 as features 8 e + 4 (lane / 32) .. of
+  // row lane % 32: they change places in LDS, a wave HF tiles at a time, so that
+  // whole lines of y are written. A slice of k leaves f32 sums.
+  void* y = a.y;
+  int64_t ldy = a.ldy;
+  int elem = a.y_elem, vec = a.y_vec;
+  if (a.kslices > 1) {
+    y = a.partial + (size_t)kz * a.m * a.ldp;
+    ldy = a.ldp;
+    elem = ELEM_F32;
+    vec = 1;
+  }
+  constexpr int ROOM = NS * (S::WU + S::XU) * 1024;
+  constexpr int HF = NF > 1 && S::NW * 32 * 68 * 4 <= ROOM ? 2 : 1, PITCH = 32 * HF + 4;
+  static_assert(S::NW * 32 * PITCH * 4 <= ROOM, "the stages hold a tile of each wave");
+  float* tile = (float*)&stage[0][0] + wv * 32 * PITCH;
+  __syncthreads();   // every wave has read its last stage
 #pragma unroll
   for (int j = 0; j < MF; ++j) {
-    const int64_t row = (((bm * WM + wm) * MF) + j) * 32 + (lane & 31);
-    if (row >= a.m) continue;
+    const int64_t row0 = (rm0 + wm * MF + j) * 32;
 #pragma unroll
-    for (int i = 0; i < NF; ++i)
+    for (int i0 = 0; i0 < NF; i0 += HF) {
+      const int64_t f0 = (rn0 + wn * NF + i0) * 32;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int64_t f = (((bn * WN + wn) * NF) + i) * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
-        if (f < a.n) store_elem(a.y_elem, a.y, row * a.ldy + f, acc[i][j][e]);
-      }
+      for (int i = 0; i < HF; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          *(f32x4*)(tile + (lane & 31) * PITCH + 32 * i + 8 * e + 4 * (lane >> 5)) =
+              f32x4{acc[i0 + i][j][4 * e], acc[i0 + i][j][4 * e + 1], acc[i0 + i][j][4 * e + 2], acc[i0 + i][j][4 * e + 3]};
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      store_tile<32 * HF, PITCH>(elem, y, ldy, row0, f0, a.m, a.n, vec, tile, lane);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
   }
+}
+
+// The k slices' sums, added in order; four features a thread.
+__global__ __launch_bounds__(256) void k_mx4_join(Mx4LinearArgs a) {
+  const int64_t f = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  const int64_t row = blockIdx.y;
+  if (f >= a.n) return;
+  const float* p = a.partial + row * a.ldp + f;   // ldp is a multiple of 4: whole vectors
+  f32x4 v = *(const f32x4*)p;
+  for (int z = 1; z < a.kslices; ++z) v += *(const f32x4*)(p + (size_t)z * a.m * a.ldp);
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (f + e < a.n) store_elem(a.y_elem, a.y, row * a.ldy + f + e, v[e]);
 }
 
 template <class T>
@@ -420,11 +697,11 @@ int quantize_t(const void* src, int64_t rows, int64_t k, int64_t ld, uint8_t* ds
 template <class T>
 int split_t(const void* src, int64_t rows, int64_t k, int64_t ld, int parts, uint8_t* dst, hipStream_t s) {
   const Mx4Layout L = mx4_layout(rows, k);
-  const dim3 grid((unsigned)L.rt, (unsigned)L.ks);
+  const dim3 grid((unsigned)L.rt, (unsigned)L.kt);
   if (aligned4<T>(src, ld))
-    hipLaunchKernelGGL((k_mx_split<T, true>), grid, dim3(256), 0, s, (const T*)src, rows, k, ld, parts, dst, L);
+    hipLaunchKernelGGL((k_mx_split<T, true>), grid, dim3(64), 0, s, (const T*)src, rows, k, ld, parts, dst, L);
   else
-    hipLaunchKernelGGL((k_mx_split<T, false>), grid, dim3(256), 0, s, (const T*)src, rows, k, ld, parts, dst, L);
+    hipLaunchKernelGGL((k_mx_split<T, false>), grid, dim3(64), 0, s, (const T*)src, rows, k, ld, parts, dst, L);
   return (int)hipGetLastError();
 }
 
@@ -462,28 +739,78 @@ int launch_mx_split(int elem, const void* src, int64_t rows, int64_t k, int64_t 
   return (int)hipErrorInvalidValue;
 }
 
-int launch_mx4_gemv(const Mx4LinearArgs& a, void* stream) {
-  const int cols = (int)a.m * a.parts;
-  const size_t lds = mx_gemv_lds(cols, a.k);
+template <class T>
+static int launch_gemv_t(const Mx4LinearArgs& a, hipStream_t s) {
+  const int cols = (int)a.m * a.parts, steps = (a.k + 127) / 128;
   const int64_t groups = (a.n + 15) / 16;
-  int kw = 8;   // waves that share 16 rows' k: as many as leave 512 blocks busy
-  while (kw > 1 && groups * kw > 8 * 512) kw >>= 1;
-  const int64_t blocks = (groups * kw + kGemvWaves - 1) / kGemvWaves;
-  hipLaunchKernelGGL(k_mx4_gemv, dim3((unsigned)(blocks < 512 ? blocks : 512)), dim3(64 * kGemvWaves), lds,
-                     (hipStream_t)stream, a, kw);
+  const size_t lds = mx_gemv_lds(cols, a.k);
+  // waves that share 16 rows' k: as many as leave a block for each CU, and each a step
+  int kw = kMxGemvWaves;
+  while (kw > 1 && (groups * kw > kMxGemvWaves * 256 || kw > steps)) kw >>= 1;
+  const int64_t blocks = (groups * kw + kMxGemvWaves - 1) / kMxGemvWaves;
+  // every block makes all parts: one a CU, and two where each has several row
+  // groups to go over and LDS holds both (more weights in flight)
+  const int64_t most = blocks >= 1024 && lds <= 80 * 1024 ? 512 : 256;
+  const dim3 grid((unsigned)(blocks < most ? blocks : most)), block(64 * kMxGemvWaves);
+  switch ((cols + 15) / 16) {
+    case 1: hipLaunchKernelGGL((k_mx4_gemv<T, 1>), grid, block, lds, s, a, kw); break;
+    case 2: hipLaunchKernelGGL((k_mx4_gemv<T, 2>), grid, block, lds, s, a, kw); break;
+    case 3: hipLaunchKernelGGL((k_mx4_gemv<T, 3>), grid, block, lds, s, a, kw); break;
+    case 4: hipLaunchKernelGGL((k_mx4_gemv<T, 4>), grid, block, lds, s, a, kw); break;
+    default: return (int)hipErrorInvalidValue;
+  }
   return (int)hipGetLastError();
 }
 
-int launch_mx4_gemm(const Mx4LinearArgs& a, bool x_mx4, void* stream) {
-  constexpr int NF = 2, MF = 2, WN = 2, WM = 2;
-  const int64_t nbn = (a.wrt + NF * WN - 1) / (NF * WN), nbm = (a.xrt + MF * WM - 1) / (MF * WM);
-  if (nbn * nbm > 0x7fffffffll) return (int)hipErrorInvalidValue;
-  const dim3 grid((unsigned)(nbn * nbm)), block(64 * WN * WM);
-  if (x_mx4)
-    hipLaunchKernelGGL((k_mx4_gemm<true, NF, MF, WN, WM>), grid, block, 0, (hipStream_t)stream, a, (int)nbn, (int)nbm);
-  else
-    hipLaunchKernelGGL((k_mx4_gemm<false, NF, MF, WN, WM>), grid, block, 0, (hipStream_t)stream, a, (int)nbn, (int)nbm);
+int launch_mx4_gemv(const Mx4LinearArgs& a, void* stream) {
+  hipStream_t s = (hipStream_t)stream;
+  switch (a.x_elem) {
+    case ELEM_F32: return launch_gemv_t<float>(a, s);
+    case ELEM_F16: return launch_gemv_t<_Float16>(a, s);
+    case ELEM_BF16: return launch_gemv_t<__bf16>(a, s);
+  }
+  return (int)hipErrorInvalidValue;
+}
+
+template <int P, bool X4, int NF, int MF, int WN, int WM, int ST, int NS, int OCC>
+static int launch_gemm_t(const Mx4LinearArgs& a, hipStream_t s) {
+  typedef GemmShape<P, X4, NF, MF, WN, WM, ST, NS> S;
+  const int64_t nbn = (a.n + S::BN - 1) / S::BN, nbm = (a.m + S::BM - 1) / S::BM;
+  if (nbn * nbm * a.kslices > 0x7fffffffll) return (int)hipErrorInvalidValue;
+  hipLaunchKernelGGL((k_mx4_gemm<P, X4, NF, MF, WN, WM, ST, NS, OCC>), dim3((unsigned)(nbn * nbm * a.kslices)),
+                     dim3(64 * WN * WM), 0, s, a, (int)nbn, (int)nbm);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.kslices == 1) return (int)e;
+  hipLaunchKernelGGL(k_mx4_join, dim3((unsigned)((a.n + 1023) / 1024), (unsigned)a.m), dim3(256), 0, s, a);
   return (int)hipGetLastError();
+}
+
+// The stages: 128 x 32 blocks, whose steps are short, copy two k groups at a
+// time, two stages ahead; packed x comes four k groups at a time.
+template <int P, bool X4>
+static int launch_gemm_p(const Mx4LinearArgs& a, int tile, hipStream_t s) {
+  switch (tile) {
+    case MT_256x256: return launch_gemm_t<P, X4, 4, 2, 2, 4, X4 ? 4 : 1, 2, 1>(a, s);
+    case MT_256x64:
+      if constexpr (!X4) return launch_gemm_t<P, X4, 2, 2, 4, 1, 1, 2, 2>(a, s);
+      break;
+    case MT_128x64:
+      if constexpr (X4) return launch_gemm_t<P, X4, 1, 2, 4, 1, 4, 2, 2>(a, s);
+      break;
+    case MT_128x32: return launch_gemm_t<P, X4, 1, 1, 4, 1, X4 ? 4 : 2, 3, 2>(a, s);
+  }
+  return (int)hipErrorInvalidValue;
+}
+
+int launch_mx4_gemm(const Mx4LinearArgs& a, bool packed, int tile, void* stream) {
+  hipStream_t s = (hipStream_t)stream;
+  if (packed) return launch_gemm_p<1, true>(a, tile, s);
+  switch (a.parts) {
+    case 3: return launch_gemm_p<3, false>(a, tile, s);
+    case 4: return launch_gemm_p<4, false>(a, tile, s);
+    case 5: return launch_gemm_p<5, false>(a, tile, s);
+  }
+  return (int)hipErrorInvalidValue;
 }
 
 }  // namespace gg

@@ -1809,12 +1809,21 @@ int gg_mxfp4_dequant(const void* packed, float* out, int64_t rows, int64_t k, in
   return launch_mx4_dequant((const uint8_t*)packed, out, rows, k, ld, stream) ? GG_ERR_HIP : GG_OK;
 }
 
-// The size holds for every y_type: the most parts that one takes.
+// Device bytes behind a product: the parts of x, then the slices' sums.
+static size_t linear_workspace(bool packed, int x_elem, int y_elem, int64_t m, int64_t n, int64_t k) {
+  const int parts = packed ? 1 : mx_parts(x_elem, y_elem);
+  if (!packed && mx_gemv_fits(m, parts, k)) return 0;
+  return (packed ? 0 : mx_parts_bytes(m, k, parts)) + mx4_sums_bytes(mx4_plan(packed, parts, m, n, k), m, n);
+}
+
+// Holds for every y_type.
 size_t gg_mxfp4_linear_workspace_size(uint32_t x_type, int64_t m, int64_t rows, int64_t k) {
+  const bool packed = x_type == GG_TYPE_MXFP4;
   const int e = elem_of(x_type);
-  if (e < 0 || !mx4_shape(m, k) || !mx4_shape(rows, k)) return 0;
-  const int parts = mx_parts(e, ELEM_F32);
-  return mx_gemv_fits(m, parts, k) ? 0 : mx_parts_bytes(m, k, parts);
+  if ((e < 0 && !packed) || !mx4_shape(m, k) || !mx4_shape(rows, k)) return 0;
+  size_t most = 0;
+  for (int ye : {ELEM_F32, ELEM_F16, ELEM_BF16}) most = std::max(most, linear_workspace(packed, e, ye, m, rows, k));
+  return most;
 }
 
 int gg_mxfp4_linear(const void* w, const void* x, uint32_t x_type, int64_t ldx, void* y, uint32_t y_type, int64_t ldy,
@@ -1841,15 +1850,19 @@ int gg_mxfp4_linear(const void* w, const void* x, uint32_t x_type, int64_t ldx, 
   a.y = y;
   a.ldy = ldy;
   a.y_elem = ye;
-  a.y_vec = aligned_to(y, 4 * elem_size(ye)) && ldy % 4 == 0;
+  a.y_vec = aligned_to(y, 16) && ldy * elem_size(ye) % 16 == 0;
   a.parts = x4 ? 1 : mx_parts(xe, ye);
+  if (!x4 && mx_gemv_fits(m, a.parts, k)) return launch_mx4_gemv(a, stream) ? GG_ERR_HIP : GG_OK;
+  if (linear_workspace(x4, xe, ye, m, rows, k) && (!workspace || !aligned_to(workspace, 16))) return GG_ERR_INVALID;
+  const Mx4Plan plan = mx4_plan(x4, a.parts, m, rows, k);
+  a.kslices = plan.slices;
+  a.ldp = (rows + 3) / 4 * 4;
+  a.partial = (float*)((uint8_t*)workspace + (x4 ? 0 : mx_parts_bytes(m, k, a.parts)));
   if (!x4) {
-    if (mx_gemv_fits(m, a.parts, k)) return launch_mx4_gemv(a, stream) ? GG_ERR_HIP : GG_OK;
-    if (!workspace || !aligned_to(workspace, 16)) return GG_ERR_INVALID;
     if (launch_mx_split(xe, x, m, k, ldx, a.parts, (uint8_t*)workspace, stream)) return GG_ERR_HIP;
     a.x = workspace;
   }
-  return launch_mx4_gemm(a, x4, stream) ? GG_ERR_HIP : GG_OK;
+  return launch_mx4_gemm(a, x4, plan.tile, stream) ? GG_ERR_HIP : GG_OK;
 }
 
 size_t gg_score_workspace_size(int64_t rows, int32_t n, int32_t top_n) {
