@@ -582,13 +582,16 @@ struct ScoreArgs {
   uint64_t* keys;        // [rows][nch][top]
 };
 constexpr int kScoreTile = 8192;       // elements a block takes at a time
-// Chunks of a row: about 1024 blocks in all, each of whole tiles. The first
-// tile may start up to 7 elements early (16-byte units of the address range).
-inline void score_plan(long long rows, int n, int* nch, int* tiles_per) {
+// Chunks of a row: about 1024 blocks in all, each of whole tiles, with at most
+// 4096 keys. The first tile may start up to 7 elements early (16-byte units of
+// the address range).
+inline void score_plan(long long rows, int n, int top, int* nch, int* tiles_per) {
   const int tiles = (int)(((long long)n + 7 + kScoreTile - 1) / kScoreTile);
-  long long c = (1024 + rows - 1) / rows;
+  long long c = (1024 + rows / 2) / rows;
+  if (c < 1) c = 1;
   if (c > tiles) c = tiles;
   if (c > kScoreMaxChunks) c = kScoreMaxChunks;
+  if (c * top > 4096) c = 4096 / top;
   *tiles_per = (int)((tiles + c - 1) / c);
   *nch = (tiles + *tiles_per - 1) / *tiles_per;
 }

@@ -12,21 +12,26 @@
 //
 // Best alternatives: a candidate is a 64-bit key, the logit as an ordered
 // integer over the complemented index, so that the largest key is the largest
-// logit with the lowest index among equals, and keys differ. A block collects
-// in LDS the elements above a threshold that is at most the n-th best so far;
-// the first tile's is the n-th largest of the 256 threads' maxima. In index
-// order few elements pass later ones (about top ln(n / tile) a row for logits
-// in random order); a tile that would overflow the buffer (ties, ascending
-// rows) is merged by repeated selection instead, whose cost is bounded.
+// logit with the lowest index among equals, and keys differ. Every wave keeps
+// its own list in LDS, without a barrier in the pass: the elements above a
+// threshold that is at most the block's n-th best so far; the first tile's is
+// the n-th largest of the lanes' maxima. In index order few elements pass
+// later ones (for logits in random order about n ln(tiles) in a block); a full
+// list is cut to its best n, so that every order of logits fits. The lists of a
+// block's waves, and then of a row's blocks, are joined by counting each key's
+// rank.
 #include "gg_device.h"
 
 namespace gg {
 
 namespace {
 
-constexpr int kScoreThreads = 256;
-constexpr int kScoreBuf = 512;       // candidates a block holds
-constexpr int kScoreCompact = 256;   // above this many they are cut to the best `top`
+constexpr int kScoreThreads = 256, kScoreWaves = kScoreThreads / 64;
+constexpr int kScoreBuf = 192;       // candidates a wave holds
+constexpr int kScoreCompact = 128;   // above this many they are cut to the best `top`
+constexpr int kScoreLane = 32;       // elements of a tile in a lane, at most
+constexpr int kScoreJoin = 4096;     // keys of a row's blocks
+static_assert(kScoreWaves * kScoreMaxTop <= kScoreThreads, "a key a thread");
 
 __device__ __forceinline__ uint32_t order_bits(float z) {
   const uint32_t b = __float_as_uint(z + 0.0f);   // -0 counts as 0
@@ -35,17 +40,10 @@ __device__ __forceinline__ uint32_t order_bits(float z) {
 __device__ __forceinline__ float order_value(uint32_t o) {
   return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xffffffffu));
 }
+// The next f32 below x (finite or +inf); below 0 it is the one below -0.
+__device__ __forceinline__ float before(float x) { return order_value(order_bits(x) - (x == 0.f ? 2u : 1u)); }
 __device__ __forceinline__ uint64_t score_key(float z, int i) {
   return ((uint64_t)order_bits(z) << 32) | (0xffffffffu - (uint32_t)i);
-}
-
-__device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const uint64_t w = __shfl_xor((unsigned long long)v, o, 64);
-    v = w > v ? w : v;
-  }
-  return v;
 }
 
 struct Stat {
@@ -71,86 +69,79 @@ __device__ __forceinline__ Stat stat_shfl(const Stat& a, int o) {
   return Stat{__shfl_xor(a.m, o, 64), __shfl_xor(a.s, o, 64), __shfl_xor(a.w, o, 64)};
 }
 
+static_assert(kScoreBuf - kScoreMaxTop >= 64 && kScoreCompact >= kScoreMaxTop, "a cut list takes what one lane holds");
+// The logit of a key, the same in every lane.
+__device__ __forceinline__ float list_value(uint64_t key) {
+  return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(order_value((uint32_t)(key >> 32)))));
+}
+
 struct ScoreShared {
-  uint64_t buf[kScoreBuf];
-  uint64_t list[kScoreMaxTop];
-  float mx[kScoreThreads];
-  uint64_t wbest[4];
-  Stat ws[4];
-  float thr;
-  int count, add;
+  uint64_t buf[kScoreWaves][kScoreBuf];
+  float mx[kScoreWaves][64];
+  float tile[kScoreWaves][kScoreLane];
+  float thr[kScoreWaves];   // the waves' thresholds
+  Stat ws[kScoreWaves];
 };
 
+__device__ __forceinline__ void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+
 // The block's merged statistic, in every thread.
-__device__ Stat block_stat(ScoreShared& sh, Stat a) {
+__device__ Stat block_stat(Stat* ws, Stat a) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) a = stat_merge(a, stat_shfl(a, o));
+  if ((threadIdx.x & 63) == 0) ws[threadIdx.x >> 6] = a;
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) sh.ws[threadIdx.x >> 6] = a;
-  __syncthreads();
-  return stat_merge(stat_merge(sh.ws[0], sh.ws[1]), stat_merge(sh.ws[2], sh.ws[3]));
+  return stat_merge(stat_merge(ws[0], ws[1]), stat_merge(ws[2], ws[3]));
 }
 
-// Largest key of the block below `last` given each thread's, in every thread.
-__device__ uint64_t block_best(ScoreShared& sh, uint64_t mine) {
-  mine = wave_max64(mine);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) sh.wbest[threadIdx.x >> 6] = mine;
-  __syncthreads();
-  const uint64_t a = sh.wbest[0] > sh.wbest[1] ? sh.wbest[0] : sh.wbest[1];
-  const uint64_t b = sh.wbest[2] > sh.wbest[3] ? sh.wbest[2] : sh.wbest[3];
-  return a > b ? a : b;
-}
-
-// The threshold that `top` of the threads' maxima reach (-inf when fewer than
-// `top` have one): at least `top` elements are as large.
-__device__ float thread_threshold(ScoreShared& sh, float mx, int top) {
-  const int tid = threadIdx.x;
-  sh.mx[tid] = mx;
-  __syncthreads();
+// The n-th largest of the lanes' maxima (-inf when fewer lanes have one): at
+// least n elements are as large.
+__device__ float lane_threshold(float* mxs, float mx, int n) {
+  const int lane = threadIdx.x & 63;
+  mxs[lane] = mx;
+  wave_fence();
   int rank = 0;
-  const float4* p = (const float4*)sh.mx;
-#pragma unroll 8
-  for (int j = 0; j < kScoreThreads / 4; ++j) {
+  const float4* p = (const float4*)mxs;
+#pragma unroll 4
+  for (int j = 0; j < 16; ++j) {
     const float4 o = p[j];
-    rank += (o.x > mx) | ((o.x == mx) & (4 * j < tid));
-    rank += (o.y > mx) | ((o.y == mx) & (4 * j + 1 < tid));
-    rank += (o.z > mx) | ((o.z == mx) & (4 * j + 2 < tid));
-    rank += (o.w > mx) | ((o.w == mx) & (4 * j + 3 < tid));
+    rank += (o.x > mx) | ((o.x == mx) & (4 * j < lane));
+    rank += (o.y > mx) | ((o.y == mx) & (4 * j + 1 < lane));
+    rank += (o.z > mx) | ((o.z == mx) & (4 * j + 2 < lane));
+    rank += (o.w > mx) | ((o.w == mx) & (4 * j + 3 < lane));
   }
-  if (rank == top - 1) sh.thr = mx;
-  __syncthreads();
-  return sh.thr;
+  const uint64_t at = __ballot(rank == n - 1);   // the ranks are a permutation
+  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mx), __builtin_ctzll(at)));
 }
 
-// buf[0, count) -> its best `top` keys in descending order at buf[0, ...);
-// returns how many. Every thread calls it; count <= kScoreBuf.
-__device__ int compact(ScoreShared& sh, int count, int top) {
-  const int tid = threadIdx.x;
-  __syncthreads();
-  uint64_t k[kScoreBuf / kScoreThreads];
-  int rank[kScoreBuf / kScoreThreads] = {};
+// buf[0, count) -> its best n keys in descending order; returns how many.
+// One wave; count <= kScoreBuf.
+__device__ int compact(uint64_t* buf, int count, int n) {
+  constexpr int PER = kScoreBuf / 64;
+  const int lane = threadIdx.x & 63;
+  wave_fence();
+  uint64_t k[PER];
+  int rank[PER] = {};
 #pragma unroll
-  for (int i = 0; i < kScoreBuf / kScoreThreads; ++i) k[i] = tid + kScoreThreads * i < count ? sh.buf[tid + kScoreThreads * i] : 0;
+  for (int i = 0; i < PER; ++i) k[i] = lane + 64 * i < count ? buf[lane + 64 * i] : 0;
+#pragma unroll 4
   for (int j = 0; j < count; ++j) {
-    const uint64_t o = sh.buf[j];
+    const uint64_t o = buf[j];
 #pragma unroll
-    for (int i = 0; i < kScoreBuf / kScoreThreads; ++i) rank[i] += o > k[i];
+    for (int i = 0; i < PER; ++i) rank[i] += o > k[i];
   }
-  __syncthreads();
+  wave_fence();
 #pragma unroll
-  for (int i = 0; i < kScoreBuf / kScoreThreads; ++i)
-    if (tid + kScoreThreads * i < count && rank[i] < top) sh.buf[rank[i]] = k[i];
-  const int left = count < top ? count : top;
-  if (tid == 0) sh.count = left;
-  __syncthreads();
-  return left;
+  for (int i = 0; i < PER; ++i)
+    if (lane + 64 * i < count && rank[i] < n) buf[rank[i]] = k[i];
+  wave_fence();
+  return __builtin_amdgcn_readfirstlane(min(count, n));
 }
 
 // What the host API reports of a row: the statistic, the given ids' log
-// probabilities, and the list buf[0, count).
+// probabilities, and the list best[0, top), 0 where there is none.
 template <class T>
-__device__ void write_row(const ScoreArgs& a, long long row, const Stat& st, const uint64_t* best, int count) {
+__device__ void write_row(const ScoreArgs& a, long long row, const Stat& st, const uint64_t* best) {
   const int tid = threadIdx.x;
   const T* z = (const T*)a.z + row * a.ld;
   const float log_s = logf(st.s);
@@ -167,20 +158,22 @@ __device__ void write_row(const ScoreArgs& a, long long row, const Stat& st, con
     a.lp[row * a.n_ids + j] = v;
   }
   for (int j = tid; j < a.top; j += kScoreThreads) {
-    const uint64_t k = j < count ? best[j] : 0;
+    const uint64_t k = best[j];
     if (a.top_ids) a.top_ids[row * a.top + j] = k ? (int)(0xffffffffu - (uint32_t)k) : -1;
     if (a.top_lp) a.top_lp[row * a.top + j] = k ? (order_value((uint32_t)(k >> 32)) - st.m) - log_s : -INFINITY;
   }
 }
 
-// One block: chunk blockIdx.x % nch of row blockIdx.x / nch. The row is taken
-// in 16-byte units of its address; the units at its ends, which may hold
-// elements of other rows, are read element by element.
+// One block: chunk blockIdx.x % nch of row blockIdx.x / nch; its waves take
+// turns at tiles of 64 EPT elements. The row is taken in 16-byte units of its
+// address; the units at its ends, which may hold elements of other rows, are
+// read element by element.
 template <class T, int EPT>
-__global__ __launch_bounds__(kScoreThreads) void k_score(ScoreArgs a) {
-  constexpr int VE = 16 / sizeof(T), NV = EPT / VE;
+__global__ __launch_bounds__(kScoreThreads, 4) void k_score(ScoreArgs a) {
+  static_assert(EPT <= kScoreLane, "a lane's part of a tile");
+  constexpr int VE = 16 / sizeof(T), NV = EPT / VE, STEP = NV * kScoreThreads;
   __shared__ ScoreShared sh;
-  const int tid = threadIdx.x, top = a.top, n = a.n;
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), top = a.top, n = a.n;
   const long long row = blockIdx.x / a.nch;
   const int ch = blockIdx.x - (int)(row * a.nch);
   const T* z = (const T*)a.z + row * a.ld;
@@ -188,116 +181,147 @@ __global__ __launch_bounds__(kScoreThreads) void k_score(ScoreArgs a) {
   const T* z0 = z - shift;
   const int units = (int)(((long long)n + shift + VE - 1) / VE);
   const int u_lo = ch * a.per, u_hi = min(units, u_lo + a.per);
-  if (tid == 0) {
-    sh.count = 0;
-    sh.add = 0;
-  }
+  uint64_t* buf = sh.buf[wv];
   typedef T vec_t __attribute__((ext_vector_type(VE)));
   vec_t nx[NV];
-  auto load = [&](int u0) {
+  auto load = [&](int u0) __attribute__((always_inline)) {
+    if (u0 * VE >= shift && u0 + 64 * NV <= u_hi && (long long)(u0 + 64 * NV) * VE - shift <= n) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int u = u0 + i * kScoreThreads + tid;
-      const long long e0 = (long long)u * VE - shift;
-      if (u < u_hi && e0 >= 0 && e0 + VE <= n) {
-        nx[i] = __builtin_nontemporal_load((const vec_t*)z0 + u);
-      } else {
+      for (int i = 0; i < NV; ++i) nx[i] = __builtin_nontemporal_load((const vec_t*)z0 + (u0 + i * 64 + lane));
+    } else {
 #pragma unroll
-        for (int e = 0; e < VE; ++e) nx[i][e] = u < u_hi && e0 + e >= 0 && e0 + e < n ? z[e0 + e] : (T)-INFINITY;
+      for (int i = 0; i < NV; ++i) {
+        const int u = u0 + i * 64 + lane;
+        const long long e0 = (long long)u * VE - shift;
+        if (u < u_hi && e0 >= 0 && e0 + VE <= n) {
+          nx[i] = __builtin_nontemporal_load((const vec_t*)z0 + u);
+        } else {
+#pragma unroll
+          for (int e = 0; e < VE; ++e) nx[i][e] = u < u_hi && e0 + e >= 0 && e0 + e < n ? z[e0 + e] : (T)-INFINITY;
+        }
       }
     }
   };
+  if (tid < kScoreWaves) sh.thr[tid] = -INFINITY;
+  __syncthreads();
   Stat st{-INFINITY, 0.f, 0.f};
   float thr = -INFINITY;
   int count = 0;
-  load(u_lo);
-  __syncthreads();
-  for (int u0 = u_lo; u0 < u_hi; u0 += NV * kScoreThreads) {
+  const int u_first = u_lo + wv * 64 * NV;
+  if (u_first < u_hi) load(u_first);
+  for (int u0 = u_first; u0 < u_hi; u0 += STEP) {
     float v[EPT];
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int e = 0; e < VE; ++e) v[i * VE + e] = (float)nx[i][e];
-    if (u0 + NV * kScoreThreads < u_hi) load(u0 + NV * kScoreThreads);
+    if (u0 + STEP < u_hi) load(u0 + STEP);
     float mx = v[0];
 #pragma unroll
     for (int i = 1; i < EPT; ++i) mx = fmaxf(mx, v[i]);
     mx = fmaxf(mx, -INFINITY);   // all NaN: no maximum
     const float m = fmaxf(st.m, mx);
-    stat_move(st, m);
+    if (__ballot(m > st.m)) stat_move(st, m);
     const float ref = m == -INFINITY ? 0.f : m;
-    float s = 0.f, w = 0.f;
+    float s[2] = {0.f, 0.f}, w[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < EPT; ++i) {
       const float d = v[i] - ref;
       const float p = __builtin_amdgcn_exp2f(d * 1.4426950408889634f);
-      s += p;
-      w = fmaf(p, fmaxf(d, -1e4f), w);   // e^-1e4 is 0: no 0 times -inf
+      s[i & 1] += p;
+      w[i & 1] = fmaf(p, fmaxf(d, -1e4f), w[i & 1]);   // e^-1e4 is 0: no 0 times -inf
     }
-    st.s += s;
-    st.w += w;
-    if (top > 0) {
-      const bool first = thr == -INFINITY;
-      float lim = thr;
-      if (first) lim = thread_threshold(sh, mx, top);
-      auto index = [&](int i) { return (u0 + (i / VE) * kScoreThreads + tid) * VE + i % VE - shift; };
-      auto passes = [&](float x) { return first ? (x >= lim) & (x > -INFINITY) : x > lim; };
-      int mine = 0;
-      if (first ? mx >= lim : mx > lim) {
+    st.s += s[0] + s[1];
+    st.w += w[0] + w[1];
+    if (top == 0) continue;
+    // Above `lim` an element may be one of the best: this wave's own n-th best
+    // came before the tile and wins a tie, another wave's may not.
+    float lim = thr;
 #pragma unroll
-        for (int i = 0; i < EPT; ++i) mine += passes(v[i]) ? 1 : 0;
-      }
-      int at = 0;
-      if (mine) at = atomicAdd(&sh.add, mine);
-      __syncthreads();
-      const int add = sh.add;
-      if (count + add <= kScoreBuf) {
-        if (mine) {
-          at += count;
-#pragma unroll
-          for (int i = 0; i < EPT; ++i)
-            if (passes(v[i])) sh.buf[at++] = score_key(v[i], index(i));
-        }
-        count += add;
-        if (add && (first || count > kScoreCompact)) {
-          count = compact(sh, count, top);
-          if (count == top) thr = order_value((uint32_t)(sh.buf[top - 1] >> 32));
-        }
-      } else {
-        // the best `top` of buffer and tile, one by one
-        uint64_t last = ~0ull;
-        int j = 0;
-        for (; j < top; ++j) {
-          uint64_t b = 0;
-          for (int q = tid; q < count; q += kScoreThreads) {
-            const uint64_t k = sh.buf[q];
-            b = k < last && k > b ? k : b;
-          }
-#pragma unroll
-          for (int i = 0; i < EPT; ++i) {
-            const uint64_t k = passes(v[i]) ? score_key(v[i], index(i)) : 0;
-            b = k < last && k > b ? k : b;
-          }
-          b = block_best(sh, b);
-          if (b == 0) break;
-          last = b;
-          if (tid == 0) sh.list[j] = b;
-        }
-        __syncthreads();
-        if (tid < j) sh.buf[tid] = sh.list[tid];
-        count = j;
-        __syncthreads();
-        if (count == top) thr = order_value((uint32_t)(sh.buf[top - 1] >> 32));
-      }
-      __syncthreads();
-      if (tid == 0) sh.add = 0;
-      __syncthreads();
+    for (int q = 0; q < kScoreWaves; ++q) {
+      const float t = __hip_atomic_load(&sh.thr[q], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+      lim = q == wv || t == -INFINITY ? lim : fmaxf(lim, before(t));
     }
+    const bool first = __builtin_amdgcn_readfirstlane(lim == -INFINITY);
+    if (first) {
+      const float t = lane_threshold(sh.mx[wv], mx, top);
+      lim = t == -INFINITY ? t : before(t);
+    }
+    uint64_t lanes = __ballot(mx > lim);
+    if (lanes == 0) continue;
+    if (__popcll(lanes) > 4) {
+      // many lanes, as in the first tile: each writes its elements to its place
+      int c = 0;
+#pragma unroll
+      for (int i = 0; i < EPT; ++i) c += v[i] > lim;
+      int at = count, sum = 0;
+#pragma unroll
+      for (int bit = 0; (EPT >> bit) > 0; ++bit) {   // prefix sums, a bit of the counts at a time
+        const uint64_t mask = __ballot((c >> bit) & 1);
+        at += __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u)) << bit;
+        sum += __popcll(mask) << bit;
+      }
+      if (count + sum <= kScoreBuf) {
+        const int e_lane = (u0 + lane) * VE - shift;
+#pragma unroll
+        for (int i = 0; i < EPT; ++i)
+          if (v[i] > lim) buf[at++] = score_key(v[i], e_lane + 64 * VE * (i / VE) + i % VE);
+        count += sum;
+        lanes = 0;
+      }
+    }
+    // one lane's elements at a time, an element a lane: any number of them fits
+    float* tile = sh.tile[wv];
+    while (lanes) {
+      const int L = __builtin_ctzll(lanes);
+      lanes &= lanes - 1;
+      if (lane == L) {
+#pragma unroll
+        for (int i = 0; i < EPT; ++i) tile[i] = v[i];
+      }
+      wave_fence();
+      const float x = lane < EPT ? tile[lane] : -INFINITY;
+      wave_fence();
+      uint64_t mask = __ballot(x > lim);
+      if (count + __popcll(mask) > kScoreBuf) {
+        count = compact(buf, count, top);   // to `top`: it was full
+        thr = list_value(buf[top - 1]);
+        lim = fmaxf(lim, before(thr));      // within the tile the order is not the indices'
+        mask = __ballot(x > lim);
+      }
+      if (x > lim)
+        buf[count + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u))] =
+            score_key(x, (u0 + 64 * (lane / VE) + L) * VE + lane % VE - shift);
+      count += __popcll(mask);
+    }
+    if (count > kScoreCompact || (first && count >= top)) {
+      count = compact(buf, count, top);
+      thr = list_value(buf[top - 1]);
+    }
+    if (lane == 0) __hip_atomic_store(&sh.thr[wv], thr, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
   }
-  st = block_stat(sh, st);
-  if (top > 0) count = compact(sh, count, top);
+  if (top > 0) {
+    count = compact(buf, count, top);
+    for (int j = count + lane; j < top; j += 64) buf[j] = 0;
+  }
+  st = block_stat(sh.ws, st);   // and the waves' lists are complete
+  // the waves' lists, a key a thread
+  uint64_t key = 0;
+  int rank = 0;
+  if (top > 0) {
+    const int lw = tid / top, lj = tid - lw * top;
+    if (lw < kScoreWaves) key = sh.buf[lw][lj];
+    for (int q = 0; q < kScoreWaves; ++q)
+      for (int j = 0; j < top; ++j) rank += sh.buf[q][j] > key;
+    __syncthreads();
+    uint64_t* best = sh.buf[0];
+    if (tid < top) best[tid] = 0;
+    __syncthreads();
+    if (key && rank < top) best[rank] = key;
+    __syncthreads();
+  }
   if (a.nch == 1) {
-    write_row<T>(a, row, st, sh.buf, count);
+    write_row<T>(a, row, st, sh.buf[0]);
     return;
   }
   if (tid == 0) {
@@ -306,13 +330,20 @@ __global__ __launch_bounds__(kScoreThreads) void k_score(ScoreArgs a) {
     p[1] = st.s;
     p[2] = st.w;
   }
-  for (int j = tid; j < top; j += kScoreThreads) a.keys[(size_t)blockIdx.x * top + j] = j < count ? sh.buf[j] : 0;
+  for (int j = tid; j < top; j += kScoreThreads) a.keys[(size_t)blockIdx.x * top + j] = sh.buf[0][j];
 }
 
-// One block per row: the chunks' statistics and lists.
+// One block per row: the chunks' statistics and lists. At most kScoreJoin keys,
+// 16 a thread; the ranks are counted of those whose logit is at least the
+// `top`-th largest of 64 groups' best (about 2 top of them without ties).
 template <class T>
 __global__ __launch_bounds__(kScoreThreads) void k_score_merge(ScoreArgs a) {
-  __shared__ ScoreShared sh;
+  constexpr int PER = kScoreJoin / kScoreThreads;
+  __shared__ Stat ws[kScoreWaves];
+  __shared__ __align__(16) float own[kScoreThreads];
+  __shared__ uint64_t cand[kScoreJoin], best[kScoreMaxTop];
+  __shared__ float limit;
+  __shared__ int count;
   const int tid = threadIdx.x, top = a.top, nch = a.nch;
   const long long row = blockIdx.x;
   Stat st{-INFINITY, 0.f, 0.f};
@@ -320,23 +351,40 @@ __global__ __launch_bounds__(kScoreThreads) void k_score_merge(ScoreArgs a) {
     const float* p = a.part + 4 * ((size_t)row * nch + tid);
     st = Stat{p[0], p[1], p[2]};
   }
-  st = block_stat(sh, st);
-  int j = 0;
+  const int total = nch * top;
+  uint64_t k[PER], b = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) k[i] = tid + kScoreThreads * i < total ? a.keys[(size_t)row * total + tid + kScoreThreads * i] : 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) b = k[i] > b ? k[i] : b;
+  own[tid] = b ? order_value((uint32_t)(b >> 32)) : -INFINITY;
+  if (tid < top) best[tid] = 0;
+  if (tid == 0) count = 0;
+  st = block_stat(ws, st);
   if (top > 0) {
-    // each list descends: a thread holds the front of its chunk's list, and
-    // the best front is taken `top` times
-    const uint64_t* list = a.keys + ((size_t)row * nch + (tid < nch ? tid : 0)) * top;
-    int at = 0;
-    uint64_t front = tid < nch ? list[0] : 0;
-    for (; j < top; ++j) {
-      const uint64_t b = block_best(sh, front);
-      if (b == 0) break;
-      if (front == b) front = ++at < top ? list[at] : 0;
-      if (tid == 0) sh.buf[j] = b;
+    if (tid < 64) {
+      const float g = fmaxf(fmaxf(own[tid], own[tid + 64]), fmaxf(own[tid + 128], own[tid + 192]));
+      wave_fence();
+      const float lim = lane_threshold(own, g, top);
+      if (tid == 0) limit = lim;
+    }
+    __syncthreads();
+    const float lim = limit;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (k[i] && order_value((uint32_t)(k[i] >> 32)) >= lim) cand[atomicAdd(&count, 1)] = k[i];
+    __syncthreads();
+    const int c = count;
+    for (int i = tid; i < c; i += kScoreThreads) {
+      const uint64_t key = cand[i];
+      int r = 0;
+#pragma unroll 4
+      for (int j = 0; j < c; ++j) r += cand[j] > key;
+      if (r < top) best[r] = key;
     }
     __syncthreads();
   }
-  write_row<T>(a, row, st, sh.buf, j);
+  write_row<T>(a, row, st, best);
 }
 
 template <class T, int EPT>
