@@ -14,35 +14,28 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x6 __attribute__((ext_vector_type(6)));
 constexpr int kFp6 = 2, kFp4 = 4;   // operand formats of the MX matrix instructions
 
-template <class T>
-__device__ __forceinline__ float load_elem(const void* p, int64_t i) { return (float)((const T*)p)[i]; }
-
-// Elements [c, c + 4) of a row of k elements, zeros past its end.
-template <class T, bool VEC>
-__device__ __forceinline__ void load4(const T* row, int64_t c, int64_t k, float (&v)[4]) {
-  typedef T vec_t __attribute__((ext_vector_type(4)));
-  if (VEC && c + 4 <= k) {
+// Elements [c, c + E) of a row of k elements, zeros past its end.
+template <class T, int E, bool VEC>
+__device__ __forceinline__ void load_row(const T* row, int64_t c, int64_t k, float (&v)[E]) {
+  typedef T vec_t __attribute__((ext_vector_type(E)));
+  if (VEC && c + E <= k) {
     const vec_t t = *(const vec_t*)(row + c);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = (float)t[i];
+    for (int i = 0; i < E; ++i) v[i] = (float)t[i];
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = c + i < k ? (float)row[c + i] : 0.f;
+    for (int i = 0; i < E; ++i) v[i] = c + i < k ? (float)row[c + i] : 0.f;
   }
 }
-
-__device__ __forceinline__ float group8_max(float x) {
-  x = fmaxf(x, dpp_mov<0xB1>(x));
-  x = fmaxf(x, dpp_mov<0x4E>(x));
-  x = fmaxf(x, dpp_mov<0x141>(x));
-  return x;
-}
+template <class T, bool VEC>
+__device__ __forceinline__ void load4(const T* row, int64_t c, int64_t k, float (&v)[4]) { load_row<T, 4, VEC>(row, c, k, v); }
 
 // ---------------------------------------------------------------------------
-// Quantisation. A block takes 32 rows x 256 k (one group of scale dwords):
-// a wave reads 256 consecutive elements of a row at a time, eight lanes to a
-// 32-block; the codes go through LDS into operand order, so that both the
-// reads and the 1 KB tiles written are whole lines.
+// Quantisation. A block takes 32 rows x 256 k (one group of scale dwords): a
+// wave reads 16 bytes a lane, 256 consecutive elements of one f32 row or of two
+// 16-bit ones at a time, 8 or 4 lanes to a 32-block; the codes go through LDS
+// into operand order, so that both the reads and the 1 KB tiles written are
+// whole lines.
 // Scale byte: the exponent field of the block's largest magnitude less 2
 // (floor(log2) - 2), at least 0; conversion to nearest, ties to even, values
 // above 6 to 6. Bound by memory: reads the input once, writes 17/32 byte an
@@ -51,43 +44,46 @@ __device__ __forceinline__ float group8_max(float x) {
 template <class T, bool VEC>
 __global__ __launch_bounds__(256) void k_mx4_quantize(const T* __restrict__ src, int64_t rows, int64_t k, int64_t ld,
                                                       uint8_t* __restrict__ dst, Mx4Layout L) {
-  __shared__ __align__(16) uint16_t codes[256][8];   // [4 tiles x 64 lanes][16 bytes]
+  constexpr int E = 16 / sizeof(T), LB = 32 / E, RW = E / 4;   // elements a lane, lanes a block, rows a wave at a time
+  __shared__ __align__(16) uint8_t codes[256][16];   // [4 tiles x 64 lanes][16 bytes]
   __shared__ __align__(4) uint8_t scales[256];       // [64 lanes][4 tiles]
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   const int64_t R = blockIdx.x;
   const int g = blockIdx.y;
-  const int64_t c = (int64_t)g * 256 + 4 * lane;
-  const int kb = lane >> 3, t = kb >> 1, b = kb & 1;   // 32-block, its tile and half
-  float v[8][4];
+  const int ln = lane % (64 / RW);
+  const int64_t c = (int64_t)g * 256 + E * ln;
+  const int kb = ln / LB, t = kb >> 1, b = kb & 1;   // 32-block, its tile and half
+  float v[8 / RW][E];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int64_t r = R * 32 + wv * 8 + i;
-    if (r < rows) {
-      load4<T, VEC>(src + r * ld, c, k, v[i]);
-    } else {
-      v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0.f;
-    }
+  for (int i = 0; i < 8 / RW; ++i) {
+    const int64_t r = R * 32 + wv * 8 + i * RW + lane / (64 / RW);
+    load_row<T, E, VEC>(src + min(r, rows - 1) * ld, c, r < rows ? k : 0, v[i]);
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int row = wv * 8 + i;
+  for (int i = 0; i < 8 / RW; ++i) {
+    const int row = wv * 8 + i * RW + lane / (64 / RW);
     // the magnitudes' bits order as the magnitudes do, Inf and NaN on top
     uint32_t a = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) a = max(a, __float_as_uint(v[i][j]) & 0x7fffffffu);
+    for (int j = 0; j < E; ++j) a = max(a, __float_as_uint(v[i][j]) & 0x7fffffffu);
     a = max(a, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)a, 0xB1, 0xf, 0xf, false));
     a = max(a, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)a, 0x4E, 0xf, 0xf, false));
-    a = max(a, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)a, 0x141, 0xf, 0xf, false));
+    if (LB == 8) a = max(a, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)a, 0x141, 0xf, 0xf, false));
     const int ex = (int)(a >> 23);
     const int byte = ex == 255 ? 255 : max(ex - 2, 0);
     const float scale = __uint_as_float(byte ? (uint32_t)byte << 23 : 0x00400000u);   // byte 0: 2^-127
     uint32_t q = 0;
     q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[i][0], v[i][1], scale, 0);
     q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[i][2], v[i][3], scale, 1);
+    if constexpr (E == 8) {
+      q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[i][4], v[i][5], scale, 2);
+      q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[i][6], v[i][7], scale, 3);
+    }
     if (byte == 255) q = 0;   // Inf or NaN in the block: its scale says NaN
     const int l = 32 * b + row;
-    codes[t * 64 + l][lane & 7] = (uint16_t)q;
-    if ((lane & 7) == 0) scales[4 * l + t] = (uint8_t)byte;
+    if constexpr (E == 8) *(uint32_t*)&codes[t * 64 + l][4 * (ln % LB)] = q;
+    else *(uint16_t*)&codes[t * 64 + l][2 * (ln % LB)] = (uint16_t)q;
+    if (ln % LB == 0) scales[4 * l + t] = (uint8_t)byte;
   }
   __syncthreads();
   if (g * 4 + wv < L.kt)
@@ -678,16 +674,17 @@ __global__ __launch_bounds__(256) void k_mx4_join(Mx4LinearArgs a) {
     if (f + e < a.n) store_elem(a.y_elem, a.y, row * a.ldy + f + e, v[e]);
 }
 
+// Rows can be read n elements at once.
 template <class T>
-bool aligned4(const void* p, int64_t ld) {
-  return ((uintptr_t)p % (4 * sizeof(T))) == 0 && (ld * sizeof(T)) % (4 * sizeof(T)) == 0;
+bool rows_aligned(const void* p, int64_t ld, int n) {
+  return ((uintptr_t)p % (n * sizeof(T))) == 0 && ld % n == 0;
 }
 
 template <class T>
 int quantize_t(const void* src, int64_t rows, int64_t k, int64_t ld, uint8_t* dst, hipStream_t s) {
   const Mx4Layout L = mx4_layout(rows, k);
   const dim3 grid((unsigned)L.rt, (unsigned)L.ks);
-  if (aligned4<T>(src, ld))
+  if (rows_aligned<T>(src, ld, 16 / (int)sizeof(T)))
     hipLaunchKernelGGL((k_mx4_quantize<T, true>), grid, dim3(256), 0, s, (const T*)src, rows, k, ld, dst, L);
   else
     hipLaunchKernelGGL((k_mx4_quantize<T, false>), grid, dim3(256), 0, s, (const T*)src, rows, k, ld, dst, L);
@@ -698,7 +695,7 @@ template <class T>
 int split_t(const void* src, int64_t rows, int64_t k, int64_t ld, int parts, uint8_t* dst, hipStream_t s) {
   const Mx4Layout L = mx4_layout(rows, k);
   const dim3 grid((unsigned)L.rt, (unsigned)L.kt);
-  if (aligned4<T>(src, ld))
+  if (rows_aligned<T>(src, ld, 4))
     hipLaunchKernelGGL((k_mx_split<T, true>), grid, dim3(64), 0, s, (const T*)src, rows, k, ld, parts, dst, L);
   else
     hipLaunchKernelGGL((k_mx_split<T, false>), grid, dim3(64), 0, s, (const T*)src, rows, k, ld, parts, dst, L);
@@ -721,7 +718,7 @@ int launch_mx4_dequant(const uint8_t* src, float* out, int64_t rows, int64_t k, 
   const Mx4Layout L = mx4_layout(rows, k);
   const dim3 grid((unsigned)L.rt, (unsigned)L.ks);
   hipStream_t s = (hipStream_t)stream;
-  if (aligned4<float>(out, ld))
+  if (rows_aligned<float>(out, ld, 4))
     hipLaunchKernelGGL((k_mx4_dequant<true>), grid, dim3(256), 0, s, src, out, rows, k, ld, L);
   else
     hipLaunchKernelGGL((k_mx4_dequant<false>), grid, dim3(256), 0, s, src, out, rows, k, ld, L);

@@ -1867,8 +1867,7 @@ int gg_mxfp4_linear(const void* w, const void* x, uint32_t x_type, int64_t ldx, 
 
 size_t gg_score_workspace_size(int64_t rows, int32_t n, int32_t top_n) {
   if (rows <= 0 || rows > (1LL << 30) || n <= 0 || n > (1 << 30) || top_n < 0 || top_n > kScoreMaxTop) return 0;
-  int nch, per;
-  score_plan(rows, n, top_n, &nch, &per);
+  const int nch = score_plan(rows, n, top_n).nch;
   return nch == 1 ? 0 : (size_t)rows * nch * (16 + 8 * (size_t)top_n);
 }
 
@@ -1887,9 +1886,10 @@ int gg_score_logits(const void* logits, uint32_t type, int64_t rows, int32_t n, 
   a.ld = ld;
   a.rows = rows;
   a.n = n;
-  int tiles;
-  score_plan(rows, n, top_n, &a.nch, &tiles);
-  a.per = tiles * (int)(kScoreTile * elem_size(e) / 16);
+  const ScorePlan plan = score_plan(rows, n, top_n);
+  a.tile = plan.tile;
+  a.nch = plan.nch;
+  a.per = plan.tiles_per * (int)(plan.tile * elem_size(e) / 16);
   a.ids = ids;
   a.n_ids = n_ids;
   a.lp = id_logprobs;

@@ -13,13 +13,13 @@
 // Best alternatives: a candidate is a 64-bit key, the logit as an ordered
 // integer over the complemented index, so that the largest key is the largest
 // logit with the lowest index among equals, and keys differ. Every wave keeps
-// its own list in LDS, without a barrier in the pass: the elements above a
-// threshold that is at most the block's n-th best so far; the first tile's is
-// the n-th largest of the lanes' maxima. In index order few elements pass
-// later ones (for logits in random order about n ln(tiles) in a block); a full
-// list is cut to its best n, so that every order of logits fits. The lists of a
-// block's waves, and then of a row's blocks, are joined by counting each key's
-// rank.
+// its own list in LDS: the elements above a bound that is below the block's
+// n-th best so far; the first tiles' is near the n-th largest of a wave's lane
+// maxima, the waves' best one. In index order few elements pass later ones (for
+// logits in random order about n ln(tiles) in a block), which need no barrier;
+// a list that grows is cut to its best n, so that every order of logits fits.
+// The lists of a block's waves, and then of a row's blocks, are joined by
+// counting each key's rank.
 #include "gg_device.h"
 
 namespace gg {
@@ -28,9 +28,9 @@ namespace {
 
 constexpr int kScoreThreads = 256, kScoreWaves = kScoreThreads / 64;
 constexpr int kScoreBuf = 192;       // candidates a wave holds
-constexpr int kScoreCompact = 128;   // above this many they are cut to the best `top`
+constexpr int kScoreMore = 16;       // this many above `top` are cut to `top`
 constexpr int kScoreLane = 32;       // elements of a tile in a lane, at most
-constexpr int kScoreJoin = 4096;     // keys of a row's blocks
+constexpr int kMergePer = 4;         // keys of a row's blocks in a thread that joins them
 static_assert(kScoreWaves * kScoreMaxTop <= kScoreThreads, "a key a thread");
 
 __device__ __forceinline__ uint32_t order_bits(float z) {
@@ -65,53 +65,50 @@ __device__ __forceinline__ Stat stat_merge(Stat a, Stat b) {
   stat_move(b, m);
   return Stat{m, a.s + b.s, a.w + b.w};
 }
-__device__ __forceinline__ Stat stat_shfl(const Stat& a, int o) {
-  return Stat{__shfl_xor(a.m, o, 64), __shfl_xor(a.s, o, 64), __shfl_xor(a.w, o, 64)};
-}
-
-static_assert(kScoreBuf - kScoreMaxTop >= 64 && kScoreCompact >= kScoreMaxTop, "a cut list takes what one lane holds");
+static_assert(kScoreBuf - kScoreMaxTop >= kScoreLane, "a cut list takes what one lane holds");
 // The logit of a key, the same in every lane.
 __device__ __forceinline__ float list_value(uint64_t key) {
   return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(order_value((uint32_t)(key >> 32)))));
 }
 
 struct ScoreShared {
-  uint64_t buf[kScoreWaves][kScoreBuf];
-  float mx[kScoreWaves][64];
+  uint64_t buf[kScoreWaves][kScoreBuf], best[kScoreMaxTop];
   float tile[kScoreWaves][kScoreLane];
-  float thr[kScoreWaves];   // the waves' thresholds
+  float thr[kScoreWaves];   // bounds: the waves' first ones, then their lists' n-th best
+  int counts[kScoreWaves];
   Stat ws[kScoreWaves];
 };
 
 __device__ __forceinline__ void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
 
-// The block's merged statistic, in every thread.
-__device__ Stat block_stat(Stat* ws, Stat a) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) a = stat_merge(a, stat_shfl(a, o));
-  if ((threadIdx.x & 63) == 0) ws[threadIdx.x >> 6] = a;
+// The block's merged statistic, in every thread: all lanes move to the wave's
+// maximum, then the sums are added.
+__device__ Stat block_stat(Stat* ws, Stat a) {   // of the first kScoreWaves waves
+  float m = a.m;
+  m = fmaxf(m, dpp_mov<0xB1>(m));
+  m = fmaxf(m, dpp_mov<0x4E>(m));
+  m = fmaxf(m, dpp_mov<0x141>(m));
+  m = across8_max(m);
+  stat_move(a, m);
+  a.s = wave_sum_dpp(a.s);
+  a.w = wave_sum_dpp(a.w);
+  if ((threadIdx.x & 63) == 0 && threadIdx.x < kScoreThreads) ws[threadIdx.x >> 6] = a;
   __syncthreads();
   return stat_merge(stat_merge(ws[0], ws[1]), stat_merge(ws[2], ws[3]));
 }
 
-// The n-th largest of the lanes' maxima (-inf when fewer lanes have one): at
-// least n elements are as large.
-__device__ float lane_threshold(float* mxs, float mx, int n) {
+// A bound that at least n lanes' maxima reach, next to the n-th largest of them
+// (-inf when fewer lanes have one). The last six bits give way to the lane, so
+// that the order is strict, and count as zero in the bound.
+__device__ float lane_threshold(float mx, int n) {
   const int lane = threadIdx.x & 63;
-  mxs[lane] = mx;
-  wave_fence();
+  const uint32_t u = (order_bits(mx) & ~63u) | (uint32_t)(63 - lane);
   int rank = 0;
-  const float4* p = (const float4*)mxs;
-#pragma unroll 4
-  for (int j = 0; j < 16; ++j) {
-    const float4 o = p[j];
-    rank += (o.x > mx) | ((o.x == mx) & (4 * j < lane));
-    rank += (o.y > mx) | ((o.y == mx) & (4 * j + 1 < lane));
-    rank += (o.z > mx) | ((o.z == mx) & (4 * j + 2 < lane));
-    rank += (o.w > mx) | ((o.w == mx) & (4 * j + 3 < lane));
-  }
-  const uint64_t at = __ballot(rank == n - 1);   // the ranks are a permutation
-  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mx), __builtin_ctzll(at)));
+#pragma unroll
+  for (int j = 0; j < 64; ++j) rank += (uint32_t)__builtin_amdgcn_readlane((int)u, j) > u;
+  const uint64_t at = __ballot(rank == n - 1);
+  const uint32_t o = (uint32_t)__builtin_amdgcn_readlane((int)u, __builtin_ctzll(at)) & ~63u;
+  return o > order_bits(-INFINITY) ? order_value(o) : -INFINITY;
 }
 
 // buf[0, count) -> its best n keys in descending order; returns how many.
@@ -120,6 +117,20 @@ __device__ int compact(uint64_t* buf, int count, int n) {
   constexpr int PER = kScoreBuf / 64;
   const int lane = threadIdx.x & 63;
   wave_fence();
+  if (count <= 64) {   // a key a lane: no LDS in the loop
+    const uint64_t key = lane < count ? buf[lane] : 0;
+    int r = 0;
+#pragma unroll 4
+    for (int j = 0; j < count; ++j) {
+      const uint64_t o = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(key >> 32), j) << 32) |
+                         (uint32_t)__builtin_amdgcn_readlane((int)key, j);
+      r += o > key;
+    }
+    wave_fence();
+    if (lane < count && r < n) buf[r] = key;
+    wave_fence();
+    return min(count, n);
+  }
   uint64_t k[PER];
   int rank[PER] = {};
 #pragma unroll
@@ -138,26 +149,53 @@ __device__ int compact(uint64_t* buf, int count, int n) {
   return __builtin_amdgcn_readfirstlane(min(count, n));
 }
 
-// What the host API reports of a row: the statistic, the given ids' log
-// probabilities, and the list best[0, top), 0 where there is none.
+// How many of keys[0, n) are above key; eight reads at a time (the last ones of
+// n again past its end, not counted).
+__device__ __forceinline__ int keys_above(const uint64_t* keys, int n, uint64_t key) {
+  int r = 0;
+  for (int j = 0; j < n; j += 8) {
+    uint64_t o[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = keys[min(j + i, n - 1)];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r += (j + i < n) & (o[i] > key);
+  }
+  return r;
+}
+
+// The thread's first given id and its logit, asked for before the pass: two
+// loads that depend on each other.
+struct Given {
+  int id;
+  float z;
+};
 template <class T>
-__device__ void write_row(const ScoreArgs& a, long long row, const Stat& st, const uint64_t* best) {
+__device__ __forceinline__ Given given(const ScoreArgs& a, long long row, int j) {
+  Given g{-1, 0.f};
+  if (j < a.n_ids) g.id = a.ids[row * a.n_ids + j];
+  if (g.id >= 0 && g.id < a.n) g.z = (float)((const T*)a.z)[row * a.ld + g.id];
+  return g;
+}
+
+// What is reported of a row: the statistic, the given ids' log probabilities,
+// and the list best[0, top), 0 where there is none.
+template <class T, int THREADS>
+__device__ void write_row(const ScoreArgs& a, long long row, const Stat& st, const uint64_t* best, Given g) {
   const int tid = threadIdx.x;
-  const T* z = (const T*)a.z + row * a.ld;
   const float log_s = logf(st.s);
   const bool none = st.s == 0.f;   // every logit is -inf: nothing has a probability
   if (tid == 0) {
     if (a.lse) a.lse[row] = none ? -INFINITY : st.m + log_s;
     if (a.entropy) a.entropy[row] = none ? 0.f : log_s - st.w / st.s;
   }
-  for (int j = tid; j < a.n_ids; j += kScoreThreads) {
-    const int id = a.ids[row * a.n_ids + j];
+  for (int j = tid; j < a.n_ids; j += THREADS) {
+    if (j != tid) g = given<T>(a, row, j);
     float v = 0.f;   // -1: no token here
-    if (id >= 0 && id < a.n) v = none ? -INFINITY : ((float)z[id] - st.m) - log_s;
-    else if (id != -1) v = NAN;
+    if (g.id >= 0 && g.id < a.n) v = none ? -INFINITY : (g.z - st.m) - log_s;
+    else if (g.id != -1) v = NAN;
     a.lp[row * a.n_ids + j] = v;
   }
-  for (int j = tid; j < a.top; j += kScoreThreads) {
+  for (int j = tid; j < a.top; j += THREADS) {
     const uint64_t k = best[j];
     if (a.top_ids) a.top_ids[row * a.top + j] = k ? (int)(0xffffffffu - (uint32_t)k) : -1;
     if (a.top_lp) a.top_lp[row * a.top + j] = k ? (order_value((uint32_t)(k >> 32)) - st.m) - log_s : -INFINITY;
@@ -182,6 +220,8 @@ __global__ __launch_bounds__(kScoreThreads, 4) void k_score(ScoreArgs a) {
   const int units = (int)(((long long)n + shift + VE - 1) / VE);
   const int u_lo = ch * a.per, u_hi = min(units, u_lo + a.per);
   uint64_t* buf = sh.buf[wv];
+  Given g{-1, 0.f};
+  if (a.nch == 1) g = given<T>(a, row, tid);
   typedef T vec_t __attribute__((ext_vector_type(VE)));
   vec_t nx[NV];
   auto load = [&](int u0) __attribute__((always_inline)) {
@@ -202,14 +242,13 @@ __global__ __launch_bounds__(kScoreThreads, 4) void k_score(ScoreArgs a) {
       }
     }
   };
-  if (tid < kScoreWaves) sh.thr[tid] = -INFINITY;
-  __syncthreads();
   Stat st{-INFINITY, 0.f, 0.f};
-  float thr = -INFINITY;
+  float lim = -INFINITY;   // elements above it may be among the best
   int count = 0;
   const int u_first = u_lo + wv * 64 * NV;
-  if (u_first < u_hi) load(u_first);
-  for (int u0 = u_first; u0 < u_hi; u0 += STEP) {
+  load(u_first);   // past the chunk's end: -inf
+  // every wave takes part in the first round, with or without a tile
+  for (int u0 = u_first; u0 < u_hi || u0 == u_first; u0 += STEP) {
     float v[EPT];
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -234,18 +273,16 @@ __global__ __launch_bounds__(kScoreThreads, 4) void k_score(ScoreArgs a) {
     st.s += s[0] + s[1];
     st.w += w[0] + w[1];
     if (top == 0) continue;
-    // Above `lim` an element may be one of the best: this wave's own n-th best
-    // came before the tile and wins a tie, another wave's may not.
-    float lim = thr;
+    if (u0 == u_first) {
+      const float t = lane_threshold(mx, top);
+      if (lane == 0) sh.thr[wv] = t;
+      __syncthreads();
+    }
+    // another wave's bound may be a logit behind this tile that loses a tie
 #pragma unroll
     for (int q = 0; q < kScoreWaves; ++q) {
       const float t = __hip_atomic_load(&sh.thr[q], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-      lim = q == wv || t == -INFINITY ? lim : fmaxf(lim, before(t));
-    }
-    const bool first = __builtin_amdgcn_readfirstlane(lim == -INFINITY);
-    if (first) {
-      const float t = lane_threshold(sh.mx[wv], mx, top);
-      lim = t == -INFINITY ? t : before(t);
+      lim = fmaxf(lim, t == -INFINITY ? t : before(t));
     }
     uint64_t lanes = __ballot(mx > lim);
     if (lanes == 0) continue;
@@ -284,9 +321,8 @@ __global__ __launch_bounds__(kScoreThreads, 4) void k_score(ScoreArgs a) {
       wave_fence();
       uint64_t mask = __ballot(x > lim);
       if (count + __popcll(mask) > kScoreBuf) {
-        count = compact(buf, count, top);   // to `top`: it was full
-        thr = list_value(buf[top - 1]);
-        lim = fmaxf(lim, before(thr));      // within the tile the order is not the indices'
+        count = compact(buf, count, top);                        // to `top`: it was full
+        lim = fmaxf(lim, before(list_value(buf[top - 1])));      // within the tile the order is not the indices'
         mask = __ballot(x > lim);
       }
       if (x > lim)
@@ -294,34 +330,38 @@ __global__ __launch_bounds__(kScoreThreads, 4) void k_score(ScoreArgs a) {
             score_key(x, (u0 + 64 * (lane / VE) + L) * VE + lane % VE - shift);
       count += __popcll(mask);
     }
-    if (count > kScoreCompact || (first && count >= top)) {
+    if (count >= top + kScoreMore) {
       count = compact(buf, count, top);
-      thr = list_value(buf[top - 1]);
+      const float t = list_value(buf[top - 1]);
+      lim = fmaxf(lim, t);   // all of the list comes before the next tile: it wins ties
+      if (lane == 0) __hip_atomic_store(&sh.thr[wv], t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
     }
-    if (lane == 0) __hip_atomic_store(&sh.thr[wv], thr, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
   }
   if (top > 0) {
-    count = compact(buf, count, top);
-    for (int j = count + lane; j < top; j += 64) buf[j] = 0;
+    if (count > kScoreThreads / kScoreWaves) count = compact(buf, count, top);
+    if (lane == 0) sh.counts[wv] = count;
   }
   st = block_stat(sh.ws, st);   // and the waves' lists are complete
-  // the waves' lists, a key a thread
-  uint64_t key = 0;
-  int rank = 0;
   if (top > 0) {
-    const int lw = tid / top, lj = tid - lw * top;
-    if (lw < kScoreWaves) key = sh.buf[lw][lj];
-    for (int q = 0; q < kScoreWaves; ++q)
-      for (int j = 0; j < top; ++j) rank += sh.buf[q][j] > key;
+    // a key a thread
+    uint64_t key = 0;
+    int rank = 0, at = tid;
+#pragma unroll
+    for (int q = 0; q < kScoreWaves; ++q) {
+      const int c = sh.counts[q];
+      if (at >= 0 && at < c) key = sh.buf[q][at];
+      at -= c;
+    }
+    if (key) {
+      for (int q = 0; q < kScoreWaves; ++q) rank += keys_above(sh.buf[q], sh.counts[q], key);
+    }
+    if (tid < top) sh.best[tid] = 0;
     __syncthreads();
-    uint64_t* best = sh.buf[0];
-    if (tid < top) best[tid] = 0;
-    __syncthreads();
-    if (key && rank < top) best[rank] = key;
+    if (key && rank < top) sh.best[rank] = key;
     __syncthreads();
   }
   if (a.nch == 1) {
-    write_row<T>(a, row, st, sh.buf[0]);
+    write_row<T, kScoreThreads>(a, row, st, sh.best, g);
     return;
   }
   if (tid == 0) {
@@ -330,61 +370,67 @@ __global__ __launch_bounds__(kScoreThreads, 4) void k_score(ScoreArgs a) {
     p[1] = st.s;
     p[2] = st.w;
   }
-  for (int j = tid; j < top; j += kScoreThreads) a.keys[(size_t)blockIdx.x * top + j] = sh.buf[0][j];
+  for (int j = tid; j < top; j += kScoreThreads) a.keys[(size_t)blockIdx.x * top + j] = sh.best[j];
 }
 
-// One block per row: the chunks' statistics and lists. At most kScoreJoin keys,
-// 16 a thread; the ranks are counted of those whose logit is at least the
-// `top`-th largest of 64 groups' best (about 2 top of them without ties).
-template <class T>
-__global__ __launch_bounds__(kScoreThreads) void k_score_merge(ScoreArgs a) {
-  constexpr int PER = kScoreJoin / kScoreThreads;
+// One block per row: the chunks' statistics and lists. At most 4096 keys, four
+// a thread; the ranks are counted of those whose logit reaches a bound
+// that `top` of 64 groups' best do (about 2 top of them without ties).
+template <class T, int THREADS>
+__global__ __launch_bounds__(THREADS) void k_score_merge(ScoreArgs a) {
+  constexpr int PER = kMergePer;
   __shared__ Stat ws[kScoreWaves];
-  __shared__ __align__(16) float own[kScoreThreads];
-  __shared__ uint64_t cand[kScoreJoin], best[kScoreMaxTop];
-  __shared__ float limit;
+  __shared__ __align__(16) float own[THREADS];
+  __shared__ uint64_t cand[THREADS * PER], best[kScoreMaxTop];
   __shared__ int count;
-  const int tid = threadIdx.x, top = a.top, nch = a.nch;
+  const int tid = threadIdx.x, lane = tid & 63, top = a.top, nch = a.nch;
   const long long row = blockIdx.x;
+  const int total = nch * top;
+  uint64_t k[PER], b = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) k[i] = tid + THREADS * i < total ? a.keys[(size_t)row * total + tid + THREADS * i] : 0;
   Stat st{-INFINITY, 0.f, 0.f};
   if (tid < nch) {
     const float* p = a.part + 4 * ((size_t)row * nch + tid);
     st = Stat{p[0], p[1], p[2]};
   }
-  const int total = nch * top;
-  uint64_t k[PER], b = 0;
-#pragma unroll
-  for (int i = 0; i < PER; ++i) k[i] = tid + kScoreThreads * i < total ? a.keys[(size_t)row * total + tid + kScoreThreads * i] : 0;
+  const Given g = given<T>(a, row, tid);
 #pragma unroll
   for (int i = 0; i < PER; ++i) b = k[i] > b ? k[i] : b;
   own[tid] = b ? order_value((uint32_t)(b >> 32)) : -INFINITY;
   if (tid < top) best[tid] = 0;
   if (tid == 0) count = 0;
+  static_assert(kScoreMaxChunks <= kScoreThreads, "the first waves hold the statistics");
   st = block_stat(ws, st);
   if (top > 0) {
-    if (tid < 64) {
-      const float g = fmaxf(fmaxf(own[tid], own[tid + 64]), fmaxf(own[tid + 128], own[tid + 192]));
-      wave_fence();
-      const float lim = lane_threshold(own, g, top);
-      if (tid == 0) limit = lim;
+    // every wave finds the bound for itself
+    float mx = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < THREADS / 256; ++i) {
+      const float4 o = *(const float4*)&own[256 * i + 4 * lane];
+      mx = fmaxf(fmaxf(fmaxf(o.x, o.y), fmaxf(o.z, o.w)), mx);
+    }
+    const float lim = lane_threshold(mx, top);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const bool take = k[i] != 0 && order_value((uint32_t)(k[i] >> 32)) >= lim;
+      const uint64_t mask = __ballot(take);
+      if (!mask) continue;
+      int at = 0;
+      if (lane == 0) at = atomicAdd(&count, (int)__popcll(mask));
+      at = __builtin_amdgcn_readfirstlane(at);
+      if (take) cand[at + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u))] = k[i];
     }
     __syncthreads();
-    const float lim = limit;
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (k[i] && order_value((uint32_t)(k[i] >> 32)) >= lim) cand[atomicAdd(&count, 1)] = k[i];
-    __syncthreads();
     const int c = count;
-    for (int i = tid; i < c; i += kScoreThreads) {
+    for (int i = tid; i < c; i += THREADS) {
       const uint64_t key = cand[i];
-      int r = 0;
-#pragma unroll 4
-      for (int j = 0; j < c; ++j) r += cand[j] > key;
+      const int r = keys_above(cand, c, key);
       if (r < top) best[r] = key;
     }
     __syncthreads();
   }
-  write_row<T>(a, row, st, best);
+  write_row<T, THREADS>(a, row, st, best, g);
 }
 
 template <class T, int EPT>
@@ -392,7 +438,10 @@ int launch_score_t(ScoreArgs a, hipStream_t s) {
   hipLaunchKernelGGL((k_score<T, EPT>), dim3((unsigned)(a.rows * a.nch)), dim3(kScoreThreads), 0, s, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.nch == 1) return (int)e;
-  hipLaunchKernelGGL((k_score_merge<T>), dim3((unsigned)a.rows), dim3(kScoreThreads), 0, s, a);
+  if (a.nch * a.top <= kScoreThreads * kMergePer)
+    hipLaunchKernelGGL((k_score_merge<T, kScoreThreads>), dim3((unsigned)a.rows), dim3(kScoreThreads), 0, s, a);
+  else
+    hipLaunchKernelGGL((k_score_merge<T, 1024>), dim3((unsigned)a.rows), dim3(1024), 0, s, a);
   return (int)hipGetLastError();
 }
 
@@ -400,10 +449,11 @@ int launch_score_t(ScoreArgs a, hipStream_t s) {
 
 int launch_score(int elem, const ScoreArgs& a, void* stream) {
   hipStream_t s = (hipStream_t)stream;
+  const bool few = a.tile < kScoreTile;
   switch (elem) {
-    case ELEM_F32: return launch_score_t<float, 32>(a, s);
-    case ELEM_F16: return launch_score_t<_Float16, 32>(a, s);
-    case ELEM_BF16: return launch_score_t<__bf16, 32>(a, s);
+    case ELEM_F32: return few ? launch_score_t<float, 8>(a, s) : launch_score_t<float, 32>(a, s);
+    case ELEM_F16: return few ? launch_score_t<_Float16, 8>(a, s) : launch_score_t<_Float16, 32>(a, s);
+    case ELEM_BF16: return few ? launch_score_t<__bf16, 8>(a, s) : launch_score_t<__bf16, 32>(a, s);
   }
   return (int)hipErrorInvalidValue;
 }
