@@ -15,11 +15,11 @@ typedef uint32_t u32x6 __attribute__((ext_vector_type(6)));
 constexpr int kFp6 = 2, kFp4 = 4;   // operand formats of the MX matrix instructions
 
 // Elements [c, c + E) of a row of k elements, zeros past its end.
-template <class T, int E, bool VEC>
+template <class T, int E, bool VEC, bool NT = false>
 __device__ __forceinline__ void load_row(const T* row, int64_t c, int64_t k, float (&v)[E]) {
   typedef T vec_t __attribute__((ext_vector_type(E)));
   if (VEC && c + E <= k) {
-    const vec_t t = *(const vec_t*)(row + c);
+    const vec_t t = NT ? __builtin_nontemporal_load((const vec_t*)(row + c)) : *(const vec_t*)(row + c);
 #pragma unroll
     for (int i = 0; i < E; ++i) v[i] = (float)t[i];
   } else {
@@ -57,7 +57,7 @@ __global__ __launch_bounds__(256) void k_mx4_quantize(const T* __restrict__ src,
 #pragma unroll
   for (int i = 0; i < 8 / RW; ++i) {
     const int64_t r = R * 32 + wv * 8 + i * RW + lane / (64 / RW);
-    load_row<T, E, VEC>(src + min(r, rows - 1) * ld, c, r < rows ? k : 0, v[i]);
+    load_row<T, E, VEC, true>(src + min(r, rows - 1) * ld, c, r < rows ? k : 0, v[i]);
   }
 #pragma unroll
   for (int i = 0; i < 8 / RW; ++i) {
@@ -129,7 +129,7 @@ __global__ __launch_bounds__(256) void k_mx4_dequant(const uint8_t* __restrict__
     for (int j = 0; j < 4; ++j) o[j] = byte == 255 ? NAN : ldexpf(v[j], byte - 127);
     float* d = out + r * ld + c;
     if (VEC && c + 4 <= k) {
-      *(f32x4*)d = o;
+      __builtin_nontemporal_store(o, (f32x4*)d);
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
