@@ -150,6 +150,16 @@ int gg_step(gg_ctx* ctx, int32_t token, int32_t pos, const gg_sample* s, double 
 int gg_step_submit(gg_ctx* ctx, int32_t token, int32_t pos, const gg_sample* s, double u);
 int gg_step_collect(gg_ctx* ctx, int32_t* out_token);
 
+/* Log probabilities behind the last selection (gg_select, gg_step or a
+ * collected step): its logits as GG_READ_LOGITS holds them, before penalty,
+ * temperature and top-p. Host pointers; what is reported, and the outputs that
+ * may be NULL, as for one row of gg_score_logits, with at most
+ * GG_SCORE_MAX_IDS given ids. Returns after the device has finished. No
+ * counterpart in the reference. */
+#define GG_SCORE_MAX_IDS 256
+int gg_score(gg_ctx* ctx, const int32_t* ids, int32_t n_ids, float* id_logprobs, float* lse, float* entropy,
+             int32_t top_n, int32_t* top_ids, float* top_logprobs);
+
 /* Repetition-penalty set (the reference's Set(allTokens), engine.ts:868-876,
  * 989, 994, 1021): cleared per turn, filled with the turn's prompt ids. */
 int gg_penalty_reset(gg_ctx* ctx);

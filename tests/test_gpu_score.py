@@ -195,3 +195,52 @@ def test_lm_head_in_four_bits_selected_and_scored(gpu, m):
     move = product_bound(h.astype(np.float64), wq, z, "f32", "f32").max()
     lse, ent, lp, order = scores(z, 5)
     assert (np.abs(got["lp"] - np.take_along_axis(lp, ids, 1)) <= 2 * move + 1e-5).all()
+
+
+@pytest.mark.parametrize("path,vocab", [("fused", 16384), ("fused", 2048), ("graph", 2048)])
+def test_score_of_the_token_loop(gpu, path, vocab):
+    """gg_score against the logits that gg_read returns, after a select, steps and collected steps, on each decode path."""
+    from dataclasses import replace
+
+    from gemma_amd import synth
+    shape = replace(synth.TINY, vocab=vocab).gemma3_mode(window=7)
+    e = capi.Engine(shape.gg_config())
+    e.set_decode_path(path)
+    e.upload_model(synth.make_model(shape, seed=3))
+    e.finalize()
+    with pytest.raises(capi.GGError) as err:
+        e.score([1])
+    assert err.value.code == capi.GG_ERR_INVALID
+    prompt = synth.prompt_ids(9, seed=11, vocab=shape.vocab)
+    e.prefill(prompt, 0)
+
+    def check_now(tok, greedy):
+        got = e.score([tok, 0, -1], top_n=5)
+        z = e.read(capi.READ_LOGITS).astype(np.float64)[None]
+        lse, ent, lp, order = scores(z, 5)
+        tol = score_rel(vocab) + 2.0 ** -22 * (1 + np.log(vocab)) + 2.0 ** -23 * np.abs(lp).max()
+        assert abs(got["lse"] - lse[0]) <= tol + 2.0 ** -23 * abs(lse[0]) and abs(got["entropy"] - ent[0]) <= tol * 2
+        assert np.array_equal(got["top_ids"], order[0])
+        assert (np.abs(got["top_logprobs"] - lp[0, order[0]]) <= tol).all()
+        assert abs(got["logprobs"][0] - lp[0, tok]) <= tol and abs(got["logprobs"][1] - lp[0, 0]) <= tol
+        assert got["logprobs"][2] == 0
+        if greedy:
+            assert got["top_ids"][0] == tok
+
+    say("score in the loop", path, vocab)
+    tok = e.select()
+    check_now(tok, True)
+    pos = len(prompt)
+    for i in range(3):
+        tok = e.step(tok, pos + i, *((0.0, 0.9, 1.0, 0.0) if i < 2 else (0.7, 0.9, 1.2, 0.4)))
+        check_now(tok, i < 2)
+    e.step_submit(tok, pos + 3)
+    with pytest.raises(capi.GGError):
+        e.score([1])
+    check_now(e.step_collect(), True)
+    for bad in (dict(ids=[1] * 257), dict(top_n=65), dict(top_n=-1)):
+        with pytest.raises(capi.GGError) as err:
+            e.score(**bad)
+        assert err.value.code == capi.GG_ERR_INVALID
+    check_now(e.step(tok, pos + 4), True)
+    e.close()

@@ -35,6 +35,14 @@ const char* kNormNames[N_NNORM] = {"attn_norm", "ffn_norm", "attn_q_norm", "attn
 enum Q8Idx { Q_ATTN_Q, Q_ATTN_K, Q_ATTN_V, Q_ATTN_O, Q_GATE, Q_UP, Q_DOWN, Q_NQ8 };
 const char* kQ8Names[Q_NQ8] = {"attn_q", "attn_k", "attn_v", "attn_output", "ffn_gate", "ffn_up", "ffn_down"};
 
+// What gg_score copies to the host.
+struct ScoreOut {
+  float lse, entropy;
+  float lp[GG_SCORE_MAX_IDS];
+  int32_t top_ids[kScoreMaxTop];
+  float top_lp[kScoreMaxTop];
+};
+
 struct Layer {
   uint8_t* qkv = nullptr;   // fused [q | k | v] rows, item-planar
   uint8_t* o = nullptr;
@@ -108,6 +116,9 @@ struct gg_ctx {
   float *logits = nullptr, *hist = nullptr, *q_dbg = nullptr;
   float* normed_tmp = nullptr;        // parity reads (GG_READ_EMBED)
   float* logits_rows = nullptr;       // class-major logits in row order (GG_READ_LOGITS)
+  uint8_t* score_ws = nullptr;        // gg_score: workspace of one row,
+  int32_t* score_ids = nullptr;       // the given ids,
+  ScoreOut* score_out = nullptr;      // the results
   float *rope_local = nullptr, *rope_global = nullptr;   // [ctx][cos|sin][128]
   float* cand_val = nullptr;
   uint32_t *cand_id = nullptr, *top = nullptr, *seen = nullptr;
@@ -1048,6 +1059,11 @@ int gg_finalize(gg_ctx* c) {
   GG_TRY(dalloc(c, &c->normed_tmp, (size_t)c->H * 4));
   GG_TRY(dalloc(c, &c->logits, (size_t)c->V * 4));
   GG_TRY(dalloc(c, &c->logits_rows, (size_t)c->V * 4));
+  size_t score_ws = 0;
+  for (int top = 0; top <= kScoreMaxTop; ++top) score_ws = std::max(score_ws, gg_score_workspace_size(1, c->V, top));
+  GG_TRY(dalloc(c, &c->score_ws, score_ws));
+  GG_TRY(dalloc(c, &c->score_ids, GG_SCORE_MAX_IDS * 4));
+  GG_TRY(dalloc(c, &c->score_out, sizeof(ScoreOut)));
   GG_TRY(dalloc(c, &c->hist, (size_t)c->L * c->H * 4));
   GG_TRY(dalloc(c, &c->q_dbg, (size_t)c->L * c->QD * 4));
   GG_TRY(dalloc(c, &c->rope_local, (size_t)c->CTX * kHeadDim * 4));
@@ -1548,6 +1564,33 @@ int gg_read(gg_ctx* c, int32_t what, int32_t layer, void* dst, size_t nbytes) {
     src = c->logits_rows;
   }
   GG_HIP(c, hipMemcpy(dst, src, sz, hipMemcpyDeviceToHost));
+  return GG_OK;
+}
+
+int gg_score(gg_ctx* c, const int32_t* ids, int32_t n_ids, float* id_logprobs, float* lse, float* entropy,
+             int32_t top_n, int32_t* top_ids, float* top_logprobs) {
+  GG_TRY(check_idle(c));
+  if (!c->have_prev) return set_err(c, GG_ERR_INVALID, "no logits to score: select or step first");
+  if (n_ids < 0 || n_ids > GG_SCORE_MAX_IDS || (n_ids > 0 && (!ids || !id_logprobs)))
+    return set_err(c, GG_ERR_INVALID, "given ids: 0 to 256, with a place for their log probabilities");
+  if (top_n < 0 || top_n > kScoreMaxTop) return set_err(c, GG_ERR_INVALID, "top_n must be 0 to 64");
+  const float* logits = c->logits;
+  if (c->logits_cm) {
+    GG_TRY(launch_rc(c, launch_logits_rows(c->logits, c->logits_rows, c->V, c->stream), "logits order"));
+    logits = c->logits_rows;
+  }
+  if (n_ids) GG_HIP(c, hipMemcpyWithStream(c->score_ids, ids, (size_t)n_ids * 4, hipMemcpyHostToDevice, c->stream));
+  const int rc = gg_score_logits(logits, GG_TYPE_F32, 1, c->V, c->V, c->score_ids, n_ids, c->score_out->lp,
+                                 &c->score_out->lse, &c->score_out->entropy, top_n, c->score_out->top_ids,
+                                 c->score_out->top_lp, c->score_ws, c->stream);
+  if (rc != GG_OK) return set_err(c, rc, "score: the kernels could not be queued");
+  ScoreOut out;
+  GG_HIP(c, hipMemcpyWithStream(&out, c->score_out, sizeof out, hipMemcpyDeviceToHost, c->stream));
+  if (lse) *lse = out.lse;
+  if (entropy) *entropy = out.entropy;
+  if (n_ids) std::memcpy(id_logprobs, out.lp, (size_t)n_ids * 4);
+  if (top_ids) std::memcpy(top_ids, out.top_ids, (size_t)top_n * 4);
+  if (top_logprobs) std::memcpy(top_logprobs, out.top_lp, (size_t)top_n * 4);
   return GG_OK;
 }
 

@@ -98,6 +98,9 @@ _SIGS = {
                                ctypes.POINTER(ctypes.c_int32)]),
     "gg_step_submit": (ctypes.c_int, [_P, ctypes.c_int32, ctypes.c_int32, ctypes.POINTER(GGSample), ctypes.c_double]),
     "gg_step_collect": (ctypes.c_int, [_P, ctypes.POINTER(ctypes.c_int32)]),
+    "gg_score": (ctypes.c_int, [_P, ctypes.POINTER(ctypes.c_int32), ctypes.c_int32, ctypes.POINTER(ctypes.c_float),
+                                ctypes.POINTER(ctypes.c_float), ctypes.POINTER(ctypes.c_float), ctypes.c_int32,
+                                ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_float)]),
     "gg_penalty_reset": (ctypes.c_int, [_P]),
     "gg_penalty_add": (ctypes.c_int, [_P, ctypes.POINTER(ctypes.c_int32), ctypes.c_int32]),
     "gg_reset_kv": (ctypes.c_int, [_P]),
@@ -233,6 +236,17 @@ class Engine:
         out = ctypes.c_int32(-1)
         _check(self.ctx, lib().gg_step_collect(self.ctx, ctypes.byref(out)))
         return out.value
+
+    def score(self, ids=(), top_n: int = 0) -> dict:
+        """Log probabilities behind the last selection's logits: of `ids`, log-sum-exp, entropy, the best alternatives."""
+        arr = np.ascontiguousarray(np.asarray(ids, dtype=np.int32))
+        lp, top_lp = np.empty(len(arr), np.float32), np.empty(max(top_n, 0), np.float32)
+        top_ids = np.empty(max(top_n, 0), np.int32)
+        lse, entropy = ctypes.c_float(), ctypes.c_float()
+        fp, ip = ctypes.POINTER(ctypes.c_float), ctypes.POINTER(ctypes.c_int32)
+        _check(self.ctx, lib().gg_score(self.ctx, arr.ctypes.data_as(ip), len(arr), lp.ctypes.data_as(fp), ctypes.byref(lse),
+                                        ctypes.byref(entropy), int(top_n), top_ids.ctypes.data_as(ip), top_lp.ctypes.data_as(fp)))
+        return {"logprobs": lp, "lse": lse.value, "entropy": entropy.value, "top_ids": top_ids, "top_logprobs": top_lp}
 
     def penalty_reset(self):
         _check(self.ctx, lib().gg_penalty_reset(self.ctx))
