@@ -464,7 +464,11 @@ struct GemmShape {
   static constexpr int GN = (BN + BM) / 32, SU = (GN + 3) / 4; // and of the row groups' scale dwords
   static constexpr int CPW = (WU + NW - 1) / NW + (XU + NW - 1) / NW + (SU + NW - 1) / NW;
   static_assert(ST == 4 || ST == 2 || ST == 1, "a stage lies within four k groups, whose scale bytes are one dword");
-  static_assert(NS >= 2 && NS <= 4, "scale dwords of two groups are held");
+  // With two stages nothing is copied twice, and the scale dwords of four k
+  // groups alternate between two places; else each stage brings its own.
+  static constexpr bool ONCE = NS == 2;
+  static constexpr int SS = ONCE ? 2 : NS;
+  static_assert(NS >= 2 && NS <= 4, "stages");
   static_assert(BM / 32 <= kMxPadGroups + 1 || X4, "the parts are padded for the last block");
   static_assert((NS - 2) * CPW < 64, "what a wave can wait for");
 };
@@ -485,7 +489,7 @@ template <int P, bool X4, int NF, int MF, int WN, int WM, int ST, int NS, int OC
 __global__ __launch_bounds__(64 * WN * WM, OCC) void k_mx4_gemm(Mx4LinearArgs a, int nbn, int nbm) {
   typedef GemmShape<P, X4, NF, MF, WN, WM, ST, NS> S;
   __shared__ __align__(1024) uint8_t stage[NS][(S::WU + S::XU) * 1024];
-  __shared__ __align__(1024) uint8_t sstage[2][S::SU * 1024];
+  __shared__ __align__(1024) uint8_t sstage[S::SS][S::SU * 1024];
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wn = wv % WN, wm = wv / WN;
   // Tile order: the blocks with one value of blockIdx % 8 share an XCD and its
@@ -532,28 +536,27 @@ __global__ __launch_bounds__(64 * WN * WM, OCC) void k_mx4_gemm(Mx4LinearArgs a,
                                : xsc + (size_t)min(rm0 + gi - S::BN / 32, xlast) * ks * 256) + 16 * (lane & 15);
   }
   // With two stages a wave waits for all its copies, and nothing is copied
-  // twice. With more their number has to be the same in every stage: units and
-  // scales of the four k groups are fetched again where there are none left.
-  constexpr bool ONCE = NS == 2;
+  // twice. With more their number has to be the same in every stage: units are
+  // fetched again where there are none left.
   auto copy = [&](int t, int buf) __attribute__((always_inline)) {
     const uint32_t dst = lds + buf * ((S::WU + S::XU) * 1024);
 #pragma unroll
     for (int i = 0; i < NWC; ++i) {
       const int u = min(i * S::NW + wv, S::WU - 1);
-      if (!ONCE || S::WU % S::NW == 0 || i * S::NW + wv < S::WU)
+      if (!S::ONCE || S::WU % S::NW == 0 || i * S::NW + wv < S::WU)
         dma16(wsrc[i] + (size_t)(ST == 1 ? t : min(t + u % ST, kt - 1)) * 1024, dst + 1024 * u);
     }
 #pragma unroll
     for (int i = 0; i < NXC; ++i) {
       const int u = min(i * S::NW + wv, S::XU - 1), q = X4 ? u % ST : u / S::XQ;
-      if (!ONCE || S::XU % S::NW == 0 || i * S::NW + wv < S::XU)
+      if (!S::ONCE || S::XU % S::NW == 0 || i * S::NW + wv < S::XU)
         dma16(xsrc[i] + (size_t)(ST == 1 ? t : min(t + q, kt - 1)) * xstep, dst + 1024 * (S::WU + u));
     }
-    if (ONCE && ST < 4 && (t & 3) != 0) return;
+    if (S::ONCE && ST < 4 && (t & 3) != 0) return;
 #pragma unroll
     for (int i = 0; i < NSC; ++i) {
       const int u = min(i * S::NW + wv, S::SU - 1);
-      if (!ONCE || i * S::NW + wv < S::SU) dma16(ssrc[i] + (t >> 2) * 256, slds + ((t >> 2) & 1) * (S::SU * 1024) + u * 1024);
+      if (!S::ONCE || i * S::NW + wv < S::SU) dma16(ssrc[i] + (t >> 2) * 256, slds + (S::ONCE ? (t >> 2) & 1 : buf) * (S::SU * 1024) + u * 1024);
     }
   };
   f32x16 acc[NF][MF];
@@ -579,8 +582,8 @@ __global__ __launch_bounds__(64 * WN * WM, OCC) void k_mx4_gemm(Mx4LinearArgs a,
     fill = fill + 1 == NS ? 0 : fill + 1;
     const uint8_t* ws = stage[buf] + 16 * lane;
     const uint8_t* xs = ws + S::WU * 1024;
+    const uint32_t* sd = (const uint32_t*)sstage[S::ONCE ? (t >> 2) & 1 : buf] + lane;
     buf = buf + 1 == NS ? 0 : buf + 1;
-    const uint32_t* sd = (const uint32_t*)sstage[(t >> 2) & 1] + lane;
     int wd[NF], xd[MF];   // scale dwords: byte t % 4 is this k group's
 #pragma unroll
     for (int i = 0; i < NF; ++i) wd[i] = sd[(wn * NF + i) * 64];
