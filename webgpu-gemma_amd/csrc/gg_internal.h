@@ -497,9 +497,13 @@ struct Mx4LinearArgs {
   int64_t ldp;
 };
 // A product with m rows and `parts` parts takes the few-row kernel when it has
-// a column of its matrix instructions for each part of each row, and LDS holds
-// them (32 bytes of each 32-block's part) and the sums.
-constexpr int kMxGemvCols = 64, kMxGemvWaves = 8;
+// a column of its matrix instructions for each part of each row, LDS holds them
+// (32 bytes of each 32-block's part) and the sums, and x has no more than 648
+// 32-blocks, since every block of the kernel makes all parts. us against the
+// many-row kernel: 2 x 1152 x 6912 (432 32-blocks) 12.0 / 15.5, 4 x 16384 x
+// 4096 (512) 15.9 / 19.2, 3 x 1152 x 6912 (648) 14.8 / 15.7; 4 x 1152 x 6912
+// (864) 16.7 / 15.9, 8 x 4096 x 4096 bf16 (1024) 15.9 / 13.4.
+constexpr int kMxGemvCols = 64, kMxGemvWaves = 8, kMxGemvBlocks = 648;
 __host__ __device__ constexpr size_t mx_gemv_sums(int col_tiles) {   // f32 [wave][16][16 col_tiles + 1]
   return (size_t)kMxGemvWaves * 16 * (16 * col_tiles + 1) * 4;
 }
@@ -507,7 +511,8 @@ inline size_t mx_gemv_lds(int cols, int k) {
   return mx_gemv_sums((cols + 15) / 16) + (size_t)((k + 127) / 128 * 4) * cols * 32;
 }
 inline bool mx_gemv_fits(int64_t m, int parts, int64_t k) {
-  return m * parts <= kMxGemvCols && mx_gemv_lds((int)m * parts, (int)k) <= 160 * 1024;
+  return m * parts <= kMxGemvCols && m * ((k + 127) / 128 * 4) <= kMxGemvBlocks &&
+         mx_gemv_lds((int)m * parts, (int)k) <= 160 * 1024;
 }
 // Tiles of the many-row kernel (features x rows) and slices of k.
 enum Mx4TileId { MT_256x256, MT_256x64, MT_128x64, MT_128x32, MT_COUNT };
