@@ -54,10 +54,34 @@ __global__ __launch_bounds__(256) void k_mx4_quantize(const T* __restrict__ src,
   const int64_t c = (int64_t)g * 256 + E * ln;
   const int kb = ln / LB, t = kb >> 1, b = kb & 1;   // 32-block, its tile and half
   float v[8 / RW][E];
+  if constexpr (VEC || sizeof(T) == 4) {
 #pragma unroll
-  for (int i = 0; i < 8 / RW; ++i) {
-    const int64_t r = R * 32 + wv * 8 + i * RW + lane / (64 / RW);
-    load_row<T, E, VEC, true>(src + min(r, rows - 1) * ld, c, r < rows ? k : 0, v[i]);
+    for (int i = 0; i < 8 / RW; ++i) {
+      const int64_t r = R * 32 + wv * 8 + i * RW + lane / (64 / RW);
+      load_row<T, E, VEC, VEC>(src + min(r, rows - 1) * ld, c, r < rows ? k : 0, v[i]);
+    }
+  } else {
+    // 16-bit rows at odd addresses: an element a lane, whole lines all the
+    // same, and to the lanes that take them through LDS (20000 x 1153 bf16 33
+    // -> 25 us; f32 rows, four loads a lane, take 25 as they are and 40 so)
+    __shared__ __align__(16) T rowbuf[4][8][256];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int64_t r = R * 32 + wv * 8 + i;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t e = (int64_t)g * 256 + 64 * j + lane;
+        rowbuf[wv][i][64 * j + lane] = r < rows && e < k ? src[r * ld + e] : (T)0.f;
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int i = 0; i < 8 / RW; ++i) {
+      typedef T vec_t __attribute__((ext_vector_type(E)));
+      const vec_t t = *(const vec_t*)&rowbuf[wv][i * RW + lane / (64 / RW)][E * ln];
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[i][j] = (float)t[j];
+    }
   }
 #pragma unroll
   for (int i = 0; i < 8 / RW; ++i) {
@@ -115,7 +139,7 @@ __global__ __launch_bounds__(256) void k_mx4_dequant(const uint8_t* __restrict__
   for (int i = 0; i < 8; ++i) {
     const int row = wv * 8 + i;
     const int64_t r = R * 32 + row;
-    if (r >= rows || c >= k) continue;
+    if (r >= rows) continue;
     const int l = 32 * b + row;
     const uint32_t q = codes[t * 64 + l][lane & 7];
     const int byte = scales[4 * l + t];
@@ -127,13 +151,27 @@ __global__ __launch_bounds__(256) void k_mx4_dequant(const uint8_t* __restrict__
     f32x4 o;
 #pragma unroll
     for (int j = 0; j < 4; ++j) o[j] = byte == 255 ? NAN : ldexpf(v[j], byte - 127);
-    float* d = out + r * ld + c;
-    if (VEC && c + 4 <= k) {
-      __builtin_nontemporal_store(o, (f32x4*)d);
-    } else {
+    float* d = out + r * ld;
+    if constexpr (VEC) {
+      if (c + 4 <= k) {
+        __builtin_nontemporal_store(o, (f32x4*)(d + c));
+      } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (c + j < k) d[j] = o[j];
+        for (int j = 0; j < 4; ++j)
+          if (c + j < k) d[c + j] = o[j];
+      }
+    } else {
+      // rows at odd addresses: an element a lane
+      __shared__ __align__(16) float rowbuf[4][256];
+      *(f32x4*)&rowbuf[wv][4 * lane] = o;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t e = (int64_t)g * 256 + 64 * j + lane;
+        const float t = rowbuf[wv][64 * j + lane];
+        if (e < k) d[e] = t;   // through the cache, which makes whole lines of them
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
   }
 }
@@ -168,15 +206,14 @@ __device__ __forceinline__ int parts_byte(uint32_t amax_bits) {
 struct Block32 {
   f32x16 ev, od;
   float magic, unit;
-  template <class T, bool VEC>
-  __device__ __forceinline__ void load(const T* row, int64_t c, int64_t k) {
-    float v[8][4];
+  __device__ __forceinline__ void load(const float* lds) {   // 16-byte aligned
 #pragma unroll
-    for (int i = 0; i < 8; ++i) load4<T, VEC>(row, c + 4 * i, k, v[i]);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      ev[i] = v[i / 2][2 * (i & 1)];
-      od[i] = v[i / 2][2 * (i & 1) + 1];
+    for (int i = 0; i < 8; ++i) {
+      const f32x4 t = *(const f32x4*)(lds + 4 * i);
+      ev[2 * i] = t[0];
+      od[2 * i] = t[1];
+      ev[2 * i + 1] = t[2];
+      od[2 * i + 1] = t[3];
     }
   }
   // the scale byte; the elements become x / 2^e
@@ -208,15 +245,43 @@ struct Block32 {
   }
 };
 
-// A wave takes 32 rows x 64 k, a thread one 32-block of them.
+// A wave takes 32 rows x 64 k, a thread one 32-block of them. The rows come in
+// whole lines, four elements a lane (one where their addresses are odd), and
+// change lanes in LDS; a pitch of 68 floats puts the 16 lanes of a read on
+// different banks. Bound by memory for long x (reads 4 or 2 bytes, writes
+// 3/4 byte a part and element), by its latency for short.
 template <class T, bool VEC>
 __global__ __launch_bounds__(64) void k_mx_split(const T* __restrict__ src, int64_t rows, int64_t k, int64_t ld,
                                                  int parts, uint8_t* __restrict__ dst, Mx4Layout L) {
+  constexpr int PITCH = 68;
+  __shared__ __align__(16) float xs[32 * PITCH];
   const int lane = threadIdx.x;
-  const int64_t R = blockIdx.x, r = R * 32 + (lane & 31);
+  const int64_t R = blockIdx.x;
   const int t = blockIdx.y;
+  if constexpr (VEC) {
+    float v[8][4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int64_t r = R * 32 + 4 * i + (lane >> 4);
+      load4<T, true>(src + min(r, rows - 1) * ld, (int64_t)t * 64 + 4 * (lane & 15), r < rows ? k : 0, v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      *(f32x4*)(xs + (4 * i + (lane >> 4)) * PITCH + 4 * (lane & 15)) = f32x4{v[i][0], v[i][1], v[i][2], v[i][3]};
+  } else {
+    const int64_t e = (int64_t)t * 64 + lane;
+    float v[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const int64_t r = R * 32 + i;
+      v[i] = r < rows && e < k ? (float)src[r * ld + e] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 32; ++i) xs[i * PITCH + lane] = v[i];
+  }
+  __syncthreads();
   Block32 v;
-  v.load<T, VEC>(src + min(r, rows - 1) * ld, (int64_t)t * 64 + 32 * (lane >> 5), r < rows ? k : 0);
+  v.load(xs + (lane & 31) * PITCH + 32 * (lane >> 5));
   dst[mx_codes_bytes(L.rt, L.kt, parts) + ((size_t)R * L.ks + (t >> 2)) * 256 + 4 * lane + (t & 3)] = (uint8_t)v.scale();
   uint8_t* out = dst + ((size_t)t * L.rt + R) * parts * kMxPartBytes;
   for (int p = 0; p < parts; ++p, out += kMxPartBytes) {
