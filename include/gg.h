@@ -319,8 +319,8 @@ int gg_mxfp4_dequant(const void* packed, float* out, int64_t rows, int64_t k, in
  * rows; ldx is not read). GG_TYPE_F32 / F16 / BF16: rows of x ldx >= k apart;
  * of every 32-block of x, 2^-24 of its largest magnitude (of 2^-106 where that
  * is smaller) is kept for f32 y, 2^-19 for f16 y (2^-14 of bf16 x), 2^-14 for
- * bf16 y, finer than the result's rounding. A row of x
- * with an infinity or a NaN gives NaN. Rows of y are ldy >= rows apart; what
+ * bf16 y, finer than the result's rounding. A row of x with an infinity or a
+ * NaN gives NaN. Rows of y are ldy >= rows apart; what
  * lies between them is left alone. y overlaps neither operand.
  * workspace: gg_mxfp4_linear_workspace_size() device bytes, 16-byte aligned
  * (NULL where that is 0), used until the call's kernels have run: calls that
@@ -331,7 +331,8 @@ int gg_mxfp4_linear(const void* w, const void* x, uint32_t x_type, int64_t ldx, 
 
 /* ---- scoring ---------------------------------------------------------------
  * Log probabilities over rows of logits: rows x n (GG_TYPE_F32 / F16 / BF16),
- * ld >= n elements apart, n from 1 to 2^30. Each output may be NULL:
+ * ld >= n elements apart, rows and n from 1 to 2^30. Each output may be NULL,
+ * id_logprobs with n_ids 0:
  *   lse[row]          ln sum e^z
  *   entropy[row]      -sum p ln p, in nats
  *   id_logprobs       [rows][n_ids]: z[ids] - lse; 0 for the id -1 (no token),

@@ -258,3 +258,38 @@ def test_linear_repeats_bit_for_bit(gpu, m):
     first = linear(wp, ptr, capi.GG_TYPE_F32, k, m, n, k, "f32")
     for _ in range(3):
         assert np.array_equal(first, linear(wp, ptr, capi.GG_TYPE_F32, k, m, n, k, "f32"))
+
+
+@pytest.mark.parametrize("x_name", ["f32", "f16", "mxfp4"])
+@pytest.mark.parametrize("m,n,k", [(12, 100, 16400), (40, 96, 8200), (70, 200, 5000), (300, 260, 3100)])
+def test_linear_long_k(gpu, x_name, m, n, k):
+    """Many stages of each tile, with and without slices of k."""
+    say("long k", x_name, m, n, k)
+    rng = np.random.default_rng(k + m)
+    x = sample(rng, m, k)
+    wp, wk = pack(rng.standard_normal((n, k)) * 0.05)
+    wq = quantised(wk)
+    if x_name == "mxfp4":
+        xp, xk = pack(x)
+        xk = quantised(xk)
+        got = linear(wp, xp.data_ptr(), MX, 0, m, n, k, "f32")
+    else:
+        buf, ptr, xk = rows_of(np.clip(x, -500, 500), x_name, k)
+        got = linear(wp, ptr, TYPES[x_name][0], k, m, n, k, "f32")
+    want = xk @ wq.T
+    assert (np.abs(got - want) <= product_bound(xk, wq, want, None if x_name == "mxfp4" else x_name, "f32")).all()
+
+
+def test_round_trip_of_many_rows(gpu):
+    """More rows than one grid's threads allow: 2^28 and a few, of one element."""
+    rows = (1 << 28) + 70
+    say("round trip", rows)
+    src = (torch.arange(rows, dtype=torch.int32, device="cuda:0") % 13).to(torch.bfloat16)
+    p = torch.empty(capi.mxfp4_packed_size(rows, 1), dtype=torch.uint8, device="cuda:0")
+    out = torch.empty(rows, device="cuda:0")
+    capi.mxfp4_quantize(src.data_ptr(), capi.GG_TYPE_BF16, rows, 1, 1, p.data_ptr(), stream())
+    capi.mxfp4_dequant(p.data_ptr(), out.data_ptr(), rows, 1, 1, stream())
+    kept = torch.from_numpy(quantised(np.arange(13.0)[:, None])[:, 0]).to("cuda:0", torch.float32)
+    for lo in range(0, rows, 1 << 26):
+        part = out[lo:lo + (1 << 26)]
+        assert torch.equal(part, kept[src[lo:lo + (1 << 26)].long()])

@@ -197,6 +197,26 @@ def test_lm_head_in_four_bits_selected_and_scored(gpu, m):
     assert (np.abs(got["lp"] - np.take_along_axis(lp, ids, 1)) <= 2 * move + 1e-5).all()
 
 
+def test_many_rows(gpu):
+    """More rows than one grid's threads allow: 2^24 and a few, of two logits."""
+    rows = (1 << 24) + 5
+    say("score", rows)
+    z = (torch.arange(2 * rows, device="cuda:0") % 7).to(torch.float32).view(rows, 2)
+    ids = (torch.arange(rows, device="cuda:0", dtype=torch.int32) % 2)
+    lp, lse, ent, top_lp = (torch.full((rows,), 9.0, device="cuda:0") for _ in range(4))
+    top = torch.full((rows,), 9, dtype=torch.int32, device="cuda:0")
+    assert capi.score_workspace_size(rows, 2, 1) == 0
+    capi.score_logits(z.data_ptr(), capi.GG_TYPE_F32, rows, 2, 2, ids.data_ptr(), 1, lp.data_ptr(), lse.data_ptr(),
+                      ent.data_ptr(), 1, top.data_ptr(), top_lp.data_ptr(), None, stream())
+    torch.cuda.synchronize()
+    all_lp = torch.log_softmax(z.double(), 1)
+    tol = score_rel(2) + 2.0 ** -20
+    assert ((lse - torch.logsumexp(z.double(), 1)).abs() <= tol + 2.0 ** -20).all()
+    assert ((lp - all_lp.gather(1, ids.long()[:, None])[:, 0]).abs() <= tol).all()
+    assert ((ent + (all_lp.exp() * all_lp).sum(1)).abs() <= 4 * tol).all()
+    assert torch.equal(top.long(), z.argmax(1)) and ((top_lp - all_lp.amax(1)).abs() <= tol).all()
+
+
 @pytest.mark.parametrize("path,vocab", [("fused", 16384), ("fused", 2048), ("graph", 2048)])
 def test_score_of_the_token_loop(gpu, path, vocab):
     """gg_score against the logits that gg_read returns, after a select, steps and collected steps, on each decode path."""

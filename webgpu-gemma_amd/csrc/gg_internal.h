@@ -522,8 +522,8 @@ struct Mx4Tile {
   // start and end; the same for each block when the CUs are full
   float lat, lat_part, lat_end, thr, thr_part, thr_end;
 };
-// Least-squares fits of 11,000 timings (240 products of 1 to 4096 rows, 64 to
-// 262144 features and k of 64 to 8192, each tile, 1 to 16 slices): 11% rms for
+// Least-squares fits of 5,400 timings (310 products of 1 to 4096 rows, 72 to
+// 250200 features and k of 65 to 8192, each tile, 1 to 16 slices): 11% rms for
 // parts, 8% for packed x; the choice costs 1.8% and 3.5% over the best of all.
 constexpr Mx4Tile kMx4PartTiles[MT_COUNT] = {{256, 256, .15f, .05f, 2.f, .006f, .326f, 12.1f},
                                              {256, 64, .127f, .094f, 4.6f, .052f, .097f, 3.1f},

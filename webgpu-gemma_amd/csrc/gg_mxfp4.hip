@@ -4,6 +4,8 @@
 // (gg_internal.h).
 #include "gg_device.h"
 
+#include <algorithm>
+
 namespace gg {
 
 namespace {
@@ -43,12 +45,12 @@ __device__ __forceinline__ void load4(const T* row, int64_t c, int64_t k, float 
 // ---------------------------------------------------------------------------
 template <class T, bool VEC>
 __global__ __launch_bounds__(256) void k_mx4_quantize(const T* __restrict__ src, int64_t rows, int64_t k, int64_t ld,
-                                                      uint8_t* __restrict__ dst, Mx4Layout L) {
+                                                      uint8_t* __restrict__ dst, Mx4Layout L, int64_t r0) {
   constexpr int E = 16 / sizeof(T), LB = 32 / E, RW = E / 4;   // elements a lane, lanes a block, rows a wave at a time
   __shared__ __align__(16) uint8_t codes[256][16];   // [4 tiles x 64 lanes][16 bytes]
   __shared__ __align__(4) uint8_t scales[256];       // [64 lanes][4 tiles]
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-  const int64_t R = blockIdx.x;
+  const int64_t R = r0 + blockIdx.x;
   const int g = blockIdx.y;
   const int ln = lane % (64 / RW);
   const int64_t c = (int64_t)g * 256 + E * ln;
@@ -122,11 +124,11 @@ __global__ __launch_bounds__(256) void k_mx4_quantize(const T* __restrict__ src,
 // ---------------------------------------------------------------------------
 template <bool VEC>
 __global__ __launch_bounds__(256) void k_mx4_dequant(const uint8_t* __restrict__ src, float* __restrict__ out,
-                                                     int64_t rows, int64_t k, int64_t ld, Mx4Layout L) {
+                                                     int64_t rows, int64_t k, int64_t ld, Mx4Layout L, int64_t r0) {
   __shared__ __align__(16) uint16_t codes[256][8];
   __shared__ __align__(4) uint8_t scales[256];
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-  const int64_t R = blockIdx.x;
+  const int64_t R = r0 + blockIdx.x;
   const int g = blockIdx.y;
   if (g * 4 + wv < L.kt)
     *(u32x4*)codes[wv * 64 + lane] = *(const u32x4*)(src + ((size_t)R * L.kt + g * 4 + wv) * 1024 + 16 * lane);
@@ -748,15 +750,27 @@ bool rows_aligned(const void* p, int64_t ld, int n) {
   return ((uintptr_t)p % (n * sizeof(T))) == 0 && ld % n == 0;
 }
 
+// A launch for each 2^23 row groups (a grid holds fewer than 2^32 threads):
+// f(first row group, grid).
+template <class F>
+int by_row_groups(const Mx4Layout& L, F f) {
+  constexpr int64_t MOST = 1 << 23;
+  for (int64_t r0 = 0; r0 < L.rt; r0 += MOST) {
+    f(r0, dim3((unsigned)std::min(L.rt - r0, MOST), (unsigned)L.ks));
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return (int)e;
+  }
+  return 0;
+}
+
 template <class T>
 int quantize_t(const void* src, int64_t rows, int64_t k, int64_t ld, uint8_t* dst, hipStream_t s) {
   const Mx4Layout L = mx4_layout(rows, k);
-  const dim3 grid((unsigned)L.rt, (unsigned)L.ks);
-  if (rows_aligned<T>(src, ld, 16 / (int)sizeof(T)))
-    hipLaunchKernelGGL((k_mx4_quantize<T, true>), grid, dim3(256), 0, s, (const T*)src, rows, k, ld, dst, L);
-  else
-    hipLaunchKernelGGL((k_mx4_quantize<T, false>), grid, dim3(256), 0, s, (const T*)src, rows, k, ld, dst, L);
-  return (int)hipGetLastError();
+  const bool vec = rows_aligned<T>(src, ld, 16 / (int)sizeof(T));
+  return by_row_groups(L, [&](int64_t r0, dim3 grid) {
+    if (vec) hipLaunchKernelGGL((k_mx4_quantize<T, true>), grid, dim3(256), 0, s, (const T*)src, rows, k, ld, dst, L, r0);
+    else hipLaunchKernelGGL((k_mx4_quantize<T, false>), grid, dim3(256), 0, s, (const T*)src, rows, k, ld, dst, L, r0);
+  });
 }
 
 template <class T>
@@ -784,13 +798,12 @@ int launch_mx4_quantize(int elem, const void* src, int64_t rows, int64_t k, int6
 
 int launch_mx4_dequant(const uint8_t* src, float* out, int64_t rows, int64_t k, int64_t ld, void* stream) {
   const Mx4Layout L = mx4_layout(rows, k);
-  const dim3 grid((unsigned)L.rt, (unsigned)L.ks);
   hipStream_t s = (hipStream_t)stream;
-  if (rows_aligned<float>(out, ld, 4))
-    hipLaunchKernelGGL((k_mx4_dequant<true>), grid, dim3(256), 0, s, src, out, rows, k, ld, L);
-  else
-    hipLaunchKernelGGL((k_mx4_dequant<false>), grid, dim3(256), 0, s, src, out, rows, k, ld, L);
-  return (int)hipGetLastError();
+  const bool vec = rows_aligned<float>(out, ld, 4);
+  return by_row_groups(L, [&](int64_t r0, dim3 grid) {
+    if (vec) hipLaunchKernelGGL((k_mx4_dequant<true>), grid, dim3(256), 0, s, src, out, rows, k, ld, L, r0);
+    else hipLaunchKernelGGL((k_mx4_dequant<false>), grid, dim3(256), 0, s, src, out, rows, k, ld, L, r0);
+  });
 }
 
 int launch_mx_split(int elem, const void* src, int64_t rows, int64_t k, int64_t ld, int parts, uint8_t* dst,
@@ -841,7 +854,7 @@ template <int P, bool X4, int NF, int MF, int WN, int WM, int ST, int NS, int OC
 static int launch_gemm_t(const Mx4LinearArgs& a, hipStream_t s) {
   typedef GemmShape<P, X4, NF, MF, WN, WM, ST, NS> S;
   const int64_t nbn = (a.n + S::BN - 1) / S::BN, nbm = (a.m + S::BM - 1) / S::BM;
-  if (nbn * nbm * a.kslices > 0x7fffffffll) return (int)hipErrorInvalidValue;
+  if (nbn * nbm * a.kslices > 0xffffffffll / (64 * WN * WM)) return (int)hipErrorInvalidValue;   // threads of a grid
   hipLaunchKernelGGL((k_mx4_gemm<P, X4, NF, MF, WN, WM, ST, NS, OCC>), dim3((unsigned)(nbn * nbm * a.kslices)),
                      dim3(64 * WN * WM), 0, s, a, (int)nbn, (int)nbm);
   const hipError_t e = hipGetLastError();

@@ -435,9 +435,26 @@ __global__ __launch_bounds__(THREADS) void k_score_merge(ScoreArgs a) {
 
 template <class T, int EPT>
 int launch_score_t(ScoreArgs a, hipStream_t s) {
-  hipLaunchKernelGGL((k_score<T, EPT>), dim3((unsigned)(a.rows * a.nch)), dim3(kScoreThreads), 0, s, a);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || a.nch == 1) return (int)e;
+  // a launch for each 2^22 rows: a grid holds fewer than 2^32 threads (more
+  // rows than 768 are one block each)
+  constexpr long long MOST = 1 << 22;
+  for (long long left = a.rows; left > 0; left -= MOST) {
+    a.rows = left < MOST ? left : MOST;
+    hipLaunchKernelGGL((k_score<T, EPT>), dim3((unsigned)(a.rows * a.nch)), dim3(kScoreThreads), 0, s, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return (int)e;
+    if (left <= MOST) break;
+    a.z = (const T*)a.z + MOST * a.ld;
+    if (a.n_ids) {
+      a.ids += MOST * a.n_ids;
+      a.lp += MOST * a.n_ids;
+    }
+    if (a.lse) a.lse += MOST;
+    if (a.entropy) a.entropy += MOST;
+    if (a.top_ids) a.top_ids += MOST * a.top;
+    if (a.top_lp) a.top_lp += MOST * a.top;
+  }
+  if (a.nch == 1) return 0;
   if (a.nch * a.top <= kScoreThreads * kMergePer)
     hipLaunchKernelGGL((k_score_merge<T, kScoreThreads>), dim3((unsigned)a.rows), dim3(kScoreThreads), 0, s, a);
   else
