@@ -517,9 +517,14 @@ __global__ __launch_bounds__(64 * kMxGemvWaves) void k_mx4_gemv(Mx4LinearArgs a,
 // rows over one slice of k, a wave NF x MF instruction tiles of it.
 // The operands lie in memory in operand order, so a stage (ST groups of 64 k)
 // goes to LDS as it is, by DMA, 1 KB an instruction, NS - 1 stages ahead of
-// the one that is multiplied; one barrier a stage. With more than two stages
-// every wave starts the same number of copies (CPW) in every stage, so that
-// the number in flight tells which stage has arrived.
+// the one that is multiplied; one barrier a stage. In the largest tile four
+// waves only copy, so that the others' matrix instructions do not queue behind
+// a stage's 44 to 72 copies: 4096 x 8192 x 8192 with both operands packed 140 ->
+// 129 us, bf16 x 388 -> 368, f32 x 656 -> 603 (with one copying wave, which
+// cannot start them fast enough, 136 and 412; with two 127, 369 and 606). In the
+// smaller tiles the waves share the copies.
+// With more than two stages every copying wave starts the same number (CPW) in
+// every stage, so that the number in flight tells which stage has arrived.
 // ---------------------------------------------------------------------------
 template <int P, bool X4, int NF, int MF, int WN, int WM, int ST, int NS>
 struct GemmShape {
@@ -529,15 +534,17 @@ struct GemmShape {
   static constexpr int XB = BM / 32 * XG;                      // bytes of a k group's x,
   static constexpr int XQ = (XB + 1023) / 1024, XU = XQ * ST;  // units of it and of a stage's,
   static constexpr int GN = (BN + BM) / 32, SU = (GN + 3) / 4; // and of the row groups' scale dwords
-  static constexpr int CPW = (WU + NW - 1) / NW + (XU + NW - 1) / NW + (SU + NW - 1) / NW;
+  static constexpr int COPIERS = NF * MF >= 8 ? 4 : 0;               // waves that only copy
+  static constexpr int THREADS = 64 * (NW + COPIERS), CW = COPIERS ? COPIERS : NW;
+  static constexpr int CPW = (WU + CW - 1) / CW + (XU + CW - 1) / CW + (SU + CW - 1) / CW;
   static_assert(ST == 4 || ST == 2 || ST == 1, "a stage lies within four k groups, whose scale bytes are one dword");
   // With two stages nothing is copied twice, and the scale dwords of four k
   // groups alternate between two places; else each stage brings its own.
   static constexpr bool ONCE = NS == 2;
   static constexpr int SS = ONCE ? 2 : NS;
-  static_assert(NS >= 2 && NS <= 4, "stages");
+  static_assert(NS == 2 || NS == 3, "stages");
   static_assert(BM / 32 <= kMxPadGroups + 1 || X4, "the parts are padded for the last block");
-  static_assert((NS - 2) * CPW < 64, "what a wave can wait for");
+  static_assert(NS == 2 || CPW < 64, "what a wave can wait for");
 };
 
 // One DMA instruction: lane l's 16 bytes at src go to dst + 16 l. Inline asm,
@@ -549,11 +556,18 @@ __device__ __forceinline__ void dma16(const uint8_t* src, uint32_t dst) {
                "v"(src)
                : "memory", "m0");
 }
+// The same from a uniform address: lane l's 16 bytes are at base + off, off = 16 l.
+__device__ __forceinline__ void dma16u(const uint8_t* base, uint32_t off, uint32_t dst) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(
+                   __builtin_amdgcn_readfirstlane(dst)),
+               "v"(off), "s"(base)
+               : "memory", "m0");
+}
 template <int N>
 __device__ __forceinline__ void wait_copies() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
 template <int P, bool X4, int NF, int MF, int WN, int WM, int ST, int NS, int OCC>
-__global__ __launch_bounds__(64 * WN * WM, OCC) void k_mx4_gemm(Mx4LinearArgs a, int nbn, int nbm) {
+__global__ __launch_bounds__((GemmShape<P, X4, NF, MF, WN, WM, ST, NS>::THREADS), OCC) void k_mx4_gemm(Mx4LinearArgs a, int nbn, int nbm) {
   typedef GemmShape<P, X4, NF, MF, WN, WM, ST, NS> S;
   __shared__ __align__(1024) uint8_t stage[NS][(S::WU + S::XU) * 1024];
   __shared__ __align__(1024) uint8_t sstage[S::SS][S::SU * 1024];
@@ -578,19 +592,20 @@ __global__ __launch_bounds__(64 * WN * WM, OCC) void k_mx4_gemm(Mx4LinearArgs a,
   // The lanes' sources at k group 0. Row groups and k groups past the matrix
   // read its last ones, parts past the last row group what follows them; their
   // results are not stored, their x is not multiplied.
-  constexpr int NWC = (S::WU + S::NW - 1) / S::NW, NXC = (S::XU + S::NW - 1) / S::NW, NSC = (S::SU + S::NW - 1) / S::NW;
+  constexpr int NWC = (S::WU + S::CW - 1) / S::CW, NXC = (S::XU + S::CW - 1) / S::CW, NSC = (S::SU + S::CW - 1) / S::CW;
+  const int cw = S::COPIERS > 0 ? wv - S::NW : wv;
   const uint8_t *wsrc[NWC], *xsrc[NXC], *ssrc[NSC];
   const int kt = a.kt, ks = a.ks;
   const int64_t wlast = a.wrt - 1, xlast = a.xrt - 1;
   const size_t xstep = X4 ? 1024 : (size_t)a.xrt * S::XG;
 #pragma unroll
   for (int i = 0; i < NWC; ++i) {
-    const int u = min(i * S::NW + wv, S::WU - 1);
+    const int u = min(i * S::CW + cw, S::WU - 1);
     wsrc[i] = a.w + (size_t)min(rn0 + u / ST, wlast) * kt * 1024 + 16 * lane;
   }
 #pragma unroll
   for (int i = 0; i < NXC; ++i) {
-    const int u = min(i * S::NW + wv, S::XU - 1);
+    const int u = min(i * S::CW + cw, S::XU - 1);
     if constexpr (X4) xsrc[i] = x + (size_t)min(rm0 + u / ST, xlast) * kt * 1024 + 16 * lane;
     // the block's row groups of one k group lie one after the other
     else xsrc[i] = x + (size_t)rm0 * S::XG + min(u % S::XQ * 1024 + 16 * lane, S::XB - 16);
@@ -598,7 +613,7 @@ __global__ __launch_bounds__(64 * WN * WM, OCC) void k_mx4_gemm(Mx4LinearArgs a,
 #pragma unroll
   for (int i = 0; i < NSC; ++i) {
     // 16 lanes a row group's 256 bytes of scales
-    const int gi = min(4 * min(i * S::NW + wv, S::SU - 1) + (lane >> 4), S::GN - 1);
+    const int gi = min(4 * min(i * S::CW + cw, S::SU - 1) + (lane >> 4), S::GN - 1);
     ssrc[i] = (gi < S::BN / 32 ? wsc + (size_t)min(rn0 + gi, wlast) * ks * 256
                                : xsc + (size_t)min(rm0 + gi - S::BN / 32, xlast) * ks * 256) + 16 * (lane & 15);
   }
@@ -609,23 +624,86 @@ __global__ __launch_bounds__(64 * WN * WM, OCC) void k_mx4_gemm(Mx4LinearArgs a,
     const uint32_t dst = lds + buf * ((S::WU + S::XU) * 1024);
 #pragma unroll
     for (int i = 0; i < NWC; ++i) {
-      const int u = min(i * S::NW + wv, S::WU - 1);
-      if (!S::ONCE || S::WU % S::NW == 0 || i * S::NW + wv < S::WU)
+      const int u = min(i * S::CW + cw, S::WU - 1);
+      if (!S::ONCE || S::WU % S::CW == 0 || i * S::CW + cw < S::WU)
         dma16(wsrc[i] + (size_t)(ST == 1 ? t : min(t + u % ST, kt - 1)) * 1024, dst + 1024 * u);
     }
 #pragma unroll
     for (int i = 0; i < NXC; ++i) {
-      const int u = min(i * S::NW + wv, S::XU - 1), q = X4 ? u % ST : u / S::XQ;
-      if (!S::ONCE || S::XU % S::NW == 0 || i * S::NW + wv < S::XU)
+      const int u = min(i * S::CW + cw, S::XU - 1), q = X4 ? u % ST : u / S::XQ;
+      if (!S::ONCE || S::XU % S::CW == 0 || i * S::CW + cw < S::XU)
         dma16(xsrc[i] + (size_t)(ST == 1 ? t : min(t + q, kt - 1)) * xstep, dst + 1024 * (S::WU + u));
     }
     if (S::ONCE && ST < 4 && (t & 3) != 0) return;
 #pragma unroll
     for (int i = 0; i < NSC; ++i) {
-      const int u = min(i * S::NW + wv, S::SU - 1);
-      if (!S::ONCE || i * S::NW + wv < S::SU) dma16(ssrc[i] + (t >> 2) * 256, slds + (S::ONCE ? (t >> 2) & 1 : buf) * (S::SU * 1024) + u * 1024);
+      const int u = min(i * S::CW + cw, S::SU - 1);
+      if (!S::ONCE || i * S::CW + cw < S::SU) dma16(ssrc[i] + (t >> 2) * 256, slds + (S::ONCE ? (t >> 2) & 1 : buf) * (S::SU * 1024) + u * 1024);
     }
   };
+  // Waits for stage t: the copies of the stage behind it, if there is one, may
+  // stay in flight.
+  auto arrived = [&](int t) __attribute__((always_inline)) {
+    if (NS == 2) wait_copies<0>();
+    else if (t + ST < t_hi) wait_copies<S::CPW>();
+    else wait_copies<0>();
+  };
+  int buf = 0, fill = NS - 1;
+  if constexpr (S::COPIERS > 0) {
+    if (wv >= S::NW) {
+      // addresses in scalar registers (64-bit sums in every lane for each copy:
+      // 147 us instead of 136 for the packed x above with one copying wave)
+      constexpr int C = S::COPIERS, GW = S::BN / 32 / C, GX = X4 ? S::BM / 32 / C : S::XB / 1024 / C, GS = S::SU / C;
+      static_assert(GW * C * ST == S::WU && GX * C * ST == S::XU && GS * C == S::SU && S::XB % 1024 == 0, "equal shares");
+      const uint8_t *wb[GW], *xb[GX], *sb[GS];
+#pragma unroll
+      for (int i = 0; i < GW; ++i) wb[i] = a.w + (size_t)min(rn0 + cw * GW + i, wlast) * kt * 1024;
+#pragma unroll
+      for (int i = 0; i < GX; ++i)
+        xb[i] = X4 ? x + (size_t)min(rm0 + cw * GX + i, xlast) * kt * 1024 : x + (size_t)rm0 * S::XG + 1024 * (cw * GX + i);
+#pragma unroll
+      for (int i = 0; i < GS; ++i) {
+        const int gi = 4 * (cw * GS + i) + (lane >> 4);
+        sb[i] = (gi < S::BN / 32 ? wsc + (size_t)min(rn0 + gi, wlast) * ks * 256
+                                 : xsc + (size_t)min(rm0 + gi - S::BN / 32, xlast) * ks * 256) + 16 * (lane & 15);
+      }
+      auto copy_share = [&](int t, int buf) __attribute__((always_inline)) {
+        const uint32_t dst = lds + buf * ((S::WU + S::XU) * 1024);
+#pragma unroll
+        for (int q = 0; q < ST; ++q) {
+          const int tq = ST == 1 ? t : min(t + q, kt - 1);
+#pragma unroll
+          for (int i = 0; i < GW; ++i)
+            dma16u(wb[i] + (size_t)tq * 1024, 16 * lane, dst + 1024 * ((cw * GW + i) * ST + q));
+#pragma unroll
+          for (int i = 0; i < GX; ++i)
+            dma16u(xb[i] + (size_t)tq * xstep, 16 * lane,
+                   dst + 1024 * (S::WU + (X4 ? (cw * GX + i) * ST + q : q * S::XQ + cw * GX + i)));
+        }
+        if (S::ONCE && ST < 4 && (t & 3) != 0) return;
+#pragma unroll
+        for (int i = 0; i < GS; ++i)
+          dma16(sb[i] + (t >> 2) * 256, slds + (S::ONCE ? (t >> 2) & 1 : buf) * (S::SU * 1024) + (cw * GS + i) * 1024);
+      };
+      __builtin_amdgcn_s_setprio(3);
+#pragma unroll
+      for (int i = 0; i < NS - 1; ++i)
+        if (t_lo + i * ST < t_hi) copy_share(t_lo + i * ST, i);
+      // the barriers of the waves that multiply, and the copies between them
+      for (int t = t_lo; t < t_hi; t += ST) {
+        arrived(t);
+        __syncthreads();
+        if (t + (NS - 1) * ST < t_hi) copy_share(t + (NS - 1) * ST, fill);
+        fill = fill + 1 == NS ? 0 : fill + 1;
+      }
+      __syncthreads();
+      return;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NS - 1; ++i)
+      if (t_lo + i * ST < t_hi) copy(t_lo + i * ST, i);
+  }
   f32x16 acc[NF][MF];
 #pragma unroll
   for (int i = 0; i < NF; ++i)
@@ -633,19 +711,10 @@ __global__ __launch_bounds__(64 * WN * WM, OCC) void k_mx4_gemm(Mx4LinearArgs a,
     for (int j = 0; j < MF; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-#pragma unroll
-  for (int i = 0; i < NS - 1; ++i)
-    if (t_lo + i * ST < t_hi) copy(t_lo + i * ST, i);
-  int buf = 0, fill = NS - 1;
   for (int t = t_lo; t < t_hi; t += ST) {
-    // the copies that may stay in flight: those of the NS - 2 stages behind
-    // this one, as far as there are any
-    if (NS == 2) wait_copies<0>();
-    else if (t + (NS - 2) * ST < t_hi) wait_copies<(NS - 2) * S::CPW>();
-    else if (NS == 4 && t + ST < t_hi) wait_copies<S::CPW>();
-    else wait_copies<0>();
+    if (S::COPIERS == 0) arrived(t);
     __syncthreads();   // the stage has arrived for every wave, and every wave has read the one before
-    if (t + (NS - 1) * ST < t_hi) copy(t + (NS - 1) * ST, fill);
+    if (S::COPIERS == 0 && t + (NS - 1) * ST < t_hi) copy(t + (NS - 1) * ST, fill);
     fill = fill + 1 == NS ? 0 : fill + 1;
     const uint8_t* ws = stage[buf] + 16 * lane;
     const uint8_t* xs = ws + S::WU * 1024;
@@ -691,6 +760,9 @@ __global__ __launch_bounds__(64 * WN * WM, OCC) void k_mx4_gemm(Mx4LinearArgs a,
           for (int i = 0; i < NF; ++i)
             acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w[i], b, acc[i][j], kFp4, X4 ? kFp4 : kFp6, 0,
                                                                         wsv[i], 0, sx);
+          // three waves a SIMD leave 168 registers, 128 of them sums: the parts
+          // one after the other (hoisted, they spill)
+          if (S::COPIERS > 0 && P > 1) __builtin_amdgcn_sched_barrier(0);
         }
       }
     }
@@ -854,9 +926,9 @@ template <int P, bool X4, int NF, int MF, int WN, int WM, int ST, int NS, int OC
 static int launch_gemm_t(const Mx4LinearArgs& a, hipStream_t s) {
   typedef GemmShape<P, X4, NF, MF, WN, WM, ST, NS> S;
   const int64_t nbn = (a.n + S::BN - 1) / S::BN, nbm = (a.m + S::BM - 1) / S::BM;
-  if (nbn * nbm * a.kslices > 0xffffffffll / (64 * WN * WM)) return (int)hipErrorInvalidValue;   // threads of a grid
+  if (nbn * nbm * a.kslices > 0xffffffffll / S::THREADS) return (int)hipErrorInvalidValue;   // threads of a grid
   hipLaunchKernelGGL((k_mx4_gemm<P, X4, NF, MF, WN, WM, ST, NS, OCC>), dim3((unsigned)(nbn * nbm * a.kslices)),
-                     dim3(64 * WN * WM), 0, s, a, (int)nbn, (int)nbm);
+                     dim3(S::THREADS), 0, s, a, (int)nbn, (int)nbm);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.kslices == 1) return (int)e;
   hipLaunchKernelGGL(k_mx4_join, dim3((unsigned)((a.n + 1023) / 1024), (unsigned)a.m), dim3(256), 0, s, a);
