@@ -8,7 +8,10 @@
 // relative to the thread's own running maximum:
 //   m' = max(m, tile):  W' = e^(m-m') (W + (m - m') S), S' = e^(m-m') S,
 // so that partial results of any split merge the same way. All sums are f32.
-// Bound by the read of the logits.
+// Bound by the read of the logits: 1021 rows of 262144 bf16 (535 MB) with five
+// alternatives take 101 us, 5.3 TB/s. One row of f32 is split over 129 blocks
+// (7.9 us) and joined by a second kernel (5.8 us): two chains of latencies, for
+// 0.2 us of reading.
 //
 // Best alternatives: a candidate is a 64-bit key, the logit as an ordered
 // integer over the complemented index, so that the largest key is the largest
