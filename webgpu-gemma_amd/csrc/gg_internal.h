@@ -525,14 +525,15 @@ struct Mx4Tile {
 // Least-squares fits of 5,400 timings (310 products of 1 to 4096 rows, 72 to
 // 250200 features and k of 65 to 8192, each tile, 1 to 16 slices): 11% rms for
 // parts, 8% for packed x; the choice costs 1.8% and 3.5% over the best of all.
-// 256 x 256 has become faster since by what its rates for full CUs say.
+// 256 x 256 and 128 x 64 have since become faster; their rates for full CUs are
+// scaled by what that measured.
 constexpr Mx4Tile kMx4PartTiles[MT_COUNT] = {{256, 256, .15f, .05f, 2.f, .006f, .304f, 12.1f},
                                              {256, 64, .127f, .094f, 4.6f, .052f, .097f, 3.1f},
                                              {},
                                              {128, 32, .222f, .005f, 1.3f, .078f, .020f, 1.4f}};
 constexpr Mx4Tile kMx4PackedTiles[MT_COUNT] = {{256, 256, .205f, 0.f, 2.4f, .391f, 0.f, 8.1f},
                                                {},
-                                               {128, 64, .114f, 0.f, 1.6f, .097f, 0.f, 1.2f},
+                                               {128, 64, .114f, 0.f, 1.6f, .089f, 0.f, 1.2f},
                                                {128, 32, .040f, 0.f, .95f, .065f, 0.f, 1.1f}};
 constexpr int kMx4MaxSlices = 16;
 constexpr int64_t kMx4MaxSums = 1 << 24;   // f32 sums that slices may leave

@@ -525,8 +525,10 @@ __global__ __launch_bounds__(64 * kMxGemvWaves) void k_mx4_gemv(Mx4LinearArgs a,
 // waves only copy, so that the others' matrix instructions do not queue behind
 // a stage's 44 to 72 copies: 4096 x 8192 x 8192 with both operands packed 140 ->
 // 129 us, bf16 x 388 -> 368, f32 x 656 -> 603 (with one copying wave, which
-// cannot start them fast enough, 136 and 412; with two 127, 369 and 606). In the
-// smaller tiles the waves share the copies.
+// cannot start them fast enough, 136 and 412; with two 127, 369 and 606). In
+// 128 x 64 blocks two do (packed x, 300 x 8192 x 4096 15.6 -> 14.1 us, 187 x 13824
+// x 1152 8.2 -> 7.7). In the others, where it gains nothing (256 x 64) or the
+// stages are short (128 x 32), the waves share the copies.
 // With more than two stages every copying wave starts the same number (CPW) in
 // every stage, so that the number in flight tells which stage has arrived.
 // Bound by the matrix units and their power. A loop on registers reaches 6.4
@@ -545,7 +547,7 @@ struct GemmShape {
   static constexpr int XB = BM / 32 * XG;                      // bytes of a k group's x,
   static constexpr int XQ = (XB + 1023) / 1024, XU = XQ * ST;  // units of it and of a stage's,
   static constexpr int GN = (BN + BM) / 32, SU = (GN + 3) / 4; // and of the row groups' scale dwords
-  static constexpr int COPIERS = NF * MF >= 8 ? 4 : 0;               // waves that only copy
+  static constexpr int COPIERS = NF * MF >= 8 ? 4 : NF * MF == 2 ? 2 : 0;   // waves that only copy
   static constexpr int THREADS = 64 * (NW + COPIERS), CW = COPIERS ? COPIERS : NW;
   static constexpr int CPW = (WU + CW - 1) / CW + (XU + CW - 1) / CW + (SU + CW - 1) / CW;
   static_assert(ST == 4 || ST == 2 || ST == 1, "a stage lies within four k groups, whose scale bytes are one dword");
