@@ -533,8 +533,8 @@ __global__ __launch_bounds__(64 * kMxGemvWaves) void k_mx4_gemv(Mx4LinearArgs a,
 // every stage, so that the number in flight tells which stage has arrived.
 // Bound by the matrix units and their power. A loop on registers reaches 6.4
 // PFLOP/s for 4-bit x and 5.9 for 6-bit parts on random operands (9.5 on constant
-// ones: the clock falls to 1.6 GHz), 256 x 256 blocks 4.4 (4096 x 8192 x 8192,
-// packed x, 126 us) and 4.6 (4000 rows, three parts, 354 us), of which 16 us are
+// ones: the clock falls to 1.6 GHz), 256 x 256 blocks 4.5 (4096 x 8192 x 8192,
+// packed x, 123 us) and 4.7 (4000 rows, three parts, 345 us), of which 16 us are
 // each block's start and the store of its results. 16 x 16 x 128 instructions reach
 // 4.6. Blocks of half the size, two to a CU, and more stages measured no faster;
 // waves of 128 x 128 spill.
