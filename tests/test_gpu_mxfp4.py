@@ -293,3 +293,25 @@ def test_round_trip_of_many_rows(gpu):
     for lo in range(0, rows, 1 << 26):
         part = out[lo:lo + (1 << 26)]
         assert torch.equal(part, kept[src[lo:lo + (1 << 26)].long()])
+
+
+@pytest.mark.parametrize("x_name,y_name", [("f32", "f32"), ("f16", "f16"), ("bf16", "bf16"), ("bf16", "f32"), ("mxfp4", "f32")])
+def test_linear_large(gpu, x_name, y_name):
+    """Sizes of the largest blocks, ragged at each edge; rows of the first, inner and last blocks are checked."""
+    m, n, k = 2500, 8300, 6020
+    say("large", x_name, y_name)
+    rng = np.random.default_rng(77)
+    wp, _ = pack(rng.standard_normal((n, k)) * 0.02)
+    w = unpack(wp, n, k)[:-4].reshape(n, k).astype(np.float64)
+    x = np.clip(sample(rng, m, k), -200, 200)
+    pick = np.r_[0:24, 244:268, 1500:1510, m - 40:m]
+    if x_name == "mxfp4":
+        xp, xk = pack(x)
+        xk = quantised(xk[pick])
+        got = linear(wp, xp.data_ptr(), MX, 0, m, n, k, y_name)
+    else:
+        buf, ptr, xk = rows_of(x, x_name, k)
+        xk = xk[pick]
+        got = linear(wp, ptr, TYPES[x_name][0], k, m, n, k, y_name)
+    want = xk @ w.T
+    assert (np.abs(got[pick] - want) <= product_bound(xk, w, want, None if x_name == "mxfp4" else x_name, y_name)).all()
