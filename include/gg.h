@@ -316,10 +316,9 @@ int gg_mxfp4_dequant(const void* packed, float* out, int64_t rows, int64_t k, in
 
 /* y[m][rows] = x[m][k] W[rows][k]^T with W packed, sums in f32, rounded once to
  * y_type (GG_TYPE_F32 / F16 / BF16). x_type GG_TYPE_MXFP4: x is packed too (m
- * rows; ldx is not read). GG_TYPE_F32 / F16 / BF16: rows of x ldx >= k apart;
- * of every 32-block of x, 2^-24 of its largest magnitude (of 2^-106 where that
- * is smaller) is kept for f32 y, 2^-19 for f16 y (2^-14 of bf16 x), 2^-14 for
- * bf16 y, finer than the result's rounding. A row of x with an infinity or a
+ * rows; ldx is not read). GG_TYPE_F32 / F16 / BF16: rows of x ldx >= k apart,
+ * each value with all its bits, whatever y_type is (of an f32 below 2^-110,
+ * what lies under 2^-133 is cut off). A row of x with an infinity or a
  * NaN gives NaN. Rows of y are ldy >= rows apart; what
  * lies between them is left alone. y overlaps neither operand.
  * workspace: gg_mxfp4_linear_workspace_size() device bytes, 16-byte aligned

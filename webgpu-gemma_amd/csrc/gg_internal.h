@@ -450,32 +450,22 @@ __host__ __device__ inline Mx4Layout mx4_layout(int64_t rows, int64_t k) {
   return Mx4Layout{(rows + 31) / 32, kt, (kt + 3) / 4};
 }
 
-// Activations of a product as P parts: with 2^e the power of two at or below
-// the largest magnitude of a 32-block, x / 2^e = sum_p d_p 2^(-3 - 5 p) + r,
-// d_p whole numbers in [-16, 16], |r| <= 2^(-4 - 5 (P - 1)). d_p / 8 is an
-// e2m3 (6-bit) value, exactly, so part p is a 6-bit MX block of scale
-// 2^(e - 5 p) and the matrix instruction multiplies it by the 4-bit weights
-// without another rounding. Parts by what the result can show: a bf16 result
-// keeps 8 bits and takes 3 parts (2^-14 of the block's maximum), an f16 result
-// 11 and takes 4 (3 from bf16, whose own 8 bits they hold), an f32 result takes
-// 5 (2^-24, as f32 itself; 4 parts of 16-bit inputs with outliers in a block
-// left errors of 1.5e-6 where f32 products of the same inputs leave 2e-8).
-__host__ __device__ inline int mx_parts(int x_elem, int y_elem) {
-  if (y_elem == ELEM_BF16) return 3;
-  if (y_elem == ELEM_F16) return x_elem == ELEM_BF16 ? 3 : 4;
-  return 5;
-}
-constexpr int kMxMaxParts = 5;
-constexpr int kMxPartBytes = 1536;   // 32 rows x 64 k of one part: 16 bytes a lane, then 8 bytes a lane
+// Activations of a product in parts: a part is the upper 16 bits of an f32, a
+// bf16 towards zero, the next one that of what is left, so that an element
+// keeps its own 8 bits in each, whatever stands beside it: bf16 x is its one
+// part, f16 (11 bits) has two and f32 (24) three, and the products of parts and
+// weights are exact in f32. What an f32 below 2^-110 has under 2^-133, the last
+// bit of bf16, is cut off. (Parts of fixed steps below the largest of 32
+// elements fit the faster 6-bit matrix instruction, but lose an element's bits
+// beside a much larger one: with a zero weight at that one the sum has nothing else.)
+__host__ __device__ constexpr int mx_parts(int x_elem) { return x_elem == ELEM_F32 ? 3 : x_elem == ELEM_F16 ? 2 : 1; }
+constexpr int kMxPartBytes = 4096;   // 32 rows x 64 k of one part: four 16-byte quarters of a 32-block, each for 64 lanes
 constexpr int kMxPadGroups = 7;      // row groups that a block of a product may read past the last
-// Workspace of m x k activations in parts: [k group][row group][part][1536]
-// and the padding, then the scale bytes of part 0 as in Mx4Layout.
-__host__ __device__ inline size_t mx_codes_bytes(int64_t rt, int kt, int parts) {
-  return ((size_t)rt * kt + kMxPadGroups) * parts * kMxPartBytes;
-}
+// Workspace of m x k activations in parts: [k group][part][row group][4096] and
+// the padding.
 inline size_t mx_parts_bytes(int64_t m, int64_t k, int parts) {
   const Mx4Layout L = mx4_layout(m, k);
-  return mx_codes_bytes(L.rt, L.kt, parts) + (size_t)L.rt * L.ks * 256;
+  return ((size_t)L.rt * L.kt * parts + kMxPadGroups) * kMxPartBytes;
 }
 
 struct Mx4LinearArgs {
@@ -490,51 +480,46 @@ struct Mx4LinearArgs {
   void* y;
   int64_t ldy;
   int y_elem;
-  int parts;
+  int parts;             // of x, 1 for packed
   int y_vec;             // rows of y are 16-byte aligned
   int kslices;           // k slices of the many-row kernel; above 1 they leave
   float* partial;        // f32 sums [kslices][m][ldp] that k_mx4_join adds
   int64_t ldp;
 };
-// A product with m rows and `parts` parts takes the few-row kernel when it has
-// a column of its matrix instructions for each part of each row, LDS holds them
-// (32 bytes of each 32-block's part) and the sums, and x has no more than 648
-// 32-blocks, since every block of the kernel makes all parts. us against the
-// many-row kernel: 2 x 1152 x 6912 (432 32-blocks) 12.0 / 15.5, 4 x 16384 x
-// 4096 (512) 15.9 / 19.2, 3 x 1152 x 6912 (648) 14.8 / 15.7; 4 x 1152 x 6912
-// (864) 16.7 / 15.9, 8 x 4096 x 4096 bf16 (1024) 15.9 / 13.4.
-constexpr int kMxGemvCols = 64, kMxGemvWaves = 8, kMxGemvBlocks = 648;
+// A product takes the few-row kernel up to 22 rows, where it has a column of
+// its matrix instructions for each part of each row and LDS holds them (64 bytes
+// of each 32-block's part) and the sums. Over 220 products of 1 to 64 rows,
+// each both ways, this costs 0.9% over the better of the two (0.7% below 20000
+// features, 1.6% above); up to 16 rows 1.2%, up to 32 rows 1.7%. us, few-row / many-row: 1 x 5493 -> 1140
+// f32 9.4 / 17.9, 11 x 1458 -> 138455 f32 49 / 65, 13 x 1507 -> 9044 f16 14.6 / 15.1, 23 x
+// 1024 -> 127133 bf16 29.4 / 26.0, 29 x 852 -> 61810 bf16 20.2 / 15.1.
+constexpr int kMxGemvRows = 22, kMxGemvCols = 64, kMxGemvWaves = 8;
 __host__ __device__ constexpr size_t mx_gemv_sums(int col_tiles) {   // f32 [wave][16][16 col_tiles + 1]
   return (size_t)kMxGemvWaves * 16 * (16 * col_tiles + 1) * 4;
 }
 inline size_t mx_gemv_lds(int cols, int k) {
-  return mx_gemv_sums((cols + 15) / 16) + (size_t)((k + 127) / 128 * 4) * cols * 32;
+  return mx_gemv_sums((cols + 15) / 16) + (size_t)((k + 127) / 128 * 4) * cols * 64;
 }
 inline bool mx_gemv_fits(int64_t m, int parts, int64_t k) {
-  return m * parts <= kMxGemvCols && m * ((k + 127) / 128 * 4) <= kMxGemvBlocks &&
-         mx_gemv_lds((int)m * parts, (int)k) <= 160 * 1024;
+  return m <= kMxGemvRows && m * parts <= kMxGemvCols && mx_gemv_lds((int)m * parts, (int)k) <= 160 * 1024;
 }
 // Tiles of the many-row kernel (features x rows) and slices of k.
 enum Mx4TileId { MT_256x256, MT_256x64, MT_128x64, MT_128x32, MT_COUNT };
 struct Mx4Tile {
   int bn, bm;
-  // us: a 64-deep step of a block alone on a CU (with parts: + for each), its
-  // start and end; the same for each block when the CUs are full
-  float lat, lat_part, lat_end, thr, thr_part, thr_end;
+  // us: a step of a block alone on a CU (64 k of one part), its start and end;
+  // the same for each block when the CUs are full
+  float lat, lat_end, thr, thr_end;
 };
-// Least-squares fits of 5,400 timings (310 products of 1 to 4096 rows, 72 to
-// 250200 features and k of 65 to 8192, each tile, 1 to 16 slices): 11% rms for
-// parts, 8% for packed x; the choice costs 1.8% and 3.5% over the best of all.
-// 256 x 256 and 128 x 64 have since become faster; their rates for full CUs are
-// scaled by what that measured.
-constexpr Mx4Tile kMx4PartTiles[MT_COUNT] = {{256, 256, .15f, .05f, 2.f, .006f, .304f, 12.1f},
-                                             {256, 64, .127f, .094f, 4.6f, .052f, .097f, 3.1f},
-                                             {},
-                                             {128, 32, .222f, .005f, 1.3f, .078f, .020f, 1.4f}};
-constexpr Mx4Tile kMx4PackedTiles[MT_COUNT] = {{256, 256, .205f, 0.f, 2.4f, .391f, 0.f, 8.1f},
-                                               {},
-                                               {128, 64, .114f, 0.f, 1.6f, .089f, 0.f, 1.2f},
-                                               {128, 32, .040f, 0.f, .95f, .065f, 0.f, 1.1f}};
+// Least-squares fits of 4,200 timings of the present kernels (270 products of 1
+// to 4096 rows, 64 to 262144 features and k of 64 to 8192 and 200 of few rows,
+// each tile, 1 to 16 slices): 10% rms for parts, 9% for packed x; the choice costs
+// 0.5% and 2.1% over the best of them. A 256 x 256 block is never bound by its
+// own latency. 256 x 128 and 128 x 64 tiles for parts would gain 0.3%.
+constexpr Mx4Tile kMx4PartTiles[MT_COUNT] = {
+    {256, 256, 1.122f, 13.2f, 1.122f, 13.2f}, {256, 64, .481f, 2.5f, .349f, 1.6f}, {}, {128, 32, .241f, 0.f, .142f, .65f}};
+constexpr Mx4Tile kMx4PackedTiles[MT_COUNT] = {
+    {256, 256, .330f, 11.2f, .330f, 11.2f}, {}, {128, 64, .084f, 2.3f, .111f, 1.7f}, {128, 32, .095f, .55f, .074f, 1.4f}};
 constexpr int kMx4MaxSlices = 16;
 constexpr int64_t kMx4MaxSums = 1 << 24;   // f32 sums that slices may leave
 struct Mx4Plan { int tile, slices; };
@@ -549,11 +534,10 @@ inline Mx4Plan mx4_plan(bool packed, int parts, int64_t m, int64_t n, int64_t k)
     const double blocks = (double)((n + T.bn - 1) / T.bn) * (double)((m + T.bm - 1) / T.bm);
     for (int s = 1; s <= kMx4MaxSlices && s <= ks; s += s < 4 ? 1 : s < 8 ? 2 : 4) {
       if (s > 1 && (m > 65535 || (int64_t)s * m > kMx4MaxSums / ((n + 3) / 4 * 4))) break;
-      const int slice = 4 * ((ks + s - 1) / s), steps = kt < slice ? kt : slice;
-      const double alone = steps * (T.lat + T.lat_part * parts) + T.lat_end;
-      const double full = steps * (T.thr + T.thr_part * parts) + T.thr_end;
+      const int slice = 4 * ((ks + s - 1) / s), steps = (kt < slice ? kt : slice) * parts;
+      const double alone = steps * T.lat + T.lat_end, full = steps * T.thr + T.thr_end;
       const double rounds = (double)(int64_t)((blocks * s + 255) / 256) * full;
-      const double cost = (alone > rounds ? alone : rounds) + (s > 1 ? 2.9 + 0.6e-6 * s * m * n : 0.0);
+      const double cost = (alone > rounds ? alone : rounds) + (s > 1 ? 2.8 + 1e-6 * s * m * n : 0.0);
       if (best.tile < 0 || cost < best_cost) {
         best_cost = cost;
         best = {t, s};
@@ -567,8 +551,7 @@ inline size_t mx4_sums_bytes(const Mx4Plan& p, int64_t m, int64_t n) {
 }
 int launch_mx4_quantize(int elem, const void* src, int64_t rows, int64_t k, int64_t ld, uint8_t* dst, void* stream);
 int launch_mx4_dequant(const uint8_t* src, float* out, int64_t rows, int64_t k, int64_t ld, void* stream);
-int launch_mx_split(int elem, const void* src, int64_t rows, int64_t k, int64_t ld, int parts, uint8_t* dst,
-                    void* stream);
+int launch_mx_split(int elem, const void* src, int64_t rows, int64_t k, int64_t ld, uint8_t* dst, void* stream);
 int launch_mx4_gemv(const Mx4LinearArgs& a, void* stream);
 int launch_mx4_gemm(const Mx4LinearArgs& a, bool packed, int tile, void* stream);
 

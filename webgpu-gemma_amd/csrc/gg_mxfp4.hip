@@ -12,9 +12,10 @@ namespace {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef uint32_t u32x6 __attribute__((ext_vector_type(6)));
-constexpr int kFp6 = 2, kFp4 = 4;   // operand formats of the MX matrix instructions
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+constexpr int kFp4 = 4;   // operand format of the MX matrix instructions
+template <class T>
+constexpr int kElem = __is_same(T, float) ? ELEM_F32 : __is_same(T, _Float16) ? ELEM_F16 : ELEM_BF16;
 
 // Elements [c, c + E) of a row of k elements, zeros past its end.
 template <class T, int E, bool VEC, bool NT = false>
@@ -181,84 +182,41 @@ __global__ __launch_bounds__(256) void k_mx4_dequant(const uint8_t* __restrict__
 }
 
 // ---------------------------------------------------------------------------
-// Activations in parts (mx_parts). A block of 32 with largest magnitude in
-// [2^e, 2^(e+1)): scale byte e + 127, at least 21 so that every part's is at
-// least 1, 255 when the block holds an Inf or a NaN (its row's results are
-// NaN). Part p of u = x / 2^e is what is left of u rounded to a multiple of
-// 2^(-3 - 5 p), to nearest: |u| <= 2 before part 0, 2^(-4 - 5 p) after part p.
+// Activations in parts (mx_parts): a part of a value is the upper 16 bits of
+// what is left of it in f32, a bf16 towards zero, so that no part rounds and
+// none overflows: 8 significant bits each, 24 in three. A subtraction of the
+// upper bits is exact. An infinity leaves NaN behind it; bf16 x, which has one
+// part, turns into NaN here.
 // ---------------------------------------------------------------------------
-
-// 32 values, even elements in a, odd ones in b, over scale -> their e2m3 codes,
-// element i at bit 6 i. The instruction writes its result while it still reads
-// its operands, so the result must not share their registers: that is asked
-// for here, since the builtin's result was placed over the scale (and the
-// elements behind the first two were divided by something else).
-__device__ __forceinline__ u32x6 to_fp6(const f32x16& a, const f32x16& b, float scale) {
-  u32x6 z;
-  asm("v_cvt_scalef32_2xpk16_fp6_f32 %0, %1, %2, %3\n\ts_nop 1" : "=&v"(z) : "v"(a), "v"(b), "v"(scale));
+__device__ __forceinline__ u32x4 take_part(float (&u)[8]) {
+  u32x4 z;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t a = __float_as_uint(u[2 * j]), b = __float_as_uint(u[2 * j + 1]);
+    z[j] = __builtin_amdgcn_perm(b, a, 0x07060302);
+    u[2 * j] -= __uint_as_float(a & 0xffff0000u);
+    u[2 * j + 1] -= __uint_as_float(b & 0xffff0000u);
+  }
   return z;
 }
-
-constexpr float kPartMagic = 1572864.0f;   // 1.5 2^20, whose last bit is 1/8: adding and subtracting it rounds to 1/8
-__device__ __forceinline__ int parts_byte(uint32_t amax_bits) {
-  const int ex = (int)(amax_bits >> 23);
-  return max(ex, 1 + 5 * (kMxMaxParts - 1));
+template <class T>
+__device__ __forceinline__ void inf_to_nan(float (&u)[8]) {
+  if constexpr (__is_same(T, __bf16)) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) u[j] = __builtin_fabsf(u[j]) == INFINITY ? NAN : u[j];
+  }
 }
-
-// A 32-block of x in a thread: its elements, even and odd ones apart as the
-// conversion takes them, and the parts one after the other.
-struct Block32 {
-  f32x16 ev, od;
-  float magic, unit;
-  __device__ __forceinline__ void load(const float* lds) {   // 16-byte aligned
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const f32x4 t = *(const f32x4*)(lds + 4 * i);
-      ev[2 * i] = t[0];
-      od[2 * i] = t[1];
-      ev[2 * i + 1] = t[2];
-      od[2 * i + 1] = t[3];
-    }
-  }
-  // the scale byte; the elements become x / 2^e
-  __device__ __forceinline__ int scale() {
-    uint32_t a = 0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      a = max(a, max(__float_as_uint(ev[i]) & 0x7fffffffu, __float_as_uint(od[i]) & 0x7fffffffu));
-    const int byte = parts_byte(a);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      ev[i] = ldexpf(ev[i], 127 - byte);
-      od[i] = ldexpf(od[i], 127 - byte);
-    }
-    return byte;
-  }
-  __device__ __forceinline__ u32x6 part(bool first) {
-    magic = first ? kPartMagic : magic * 0.03125f;
-    unit = first ? 1.f : unit * 0.03125f;
-    f32x16 qe, qo;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      qe[i] = (ev[i] + magic) - magic;
-      qo[i] = (od[i] + magic) - magic;
-      ev[i] -= qe[i];
-      od[i] -= qo[i];
-    }
-    return to_fp6(qe, qo, unit);
-  }
-};
 
 // A wave takes 32 rows x 64 k, a thread one 32-block of them. The rows come in
 // whole lines, four elements a lane (one where their addresses are odd), and
 // change lanes in LDS; a pitch of 68 floats puts the 16 lanes of a read on
-// different banks. Bound by memory for long x (reads 4 or 2 bytes, writes
-// 3/4 byte a part and element; 4000 x 8192 bf16 in three parts, 139 MB: 29 us,
-// 4.7 TB/s), by its latency for short.
+// different banks. Bound by memory for long x (reads 4 or 2 bytes, writes 2 a
+// part and element; 4000 x 8192 bf16, 131 MB: 24 us, 5.5 TB/s), by its latency for
+// short (2048 x 1152 f32, 24 MB: 8 us).
 template <class T, bool VEC>
 __global__ __launch_bounds__(64) void k_mx_split(const T* __restrict__ src, int64_t rows, int64_t k, int64_t ld,
-                                                 int parts, uint8_t* __restrict__ dst, Mx4Layout L) {
-  constexpr int PITCH = 68;
+                                                 uint8_t* __restrict__ dst, Mx4Layout L) {
+  constexpr int PITCH = 68, P = mx_parts(kElem<T>);
   __shared__ __align__(16) float xs[32 * PITCH];
   const int lane = threadIdx.x;
   const int64_t R = blockIdx.x;
@@ -285,16 +243,27 @@ __global__ __launch_bounds__(64) void k_mx_split(const T* __restrict__ src, int6
     for (int i = 0; i < 32; ++i) xs[i * PITCH + lane] = v[i];
   }
   __syncthreads();
-  Block32 v;
-  v.load(xs + (lane & 31) * PITCH + 32 * (lane >> 5));
-  dst[mx_codes_bytes(L.rt, L.kt, parts) + ((size_t)R * L.ks + (t >> 2)) * 256 + 4 * lane + (t & 3)] = (uint8_t)v.scale();
-  uint8_t* out = dst + ((size_t)t * L.rt + R) * parts * kMxPartBytes;
-  for (int p = 0; p < parts; ++p, out += kMxPartBytes) {
-    const u32x6 z = v.part(p == 0);
-    *(u32x4*)(out + 16 * lane) = u32x4{z[0], z[1], z[2], z[3]};
-    *(u32x2*)(out + 1024 + 8 * lane) = u32x2{z[4], z[5]};
+  const float* mine = xs + (lane & 31) * PITCH + 32 * (lane >> 5);
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    const f32x4 lo = *(const f32x4*)(mine + 8 * s), hi = *(const f32x4*)(mine + 8 * s + 4);
+    float u[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    inf_to_nan<T>(u);
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+      *(u32x4*)(dst + (((size_t)t * P + p) * L.rt + R) * kMxPartBytes + 1024 * s + 16 * lane) = take_part(u);
   }
 }
+
+// Eight consecutive 4-bit weights in bf16: element times the power of two, exactly (bf16 holds what is
+// denormal there too, and the matrix instruction takes it), NaN where the scale is the one of byte 255.
+__device__ __forceinline__ bf16x8 expand8(uint32_t q, float scale) {
+  const auto a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, scale, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, scale, 1),
+             c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, scale, 2), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, scale, 3);
+  return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+// The factor of a scale byte as the conversion reads it, from its exponent field: 0 is 2^-127 there.
+__device__ __forceinline__ float scale_of(int byte) { return __uint_as_float((uint32_t)byte << 23); }
 
 template <class T>
 __device__ __forceinline__ void store_y(void* y, int64_t i, float v) { ((T*)y)[i] = (T)v; }
@@ -342,28 +311,31 @@ __device__ __forceinline__ void store_tile(int elem, void* y, int64_t ldy, int64
 }
 
 // ---------------------------------------------------------------------------
-// Few rows: m x parts columns in NC tiles of the 16 x 16 x 128 matrix
-// instruction, column r parts + p holding part p of row r, so that one
-// instruction multiplies 16 weight rows x 128 k by 16 of them at once; the sum
-// over the parts is taken once, at the end, in f32. One block a CU makes the
+// Few rows: m x parts columns in NC tiles of the 16 x 16 x 32 bf16 matrix
+// instruction, column r parts + p holding part p of row r, so that four of them
+// multiply 16 weight rows x 128 k by 16 columns; the weights are expanded to
+// bf16 on the way, and the sum over the parts is taken once, at the end, in
+// f32. One block a CU makes the
 // parts in its LDS (one launch, no workspace) and goes over its share of the
 // weights, which travel from memory to registers, kGemvAhead KB ahead in each
 // wave. A wave takes 16 weight rows; `kw` waves of a block share their k.
-// Bound by the read of the weights (17/32 byte each): 262144 x 1152 f32 27 us,
-// 6.0 TB/s. A small product by its chain of x, parts, weights, sums: 1536 x 1152
-// 5.5 us and 1152 x 6912 8.2 us, an empty kernel 1.3.
+// Bound by the read of the weights (17/32 byte each): 262144 x 1152 f32 28 us,
+// 5.8 TB/s (30 to 32 with the addresses of a step computed from the row and k
+// indices each time; 12 KB ahead spill). A small product by its chain of x,
+// parts, weights, sums: 1 row, 1536 x 1152 4.8 us and 1152 x 6912 6.2 us, 7 rows of
+// 13824 x 1152 6.9 us, an empty kernel 1.3.
 // ---------------------------------------------------------------------------
 constexpr int kGemvAhead = 8;
-constexpr int kGemvRec = 32;         // bytes of a 32-block's part: 24 of elements, the scale byte, 7 unused
 
 template <class T, int NC>
 __global__ __launch_bounds__(64 * kMxGemvWaves) void k_mx4_gemv(Mx4LinearArgs a, int kw) {
   constexpr int RP = 16 * NC + 1;
   extern __shared__ f32x4 gemv_lds[];
   float* red = (float*)gemv_lds;                                       // the waves' sums
-  uint8_t* rec = (uint8_t*)gemv_lds + mx_gemv_sums(NC);                // the parts
+  uint8_t* rec = (uint8_t*)gemv_lds + mx_gemv_sums(NC);                // the parts: [32-block][quarter][column][16 bytes]
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int nb = (a.k + 127) / 128 * 4, P = a.parts, cols = (int)a.m * P;
+  constexpr int P = mx_parts(kElem<T>);
+  const int nb = (a.k + 127) / 128 * 4, cols = (int)a.m * P;
   const int gb = kMxGemvWaves / kw, slot = wv / kw, kz = wv % kw;
   const int steps = nb / 4, ns = (steps + kw - 1) / kw, s0 = kz * ns;   // this wave's steps [s0, s0 + ns), as far as they exist
   const int g = lane >> 4, c16 = lane & 15;
@@ -376,38 +348,43 @@ __global__ __launch_bounds__(64 * kMxGemvWaves) void k_mx4_gemv(Mx4LinearArgs a,
   int wsr[kGemvAhead];
   int64_t lbase = (int64_t)blockIdx.x * gb;
   int ls = 0;
-  auto issue = [&](int r) __attribute__((always_inline)) {
-    // reads past the end repeat the last row group or k group: past the k
-    // groups x is zero (the last step's second tile) or the step is not used
+  const uint8_t *wp, *sp;
+  auto row_group = [&]() __attribute__((always_inline)) {
+    // reads past the end repeat the last row group
     const int64_t q = min(lbase + slot, groups - 1), R = q >> 1;
     const int in = 32 * (g & 1) + 16 * (int)(q & 1) + c16;
-    const int t = min(2 * (s0 + ls) + (g >> 1), kt - 1);
-    wr[r] = __builtin_nontemporal_load((const u32x4*)(a.w + ((size_t)R * kt + t) * 1024 + 16 * in));
-    wsr[r] = wsc[((size_t)R * ks + (t >> 2)) * 256 + 4 * in + (t & 3)];
+    wp = a.w + (size_t)R * kt * 1024 + 16 * in;
+    sp = wsc + (size_t)R * ks * 256 + 4 * in;
+  };
+  row_group();
+  const int t0 = 2 * s0 + (g >> 1);
+  auto issue = [&](int r) __attribute__((always_inline)) {
+    // or the last k group: past the k groups x is zero (the last step's second
+    // tile) or the step is not used
+    const int t = min(t0 + 2 * ls, kt - 1);
+    wr[r] = __builtin_nontemporal_load((const u32x4*)(wp + (size_t)t * 1024));
+    wsr[r] = sp[(t >> 2) * 256 + (t & 3)];
     if (++ls == ns) {
       ls = 0;
       lbase += (int64_t)gridDim.x * gb;
+      row_group();
     }
   };
 
-  // The parts: four lanes to a 32-block, eight elements each, the low 48 bits
-  // of a conversion. Loads return in order, so x is asked for before the
-  // weights are.
+  // The parts: four lanes to a 32-block, eight elements each. Loads return in
+  // order, so x is asked for before the weights are.
   {
     const T* x = (const T*)a.x;
-    const int items = (int)a.m * nb, unit = lane & 3;
+    const int items = (int)a.m * nb, unit = tid & 3;
     const bool vec = ((uintptr_t)x % (4 * sizeof(T))) == 0 && a.ldx % 4 == 0;
-    f32x16 qe, qo;
-#pragma unroll
-    for (int j = 4; j < 16; ++j) qe[j] = qo[j] = 0.f;
     for (int i0 = 0; i0 < items; i0 += kMxGemvWaves * 16) {
       const int it = i0 + (tid >> 2), ic = min(it, items - 1), r = ic / nb, kb = ic - r * nb;
       const int64_t c = (int64_t)kb * 32 + 8 * unit;
-      float u[2][4];
+      float h[2][4];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (vec) load4<T, true>(x + r * a.ldx, c + 4 * h, a.k, u[h]);
-        else load4<T, false>(x + r * a.ldx, c + 4 * h, a.k, u[h]);
+      for (int q = 0; q < 2; ++q) {
+        if (vec) load4<T, true>(x + r * a.ldx, c + 4 * q, a.k, h[q]);
+        else load4<T, false>(x + r * a.ldx, c + 4 * q, a.k, h[q]);
       }
       __builtin_amdgcn_sched_barrier(0);
       if (i0 == 0) {
@@ -415,48 +392,22 @@ __global__ __launch_bounds__(64 * kMxGemvWaves) void k_mx4_gemv(Mx4LinearArgs a,
         for (int q = 0; q < kGemvAhead; ++q) issue(q);
       }
       __builtin_amdgcn_sched_barrier(0);
-      uint32_t mx = 0;
+      float u[8] = {h[0][0], h[0][1], h[0][2], h[0][3], h[1][0], h[1][1], h[1][2], h[1][3]};
+      inf_to_nan<T>(u);
+      uint8_t* d = rec + ((size_t)(4 * kb + unit) * cols + r * P) * 16;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) mx = max(mx, __float_as_uint(u[j >> 2][j & 3]) & 0x7fffffffu);
-      mx = max(mx, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)mx, 0xB1, 0xf, 0xf, false));
-      mx = max(mx, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)mx, 0x4E, 0xf, 0xf, false));
-      const int byte = parts_byte(mx);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) u[j >> 2][j & 3] = ldexpf(u[j >> 2][j & 3], 127 - byte);
-      float magic = kPartMagic, scale = 1.f;
-      uint8_t* d = rec + ((size_t)kb * cols + r * P) * kGemvRec;
       for (int p = 0; p < P; ++p) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float &e = u[j >> 1][2 * (j & 1)], &o = u[j >> 1][2 * (j & 1) + 1];
-          qe[j] = (e + magic) - magic;
-          qo[j] = (o + magic) - magic;
-          e -= qe[j];
-          o -= qo[j];
-        }
-        const u32x6 z = to_fp6(qe, qo, scale);
-        // two lanes' 48 bits are three dwords: the first lane's low one, its
-        // high half with its neighbour's low half, the neighbour's rest
-        const uint32_t nz = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)z[0], 0xB1, 0xf, 0xf, false);
-        uint32_t* dw = (uint32_t*)(d + 12 * (unit >> 1));
-        if (it < items) {
-          dw[2 * (unit & 1)] = unit & 1 ? (z[0] >> 16) | (z[1] << 16) : z[0];
-          if ((unit & 1) == 0) dw[1] = (z[1] & 0xffffu) | (nz << 16);
-          else if (unit == 3) *(uint32_t*)(d + 24) = byte == 255 ? 255 : byte - 5 * p;
-        }
-        d += kGemvRec;
-        magic *= 0.03125f;
-        scale *= 0.03125f;
+        const u32x4 z = take_part(u);
+        if (it < items) *(u32x4*)(d + 16 * p) = z;
       }
     }
   }
   __syncthreads();
   const int64_t iters = (groups + (int64_t)gridDim.x * gb - 1) / ((int64_t)gridDim.x * gb);
   const int64_t total = iters * ns;
-  const uint8_t* xr[NC];   // this lane's records of the wave's next step
+  const uint8_t* xr[NC];   // this lane's part of the wave's first step
 #pragma unroll
-  for (int c = 0; c < NC; ++c)
-    xr[c] = rec + ((size_t)(4 * s0 + g) * cols + min(16 * c + c16, cols - 1)) * kGemvRec;
+  for (int c = 0; c < NC; ++c) xr[c] = rec + ((size_t)(4 * s0 + g) * 4 * cols + min(16 * c + c16, cols - 1)) * 16;
   f32x4 acc[NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -467,17 +418,15 @@ __global__ __launch_bounds__(64 * kMxGemvWaves) void k_mx4_gemv(Mx4LinearArgs a,
     for (int r = 0; r < kGemvAhead; ++r) {
       if (i + r >= total) break;
       if (s0 + s < steps) {
-        const i32x8 wa = {(int)wr[r][0], (int)wr[r][1], (int)wr[r][2], (int)wr[r][3], 0, 0, 0, 0};
-        u32x4 x0[NC], x1[NC];
+        const float scale = scale_of(wsr[r]);
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          x0[c] = *(const u32x4*)(xr[c] + (size_t)s * 4 * cols * kGemvRec);
-          x1[c] = *(const u32x4*)(xr[c] + (size_t)s * 4 * cols * kGemvRec + 16);
-        }
+        for (int e = 0; e < 4; ++e) {
+          const bf16x8 w = expand8(wr[r][e], scale);
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          const i32x8 xb = {(int)x0[c][0], (int)x0[c][1], (int)x0[c][2], (int)x0[c][3], (int)x1[c][0], (int)x1[c][1], 0, 0};
-          acc[c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wa, xb, acc[c], kFp4, kFp6, 0, wsr[r], 0, (int)x1[c][2]);
+          for (int c = 0; c < NC; ++c) {
+            const u32x4 x = *(const u32x4*)(xr[c] + (size_t)(16 * s + e) * cols * 16);
+            acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, __builtin_bit_cast(bf16x8, x), acc[c], 0, 0, 0);
+          }
         }
       }
       issue(r);
@@ -498,11 +447,9 @@ __global__ __launch_bounds__(64 * kMxGemvWaves) void k_mx4_gemv(Mx4LinearArgs a,
         const int o = o0 + tid / kw, oc = min(o, outs - 1);
         const int row = oc & 15, sl = (oc >> 4) & (gb - 1), mr = oc / (16 * gb);
         const float* q = red + ((sl * kw + z) * 16 + row) * RP + mr * P;
-        float t[kMxMaxParts], v = 0.f;
+        float v = q[P - 1];
 #pragma unroll
-        for (int p = 0; p < kMxMaxParts; ++p) t[p] = q[min(p, P - 1)];
-#pragma unroll
-        for (int p = kMxMaxParts - 1; p >= 0; --p) v += p < P ? t[p] : 0.f;
+        for (int p = P - 2; p >= 0; --p) v += q[p];
         if (kw >= 2) v += dpp_mov<0xB1>(v);
         if (kw >= 4) v += dpp_mov<0x4E>(v);
         if (kw >= 8) v += dpp_mov<0x141>(v);
@@ -516,41 +463,47 @@ __global__ __launch_bounds__(64 * kMxGemvWaves) void k_mx4_gemv(Mx4LinearArgs a,
 }
 
 // ---------------------------------------------------------------------------
-// Many rows: 32 x 32 x 64 matrix instructions, weights as the first operand
-// (rows of the result), x as the second; a block computes BN features of BM
-// rows over one slice of k, a wave NF x MF instruction tiles of it.
-// The operands lie in memory in operand order, so a stage (ST groups of 64 k)
-// goes to LDS as it is, by DMA, 1 KB an instruction, NS - 1 stages ahead of
-// the one that is multiplied; one barrier a stage. In the largest tile four
-// waves only copy, so that the others' matrix instructions do not queue behind
-// a stage's 44 to 72 copies: 4096 x 8192 x 8192 with both operands packed 140 ->
-// 129 us, bf16 x 388 -> 368, f32 x 656 -> 603 (with one copying wave, which
-// cannot start them fast enough, 136 and 412; with two 127, 369 and 606). In
-// 128 x 64 blocks two do (packed x, 300 x 8192 x 4096 15.6 -> 14.1 us, 187 x 13824
-// x 1152 8.2 -> 7.7). In the others, where it gains nothing (256 x 64) or the
-// stages are short (128 x 32), the waves share the copies.
+// Many rows: weights as the first operand (rows of the result), x as the
+// second; a block computes BN features of BM rows over one slice of k, a wave
+// NF x MF tiles of 32 x 32. Packed x goes with the weights as they are through the
+// 32 x 32 x 64 MX instruction; parts of x through 32 x 32 x 16 bf16 ones, for which a
+// wave expands its weights, eight a lane before each (a conversion makes two
+// in 5 cycles, an instruction takes 32). The parts of a k group are further steps
+// of the same sums.
+// The operands lie in memory in operand order, so a stage (ST steps) goes to
+// LDS as it is, by DMA, 1 KB an instruction, NS - 1 stages ahead of the one
+// that is multiplied; one barrier a stage. In the largest tile of packed x
+// four waves only copy, so that the others' matrix instructions do not queue
+// behind a stage's 72 copies: 4096 x 8192 x 8192 140 -> 129 us (with one copying
+// wave, which cannot start them fast enough, 136; with two 127). In 128 x 64
+// blocks two do (300 x 8192 x 4096 15.6 -> 14.1 us, 187 x 13824 x 1152 8.2 -> 7.7). In the
+// others, whose stages are short (128 x 32) or long in cycles (parts), the waves
+// share the copies.
 // With more than two stages every copying wave starts the same number (CPW) in
 // every stage, so that the number in flight tells which stage has arrived.
-// Bound by the matrix units and their power. A loop on registers reaches 6.4
-// PFLOP/s for 4-bit x and 5.9 for 6-bit parts on random operands (9.5 on constant
-// ones: the clock falls to 1.6 GHz), 256 x 256 blocks 4.5 (4096 x 8192 x 8192,
-// packed x, 123 us) and 4.7 (4000 rows, three parts, 345 us), of which 16 us are
-// each block's start and the store of its results. 16 x 16 x 128 instructions reach
-// 4.6. Blocks of half the size, two to a CU, and more stages measured no faster;
-// waves of 128 x 128 spill.
+// Bound by the matrix units and their power. Packed x: a loop on registers
+// reaches 6.4 PFLOP/s on random operands (9.3 on constant ones: the clock
+// falls to 1.6 GHz), 256 x 256 blocks 4.2 (4096 x 8192 x 8192, 123 to 131 us from box to
+// box), of which 16 us are each block's start and the store of its results. 16 x 16 x 128
+// instructions reach 4.6 in the loop. Blocks of half the size, two to a CU, and
+// more stages measured no faster.
+// Parts: 4000 x 8192 x 8192 bf16 417 to 440 us with their making (1.2 to 1.3 PFLOP/s;
+// a bf16 library product of 8192 x 8192 x 8192 reaches 1.19), 2048 x 8192 x 8192 f32, three
+// parts, 611 us (1.35 of them). 256 x 256 blocks: waves of 64 features x 128 rows 417 us,
+// of 128 x 64 423, four of 128 x 128 456; three stages 429.
 // ---------------------------------------------------------------------------
-template <int P, bool X4, int NF, int MF, int WN, int WM, int ST, int NS>
+template <bool X4, int NF, int MF, int WN, int WM, int ST, int NS>
 struct GemmShape {
   static constexpr int BN = 32 * NF * WN, BM = 32 * MF * WM, NW = WN * WM;
-  static constexpr int XG = X4 ? 1024 : P * kMxPartBytes;      // bytes of a row group's x per k group
+  static constexpr int XG = X4 ? 1024 : kMxPartBytes;          // bytes of a row group's x in a step
   static constexpr int WU = BN / 32 * ST;                      // DMA units of a stage's weights,
-  static constexpr int XB = BM / 32 * XG;                      // bytes of a k group's x,
-  static constexpr int XQ = (XB + 1023) / 1024, XU = XQ * ST;  // units of it and of a stage's,
-  static constexpr int GN = (BN + BM) / 32, SU = (GN + 3) / 4; // and of the row groups' scale dwords
-  static constexpr int COPIERS = NF * MF >= 8 ? 4 : NF * MF == 2 ? 2 : 0;   // waves that only copy
+  static constexpr int XQ = BM / 32 * XG / 1024, XU = XQ * ST; // of a step's and a stage's x,
+  static constexpr int GN = (BN + (X4 ? BM : 0)) / 32, SU = (GN + 3) / 4;   // and of the row groups' scale dwords
+  static constexpr int COPIERS = !X4 ? 0 : NF * MF >= 8 ? 4 : NF * MF == 2 ? 2 : 0;   // waves that only copy
   static constexpr int THREADS = 64 * (NW + COPIERS), CW = COPIERS ? COPIERS : NW;
   static constexpr int CPW = (WU + CW - 1) / CW + (XU + CW - 1) / CW + (SU + CW - 1) / CW;
   static_assert(ST == 4 || ST == 2 || ST == 1, "a stage lies within four k groups, whose scale bytes are one dword");
+  static_assert(X4 || ST < 4, "the steps of a stage are looked at one by one");
   // With two stages nothing is copied twice, and the scale dwords of four k
   // groups alternate between two places; else each stage brings its own.
   static constexpr bool ONCE = NS == 2;
@@ -579,9 +532,9 @@ __device__ __forceinline__ void dma16u(const uint8_t* base, uint32_t off, uint32
 template <int N>
 __device__ __forceinline__ void wait_copies() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
-template <int P, bool X4, int NF, int MF, int WN, int WM, int ST, int NS, int OCC>
-__global__ __launch_bounds__((GemmShape<P, X4, NF, MF, WN, WM, ST, NS>::THREADS), OCC) void k_mx4_gemm(Mx4LinearArgs a, int nbn, int nbm) {
-  typedef GemmShape<P, X4, NF, MF, WN, WM, ST, NS> S;
+template <bool X4, int NF, int MF, int WN, int WM, int ST, int NS, int OCC>
+__global__ __launch_bounds__((GemmShape<X4, NF, MF, WN, WM, ST, NS>::THREADS), OCC) void k_mx4_gemm(Mx4LinearArgs a, int nbn, int nbm) {
+  typedef GemmShape<X4, NF, MF, WN, WM, ST, NS> S;
   __shared__ __align__(1024) uint8_t stage[NS][(S::WU + S::XU) * 1024];
   __shared__ __align__(1024) uint8_t sstage[S::SS][S::SU * 1024];
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -598,11 +551,14 @@ __global__ __launch_bounds__((GemmShape<P, X4, NF, MF, WN, WM, ST, NS>::THREADS)
   const int t_lo = 4 * (int)((int64_t)a.ks * kz / a.kslices), t_hi = min(4 * (int)((int64_t)a.ks * (kz + 1) / a.kslices), a.kt);
   const uint8_t* x = (const uint8_t*)a.x;
   const uint8_t* wsc = a.w + (size_t)a.wrt * a.kt * 1024;
-  const uint8_t* xsc = x + (X4 ? (size_t)a.xrt * a.kt * 1024 : mx_codes_bytes(a.xrt, a.kt, P));
+  const uint8_t* xsc = x + (size_t)a.xrt * a.kt * 1024;   // of packed x
   const int64_t rn0 = bn * (S::BN / 32), rm0 = bm * (S::BM / 32);   // first row groups
   const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)&stage[0][0];
   const uint32_t slds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)&sstage[0][0];
-  // The lanes' sources at k group 0. Row groups and k groups past the matrix
+  // A step is a k group of packed x, a part of a k group of x otherwise: step
+  // P t + p multiplies the weights of k group t by part p.
+  const int P = X4 ? 1 : a.parts, u_lo = P * t_lo, u_hi = P * t_hi;
+  // The lanes' sources at step 0. Row groups and k groups past the matrix
   // read its last ones, parts past the last row group what follows them; their
   // results are not stored, their x is not multiplied.
   constexpr int NWC = (S::WU + S::CW - 1) / S::CW, NXC = (S::XU + S::CW - 1) / S::CW, NSC = (S::SU + S::CW - 1) / S::CW;
@@ -620,8 +576,8 @@ __global__ __launch_bounds__((GemmShape<P, X4, NF, MF, WN, WM, ST, NS>::THREADS)
   for (int i = 0; i < NXC; ++i) {
     const int u = min(i * S::CW + cw, S::XU - 1);
     if constexpr (X4) xsrc[i] = x + (size_t)min(rm0 + u / ST, xlast) * kt * 1024 + 16 * lane;
-    // the block's row groups of one k group lie one after the other
-    else xsrc[i] = x + (size_t)rm0 * S::XG + min(u % S::XQ * 1024 + 16 * lane, S::XB - 16);
+    // the block's row groups of one step lie one after the other
+    else xsrc[i] = x + (size_t)rm0 * S::XG + u % S::XQ * 1024 + 16 * lane;
   }
 #pragma unroll
   for (int i = 0; i < NSC; ++i) {
@@ -633,32 +589,46 @@ __global__ __launch_bounds__((GemmShape<P, X4, NF, MF, WN, WM, ST, NS>::THREADS)
   // With two stages a wave waits for all its copies, and nothing is copied
   // twice. With more their number has to be the same in every stage: units are
   // fetched again where there are none left.
-  auto copy = [&](int t, int buf) __attribute__((always_inline)) {
+  int ct = t_lo, cp = 0;   // k group and part of the next step to copy
+  auto copy = [&](int u0, int buf) __attribute__((always_inline)) {
     const uint32_t dst = lds + buf * ((S::WU + S::XU) * 1024);
+    const int t = ct;
+    const bool scales = !S::ONCE || ((t & 3) == 0 && cp == 0);
+    int tq[ST];   // the steps' k groups
+#pragma unroll
+    for (int q = 0; q < ST; ++q) {
+      tq[q] = ST == 1 ? ct : min(ct, kt - 1);
+      if (X4 || ++cp == P) {
+        cp = 0;
+        ++ct;
+      }
+    }
 #pragma unroll
     for (int i = 0; i < NWC; ++i) {
       const int u = min(i * S::CW + cw, S::WU - 1);
-      if (!S::ONCE || S::WU % S::CW == 0 || i * S::CW + cw < S::WU)
-        dma16(wsrc[i] + (size_t)(ST == 1 ? t : min(t + u % ST, kt - 1)) * 1024, dst + 1024 * u);
+      int tw = tq[0];
+#pragma unroll
+      for (int q = 1; q < ST; ++q) tw = u % ST == q ? tq[q] : tw;
+      if (!S::ONCE || S::WU % S::CW == 0 || i * S::CW + cw < S::WU) dma16(wsrc[i] + (size_t)tw * 1024, dst + 1024 * u);
     }
 #pragma unroll
     for (int i = 0; i < NXC; ++i) {
       const int u = min(i * S::CW + cw, S::XU - 1), q = X4 ? u % ST : u / S::XQ;
       if (!S::ONCE || S::XU % S::CW == 0 || i * S::CW + cw < S::XU)
-        dma16(xsrc[i] + (size_t)(ST == 1 ? t : min(t + q, kt - 1)) * xstep, dst + 1024 * (S::WU + u));
+        dma16(xsrc[i] + (size_t)(ST == 1 ? u0 : min(u0 + q, kt * P - 1)) * xstep, dst + 1024 * (S::WU + u));
     }
-    if (S::ONCE && ST < 4 && (t & 3) != 0) return;
+    if (!scales) return;
 #pragma unroll
     for (int i = 0; i < NSC; ++i) {
       const int u = min(i * S::CW + cw, S::SU - 1);
       if (!S::ONCE || i * S::CW + cw < S::SU) dma16(ssrc[i] + (t >> 2) * 256, slds + (S::ONCE ? (t >> 2) & 1 : buf) * (S::SU * 1024) + u * 1024);
     }
   };
-  // Waits for stage t: the copies of the stage behind it, if there is one, may
-  // stay in flight.
-  auto arrived = [&](int t) __attribute__((always_inline)) {
+  // Waits for the stage at step u: the copies of the stage behind it, if there
+  // is one, may stay in flight.
+  auto arrived = [&](int u) __attribute__((always_inline)) {
     if (NS == 2) wait_copies<0>();
-    else if (t + ST < t_hi) wait_copies<S::CPW>();
+    else if (u + ST < u_hi) wait_copies<S::CPW>();
     else wait_copies<0>();
   };
   int buf = 0, fill = NS - 1;
@@ -666,14 +636,13 @@ __global__ __launch_bounds__((GemmShape<P, X4, NF, MF, WN, WM, ST, NS>::THREADS)
     if (wv >= S::NW) {
       // addresses in scalar registers (64-bit sums in every lane for each copy:
       // 147 us instead of 136 for the packed x above with one copying wave)
-      constexpr int C = S::COPIERS, GW = S::BN / 32 / C, GX = X4 ? S::BM / 32 / C : S::XB / 1024 / C, GS = S::SU / C;
-      static_assert(GW * C * ST == S::WU && GX * C * ST == S::XU && GS * C == S::SU && S::XB % 1024 == 0, "equal shares");
+      constexpr int C = S::COPIERS, GW = S::BN / 32 / C, GX = S::BM / 32 / C, GS = S::SU / C;
+      static_assert(X4 && GW * C * ST == S::WU && GX * C * ST == S::XU && GS * C == S::SU, "equal shares");
       const uint8_t *wb[GW], *xb[GX], *sb[GS];
 #pragma unroll
       for (int i = 0; i < GW; ++i) wb[i] = a.w + (size_t)min(rn0 + cw * GW + i, wlast) * kt * 1024;
 #pragma unroll
-      for (int i = 0; i < GX; ++i)
-        xb[i] = X4 ? x + (size_t)min(rm0 + cw * GX + i, xlast) * kt * 1024 : x + (size_t)rm0 * S::XG + 1024 * (cw * GX + i);
+      for (int i = 0; i < GX; ++i) xb[i] = x + (size_t)min(rm0 + cw * GX + i, xlast) * kt * 1024;
 #pragma unroll
       for (int i = 0; i < GS; ++i) {
         const int gi = 4 * (cw * GS + i) + (lane >> 4);
@@ -690,8 +659,7 @@ __global__ __launch_bounds__((GemmShape<P, X4, NF, MF, WN, WM, ST, NS>::THREADS)
             dma16u(wb[i] + (size_t)tq * 1024, 16 * lane, dst + 1024 * ((cw * GW + i) * ST + q));
 #pragma unroll
           for (int i = 0; i < GX; ++i)
-            dma16u(xb[i] + (size_t)tq * xstep, 16 * lane,
-                   dst + 1024 * (S::WU + (X4 ? (cw * GX + i) * ST + q : q * S::XQ + cw * GX + i)));
+            dma16u(xb[i] + (size_t)tq * 1024, 16 * lane, dst + 1024 * (S::WU + (cw * GX + i) * ST + q));
         }
         if (S::ONCE && ST < 4 && (t & 3) != 0) return;
 #pragma unroll
@@ -715,7 +683,7 @@ __global__ __launch_bounds__((GemmShape<P, X4, NF, MF, WN, WM, ST, NS>::THREADS)
   } else {
 #pragma unroll
     for (int i = 0; i < NS - 1; ++i)
-      if (t_lo + i * ST < t_hi) copy(t_lo + i * ST, i);
+      if (u_lo + i * ST < u_hi) copy(u_lo + i * ST, i);
   }
   f32x16 acc[NF][MF];
 #pragma unroll
@@ -724,58 +692,62 @@ __global__ __launch_bounds__((GemmShape<P, X4, NF, MF, WN, WM, ST, NS>::THREADS)
     for (int j = 0; j < MF; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-  for (int t = t_lo; t < t_hi; t += ST) {
-    if (S::COPIERS == 0) arrived(t);
+  int mt = t_lo, mp = 0;   // k group and part of the step to multiply
+  for (int u = u_lo; u < u_hi; u += ST) {
+    if (S::COPIERS == 0) arrived(u);
     __syncthreads();   // the stage has arrived for every wave, and every wave has read the one before
-    if (S::COPIERS == 0 && t + (NS - 1) * ST < t_hi) copy(t + (NS - 1) * ST, fill);
+    if (S::COPIERS == 0 && u + (NS - 1) * ST < u_hi) copy(u + (NS - 1) * ST, fill);
     fill = fill + 1 == NS ? 0 : fill + 1;
     const uint8_t* ws = stage[buf] + 16 * lane;
     const uint8_t* xs = ws + S::WU * 1024;
-    const uint32_t* sd = (const uint32_t*)sstage[S::ONCE ? (t >> 2) & 1 : buf] + lane;
+    const uint32_t* sd = (const uint32_t*)sstage[S::ONCE ? (mt >> 2) & 1 : buf] + lane;
     buf = buf + 1 == NS ? 0 : buf + 1;
-    int wd[NF], xd[MF];   // scale dwords: byte t % 4 is this k group's
+    int wd[NF], xd[MF];   // scale dwords: byte t % 4 is k group t's
 #pragma unroll
     for (int i = 0; i < NF; ++i) wd[i] = sd[(wn * NF + i) * 64];
 #pragma unroll
-    for (int j = 0; j < MF; ++j) xd[j] = sd[(S::BN / 32 + wm * MF + j) * 64];
+    for (int j = 0; j < MF; ++j) xd[j] = X4 ? sd[(S::BN / 32 + wm * MF + j) * 64] : 0;
 #pragma unroll
     for (int q = 0; q < ST; ++q) {
-      if (ST > 1 && t + q >= t_hi) break;
-      i32x8 w[NF];
+      if (ST > 1 && u + q >= u_hi) break;
+      u32x4 w[NF];
 #pragma unroll
-      for (int i = 0; i < NF; ++i) {
-        const u32x4 v = *(const u32x4*)(ws + ((wn * NF + i) * ST + q) * 1024);
-        w[i] = i32x8{(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0};
-      }
-      const int sh = 8 * ((t & 3) + q);
-      int wsv[NF], xsv[MF];
-#pragma unroll
-      for (int i = 0; i < NF; ++i) wsv[i] = (uint32_t)wd[i] >> sh;
-#pragma unroll
-      for (int j = 0; j < MF; ++j) xsv[j] = ((uint32_t)xd[j] >> sh) & 255;
-#pragma unroll
-      for (int p = 0; p < P; ++p) {
+      for (int i = 0; i < NF; ++i) w[i] = *(const u32x4*)(ws + ((wn * NF + i) * ST + q) * 1024);
+      const int sh = 8 * (mt & 3);
+      if constexpr (X4) {
 #pragma unroll
         for (int j = 0; j < MF; ++j) {
-          i32x8 b;
-          if constexpr (X4) {
-            const u32x4 v = *(const u32x4*)(xs + ((wm * MF + j) * ST + q) * 1024);
-            b = i32x8{(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0};
-          } else {
-            const uint8_t* xp = xs + q * (S::XQ * 1024) + ((wm * MF + j) * P + p) * kMxPartBytes;
-            const u32x4 v = *(const u32x4*)xp;
-            const u32x2 h = *(const u32x2*)(xp + 1024 - 8 * lane);
-            b = i32x8{(int)v[0], (int)v[1], (int)v[2], (int)v[3], (int)h[0], (int)h[1], 0, 0};
-          }
-          // a NaN scale (255) stays one in part 0; the later parts' scales are 5 less each
-          const int sx = xsv[j] - 5 * p;
+          const u32x4 v = *(const u32x4*)(xs + ((wm * MF + j) * ST + q) * 1024);
+          const i32x8 b = {(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0};
 #pragma unroll
-          for (int i = 0; i < NF; ++i)
-            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w[i], b, acc[i][j], kFp4, X4 ? kFp4 : kFp6, 0,
-                                                                        wsv[i], 0, sx);
-          // three waves a SIMD leave 168 registers, 128 of them sums: the parts
-          // one after the other (hoisted, they spill)
-          if (S::COPIERS > 0 && P > 1) __builtin_amdgcn_sched_barrier(0);
+          for (int i = 0; i < NF; ++i) {
+            const i32x8 wi = {(int)w[i][0], (int)w[i][1], (int)w[i][2], (int)w[i][3], 0, 0, 0, 0};
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wi, b, acc[i][j], kFp4, kFp4, 0, (uint32_t)wd[i] >> sh, 0,
+                                                                        (uint32_t)xd[j] >> sh);
+          }
+        }
+        ++mt;
+      } else {
+        float scale[NF];
+#pragma unroll
+        for (int i = 0; i < NF; ++i) scale[i] = scale_of(((uint32_t)wd[i] >> sh) & 255);
+        // a quarter of each 32-block at a time: instruction e takes elements 8 e .. 8 e + 7 of both
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          bf16x8 we[NF];
+#pragma unroll
+          for (int i = 0; i < NF; ++i) we[i] = expand8(w[i][e], scale[i]);
+#pragma unroll
+          for (int j = 0; j < MF; ++j) {
+            const u32x4 v = *(const u32x4*)(xs + (q * S::XQ + (wm * MF + j) * 4 + e) * 1024);
+#pragma unroll
+            for (int i = 0; i < NF; ++i)
+              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(we[i], __builtin_bit_cast(bf16x8, v), acc[i][j], 0, 0, 0);
+          }
+        }
+        if (++mp == P) {
+          mp = 0;
+          ++mt;
         }
       }
     }
@@ -860,13 +832,13 @@ int quantize_t(const void* src, int64_t rows, int64_t k, int64_t ld, uint8_t* ds
 }
 
 template <class T>
-int split_t(const void* src, int64_t rows, int64_t k, int64_t ld, int parts, uint8_t* dst, hipStream_t s) {
+int split_t(const void* src, int64_t rows, int64_t k, int64_t ld, uint8_t* dst, hipStream_t s) {
   const Mx4Layout L = mx4_layout(rows, k);
   const dim3 grid((unsigned)L.rt, (unsigned)L.kt);
   if (rows_aligned<T>(src, ld, 4))
-    hipLaunchKernelGGL((k_mx_split<T, true>), grid, dim3(64), 0, s, (const T*)src, rows, k, ld, parts, dst, L);
+    hipLaunchKernelGGL((k_mx_split<T, true>), grid, dim3(64), 0, s, (const T*)src, rows, k, ld, dst, L);
   else
-    hipLaunchKernelGGL((k_mx_split<T, false>), grid, dim3(64), 0, s, (const T*)src, rows, k, ld, parts, dst, L);
+    hipLaunchKernelGGL((k_mx_split<T, false>), grid, dim3(64), 0, s, (const T*)src, rows, k, ld, dst, L);
   return (int)hipGetLastError();
 }
 
@@ -892,13 +864,12 @@ int launch_mx4_dequant(const uint8_t* src, float* out, int64_t rows, int64_t k, 
   });
 }
 
-int launch_mx_split(int elem, const void* src, int64_t rows, int64_t k, int64_t ld, int parts, uint8_t* dst,
-                    void* stream) {
+int launch_mx_split(int elem, const void* src, int64_t rows, int64_t k, int64_t ld, uint8_t* dst, void* stream) {
   hipStream_t s = (hipStream_t)stream;
   switch (elem) {
-    case ELEM_F32: return split_t<float>(src, rows, k, ld, parts, dst, s);
-    case ELEM_F16: return split_t<_Float16>(src, rows, k, ld, parts, dst, s);
-    case ELEM_BF16: return split_t<__bf16>(src, rows, k, ld, parts, dst, s);
+    case ELEM_F32: return split_t<float>(src, rows, k, ld, dst, s);
+    case ELEM_F16: return split_t<_Float16>(src, rows, k, ld, dst, s);
+    case ELEM_BF16: return split_t<__bf16>(src, rows, k, ld, dst, s);
   }
   return (int)hipErrorInvalidValue;
 }
@@ -936,12 +907,12 @@ int launch_mx4_gemv(const Mx4LinearArgs& a, void* stream) {
   return (int)hipErrorInvalidValue;
 }
 
-template <int P, bool X4, int NF, int MF, int WN, int WM, int ST, int NS, int OCC>
+template <bool X4, int NF, int MF, int WN, int WM, int ST, int NS, int OCC>
 static int launch_gemm_t(const Mx4LinearArgs& a, hipStream_t s) {
-  typedef GemmShape<P, X4, NF, MF, WN, WM, ST, NS> S;
+  typedef GemmShape<X4, NF, MF, WN, WM, ST, NS> S;
   const int64_t nbn = (a.n + S::BN - 1) / S::BN, nbm = (a.m + S::BM - 1) / S::BM;
   if (nbn * nbm * a.kslices > 0xffffffffll / S::THREADS) return (int)hipErrorInvalidValue;   // threads of a grid
-  hipLaunchKernelGGL((k_mx4_gemm<P, X4, NF, MF, WN, WM, ST, NS, OCC>), dim3((unsigned)(nbn * nbm * a.kslices)),
+  hipLaunchKernelGGL((k_mx4_gemm<X4, NF, MF, WN, WM, ST, NS, OCC>), dim3((unsigned)(nbn * nbm * a.kslices)),
                      dim3(S::THREADS), 0, s, a, (int)nbn, (int)nbm);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.kslices == 1) return (int)e;
@@ -949,30 +920,22 @@ static int launch_gemm_t(const Mx4LinearArgs& a, hipStream_t s) {
   return (int)hipGetLastError();
 }
 
-// The stages: 128 x 32 blocks, whose steps are short, copy two k groups at a
+// The stages: 128 x 32 blocks, whose steps are short, copy two of them at a
 // time, two stages ahead; packed x comes four k groups at a time.
-template <int P, bool X4>
-static int launch_gemm_p(const Mx4LinearArgs& a, int tile, hipStream_t s) {
-  switch (tile) {
-    case MT_256x256: return launch_gemm_t<P, X4, 4, 2, 2, 4, X4 ? 4 : 1, 2, 1>(a, s);
-    case MT_256x64:
-      if constexpr (!X4) return launch_gemm_t<P, X4, 2, 2, 4, 1, 1, 2, 2>(a, s);
-      break;
-    case MT_128x64:
-      if constexpr (X4) return launch_gemm_t<P, X4, 1, 2, 4, 1, 4, 2, 2>(a, s);
-      break;
-    case MT_128x32: return launch_gemm_t<P, X4, 1, 1, 4, 1, X4 ? 4 : 2, 3, 2>(a, s);
-  }
-  return (int)hipErrorInvalidValue;
-}
-
 int launch_mx4_gemm(const Mx4LinearArgs& a, bool packed, int tile, void* stream) {
   hipStream_t s = (hipStream_t)stream;
-  if (packed) return launch_gemm_p<1, true>(a, tile, s);
-  switch (a.parts) {
-    case 3: return launch_gemm_p<3, false>(a, tile, s);
-    case 4: return launch_gemm_p<4, false>(a, tile, s);
-    case 5: return launch_gemm_p<5, false>(a, tile, s);
+  if (packed) {
+    switch (tile) {
+      case MT_256x256: return launch_gemm_t<true, 4, 2, 2, 4, 4, 2, 1>(a, s);
+      case MT_128x64: return launch_gemm_t<true, 1, 2, 4, 1, 4, 2, 2>(a, s);
+      case MT_128x32: return launch_gemm_t<true, 1, 1, 4, 1, 4, 3, 2>(a, s);
+    }
+  } else {
+    switch (tile) {
+      case MT_256x256: return launch_gemm_t<false, 2, 4, 4, 2, 1, 2, 1>(a, s);
+      case MT_256x64: return launch_gemm_t<false, 2, 2, 4, 1, 1, 2, 2>(a, s);
+      case MT_128x32: return launch_gemm_t<false, 1, 1, 4, 1, 2, 3, 2>(a, s);
+    }
   }
   return (int)hipErrorInvalidValue;
 }

@@ -1853,20 +1853,17 @@ int gg_mxfp4_dequant(const void* packed, float* out, int64_t rows, int64_t k, in
 }
 
 // Device bytes behind a product: the parts of x, then the slices' sums.
-static size_t linear_workspace(bool packed, int x_elem, int y_elem, int64_t m, int64_t n, int64_t k) {
-  const int parts = packed ? 1 : mx_parts(x_elem, y_elem);
+static size_t linear_workspace(bool packed, int x_elem, int64_t m, int64_t n, int64_t k) {
+  const int parts = packed ? 1 : mx_parts(x_elem);
   if (!packed && mx_gemv_fits(m, parts, k)) return 0;
   return (packed ? 0 : mx_parts_bytes(m, k, parts)) + mx4_sums_bytes(mx4_plan(packed, parts, m, n, k), m, n);
 }
 
-// Holds for every y_type.
 size_t gg_mxfp4_linear_workspace_size(uint32_t x_type, int64_t m, int64_t rows, int64_t k) {
   const bool packed = x_type == GG_TYPE_MXFP4;
   const int e = elem_of(x_type);
   if ((e < 0 && !packed) || !mx4_shape(m, k) || !mx4_shape(rows, k)) return 0;
-  size_t most = 0;
-  for (int ye : {ELEM_F32, ELEM_F16, ELEM_BF16}) most = std::max(most, linear_workspace(packed, e, ye, m, rows, k));
-  return most;
+  return linear_workspace(packed, e, m, rows, k);
 }
 
 int gg_mxfp4_linear(const void* w, const void* x, uint32_t x_type, int64_t ldx, void* y, uint32_t y_type, int64_t ldy,
@@ -1894,15 +1891,15 @@ int gg_mxfp4_linear(const void* w, const void* x, uint32_t x_type, int64_t ldx, 
   a.ldy = ldy;
   a.y_elem = ye;
   a.y_vec = aligned_to(y, 16) && ldy * elem_size(ye) % 16 == 0;
-  a.parts = x4 ? 1 : mx_parts(xe, ye);
+  a.parts = x4 ? 1 : mx_parts(xe);
   if (!x4 && mx_gemv_fits(m, a.parts, k)) return launch_mx4_gemv(a, stream) ? GG_ERR_HIP : GG_OK;
-  if (linear_workspace(x4, xe, ye, m, rows, k) && (!workspace || !aligned_to(workspace, 16))) return GG_ERR_INVALID;
+  if (linear_workspace(x4, xe, m, rows, k) && (!workspace || !aligned_to(workspace, 16))) return GG_ERR_INVALID;
   const Mx4Plan plan = mx4_plan(x4, a.parts, m, rows, k);
   a.kslices = plan.slices;
   a.ldp = (rows + 3) / 4 * 4;
   a.partial = (float*)((uint8_t*)workspace + (x4 ? 0 : mx_parts_bytes(m, k, a.parts)));
   if (!x4) {
-    if (launch_mx_split(xe, x, m, k, ldx, a.parts, (uint8_t*)workspace, stream)) return GG_ERR_HIP;
+    if (launch_mx_split(xe, x, m, k, ldx, (uint8_t*)workspace, stream)) return GG_ERR_HIP;
     a.x = workspace;
   }
   return launch_mx4_gemm(a, x4, plan.tile, stream) ? GG_ERR_HIP : GG_OK;
