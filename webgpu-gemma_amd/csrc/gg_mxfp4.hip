@@ -533,7 +533,7 @@ template <int N>
 __device__ __forceinline__ void wait_copies() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
 template <bool X4, int NF, int MF, int WN, int WM, int ST, int NS, int OCC>
-__global__ __launch_bounds__((GemmShape<X4, NF, MF, WN, WM, ST, NS>::THREADS), OCC) void k_mx4_gemm(Mx4LinearArgs a, int nbn, int nbm) {
+__global__ __launch_bounds__((GemmShape<X4, NF, MF, WN, WM, ST, NS>::THREADS), OCC) void k_mx4_gemm(Mx4LinearArgs a, int nbn, int nbm, int bm0) {
   typedef GemmShape<X4, NF, MF, WN, WM, ST, NS> S;
   __shared__ __align__(1024) uint8_t stage[NS][(S::WU + S::XU) * 1024];
   __shared__ __align__(1024) uint8_t sstage[S::SS][S::SU * 1024];
@@ -547,7 +547,7 @@ __global__ __launch_bounds__((GemmShape<X4, NF, MF, WN, WM, ST, NS>::THREADS), O
   const int LL = xcd * (G >> 3) + min(xcd, G & 7) + (blockIdx.x >> 3);
   const int kz = LL / (nbn * nbm), L = LL - kz * (nbn * nbm);
   const int fm = L / (GROUP * nbn) * GROUP, gm = min(nbm - fm, GROUP), Lp = L % (GROUP * nbn);
-  const int64_t bm = fm + Lp % gm, bn = Lp / gm;
+  const int64_t bm = bm0 + fm + Lp % gm, bn = Lp / gm;
   const int t_lo = 4 * (int)((int64_t)a.ks * kz / a.kslices), t_hi = min(4 * (int)((int64_t)a.ks * (kz + 1) / a.kslices), a.kt);
   const uint8_t* x = (const uint8_t*)a.x;
   const uint8_t* wsc = a.w + (size_t)a.wrt * a.kt * 1024;
@@ -911,10 +911,18 @@ template <bool X4, int NF, int MF, int WN, int WM, int ST, int NS, int OCC>
 static int launch_gemm_t(const Mx4LinearArgs& a, hipStream_t s) {
   typedef GemmShape<X4, NF, MF, WN, WM, ST, NS> S;
   const int64_t nbn = (a.n + S::BN - 1) / S::BN, nbm = (a.m + S::BM - 1) / S::BM;
-  if (nbn * nbm * a.kslices > 0xffffffffll / S::THREADS) return (int)hipErrorInvalidValue;   // threads of a grid
-  hipLaunchKernelGGL((k_mx4_gemm<X4, NF, MF, WN, WM, ST, NS, OCC>), dim3((unsigned)(nbn * nbm * a.kslices)),
-                     dim3(S::THREADS), 0, s, a, (int)nbn, (int)nbm);
-  const hipError_t e = hipGetLastError();
+  // a grid holds fewer than 2^32 threads: as many tile rows as fit in each
+  // launch. 2^30 features are at most 2^23 tiles of 128, so that one row fits;
+  // slices come only with few sums (kMx4MaxSums), in one launch.
+  const int64_t rows = 0xffffffffll / S::THREADS / (nbn * a.kslices);
+  if (rows < 1 || (a.kslices > 1 && rows < nbm)) return (int)hipErrorInvalidValue;
+  hipError_t e = hipSuccess;
+  for (int64_t b = 0; b < nbm && e == hipSuccess; b += rows) {
+    const int64_t now = std::min(nbm - b, rows);
+    hipLaunchKernelGGL((k_mx4_gemm<X4, NF, MF, WN, WM, ST, NS, OCC>), dim3((unsigned)(nbn * now * a.kslices)),
+                       dim3(S::THREADS), 0, s, a, (int)nbn, (int)now, (int)b);
+    e = hipGetLastError();
+  }
   if (e != hipSuccess || a.kslices == 1) return (int)e;
   hipLaunchKernelGGL(k_mx4_join, dim3((unsigned)((a.n + 1023) / 1024), (unsigned)a.m), dim3(256), 0, s, a);
   return (int)hipGetLastError();
