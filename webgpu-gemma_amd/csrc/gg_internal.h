@@ -520,6 +520,13 @@ constexpr Mx4Tile kMx4PartTiles[MT_COUNT] = {
     {256, 256, 1.122f, 13.2f, 1.122f, 13.2f}, {256, 64, .481f, 2.5f, .349f, 1.6f}, {}, {128, 32, .241f, 0.f, .142f, .65f}};
 constexpr Mx4Tile kMx4PackedTiles[MT_COUNT] = {
     {256, 256, .330f, 11.2f, .330f, 11.2f}, {}, {128, 64, .084f, 2.3f, .111f, 1.7f}, {128, 32, .095f, .55f, .074f, 1.4f}};
+// Waves of a block of the few-row kernel that share 16 weight rows' k: as many
+// as leave a block for each CU, and each a step of 128 k.
+inline int mx_gemv_waves(int64_t n, int64_t k) {
+  int kw = kMxGemvWaves;
+  while (kw > 1 && ((n + 15) / 16 * kw > kMxGemvWaves * 256 || kw > (k + 127) / 128)) kw >>= 1;
+  return kw;
+}
 constexpr int kMx4MaxSlices = 16;
 constexpr int64_t kMx4MaxSums = 1 << 24;   // f32 sums that slices may leave
 struct Mx4Plan { int tile, slices; };

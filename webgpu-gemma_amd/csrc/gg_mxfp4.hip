@@ -876,24 +876,21 @@ int launch_mx_split(int elem, const void* src, int64_t rows, int64_t k, int64_t 
 
 template <class T>
 static int launch_gemv_t(const Mx4LinearArgs& a, hipStream_t s) {
-  const int cols = (int)a.m * a.parts, steps = (a.k + 127) / 128;
+  const int cols = (int)a.m * a.parts, kw = mx_gemv_waves(a.n, a.k);
   const int64_t groups = (a.n + 15) / 16;
   const size_t lds = mx_gemv_lds(cols, a.k);
-  // waves that share 16 rows' k: as many as leave a block for each CU, and each a step
-  int kw = kMxGemvWaves;
-  while (kw > 1 && (groups * kw > kMxGemvWaves * 256 || kw > steps)) kw >>= 1;
   const int64_t blocks = (groups * kw + kMxGemvWaves - 1) / kMxGemvWaves;
   // every block makes all parts: one a CU, and two where each has several row
   // groups to go over and LDS holds both (more weights in flight)
   const int64_t most = blocks >= 1024 && lds <= 80 * 1024 ? 512 : 256;
   const dim3 grid((unsigned)(blocks < most ? blocks : most)), block(64 * kMxGemvWaves);
-  switch ((cols + 15) / 16) {
-    case 1: hipLaunchKernelGGL((k_mx4_gemv<T, 1>), grid, block, lds, s, a, kw); break;
-    case 2: hipLaunchKernelGGL((k_mx4_gemv<T, 2>), grid, block, lds, s, a, kw); break;
-    case 3: hipLaunchKernelGGL((k_mx4_gemv<T, 3>), grid, block, lds, s, a, kw); break;
-    case 4: hipLaunchKernelGGL((k_mx4_gemv<T, 4>), grid, block, lds, s, a, kw); break;
-    default: return (int)hipErrorInvalidValue;
-  }
+  constexpr int MOST = (mx_parts(kElem<T>) * kMxGemvRows + 15) / 16;   // column tiles
+  const int tiles = (cols + 15) / 16;
+  if (tiles == 1) hipLaunchKernelGGL((k_mx4_gemv<T, 1>), grid, block, lds, s, a, kw);
+  else if (tiles == 2) hipLaunchKernelGGL((k_mx4_gemv<T, 2>), grid, block, lds, s, a, kw);
+  else if (tiles == 3 && MOST >= 3) hipLaunchKernelGGL((k_mx4_gemv<T, MOST >= 3 ? 3 : 2>), grid, block, lds, s, a, kw);
+  else if (tiles == 4 && MOST >= 4) hipLaunchKernelGGL((k_mx4_gemv<T, MOST >= 4 ? 4 : 2>), grid, block, lds, s, a, kw);
+  else return (int)hipErrorInvalidValue;
   return (int)hipGetLastError();
 }
 
