@@ -33,7 +33,8 @@ extern "C" {
 #define GG_TYPE_F32 0u
 #define GG_TYPE_F16 1u
 #define GG_TYPE_Q8_0 8u
-/* further types of the kernel-level entry points (ggml's numbers) */
+/* further types of the kernel-level entry points (ggml's numbers; MXFP4 stands
+ * for a matrix packed by gg_mxfp4_quantize, not for ggml's order of blocks) */
 #define GG_TYPE_BF16 30u
 #define GG_TYPE_MXFP4 39u
 

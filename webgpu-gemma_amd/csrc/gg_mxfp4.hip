@@ -42,7 +42,7 @@ __device__ __forceinline__ void load4(const T* row, int64_t c, int64_t k, float 
 // Scale byte: the exponent field of the block's largest magnitude less 2
 // (floor(log2) - 2), at least 0; conversion to nearest, ties to even, values
 // above 6 to 6. Bound by memory: reads the input once, writes 17/32 byte an
-// element (262144 x 1152 bf16, 764 MB: 144 us, 5.3 TB/s; 187 x 6912 f32 3.9 us,
+// element (262144 x 1152 bf16, 764 MB: 141 us, 5.4 TB/s; 187 x 6912 f32 3.8 us,
 // three times an empty kernel).
 // ---------------------------------------------------------------------------
 template <class T, bool VEC>
@@ -123,7 +123,7 @@ __global__ __launch_bounds__(256) void k_mx4_quantize(const T* __restrict__ src,
 // ---------------------------------------------------------------------------
 // Expansion to f32, the same tile the other way: each value is its 4-bit
 // element times 2^(byte - 127), NaN where the byte is 255. Bound by the f32
-// write (262144 x 1152, 1.37 GB: 237 us, 5.8 TB/s).
+// write (262144 x 1152, 1.37 GB: 235 us, 5.8 TB/s).
 // ---------------------------------------------------------------------------
 template <bool VEC>
 __global__ __launch_bounds__(256) void k_mx4_dequant(const uint8_t* __restrict__ src, float* __restrict__ out,
@@ -211,7 +211,7 @@ __device__ __forceinline__ void inf_to_nan(float (&u)[8]) {
 // whole lines, four elements a lane (one where their addresses are odd), and
 // change lanes in LDS; a pitch of 68 floats puts the 16 lanes of a read on
 // different banks. Bound by memory for long x (reads 4 or 2 bytes, writes 2 a
-// part and element; 4000 x 8192 bf16, 131 MB: 24 us, 5.5 TB/s), by its latency for
+// part and element; 4000 x 8192 bf16, 131 MB: 23 us, 5.7 TB/s), by its latency for
 // short (2048 x 1152 f32, 24 MB: 8 us).
 template <class T, bool VEC>
 __global__ __launch_bounds__(64) void k_mx_split(const T* __restrict__ src, int64_t rows, int64_t k, int64_t ld,
@@ -483,14 +483,16 @@ __global__ __launch_bounds__(64 * kMxGemvWaves) void k_mx4_gemv(Mx4LinearArgs a,
 // every stage, so that the number in flight tells which stage has arrived.
 // Bound by the matrix units and their power. Packed x: a loop on registers
 // reaches 6.4 PFLOP/s on random operands (9.3 on constant ones: the clock
-// falls to 1.6 GHz), 256 x 256 blocks 4.2 (4096 x 8192 x 8192, 123 to 131 us from box to
-// box), of which 16 us are each block's start and the store of its results. 16 x 16 x 128
+// falls to 1.6 GHz), 256 x 256 blocks 4.0 to 4.3 (4096 x 8192 x 8192, 128 to 136 us from box
+// to box), of which 16 us are each block's start and the store of its results. 16 x 16 x 128
 // instructions reach 4.6 in the loop. Blocks of half the size, two to a CU, and
 // more stages measured no faster.
-// Parts: 4000 x 8192 x 8192 bf16 417 to 440 us with their making (1.2 to 1.3 PFLOP/s;
-// a bf16 library product of 8192 x 8192 x 8192 reaches 1.19), 2048 x 8192 x 8192 f32, three
-// parts, 611 us (1.35 of them). 256 x 256 blocks: waves of 64 features x 128 rows 417 us,
-// of 128 x 64 423, four of 128 x 128 456; three stages 429.
+// Parts: 4000 x 8192 x 8192 bf16 401 to 466 us from box to box (1.15 to 1.34 PFLOP/s; a
+// bf16 library product of 8192 x 8192 x 8192 reaches 1.19), 2048 x 13824 x 1152 f32, three
+// parts, 170 to 180 us in 256 x 64 blocks (1.09 to 1.15 of them). 4000 x 8192 x 8192 with
+// the making of the parts, one box: 256 x 256 blocks with waves of 64 features x 128 rows
+// 417 us, of 128 x 64 423, four of 128 x 128 456, three stages 429; another: 430, two blocks of 256 x
+// 128 a CU 435 to 452.
 // ---------------------------------------------------------------------------
 template <bool X4, int NF, int MF, int WN, int WM, int ST, int NS>
 struct GemmShape {
