@@ -319,9 +319,9 @@ __device__ __forceinline__ void store_tile(int elem, void* y, int64_t ldy, int64
 // parts in its LDS (one launch, no workspace) and goes over its share of the
 // weights, which travel from memory to registers, kGemvAhead KB ahead in each
 // wave. A wave takes 16 weight rows; `kw` waves of a block share their k.
-// Bound by the read of the weights (17/32 byte each): 262144 x 1152 f32 28 us,
-// 5.8 TB/s (30 to 32 with the addresses of a step computed from the row and k
-// indices each time; 12 KB ahead spill). A small product by its chain of x,
+// Bound by the read of the weights (17/32 byte each): 262144 x 1152 f32 28 to 30 us,
+// 5.4 to 5.8 TB/s (2 us more with the addresses of a step computed from the row and
+// k indices each time; 12 KB ahead are no longer kept in registers: 88 us). A small product by its chain of x,
 // parts, weights, sums: 1 row, 1536 x 1152 4.8 us and 1152 x 6912 6.2 us, 7 rows of
 // 13824 x 1152 6.9 us, an empty kernel 1.3.
 // ---------------------------------------------------------------------------
