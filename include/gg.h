@@ -37,6 +37,7 @@ extern "C" {
  * for a matrix packed by gg_mxfp4_quantize, not for ggml's order of blocks) */
 #define GG_TYPE_BF16 30u
 #define GG_TYPE_MXFP4 39u
+#define GG_TYPE_E4M3 256u   /* 8-bit K/V rows, each with a scale (gg_kv_pages); not a ggml number */
 
 /* attention modes: 0 = reference (src/ as shipped: one RoPE theta, full
  * attention on every layer, types.ts:32-33, shaders.ts:229-325);
@@ -350,6 +351,131 @@ size_t gg_score_workspace_size(int64_t rows, int32_t n, int32_t top_n);
 int gg_score_logits(const void* logits, uint32_t type, int64_t rows, int32_t n, int64_t ld, const int32_t* ids,
                     int32_t n_ids, float* id_logprobs, float* lse, float* entropy, int32_t top_n, int32_t* top_ids,
                     float* top_logprobs, void* workspace, void* stream);
+
+/* ---- K/V pages and attention over them -------------------------------------
+ * For callers that serve several sequences with the products above: keys and
+ * values in pages of a few positions, a table of pages for each sequence, and
+ * one call for the new rows of all of them. No counterpart in the reference,
+ * and apart from a context's own cache. Same rules for pointers and streams as
+ * gg_mxfp4_linear; the calls read the structures before they return.
+ *
+ * gg_kv_pages describes a pool: the row of a (page, place, head) is head_dim
+ * consecutive values at page * page_stride + place * pos_stride +
+ * head * head_stride (elements) behind k, and at the same distance behind v.
+ * type GG_TYPE_BF16, GG_TYPE_F16 or GG_TYPE_E4M3; head_dim a multiple of 16 up
+ * to 256; k, v and the strides multiples of 16 bytes. E4M3 rows (sign, 4
+ * exponent bits, 3 of mantissa, up to 448) stand for their values times one
+ * f32 scale at k_scale / v_scale [page][place][head].
+ *
+ * gg_kv_seqs names the sequences of a call. Rows row_start[s] up to
+ * row_start[s + 1] of its operands are the last ones of the len[s] positions
+ * that sequence s has, with the new ones: row i of them is at position
+ * len[s] - rows + i. Position p lies in page table[s][p / page_size], place
+ * p % page_size. Entries outside [0, n_pages), positions below 0 and those past
+ * max_len or the table have no place: nothing is stored there or seen.
+ * row_start ascends from 0 or more to n_rows or less; rows outside are left alone. The device
+ * reads the arrays, so a captured call follows them; the counts and bounds in
+ * the structure are the host's: max_rows a bound of a sequence's rows that only
+ * chooses kernels, max_len one of len (lengths above it count as max_len). */
+typedef struct gg_kv_pages {
+  void* k;
+  void* v;
+  float* k_scale;       /* E4M3 only */
+  float* v_scale;
+  int64_t page_stride;
+  int64_t pos_stride;
+  int64_t head_stride;
+  uint32_t type;
+  int32_t n_pages;
+  int32_t page_size;
+  int32_t n_kv_heads;
+  int32_t head_dim;
+} gg_kv_pages;
+
+typedef struct gg_kv_seqs {
+  const int32_t* row_start;   /* [n_seqs + 1] */
+  const int32_t* len;         /* [n_seqs] */
+  const int32_t* table;       /* [n_seqs][table_ld] */
+  int32_t n_seqs;
+  int32_t n_rows;
+  int32_t max_rows;
+  int32_t max_len;
+  int32_t table_ld;
+} gg_kv_seqs;
+
+/* New rows of a QKV product into the pages. q rows hold n_q_heads * head_dim
+ * values, k and v rows n_kv_heads * head_dim (type GG_TYPE_F32 / F16 / BF16,
+ * rows ldq, ldk, ldv apart). Every head of q and k is divided by
+ * sqrt(mean x^2 + eps) and multiplied by q_norm / k_norm (f32[head_dim]; NULL:
+ * neither), then rotated in halves: with a = position * rope_theta^(-2j /
+ * head_dim), values j and j + head_dim / 2 turn by a (rope_theta 0: no
+ * rotation). q goes to q_out (rows ldqo apart), k and v to their places; a row
+ * without a place goes nowhere but to q_out, where its position counts all the
+ * same. q may be NULL, with n_q_heads 0.
+ * All between reading and storing is 64-bit: each stored value is the formula's, rounded once to nearest
+ * (even). An E4M3 row's scale is the least power of two from 2^-126 on that
+ * holds its largest magnitude within 448; a row with an infinity or a NaN gets
+ * the scale NaN. Two rows of a call must not have the same place. */
+int gg_kv_store(const gg_kv_pages* pages, const gg_kv_seqs* seqs, uint32_t type, const void* q, int64_t ldq, const void* k,
+                int64_t ldk, const void* v, int64_t ldv, int32_t n_q_heads, const float* q_norm, const float* k_norm,
+                double eps, double rope_theta, void* q_out, uint32_t q_out_type, int64_t ldqo, void* stream);
+
+/* The values that the rows' places hold, n_kv_heads * head_dim a row (type
+ * GG_TYPE_F32 / F16 / BF16; 0 for a row without a place). k_out or v_out may be
+ * NULL. Rows may be any last part of a sequence, all of it too. */
+int gg_kv_load(const gg_kv_pages* pages, const gg_kv_seqs* seqs, void* k_out, int64_t ldk, void* v_out, int64_t ldv,
+               uint32_t type, void* stream);
+
+/* Attention of the rows over what their sequences have in the pages (the rows'
+ * own keys among it). q and out: n_q_heads * head_dim values a row, ldq / ldo
+ * apart, of one type (GG_TYPE_F32 / F16 / BF16; with F16 pages GG_TYPE_F16);
+ * query head h reads K/V head h / (n_q_heads / n_kv_heads). The row at
+ * position p sees position j if j <= p and, with window > 0, if also
+ * j > p - window or j < sinks:
+ *   out = sum_j softmax_j(scale q.k_j) v_j
+ *   lse = ln sum_j e^(scale q.k_j)          [n_rows][n_q_heads], may be NULL
+ * A row that sees nothing has out 0 and lse -inf. What a row does not see has
+ * no effect on it, infinities and NaN included. Products take every bit of f32
+ * q; the weights keep 24 bits with f32, 16 with f16 on other than F16 pages,
+ * else those of the pages' type; sums are f32. out overlaps neither q nor the
+ * pages. */
+size_t gg_kv_attention_workspace_size(const gg_kv_pages* pages, const gg_kv_seqs* seqs, int32_t n_q_heads, int32_t window,
+                                      int32_t sinks);
+int gg_kv_attention(const gg_kv_pages* pages, const gg_kv_seqs* seqs, const void* q, uint32_t type, int64_t ldq,
+                    int32_t n_q_heads, float scale, int32_t window, int32_t sinks, void* out, int64_t ldo, float* lse,
+                    void* workspace, void* stream);
+
+/* ---- verification of drafted tokens -----------------------------------------
+ * Which of a sequence's drafted tokens stand, and the token behind them, such
+ * that tokens are distributed as if drawn from the target's logits one by one.
+ * Rows row_start[s] .. row_start[s + 1] - 1 belong to sequence s (row_start
+ * [n_seqs + 1] on the device, ascending within 0 .. rows): the target's logits z behind its tokens
+ * so far and 0, 1, .. of its drafts; draft[row] is the token drafted at that row (not read in
+ * the last one, which a draft never follows). rows x n logits of type GG_TYPE_F32 /
+ * F16 / BF16, ldz apart; y: the draft model's logits that each draft was drawn
+ * from (same type, rows ldy apart, a sequence's last row not read), or NULL
+ * for drafts that were no draw. With T = temperature[s] and p, q the softmax of
+ * z / T and y / T (q = 1 at the draft without y):
+ *   row by row the draft d stands while accept_u[row] * q(d) < p(d);
+ *   where one does not, the token is drawn from max(p - q, 0), or from p with d
+ *   left out where there is no y (from p if nothing is left); behind the last
+ *   draft from p: the least id whose sum of weights up to it exceeds
+ *   draw_u[s] times the sum of all;
+ * temperature 0: a draft stands while it is the largest logit's id (the lowest
+ * among equals), and the token is that id. Random numbers in [0, 1).
+ *   accepted[s]   drafts that stand
+ *   tokens[rows]  they, the token behind them, then -1 up to the sequence's end
+ *   logprobs[rows]  ln p of each of those tokens (temperature 0: of softmax z), 0 behind them; may be NULL
+ * A draft outside [0, n) does not stand. Logits of -inf have probability 0. A row that is reached and has a NaN or
+ * +inf, or nothing above -inf, in z or (before its last row) y ends its sequence: token -1, log
+ * probability NaN. A sequence without rows: accepted 0. rows and n from 1 to 2^30, n_seqs from 1 to 2^22. What decides a
+ * token is summed in 64 bits. Same rules for pointers, streams and the
+ * workspace as gg_mxfp4_linear. */
+size_t gg_verify_drafts_workspace_size(int64_t rows, int32_t n_seqs, int32_t n);
+int gg_verify_drafts(const void* z, const void* y, uint32_t type, int64_t rows, int32_t n, int64_t ldz, int64_t ldy,
+                     const int32_t* draft, const int32_t* row_start, int32_t n_seqs, const float* temperature,
+                     const double* accept_u, const double* draw_u, int32_t* accepted, int32_t* tokens, float* logprobs,
+                     void* workspace, void* stream);
 
 #ifdef __cplusplus
 }

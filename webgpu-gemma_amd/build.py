@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import os
 import subprocess
+from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -16,7 +17,7 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # -packed-fp32-ops: hipcc must not form v_pk_{add,mul,fma}_f32 from scalar code.
 HIP_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
              "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-SOURCES = ["gg_kernels.hip", "gg_mxfp4.hip", "gg_score.hip", "gg_decode.hip", "gg_runtime.hip"]
+SOURCES = ["gg_kernels.hip", "gg_mxfp4.hip", "gg_score.hip", "gg_kv.hip", "gg_attn.hip", "gg_verify.hip", "gg_decode.hip", "gg_runtime.hip"]
 # Per-source options: the persistent decode kernel is one long latency chain
 # at one wave per SIMD. Per step, on two boxes each:
 # - MFMA results in ordinary VGPRs rather than accumulation registers
@@ -40,12 +41,13 @@ def build_lib() -> str:
     os.makedirs(LIBDIR, exist_ok=True)
     out = os.path.join(LIBDIR, "libgg.so")
     tmp = out + ".tmp"
-    objs = []
-    for s in SOURCES:
-        o = os.path.join(LIBDIR, s.replace(".hip", ".o"))
-        _run([HIPCC, *HIP_FLAGS, *EXTRA.get(s, []), "-I", os.path.join(ROOT, "include"), "-c", os.path.join(CSRC, s),
-              "-o", o])
-        objs.append(o)
+    objs = [os.path.join(LIBDIR, s.replace(".hip", ".o")) for s in SOURCES]
+
+    def compile_one(s, o):
+        _run([HIPCC, *HIP_FLAGS, *EXTRA.get(s, []), "-I", os.path.join(ROOT, "include"), "-c", os.path.join(CSRC, s), "-o", o])
+
+    with ThreadPoolExecutor(max_workers=4) as pool:
+        list(pool.map(compile_one, SOURCES, objs))
     _run([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", tmp, *objs])
     os.replace(tmp, out)
     for o in objs:

@@ -610,4 +610,122 @@ inline ScorePlan score_plan(long long rows, int n, int top) {
 }
 int launch_score(int elem, const ScoreArgs& a, void* stream);
 
+// ---- K/V pages (gg_kv.hip), attention over them (gg_attn.hip) ------------------
+enum KvType { KV_BF16 = 0, KV_F16 = 1, KV_E4M3 = 2 };
+constexpr int kKvMaxDim = 256;
+
+// n / d for n below 2^31: n * mul >> shift, with mul = ceil(2^shift / d) and
+// shift = 31 + ceil(log2 d). mul d is at most 2^ceil(log2 d) above 2^shift, so n
+// times that stays below 2^shift.
+struct FastDiv {
+  uint32_t mul, shift;
+  __host__ __device__ uint32_t operator()(uint32_t n) const { return (uint32_t)(((uint64_t)n * mul) >> shift); }
+};
+inline FastDiv fast_div(uint32_t d) {
+  uint32_t l = 0;
+  while ((1ull << l) < d) ++l;
+  return FastDiv{(uint32_t)(((1ull << (31 + l)) + d - 1) / d), 31 + l};
+}
+
+// gg_kv_pages and gg_kv_seqs as the kernels take them.
+struct KvArgs {
+  void *k, *v;
+  float *k_scale, *v_scale;
+  long long page_stride, pos_stride, head_stride;   // elements
+  int n_pages, page_size, n_kv, dim;
+  FastDiv page_div;
+  const int32_t *row_start, *len, *table;
+  int n_seqs, n_rows, max_len, table_ld;
+  int places;           // positions that a table row covers, at most max_len
+};
+
+struct KvStoreArgs {
+  KvArgs kv;
+  const void *q, *k, *v;
+  long long ldq, ldk, ldv;
+  const float *q_norm, *k_norm;
+  double eps, log2_theta;
+  int n_q, rotate;
+  bool vec, vec_q;      // rows of the operands, of q_out, aligned to four elements
+  void* q_out;
+  long long ldqo;
+  int row0;             // first row of this launch
+};
+int launch_kv_store(int kv_type, int elem, int q_elem, const KvStoreArgs& a, void* stream);
+
+struct KvLoadArgs {
+  KvArgs kv;
+  void *k, *v;
+  long long ldk, ldv;
+  int row0;
+};
+int launch_kv_load(int kv_type, int elem, const KvLoadArgs& a, void* stream);
+
+// Attention of few rows a sequence (k_attn_few) and of many (k_attn_many).
+struct KvAttnArgs {
+  KvArgs kv;
+  const void* q;
+  long long ldq;
+  void* out;
+  long long ldo;
+  float* lse;
+  float scale2;          // softmax scale times log2(e)
+  int n_q, group;        // query heads, and those of a K/V head
+  int window, sinks;     // window 0: none
+  bool q_vec;            // q rows aligned to 16 bytes
+  int few_rows;          // sequences of at most this many rows (times group) go to k_attn_few
+  int chunk;             // keys of a block, a multiple of kKvChunk
+  int splits;            // blocks that share a tile at most
+  float *part_o, *part_ml;   // [splits][n_rows][n_q][dim]: sums not yet divided; [..][4]: reference, sum of weights as rounded, as they were
+};
+constexpr int kKvChunk = 128;       // keys of the smallest chunk: 32 for each of four waves
+constexpr int kKvFewTile = 16;      // packed rows (row, head of the group) of a block of k_attn_few
+struct KvAttnPlan {
+  int few_rows, chunk, splits;
+};
+KvAttnPlan kv_attn_plan(int n_seqs, int n_rows, int max_rows, int max_len, int n_kv, int group, int dim, int window, int sinks);
+int launch_kv_attention(int kv_type, int elem, const KvAttnArgs& a, int max_rows, void* stream);
+
+// ---- verification of drafted tokens (gg_verify.hip) ----------------------------
+// What one block found in its part of a row of logits.
+struct VerifyPart {
+  double sum;            // of e^((z - max) / T)
+  uint64_t best;         // largest logit over the complemented id
+  float max;
+  int bad;               // a NaN or +inf
+};
+// Where a sequence stops, and what the draw behind it needs.
+struct VerifyStop {
+  int row, draw;         // draw: 0 no token is drawn, 1 from p, 2 from p without the draft, 3 from max(p - q, 0)
+  float mp, mq;          // maxima
+  double sp, sq;         // sums, as the parts give them
+};
+constexpr int kVerifyTile = 4096;   // logits of a block of the 64-bit sums
+struct VerifyArgs {
+  const void *z, *y;
+  long long ldz, ldy, rows;
+  int n, n_seqs;
+  const int32_t *draft, *row_start;
+  const float* temperature;
+  const double *accept_u, *draw_u;
+  int32_t *accepted, *tokens;
+  float* logprobs;
+  int parts;             // parts of a row
+  int per;               // 16-byte units of one, 256 threads each
+  VerifyPart* part;      // [z, y][rows][parts]
+  int tiles;
+  VerifyStop* stop;      // [n_seqs]
+  double* sums;          // [n_seqs][tiles][4]: p, q where p is the larger; p, q
+  long long block0;
+};
+// 32 logits a thread, or 8 where that leaves CUs without work.
+constexpr int kVerifyLong = 32, kVerifyShort = 8;
+inline bool verify_short(long long rows, int n) { return rows * ((n + 256LL * kVerifyLong - 1) / (256 * kVerifyLong)) < 512; }
+inline int verify_parts(long long rows, int n) {
+  const int tile = 256 * (verify_short(rows, n) ? kVerifyShort : kVerifyLong);
+  return (int)(((long long)n + 7 + tile - 1) / tile);   // a row may begin up to 7 elements into its first 16 bytes
+}
+inline int verify_tiles(int n) { return (n + kVerifyTile - 1) / kVerifyTile; }
+int launch_verify(int elem, const VerifyArgs& a, void* stream);
+
 }  // namespace gg

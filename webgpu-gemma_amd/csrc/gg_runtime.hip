@@ -1944,3 +1944,208 @@ int gg_score_logits(const void* logits, uint32_t type, int64_t rows, int32_t n, 
 }
 
 }  // extern "C"
+
+// ---- K/V pages, attention over them, verification of drafts ------------------
+
+namespace {
+
+int kv_type_of(uint32_t type) {
+  switch (type) {
+    case GG_TYPE_BF16: return KV_BF16;
+    case GG_TYPE_F16: return KV_F16;
+    case GG_TYPE_E4M3: return KV_E4M3;
+  }
+  return -1;
+}
+
+// Counts up to 2^30, so that positions and rows are ints with room.
+bool count_ok(int32_t n) { return n > 0 && n <= (1 << 30); }
+
+bool kv_shape_ok(const gg_kv_pages* p, const gg_kv_seqs* s) {
+  return p && s && kv_type_of(p->type) >= 0 && count_ok(p->n_pages) && count_ok(p->page_size) && count_ok(p->n_kv_heads) &&
+         p->n_kv_heads <= 1024 && p->head_dim >= 16 && p->head_dim <= kKvMaxDim && p->head_dim % 16 == 0 &&
+         count_ok(s->n_seqs) && s->n_seqs <= (1 << 22) && count_ok(s->n_rows) && count_ok(s->max_rows) && count_ok(s->max_len) &&
+         count_ok(s->table_ld);
+}
+
+// The structures as the kernels take them; false where a call is refused.
+bool kv_args(const gg_kv_pages* p, const gg_kv_seqs* s, KvArgs* a) {
+  if (!kv_shape_ok(p, s)) return false;
+  const int t = kv_type_of(p->type);
+  const int64_t unit = t == KV_E4M3 ? 16 : 8;   // elements of 16 bytes
+  if (!p->k || !p->v || !aligned_to(p->k, 16) || !aligned_to(p->v, 16) || p->page_stride % unit || p->pos_stride % unit ||
+      p->head_stride % unit || (p->n_pages > 1 && p->page_stride < p->head_dim) ||
+      (p->page_size > 1 && p->pos_stride < p->head_dim) || (p->n_kv_heads > 1 && p->head_stride < p->head_dim) ||
+      p->page_stride < 0 || p->pos_stride < 0 || p->head_stride < 0 || p->page_stride > (1LL << 50) ||
+      p->pos_stride > (1LL << 50) || p->head_stride > (1LL << 50) ||
+      (t == KV_E4M3 && (!p->k_scale || !p->v_scale || !aligned_to(p->k_scale, 4) || !aligned_to(p->v_scale, 4))) ||
+      !s->row_start || !s->len || !s->table || !aligned_to(s->row_start, 4) || !aligned_to(s->len, 4) || !aligned_to(s->table, 4))
+    return false;
+  *a = KvArgs{};
+  a->k = p->k;
+  a->v = p->v;
+  a->k_scale = p->k_scale;
+  a->v_scale = p->v_scale;
+  a->page_stride = p->page_stride;
+  a->pos_stride = p->pos_stride;
+  a->head_stride = p->head_stride;
+  a->n_pages = p->n_pages;
+  a->page_size = p->page_size;
+  a->n_kv = p->n_kv_heads;
+  a->dim = p->head_dim;
+  a->page_div = fast_div((uint32_t)p->page_size);
+  a->row_start = s->row_start;
+  a->len = s->len;
+  a->table = s->table;
+  a->n_seqs = s->n_seqs;
+  a->n_rows = s->n_rows;
+  a->max_len = s->max_len;
+  a->table_ld = s->table_ld;
+  a->places = (int)std::min<int64_t>(s->max_len, (int64_t)s->table_ld * p->page_size);
+  return true;
+}
+
+bool attn_shape_ok(const gg_kv_pages* p, const gg_kv_seqs* s, int32_t n_q_heads, int32_t window, int32_t sinks) {
+  return kv_shape_ok(p, s) && n_q_heads > 0 && n_q_heads <= (1 << 16) && n_q_heads % p->n_kv_heads == 0 &&
+         (int64_t)s->n_rows * n_q_heads <= (1LL << 30) && window >= 0 && sinks >= 0 && window <= (1 << 30) && sinks <= (1 << 30);
+}
+KvAttnPlan attn_plan(const gg_kv_pages* p, const gg_kv_seqs* s, int32_t n_q_heads, int32_t window, int32_t sinks) {
+  return kv_attn_plan(s->n_seqs, s->n_rows, s->max_rows, s->max_len, p->n_kv_heads, n_q_heads / p->n_kv_heads, p->head_dim, window,
+                      sinks);
+}
+
+}  // namespace
+
+extern "C" {
+
+int gg_kv_store(const gg_kv_pages* pages, const gg_kv_seqs* seqs, uint32_t type, const void* q, int64_t ldq, const void* k,
+                int64_t ldk, const void* v, int64_t ldv, int32_t n_q_heads, const float* q_norm, const float* k_norm,
+                double eps, double rope_theta, void* q_out, uint32_t q_out_type, int64_t ldqo, void* stream) {
+  KvStoreArgs a{};
+  const int e = elem_of(type), qe = q ? elem_of(q_out_type) : ELEM_F32;
+  if (!kv_args(pages, seqs, &a.kv) || e < 0 || qe < 0 || !k || !v || n_q_heads < 0 || n_q_heads > (1 << 16) ||
+      (q != nullptr) != (n_q_heads > 0) || !(eps >= 0) || !(rope_theta >= 0) || !std::isfinite(eps) || !std::isfinite(rope_theta))
+    return GG_ERR_INVALID;
+  const size_t es = elem_size(e), qs = elem_size(qe);
+  const int64_t kv_width = (int64_t)a.kv.n_kv * a.kv.dim, q_width = (int64_t)n_q_heads * a.kv.dim;
+  if (ldk < kv_width || ldv < kv_width || !aligned_to(k, es) || !aligned_to(v, es) || !aligned_to(q_norm, 4) || !aligned_to(k_norm, 4) ||
+      (q && (!q_out || ldq < q_width || ldqo < q_width || !aligned_to(q, es) || !aligned_to(q_out, qs))) || !stream_here(stream))
+    return GG_ERR_INVALID;
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.ldq = ldq;
+  a.ldk = ldk;
+  a.ldv = ldv;
+  a.q_norm = q_norm;
+  a.k_norm = k_norm;
+  a.eps = eps;
+  a.rotate = rope_theta > 0;
+  a.log2_theta = a.rotate ? std::log2(rope_theta) : 0.0;
+  a.n_q = n_q_heads;
+  a.vec = aligned_to(k, 4 * es) && aligned_to(v, 4 * es) && ldk % 4 == 0 && ldv % 4 == 0 &&
+          (!q || (aligned_to(q, 4 * es) && ldq % 4 == 0));
+  a.q_out = q_out;
+  a.ldqo = ldqo;
+  a.vec_q = q && aligned_to(q_out, 4 * qs) && ldqo % 4 == 0;
+  return launch_kv_store(kv_type_of(pages->type), e, qe, a, stream) ? GG_ERR_HIP : GG_OK;
+}
+
+int gg_kv_load(const gg_kv_pages* pages, const gg_kv_seqs* seqs, void* k_out, int64_t ldk, void* v_out, int64_t ldv,
+               uint32_t type, void* stream) {
+  KvLoadArgs a{};
+  const int e = elem_of(type);
+  if (!kv_args(pages, seqs, &a.kv) || e < 0 || (!k_out && !v_out)) return GG_ERR_INVALID;
+  const int64_t width = (int64_t)a.kv.n_kv * a.kv.dim;
+  if ((k_out && (ldk < width || !aligned_to(k_out, elem_size(e)))) || (v_out && (ldv < width || !aligned_to(v_out, elem_size(e)))) ||
+      !stream_here(stream))
+    return GG_ERR_INVALID;
+  a.k = k_out;
+  a.v = v_out;
+  a.ldk = ldk;
+  a.ldv = ldv;
+  return launch_kv_load(kv_type_of(pages->type), e, a, stream) ? GG_ERR_HIP : GG_OK;
+}
+
+size_t gg_kv_attention_workspace_size(const gg_kv_pages* pages, const gg_kv_seqs* seqs, int32_t n_q_heads, int32_t window,
+                                      int32_t sinks) {
+  if (!attn_shape_ok(pages, seqs, n_q_heads, window, sinks)) return 0;
+  const KvAttnPlan p = attn_plan(pages, seqs, n_q_heads, window, sinks);
+  return p.splits == 1 ? 0 : (size_t)p.splits * seqs->n_rows * n_q_heads * (pages->head_dim + 4) * 4;
+}
+
+int gg_kv_attention(const gg_kv_pages* pages, const gg_kv_seqs* seqs, const void* q, uint32_t type, int64_t ldq,
+                    int32_t n_q_heads, float scale, int32_t window, int32_t sinks, void* out, int64_t ldo, float* lse,
+                    void* workspace, void* stream) {
+  KvAttnArgs a{};
+  const int e = elem_of(type);
+  if (!kv_args(pages, seqs, &a.kv) || !attn_shape_ok(pages, seqs, n_q_heads, window, sinks) || e < 0 || !q || !out ||
+      (pages->type == GG_TYPE_F16 && type != GG_TYPE_F16) || !std::isfinite(scale))
+    return GG_ERR_INVALID;
+  const int64_t width = (int64_t)n_q_heads * a.kv.dim;
+  if (ldq < width || ldo < width || !aligned_to(q, elem_size(e)) || !aligned_to(out, elem_size(e)) || !aligned_to(lse, 4) ||
+      !stream_here(stream))
+    return GG_ERR_INVALID;
+  const KvAttnPlan p = attn_plan(pages, seqs, n_q_heads, window, sinks);
+  if (p.splits > 1 && (!workspace || !aligned_to(workspace, 16))) return GG_ERR_INVALID;
+  a.q = q;
+  a.ldq = ldq;
+  a.out = out;
+  a.ldo = ldo;
+  a.lse = lse;
+  a.scale2 = scale * 1.4426950408889634f;
+  a.n_q = n_q_heads;
+  a.group = n_q_heads / a.kv.n_kv;
+  a.window = window;
+  a.sinks = sinks;
+  a.q_vec = aligned_to(q, 16) && ldq * (int64_t)elem_size(e) % 16 == 0;
+  a.few_rows = p.few_rows;
+  a.chunk = p.chunk;
+  a.splits = p.splits;
+  a.part_o = (float*)workspace;
+  a.part_ml = a.part_o + (size_t)p.splits * seqs->n_rows * n_q_heads * a.kv.dim;
+  return launch_kv_attention(kv_type_of(pages->type), e, a, seqs->max_rows, stream) ? GG_ERR_HIP : GG_OK;
+}
+
+size_t gg_verify_drafts_workspace_size(int64_t rows, int32_t n_seqs, int32_t n) {
+  if (rows <= 0 || rows > (1LL << 30) || !count_ok(n) || n_seqs <= 0 || n_seqs > (1 << 22)) return 0;
+  return (size_t)rows * 2 * verify_parts(rows, n) * sizeof(VerifyPart) + (size_t)n_seqs * verify_tiles(n) * 32 +
+         (size_t)n_seqs * sizeof(VerifyStop);
+}
+
+int gg_verify_drafts(const void* z, const void* y, uint32_t type, int64_t rows, int32_t n, int64_t ldz, int64_t ldy,
+                     const int32_t* draft, const int32_t* row_start, int32_t n_seqs, const float* temperature,
+                     const double* accept_u, const double* draw_u, int32_t* accepted, int32_t* tokens, float* logprobs,
+                     void* workspace, void* stream) {
+  const int e = elem_of(type);
+  if (!z || e < 0 || gg_verify_drafts_workspace_size(rows, n_seqs, n) == 0 || ldz < n || (y && ldy < n) || !draft || !row_start ||
+      !temperature || !accept_u || !draw_u || !accepted || !tokens || !workspace || !aligned_to(z, elem_size(e)) ||
+      !aligned_to(y, elem_size(e)) || !aligned_to(draft, 4) || !aligned_to(row_start, 4) || !aligned_to(temperature, 4) ||
+      !aligned_to(accept_u, 8) || !aligned_to(draw_u, 8) || !aligned_to(accepted, 4) || !aligned_to(tokens, 4) ||
+      !aligned_to(logprobs, 4) || !aligned_to(workspace, 16) || !stream_here(stream))
+    return GG_ERR_INVALID;
+  VerifyArgs a{};
+  a.z = z;
+  a.y = y;
+  a.ldz = ldz;
+  a.ldy = ldy;
+  a.rows = rows;
+  a.n = n;
+  a.n_seqs = n_seqs;
+  a.draft = draft;
+  a.row_start = row_start;
+  a.temperature = temperature;
+  a.accept_u = accept_u;
+  a.draw_u = draw_u;
+  a.accepted = accepted;
+  a.tokens = tokens;
+  a.logprobs = logprobs;
+  a.parts = verify_parts(rows, n);
+  a.tiles = verify_tiles(n);
+  a.part = (VerifyPart*)workspace;
+  a.sums = (double*)(a.part + 2 * (size_t)rows * a.parts);
+  a.stop = (VerifyStop*)(a.sums + 4 * (size_t)n_seqs * a.tiles);
+  return launch_verify(e, a, stream) ? GG_ERR_HIP : GG_OK;
+}
+
+}  // extern "C"

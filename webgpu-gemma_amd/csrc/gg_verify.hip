@@ -1,0 +1,460 @@
+// gg_verify.hip -- drafted tokens against the target's logits.
+//
+// With p = softmax(z / T) of a row and q the softmax(y / T) that its draft d was
+// drawn from, d stands with probability min(1, p(d) / q(d)); else the token is
+// drawn from max(p - q, 0): p again in all. Without y, q is 1 at d.
+//
+// Three launches. k_verify_stat reads all rows once: each part's maximum, sum
+// of e^((z - m) / T) and best logit. k_verify_sums finds, in every block, the
+// row at which its sequence stops, and sums that row's weights in f64,
+// kVerifyTile logits a block. k_verify_draw finds the tile and the token that
+// the draw falls on.
+//
+// The draw picks among borders that lie closer than f32 tells apart: with f32
+// sums one draw in a hundred over 262144 logits gives a neighbour of the
+// right token. So all that a draw compares is f64. Whether p exceeds q at a token is taken from
+// the sums of the first launch (2^-22 off): that changes the sum over them in the
+// second order only, and their scale is put right afterwards, since
+// sum (p - q) over a set = sum p - c sum q with any c.
+#include "gg_kv_device.h"
+
+namespace gg {
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ uint64_t logit_key(float z, int i) {
+  const uint32_t b = __float_as_uint(z + 0.0f);   // -0 counts as 0
+  return ((uint64_t)(b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u)) << 32) | (0xffffffffu - (uint32_t)i);
+}
+__device__ __forceinline__ uint64_t shfl_xor64(uint64_t x, int o) {
+  return ((uint64_t)(uint32_t)__shfl_xor((int)(x >> 32), o, 64) << 32) | (uint32_t)__shfl_xor((int)x, o, 64);
+}
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+// Temperature of a sequence; 0 (or what is none): greedy.
+__device__ __forceinline__ bool greedy(float t) { return !(t > 0.f); }
+
+// One block: part blockIdx % parts of a row of z, or of y behind all of z's.
+template <class T, int EPT>
+__global__ __launch_bounds__(256) void k_verify_stat(VerifyArgs a) {
+  constexpr int VE = 16 / sizeof(T), NV = EPT / VE;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const long long at = a.block0 + blockIdx.x;
+  long long row = at / a.parts;
+  const int part = (int)(at - row * a.parts);
+  const bool draft = row >= a.rows;
+  if (draft) row -= a.rows;
+  const int s = last_at_most(a.n_seqs, [&](int i) { return a.row_start[i] <= row; });
+  if (s < 0) return;
+  const int end = a.row_start[s + 1];
+  const float t = a.temperature[s];
+  if (row >= end || (draft && (row == end - 1 || greedy(t)))) return;   // no row of y
+  const float c = greedy(t) ? kLog2e : kLog2e / t;
+  const T* z = draft ? (const T*)a.y + row * a.ldy : (const T*)a.z + row * a.ldz;
+  const int shift = (int)(((uintptr_t)z & 15) / sizeof(T));
+  const T* z0 = z - shift;
+  typedef T vec_t __attribute__((ext_vector_type(VE)));
+  float v[EPT];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const long long e0 = ((long long)part * 256 * NV + i * 256 + tid) * VE - shift;
+    if (e0 >= 0 && e0 + VE <= a.n) {
+      const vec_t x = __builtin_nontemporal_load((const vec_t*)(z + e0));
+#pragma unroll
+      for (int e = 0; e < VE; ++e) v[i * VE + e] = (float)x[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) v[i * VE + e] = e0 + e >= 0 && e0 + e < a.n ? (float)z[e0 + e] : -INFINITY;
+    }
+  }
+  float m = -INFINITY;
+  uint64_t best = 0;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < EPT; ++i) {
+    bad |= !(v[i] < INFINITY);
+    m = fmaxf(m, v[i]);
+  }
+#pragma unroll
+  for (int i = EPT - 1; i >= 0; --i)
+    if (v[i] == m) best = logit_key(m, (int)(((long long)part * 256 * NV + (i / VE) * 256 + tid) * VE - shift) + i % VE);
+  __shared__ float ms[4];
+  __shared__ double ss[4];
+  __shared__ uint64_t bs[4];
+  __shared__ int bads[4];
+  const float wm = wave_max(m);
+  if (lane == 0) ms[tid >> 6] = wm;
+  __syncthreads();
+  m = fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3]));
+  const float ref = m == -INFINITY ? 0.f : m;
+  float sum[4] = {};
+#pragma unroll
+  for (int i = 0; i < EPT; ++i) sum[i & 3] += __builtin_amdgcn_exp2f((v[i] - ref) * c);
+  const double total = wave_sum((double)((sum[0] + sum[1]) + (sum[2] + sum[3])));
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const uint64_t x = shfl_xor64(best, o);
+    best = x > best ? x : best;
+  }
+  const int any = __ballot(bad) != 0;
+  if (lane == 0) {
+    ss[tid >> 6] = total;
+    bs[tid >> 6] = best;
+    bads[tid >> 6] = any;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    VerifyPart p;
+    p.sum = (ss[0] + ss[1]) + (ss[2] + ss[3]);
+    p.best = bs[0];
+#pragma unroll
+    for (int i = 1; i < 4; ++i) p.best = bs[i] > p.best ? bs[i] : p.best;
+    p.max = m;
+    p.bad = bads[0] | bads[1] | bads[2] | bads[3];
+    a.part[at] = p;
+  }
+}
+
+// A row's parts together, in every lane of a wave.
+struct Row {
+  float m;
+  double sum;
+  uint64_t best;
+  bool bad;
+};
+__device__ Row join_parts(const VerifyPart* p, int n, double heat) {
+  const int lane = threadIdx.x & 63;
+  Row r{-INFINITY, 0.0, 0, false};
+  int bad = 0;
+  for (int i = lane; i < n; i += 64) {
+    r.m = fmaxf(r.m, p[i].max);
+    r.best = p[i].best > r.best ? p[i].best : r.best;
+    bad |= p[i].bad;
+  }
+  r.m = wave_max(r.m);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const uint64_t x = shfl_xor64(r.best, o);
+    r.best = x > r.best ? x : r.best;
+  }
+  for (int i = lane; i < n; i += 64)
+    if (p[i].max > -INFINITY) r.sum += p[i].sum * exp(((double)p[i].max - r.m) / heat);
+  r.sum = wave_sum(r.sum);
+  r.bad = __ballot(bad) != 0 || r.m == -INFINITY;
+  return r;
+}
+
+struct Decision {
+  VerifyStop stop;
+  int first, end, token;   // token: the one at the stop where none is drawn
+  bool greedy;
+};
+
+// Where sequence s stops: four rows at a time, one a wave, up to the first that
+// stops. The block with `write` also reports the rows before.
+template <class T>
+__device__ Decision decide(const VerifyArgs& a, int s, bool write) {
+  __shared__ VerifyStop stops[4];
+  __shared__ int halts[4], tokens[4];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  Decision d{};
+  d.first = (int)min(max((long long)a.row_start[s], 0ll), a.rows);
+  d.end = (int)min(max((long long)a.row_start[s + 1], 0ll), a.rows);
+  const float t = a.temperature[s];
+  d.greedy = greedy(t);
+  const double heat = d.greedy ? 1.0 : (double)t;
+  d.stop.row = -1;
+  for (int r0 = d.first; r0 < d.end; r0 += 4) {
+    const int row = r0 + wv;
+    if (row < d.end) {
+      const bool last = row == d.end - 1;
+      const Row p = join_parts(a.part + (long long)row * a.parts, a.parts, heat);
+      const int id = last ? -1 : a.draft[row];
+      const bool real = id >= 0 && id < a.n;
+      VerifyStop st{row, 0, p.m, 0.f, p.sum, 0.0};
+      const int best = (int)(0xffffffffu - (uint32_t)p.best);
+      bool halt = last, bad = p.bad;
+      int token = best;
+      const double z_id = real ? (double)(float)((const T*)a.z)[row * a.ldz + id] : 0.0;
+      if (d.greedy) {
+        halt |= id != best;
+      } else {
+        double q = 1.0;
+        if (a.y && !last) {
+          const Row y = join_parts(a.part + (a.rows + (long long)row) * a.parts, a.parts, heat);
+          bad |= y.bad;
+          st.mq = y.m;
+          st.sq = y.sum;
+          q = real ? exp(((double)(float)((const T*)a.y)[row * a.ldy + id] - y.m) / heat) / y.sum : 0.0;
+        }
+        const bool stands = real && !last && a.accept_u[row] * q < exp((z_id - p.m) / heat) / p.sum;
+        halt |= !stands;
+        if (halt) st.draw = last ? 1 : a.y ? 3 : 2;
+      }
+      if (bad) {
+        halt = true;
+        token = -1;
+        st.draw = 0;
+      }
+      if (lane == 0) {
+        stops[wv] = st;
+        halts[wv] = halt;
+        tokens[wv] = halt ? token : id;
+        // whether an earlier wave's row stops is not known yet: what is written here for
+        // rows behind the stop is written over below
+        if (write) {
+          const double z = halt ? (double)p.m : z_id;
+          if (a.logprobs) a.logprobs[row] = bad ? NAN : (float)((z - p.m) / heat - log(p.sum));
+          a.tokens[row] = halt ? token : id;
+        }
+      }
+    } else if (lane == 0) {
+      halts[wv] = 0;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 3; i >= 0; --i)
+      if (halts[i]) {
+        d.stop = stops[i];
+        d.token = tokens[i];
+      }
+    __syncthreads();
+    if (d.stop.row >= 0) break;
+  }
+  return d;
+}
+
+// The weights of 16 logits from e0 on, f64: of p, and of q where it counts.
+template <class T>
+__device__ __forceinline__ void load16(const T* row, long long e0, int n, float (&v)[16]) {
+  constexpr int VE = 16 / sizeof(T);
+  typedef T vec_t __attribute__((ext_vector_type(VE)));
+  if (e0 + 16 <= n && ((uintptr_t)(row + e0) & 15) == 0) {
+#pragma unroll
+    for (int i = 0; i < 16; i += VE) {
+      const vec_t x = *(const vec_t*)(row + e0 + i);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) v[i + e] = (float)x[e];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = e0 + i < n ? (float)row[e0 + i] : -INFINITY;
+  }
+}
+__device__ __forceinline__ double weight(float z, float m, double inv_heat) { return exp(((double)z - (double)m) * inv_heat); }
+
+// Block = a tile of a sequence's stop row.
+template <class T>
+__global__ __launch_bounds__(256) void k_verify_sums(VerifyArgs a) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  const long long at = a.block0 + blockIdx.x;
+  const int s = (int)(at / a.tiles), tile = (int)(at - (long long)s * a.tiles);
+  const Decision d = decide<T>(a, s, tile == 0);
+  if (tile == 0) {
+    if (tid == 0) {
+      a.accepted[s] = d.stop.row >= 0 ? d.stop.row - d.first : 0;
+      a.stop[s] = d.stop;
+    }
+    if (d.stop.row >= 0)
+      for (long long r = d.stop.row + 1ll + tid; r < d.end; r += 256) {
+        a.tokens[r] = -1;
+        if (a.logprobs) a.logprobs[r] = 0.f;
+      }
+  }
+  const VerifyStop& st = d.stop;
+  if (st.row < 0 || st.draw == 0) return;
+  const double inv_heat = 1.0 / (double)a.temperature[s];
+  const long long e0 = (long long)tile * kVerifyTile + 16 * tid;
+  const bool both = st.draw == 3;
+  const int skip = st.draw == 2 ? a.draft[st.row] : -1;
+  double sum[4] = {};
+  if (e0 < a.n) {
+    float z[16], y[16];
+    load16((const T*)a.z + st.row * a.ldz, e0, a.n, z);
+    if (both) load16((const T*)a.y + st.row * a.ldy, e0, a.n, y);
+#pragma unroll 4
+    for (int i = 0; i < 16; ++i) {
+      const double p = weight(z[i], st.mp, inv_heat);
+      sum[2] += p;
+      if (both) {
+        const double q = weight(y[i], st.mq, inv_heat);
+        sum[3] += q;
+        if (p * st.sq > q * st.sp) {
+          sum[0] += p;
+          sum[1] += q;
+        }
+      } else if (e0 + i != skip) {
+        sum[0] += p;
+      }
+    }
+  }
+  __shared__ double part[4][4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const double x = wave_sum(sum[k]);
+    if (lane == 0) part[tid >> 6][k] = x;
+  }
+  __syncthreads();
+  if (tid < 4) a.sums[(at * 4) + tid] = (part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid]);
+}
+
+// Inclusive sums over the block's 256 threads in order.
+__device__ double block_scan(double v, double* sh, double* total) {
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  double x = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const double up = __shfl_up(x, o, 64);
+    if (lane >= o) x += up;
+  }
+  __syncthreads();
+  if (lane == 63) sh[wv] = x;
+  __syncthreads();
+  double before = 0;
+  for (int i = 0; i < wv; ++i) before += sh[i];
+  *total = ((sh[0] + sh[1]) + sh[2]) + sh[3];
+  return before + x;
+}
+
+// One block per sequence: the token that the draw falls on.
+template <class T>
+__global__ __launch_bounds__(256) void k_verify_draw(VerifyArgs a, int seq0) {
+  __shared__ double sh[4];
+  __shared__ int hit, last;
+  __shared__ double rest;
+  const int tid = threadIdx.x, s = seq0 + blockIdx.x;
+  const VerifyStop st = a.stop[s];
+  if (st.row < 0 || st.draw == 0) return;
+  const double* sums = a.sums + (long long)s * a.tiles * 4;
+  const int per = (a.tiles + 255) / 256, t0 = min(tid * per, a.tiles), t1 = min(t0 + per, a.tiles);
+  // the sums of all p and q first: their quotient scales q
+  double p_all = 0, q_all = 0;
+  for (int t = t0; t < t1; ++t) {
+    p_all += sums[4 * t + 2];
+    q_all += sums[4 * t + 3];
+  }
+  double p_sum, q_sum, all;
+  block_scan(p_all, sh, &p_sum);
+  block_scan(q_all, sh, &q_sum);
+  const double c = st.draw == 3 ? p_sum / q_sum : 0.0;
+  double mine = 0;
+  auto tile_weight = [&](int t) { return fmax(sums[4 * t] - c * sums[4 * t + 1], 0.0); };
+  for (int t = t0; t < t1; ++t) mine += tile_weight(t);
+  double up_to = block_scan(mine, sh, &all);
+  const bool plain = st.draw == 1 || !(all > 0.0);   // nothing left: from p
+  if (plain) {
+    mine = p_all;
+    up_to = block_scan(mine, sh, &all);
+  }
+  const double target = a.draw_u[s] * all;
+  if (tid == 0) {
+    hit = a.tiles;
+    last = -1;
+  }
+  __syncthreads();
+  {
+    // the first tile whose sums pass the target, and the last with any weight
+    double x = up_to - mine;
+    int first = a.tiles, some = -1;
+    double before = 0;
+    for (int t = t0; t < t1; ++t) {
+      const double w = plain ? sums[4 * t + 2] : tile_weight(t);
+      if (w > 0) some = t;
+      if (first == a.tiles && w > 0 && x + w > target) {
+        first = t;
+        before = x;
+      }
+      x += w;
+    }
+    if (first < a.tiles) atomicMin(&hit, first);
+    atomicMax(&last, some);
+    __syncthreads();
+    if (first < a.tiles && first == hit) rest = target - before;
+    if (hit == a.tiles && tid == 0) rest = INFINITY;   // rounding left none: the last weight
+    __syncthreads();
+  }
+  const int tile = hit < a.tiles ? hit : max(last, 0);
+  const double within = rest;
+  const double inv_heat = 1.0 / (double)a.temperature[s];
+  const long long e0 = (long long)tile * kVerifyTile + 16 * tid;
+  const int skip = st.draw == 2 && !plain ? a.draft[st.row] : -1;
+  double w[16];
+  mine = 0;
+  {
+    float z[16], y[16];
+    load16((const T*)a.z + st.row * a.ldz, e0, a.n, z);
+    if (st.draw == 3 && !plain) load16((const T*)a.y + st.row * a.ldy, e0, a.n, y);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      w[i] = weight(z[i], st.mp, inv_heat);
+      if (st.draw == 3 && !plain) w[i] = fmax(w[i] - c * weight(y[i], st.mq, inv_heat), 0.0);
+      if (e0 + i == skip || e0 + i >= a.n) w[i] = 0;
+      mine += w[i];
+    }
+  }
+  __syncthreads();
+  up_to = block_scan(mine, sh, &all);
+  if (tid == 0) {
+    hit = 0x7fffffff;
+    last = -1;
+  }
+  __syncthreads();
+  double x = up_to - mine;
+  int first = 0x7fffffff, some = -1;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    if (w[i] > 0) some = (int)(e0 + i);
+    x += w[i];
+    if (first == 0x7fffffff && w[i] > 0 && x > within) first = (int)(e0 + i);
+  }
+  atomicMin(&hit, first);
+  atomicMax(&last, some);
+  __syncthreads();
+  if (tid == 0) {
+    const int token = hit != 0x7fffffff ? hit : max(last, 0);
+    a.tokens[st.row] = token;
+    if (a.logprobs)
+      a.logprobs[st.row] = (float)(((double)(float)((const T*)a.z)[st.row * a.ldz + token] - (double)st.mp) * inv_heat - log(p_sum));
+  }
+}
+
+template <class T>
+int verify_t(VerifyArgs a, hipStream_t s) {
+  constexpr long long MOST = (1 << 24) - 1;   // a grid holds fewer than 2^32 threads
+  const bool few = verify_short(a.rows, a.n);
+  const long long stats = (a.y ? 2 : 1) * a.rows * a.parts;
+  for (a.block0 = 0; a.block0 < stats; a.block0 += MOST) {
+    const unsigned n = (unsigned)(stats - a.block0 < MOST ? stats - a.block0 : MOST);
+    if (few) hipLaunchKernelGGL((k_verify_stat<T, kVerifyShort>), dim3(n), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_verify_stat<T, kVerifyLong>), dim3(n), dim3(256), 0, s, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return (int)e;
+  }
+  const long long sums = (long long)a.n_seqs * a.tiles;
+  for (a.block0 = 0; a.block0 < sums; a.block0 += MOST) {
+    hipLaunchKernelGGL((k_verify_sums<T>), dim3((unsigned)(sums - a.block0 < MOST ? sums - a.block0 : MOST)), dim3(256), 0, s, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return (int)e;
+  }
+  hipLaunchKernelGGL((k_verify_draw<T>), dim3((unsigned)a.n_seqs), dim3(256), 0, s, a, 0);
+  return (int)hipGetLastError();
+}
+
+}  // namespace
+
+int launch_verify(int elem, const VerifyArgs& a, void* stream) {
+  switch (elem) {
+    case ELEM_F32: return verify_t<float>(a, (hipStream_t)stream);
+    case ELEM_F16: return verify_t<_Float16>(a, (hipStream_t)stream);
+    case ELEM_BF16: return verify_t<__bf16>(a, (hipStream_t)stream);
+  }
+  return (int)hipErrorInvalidValue;
+}
+
+}  // namespace gg

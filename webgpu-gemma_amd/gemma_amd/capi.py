@@ -27,6 +27,7 @@ GG_TYPE_F16 = 1
 GG_TYPE_Q8_0 = 8
 GG_TYPE_BF16 = 30
 GG_TYPE_MXFP4 = 39
+GG_TYPE_E4M3 = 256
 
 GG_ATTN_REFERENCE = 0
 GG_ATTN_GEMMA3 = 1
@@ -74,6 +75,36 @@ class GGSample(ctypes.Structure):
         ("temperature", ctypes.c_double),
         ("top_p", ctypes.c_double),
         ("rep_penalty", ctypes.c_double),
+    ]
+
+
+class GGKvPages(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("page_stride", ctypes.c_int64),
+        ("pos_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+        ("type", ctypes.c_uint32),
+        ("n_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("n_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+    ]
+
+
+class GGKvSeqs(ctypes.Structure):
+    _fields_ = [
+        ("row_start", ctypes.c_void_p),
+        ("len", ctypes.c_void_p),
+        ("table", ctypes.c_void_p),
+        ("n_seqs", ctypes.c_int32),
+        ("n_rows", ctypes.c_int32),
+        ("max_rows", ctypes.c_int32),
+        ("max_len", ctypes.c_int32),
+        ("table_ld", ctypes.c_int32),
     ]
 
 
@@ -133,6 +164,18 @@ _SIGS = {
     "gg_score_workspace_size": (ctypes.c_size_t, [_I64, ctypes.c_int32, ctypes.c_int32]),
     "gg_score_logits": (ctypes.c_int, [_P, ctypes.c_uint32, _I64, ctypes.c_int32, _I64, _P, ctypes.c_int32, _P, _P, _P,
                                        ctypes.c_int32, _P, _P, _P, _P]),
+    "gg_kv_store": (ctypes.c_int, [ctypes.POINTER(GGKvPages), ctypes.POINTER(GGKvSeqs), ctypes.c_uint32, _P, _I64, _P, _I64,
+                                   _P, _I64, ctypes.c_int32, _P, _P, ctypes.c_double, ctypes.c_double, _P, ctypes.c_uint32,
+                                   _I64, _P]),
+    "gg_kv_load": (ctypes.c_int, [ctypes.POINTER(GGKvPages), ctypes.POINTER(GGKvSeqs), _P, _I64, _P, _I64, ctypes.c_uint32,
+                                  _P]),
+    "gg_kv_attention_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(GGKvPages), ctypes.POINTER(GGKvSeqs), ctypes.c_int32,
+                                                         ctypes.c_int32, ctypes.c_int32]),
+    "gg_kv_attention": (ctypes.c_int, [ctypes.POINTER(GGKvPages), ctypes.POINTER(GGKvSeqs), _P, ctypes.c_uint32, _I64,
+                                       ctypes.c_int32, ctypes.c_float, ctypes.c_int32, ctypes.c_int32, _P, _I64, _P, _P, _P]),
+    "gg_verify_drafts_workspace_size": (ctypes.c_size_t, [_I64, ctypes.c_int32, ctypes.c_int32]),
+    "gg_verify_drafts": (ctypes.c_int, [_P, _P, ctypes.c_uint32, _I64, ctypes.c_int32, _I64, _I64, _P, _P, ctypes.c_int32, _P,
+                                        _P, _P, _P, _P, _P, _P, _P]),
 }
 
 
@@ -395,3 +438,61 @@ def score_logits(logits_ptr: int, ggml_type: int, rows: int, n: int, ld: int, id
                                        id_logprobs_ptr or None, lse_ptr or None, entropy_ptr or None, top_n,
                                        top_ids_ptr or None, top_logprobs_ptr or None, ws_ptr or None,
                                        _stream_ptr(stream)))
+
+
+def kv_pages(k_ptr: int, v_ptr: int, ggml_type: int, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int,
+             page_stride: int | None = None, pos_stride: int | None = None, head_stride: int | None = None,
+             k_scale: int | None = None, v_scale: int | None = None) -> GGKvPages:
+    """A pool of K/V pages; strides in elements, [page][place][head][head_dim] without gaps where they are not given."""
+    head = head_dim if head_stride is None else head_stride
+    pos = n_kv_heads * head_dim if pos_stride is None else pos_stride
+    page = page_size * n_kv_heads * head_dim if page_stride is None else page_stride
+    return GGKvPages(k_ptr, v_ptr, k_scale or None, v_scale or None, page, pos, head, ggml_type, n_pages, page_size,
+                     n_kv_heads, head_dim)
+
+
+def kv_seqs(row_start_ptr: int, len_ptr: int, table_ptr: int, n_seqs: int, n_rows: int, max_rows: int, max_len: int,
+            table_ld: int) -> GGKvSeqs:
+    """The sequences of a call (device arrays), with the host's bounds."""
+    return GGKvSeqs(row_start_ptr, len_ptr, table_ptr, n_seqs, n_rows, max_rows, max_len, table_ld)
+
+
+def kv_store(pages: GGKvPages, seqs: GGKvSeqs, ggml_type: int, q_ptr: int | None, ldq: int, k_ptr: int, ldk: int, v_ptr: int,
+             ldv: int, n_q_heads: int, q_norm_ptr: int | None, k_norm_ptr: int | None, eps: float, rope_theta: float,
+             q_out_ptr: int | None, q_out_type: int, ldqo: int, stream=None):
+    """Norm and rotation of new rows; q to q_out, k and v into their pages."""
+    _check(None, lib().gg_kv_store(ctypes.byref(pages), ctypes.byref(seqs), ggml_type, q_ptr or None, ldq, k_ptr, ldk, v_ptr,
+                                   ldv, n_q_heads, q_norm_ptr or None, k_norm_ptr or None, eps, rope_theta, q_out_ptr or None,
+                                   q_out_type, ldqo, _stream_ptr(stream)))
+
+
+def kv_load(pages: GGKvPages, seqs: GGKvSeqs, k_out_ptr: int | None, ldk: int, v_out_ptr: int | None, ldv: int,
+            ggml_type: int, stream=None):
+    """The values that the rows' places hold."""
+    _check(None, lib().gg_kv_load(ctypes.byref(pages), ctypes.byref(seqs), k_out_ptr or None, ldk, v_out_ptr or None, ldv,
+                                  ggml_type, _stream_ptr(stream)))
+
+
+def kv_attention_workspace_size(pages: GGKvPages, seqs: GGKvSeqs, n_q_heads: int, window: int = 0, sinks: int = 0) -> int:
+    return int(lib().gg_kv_attention_workspace_size(ctypes.byref(pages), ctypes.byref(seqs), n_q_heads, window, sinks))
+
+
+def kv_attention(pages: GGKvPages, seqs: GGKvSeqs, q_ptr: int, ggml_type: int, ldq: int, n_q_heads: int, scale: float,
+                 window: int, sinks: int, out_ptr: int, ldo: int, lse_ptr: int | None = None, ws_ptr: int | None = None,
+                 stream=None):
+    """Attention of each sequence's new rows over its pages, all of them or a window and a few first positions."""
+    _check(None, lib().gg_kv_attention(ctypes.byref(pages), ctypes.byref(seqs), q_ptr, ggml_type, ldq, n_q_heads, scale, window,
+                                       sinks, out_ptr, ldo, lse_ptr or None, ws_ptr or None, _stream_ptr(stream)))
+
+
+def verify_drafts_workspace_size(rows: int, n_seqs: int, n: int) -> int:
+    return int(lib().gg_verify_drafts_workspace_size(rows, n_seqs, n))
+
+
+def verify_drafts(z_ptr: int, y_ptr: int | None, ggml_type: int, rows: int, n: int, ldz: int, ldy: int, draft_ptr: int,
+                  row_start_ptr: int, n_seqs: int, temperature_ptr: int, accept_u_ptr: int, draw_u_ptr: int, accepted_ptr: int,
+                  tokens_ptr: int, logprobs_ptr: int | None = None, ws_ptr: int | None = None, stream=None):
+    """Drafted tokens against the target's logits: how many stand, and the tokens that follow."""
+    _check(None, lib().gg_verify_drafts(z_ptr, y_ptr or None, ggml_type, rows, n, ldz, ldy, draft_ptr, row_start_ptr, n_seqs,
+                                        temperature_ptr, accept_u_ptr, draw_u_ptr, accepted_ptr, tokens_ptr,
+                                        logprobs_ptr or None, ws_ptr or None, _stream_ptr(stream)))
