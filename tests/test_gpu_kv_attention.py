@@ -208,7 +208,10 @@ def test_what_a_row_does_not_see_has_no_effect(gpu, rows, cache, x, bad):
             meets = any(sq == s and p <= pos and (p > pos - window or p < sinks) for sq, p, _ in places)
             touched += meets
             if not meets:
-                assert np.array_equal(out[at + i], clean[at + i]) and np.array_equal(lse[at + i], clean_lse[at + i])
+                # rows beside ones that need care may be summed in another order: within the bounds of the clean values
+                for h in range(4) if not np.array_equal(out[at + i], clean[at + i]) or not np.array_equal(lse[at + i], clean_lse[at + i]) else ():
+                    ro, rl, bo, bl = attention(c.q[at + i:at + i + 1, h], c.k[s][:, 0], c.v[s][:, 0], [pos], 0.125, window, sinks, cache, x)
+                    assert (np.abs(out[at + i, h] - ro[0]) <= bo[0]).all() and abs(lse[at + i, h] - rl[0]) <= bl[0]
             else:
                 # a score of -inf has weight 0: an infinity in K that every head's q meets with one sign may leave lse finite
                 assert np.isnan(lse[at + i]).all() if cache == "e4m3" or np.isnan(bad) else not np.isfinite(out[at + i]).all()
@@ -228,10 +231,12 @@ def test_infinite_values_of_seen_keys(gpu, rows, x, cache, bad):
     c.pool.views()[1][c.pool.table[0, p // 16], p % 16, 0, 17] = bad
     out, lse = c.run()
     see = (40 + np.arange(n)) >= p
-    assert np.array_equal(lse, clean_lse)
-    assert np.array_equal(out[~see], clean[~see])
-    others = np.arange(64) != 17
-    assert np.array_equal(out[see][:, :, others], clean[see][:, :, others])
+    # rows that need care may be summed in another order
+    for i in range(n):
+        for h in range(2):
+            ro, rl, bo, bl = attention(c.q[i:i + 1, h], c.k[0][:, 0], c.v[0][:, 0], [40 + i], 0.125, 0, 0, cache, x)
+            good = (np.arange(64) != 17) | (not see[i])
+            assert (np.abs(out[i, h] - ro[0]) <= bo[0])[good].all() and abs(lse[i, h] - rl[0]) <= bl[0]
     assert (np.isnan(out[see][:, :, 17]) if np.isnan(bad) else out[see][:, :, 17] == bad).all()
 
 

@@ -96,6 +96,7 @@ __device__ __forceinline__ float value_hi(uint32_t w) {
 struct Span {
   int lo, a, sink, n;
 };
+template <int STEP>   // keys that a kernel takes at a time
 __device__ __forceinline__ Span kv_span(const KvAttnArgs& g, const KvSeq& sq, int row_first, int row_last) {
   Span s{};
   const int before = sq.len - sq.rows;
@@ -103,7 +104,7 @@ __device__ __forceinline__ Span kv_span(const KvAttnArgs& g, const KvSeq& sq, in
   if (hi <= 0) return s;
   s.lo = g.window > 0 ? max(0, before + row_first - g.window + 1) : 0;
   s.sink = g.window > 0 ? min(min(g.sinks, s.lo), hi) : 0;
-  s.a = (s.sink + 31) / 32 * 32;
+  s.a = (s.sink + STEP - 1) / STEP * STEP;
   s.n = s.a + max(0, hi - s.lo);
   return s;
 }
@@ -159,7 +160,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attn_few(KvAttnArgs 
   const int packed = sq.rows * g.group;
   if (tile_l < 0 || tile_l * kKvFewTile >= packed || packed > g.few_rows) return;
   const int p0 = (int)tile_l * kKvFewTile;
-  const Span sp = kv_span(g, sq, p0 / g.group, min((p0 + kKvFewTile - 1) / g.group, sq.rows - 1));
+  const Span sp = kv_span<32>(g, sq, p0 / g.group, min((p0 + kKvFewTile - 1) / g.group, sq.rows - 1));
   const int u0 = split * g.chunk, u1 = min(sp.n, u0 + g.chunk);
   if (split > 0 && u0 >= sp.n) return;
   const bool joined = kv_splits(g, sp) > 1;
@@ -514,6 +515,409 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attn_few(KvAttnArgs 
   }
 }
 
+// ---------------------------------------------------------------------------
+// Many rows: a block takes 128 packed rows of a K/V head, 32 a wave, and a chunk
+// of keys, 64 (heads above 128: 32) at a time. The waves share K and V through
+// LDS, two tiles of each: while one is used the next arrives by DMA, 16-byte
+// units of a row at places that a row's lowest bits permute, so that neither
+// the reads of K (a row a lane) nor those of V (transposed by the read, four
+// rows to 16 lanes) meet in a bank. 8-bit rows pass through registers and lie in
+// LDS as bf16. One barrier a tile.
+// ---------------------------------------------------------------------------
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+template <int KV>
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (KV == KV_F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+// The sum of two 16-bit weights and c.
+template <int KV>
+__device__ __forceinline__ float add2(uint32_t w, float c) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  if constexpr (KV == KV_F16) return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), f16x2{1, 1}, c, false);
+  else return value_lo<KV>(w) + (value_hi<KV>(w) + c);
+}
+// A product that is rounded before what follows.
+__device__ __forceinline__ float times(float a, float b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
+// One DMA instruction: lane l's 16 bytes at src go to dst + 16 l. Inline asm,
+// because the compiler would wait for every copy in flight before any LDS read;
+// the wait before the barrier that precedes the readers is written out.
+__device__ __forceinline__ void dma16(const void* src, uint32_t dst) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(dst)), "v"(src)
+               : "memory", "m0");
+}
+__device__ __forceinline__ uint32_t lds_at(const void* p) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)p; }
+
+// What a key without a place is read from.
+__device__ __attribute__((aligned(16))) const uint8_t kv_zeros[kKvMaxDim * 2] = {};
+
+// One packed row over [u0, u1) in plain f32, a value or four of the head a
+// lane: for rows whose sums are not finite, where an infinity or a NaN in V must
+// reach the rows that see its key and no others.
+template <int KV, int DP, class T>
+__device__ void slow_row(const KvAttnArgs& g, int s, const KvSeq& sq, const Span& sp, int u0, int u1, int kvh, int p, float scale2,
+                         float (&o)[DP / 64], float* m_out, float* l_out) {
+  constexpr int N = DP / 64;
+  const int lane = threadIdx.x & 63, D = g.kv.dim, row = sq.first + p / g.group, head = kvh * g.group + p % g.group;
+  const int pos = sq.len - sq.rows + p / g.group;
+  float q[N], m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int d = lane + 64 * i;
+    q[i] = d < D ? (float)((const T*)g.q)[row * g.ldq + (long long)head * D + d] : 0.f;
+    o[i] = 0.f;
+  }
+#pragma unroll 1
+  for (int u = u0; u < u1; ++u) {
+    const int key = u < sp.a ? u : sp.lo + u - sp.a;
+    if ((u < sp.a && u >= sp.sink) || key > pos || (g.window > 0 && key <= pos - g.window && key >= g.sinks)) continue;
+    KvPlace at{};
+    if (!kv_place(g.kv, s, key, &at)) continue;
+    const long long off = kv_offset(g.kv, at, kvh);
+    float k[N], v[N], ks = 1.f, vs = 1.f;
+    if constexpr (KV == KV_E4M3) {
+      ks = g.kv.k_scale[kv_scale_at(g.kv, at, kvh)];
+      vs = g.kv.v_scale[kv_scale_at(g.kv, at, kvh)];
+    }
+    float x = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int d = lane + 64 * i;
+      k[i] = v[i] = 0.f;
+      if (d < D) {
+        if constexpr (KV == KV_E4M3) {
+          k[i] = ks * __builtin_amdgcn_cvt_f32_fp8((uint32_t)((const uint8_t*)g.kv.k)[off + d], 0);
+          v[i] = vs * __builtin_amdgcn_cvt_f32_fp8((uint32_t)((const uint8_t*)g.kv.v)[off + d], 0);
+        } else {
+          typedef typename std::conditional<KV == KV_BF16, __bf16, _Float16>::type C;
+          k[i] = (float)((const C*)g.kv.k)[off + d];
+          v[i] = (float)((const C*)g.kv.v)[off + d];
+        }
+      }
+      x = fmaf(q[i], k[i], x);
+    }
+    x = gg::wave_sum(x) * scale2;
+    if (x > m) {
+      const float f = __builtin_amdgcn_exp2f(m - x);
+      m = x;
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < N; ++i) o[i] = scaled(o[i], f);
+    }
+    // a weight that rounds to 0 is none: an infinity counts
+    const float w = x == -INFINITY ? 0.f : fmaxf(__builtin_amdgcn_exp2f(x - (m == -INFINITY ? 0.f : m)), x != x ? NAN : 1e-38f);
+    l += x != x ? NAN : w;
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = fmaf(x != x ? NAN : w, v[i], o[i]);
+  }
+  *m_out = m;
+  *l_out = l;
+}
+
+template <int KV, int DP, class T>
+__global__ __launch_bounds__(256, (kParts<KV, T> > 1 ? 1 : 2)) void k_attn_many(KvAttnArgs g, int slot0, int slots) {
+  constexpr int NP = kParts<KV, T>, KT = DP <= 128 ? 64 : 32, UN = DP / 8, RPI = 64 / UN, IPW = KT / RPI / 4;
+  constexpr int KH = KT / 32, DT = DP / 32, CH = DP / 16, ES = KV == KV_E4M3 ? 1 : 2;
+  constexpr int KMASK = UN < 16 ? UN - 1 : 15, VMASK = UN < 16 ? 3 : 7;
+  __shared__ __align__(1024) uint8_t kbuf[2][KT * DP * 2], vbuf[2][KT * DP * 2];
+  __shared__ __align__(16) float hole[2][KT];   // -inf where a key has no place
+  __shared__ __align__(16) int holes[2][4];     // whether a wave's keys have any
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c32 = lane & 31, half = lane >> 5, D = g.kv.dim;
+  // Blocks with one value of blockIdx % 8 share an XCD and its L2: they take a
+  // contiguous range of an order with the tiles fastest, which read the same keys.
+  const int G = gridDim.x, xcd = blockIdx.x & 7;
+  const int unit = xcd * (G >> 3) + min(xcd, G & 7) + (blockIdx.x >> 3);
+  const int slot = slot0 + unit % slots, ks_ = unit / slots;
+  const int split = ks_ % g.splits, kvh = ks_ / g.splits;
+  const int s = last_at_most(g.kv.n_seqs, [&](int i) { return tile_slot(g, i, kKvManyTile) <= slot; });
+  if (s < 0) return;
+  const KvSeq sq = kv_seq(g.kv, s);
+  const long long tile_l = slot - tile_slot(g, s, kKvManyTile);
+  const int packed = sq.rows * g.group;
+  if (tile_l < 0 || tile_l * kKvManyTile >= packed || packed <= g.few_rows) return;
+  const int p0 = (int)tile_l * kKvManyTile;
+  const Span sp = kv_span<64>(g, sq, p0 / g.group, min((p0 + kKvManyTile - 1) / g.group, sq.rows - 1));
+  const int u0 = split * g.chunk, u1 = min(sp.n, u0 + g.chunk);
+  if (split > 0 && u0 >= sp.n) return;
+  const bool joined = kv_splits(g, sp) > 1;
+  const int before = sq.len - sq.rows;
+  const int pw = p0 + 32 * wv, p = pw + c32, row = sq.first + p / g.group, head = kvh * g.group + p % g.group;
+  const int pos = p < packed ? before + p / g.group : -1;
+  const bool active = pw < packed;   // this wave has rows
+  const int pos_min = before + pw / g.group, pos_max = before + min((pw + 31) / g.group, sq.rows - 1);
+
+  // queries as operand columns; a negative scale turns their signs, so that the
+  // largest product is the largest score, and scale 0 takes them out
+  const float scale2 = g.scale2 == 0.f ? 1.f : fabsf(g.scale2), sign = g.scale2 > 0.f ? 1.f : g.scale2 < 0.f ? -1.f : 0.f;
+  u32x4 qb[NP][CH];
+  {
+    const T* q = (const T*)g.q + (p < packed ? row * g.ldq + (long long)head * D : 0);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int d = 16 * c + 8 * half;
+      float f[8] = {};
+      if (p < packed && d < D) {
+        if (g.q_vec) {
+          constexpr int V = 16 / sizeof(T);
+          typedef T vec_t __attribute__((ext_vector_type(V)));
+#pragma unroll
+          for (int i = 0; i < 8; i += V) {
+            const vec_t t = *(const vec_t*)(q + d + i);
+#pragma unroll
+            for (int k = 0; k < V; ++k) f[i + k] = sign * (float)t[k];
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] = sign * (float)q[d + i];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t w[NP];
+        split2<KV, NP>(f[2 * i], f[2 * i + 1], w);
+#pragma unroll
+        for (int k = 0; k < NP; ++k) qb[k][c][i] = w[k];
+      }
+    }
+  }
+
+  // This lane's rows of a tile: (wv IPW + i) RPI + lane / UN, unit lane % UN of each in LDS.
+  const int urow = lane / UN, unit16 = lane % UN;
+  long long off[IPW];
+  auto places = [&](int u) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < IPW; ++i) {
+      const int x = u + (wv * IPW + i) * RPI + urow, key = x < sp.a ? x : sp.lo + x - sp.a;
+      KvPlace at{};
+      const bool ok = x < u1 && (x >= sp.a || x < sp.sink) && kv_place(g.kv, s, key, &at);
+      off[i] = ok ? kv_offset(g.kv, at, kvh) : -1;
+    }
+  };
+  uint2 kreg[KV == KV_E4M3 ? IPW : 1], vreg[KV == KV_E4M3 ? IPW : 1];
+  float kscale[KV == KV_E4M3 ? IPW : 1], vscale[KV == KV_E4M3 ? IPW : 1];
+  // Sends for a tile: into LDS stage st, or (8 bits) into registers.
+  auto fetch = [&](int u, int st) __attribute__((always_inline)) {
+    bool none = false;
+#pragma unroll
+    for (int i = 0; i < IPW; ++i) {
+      const int r = (wv * IPW + i) * RPI + urow;
+      const int ku = unit16 ^ (r & KMASK), vu = unit16 ^ ((r & VMASK) << 1);
+      const bool ok = off[i] >= 0;
+      none |= !ok;
+      if constexpr (KV == KV_E4M3) {
+        const uint8_t* kz = ok && 8 * ku < D ? (const uint8_t*)g.kv.k + off[i] + 8 * ku : kv_zeros;
+        const uint8_t* vz = ok && 8 * vu < D ? (const uint8_t*)g.kv.v + off[i] + 8 * vu : kv_zeros;
+        kreg[i] = *(const uint2*)kz;
+        vreg[i] = *(const uint2*)vz;
+        const int x = u + r, key = x < sp.a ? x : sp.lo + x - sp.a;
+        KvPlace at{};
+        kscale[i] = vscale[i] = 1.f;
+        if (ok && kv_place(g.kv, s, key, &at)) {
+          kscale[i] = g.kv.k_scale[kv_scale_at(g.kv, at, kvh)];
+          vscale[i] = g.kv.v_scale[kv_scale_at(g.kv, at, kvh)];
+        }
+      } else {
+        const void* kz = ok && 8 * ku < D ? (const void*)((const uint8_t*)g.kv.k + (off[i] + 8 * ku) * ES) : (const void*)kv_zeros;
+        const void* vz = ok && 8 * vu < D ? (const void*)((const uint8_t*)g.kv.v + (off[i] + 8 * vu) * ES) : (const void*)kv_zeros;
+        dma16(kz, lds_at(&kbuf[st][(wv * IPW + i) * 1024]));
+        dma16(vz, lds_at(&vbuf[st][(wv * IPW + i) * 1024]));
+      }
+      if (unit16 == 0) hole[st][r] = ok ? 0.f : -INFINITY;
+    }
+    const int any = __ballot(none) != 0;
+    if (lane == 0) holes[st][wv] = any;
+  };
+  auto bf16x8_of = [&](uint2 w, float sc) __attribute__((always_inline)) {
+    u32x4 r;
+    r.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, sc, false));
+    r.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, sc, true));
+    r.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, sc, false));
+    r.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, sc, true));
+    return sc == sc ? r : u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
+  };
+  auto settle = [&](int st) __attribute__((always_inline)) {
+    if constexpr (KV == KV_E4M3) {
+#pragma unroll
+      for (int i = 0; i < IPW; ++i) {
+        *(u32x4*)&kbuf[st][(wv * IPW + i) * 1024 + 16 * lane] = bf16x8_of(kreg[i], kscale[i]);
+        *(u32x4*)&vbuf[st][(wv * IPW + i) * 1024 + 16 * lane] = bf16x8_of(vreg[i], vscale[i]);
+      }
+    }
+  };
+
+  f32x16 o[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
+  float m = -INFINITY, l = 0.f, le = 0.f;
+  const int kswz = c32 & KMASK;
+  const int g16 = lane >> 4, vr = 4 * (g16 >> 1) + ((lane & 15) >> 2), vswz = (vr & VMASK) << 1;
+  const int vunit = 2 * (g16 & 1) + ((lane & 3) >> 1), vbase = vr * DP * 2 + 8 * (lane & 1);
+
+  const int tiles = (u1 - u0 + KT - 1) / KT;
+  if (tiles > 0) {
+    places(u0);
+    fetch(u0, 0);
+    settle(0);
+    if (tiles > 1) places(u0 + KT);
+  }
+  for (int t = 0; t < tiles; ++t) {
+    const int st = t & 1, u = u0 + t * KT;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wave's copies of tile t
+    __syncthreads();                                   // and everybody's; the other stage is free
+    if (t + 1 < tiles) {
+      fetch(u + KT, st ^ 1);
+      if (t + 2 < tiles) places(u + 2 * KT);
+    }
+    const int key0 = u < sp.a ? u : sp.lo + u - sp.a, key1 = key0 + KT - 1;
+    const bool out_of_sight = !active || key0 > pos_max || (g.window > 0 && key1 <= pos_min - g.window && key0 >= g.sinks);
+    if (!out_of_sight) {
+      const int4 hs = *(const int4*)holes[st];
+      const bool some = (hs.x | hs.y | hs.z | hs.w) != 0;
+      const bool masked = key1 > pos_min || (g.window > 0 && !(key0 > pos_max - g.window || key1 < g.sinks)) || some;
+      // S^T: KT keys x 32 packed rows
+      f32x16 sc[KH];
+#pragma unroll
+      for (int h = 0; h < KH; ++h) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[h][i] = 0.f;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          const u32x4 ka = *(const u32x4*)&kbuf[st][(32 * h + c32) * DP * 2 + (((2 * c + half) ^ kswz) << 4)];
+#pragma unroll
+          for (int k = NP - 1; k >= 0; --k) sc[h] = mfma32<KV>(ka, qb[k][c], sc[h]);
+        }
+      }
+      float mx = -INFINITY;
+      if (masked) {
+#pragma unroll
+        for (int h = 0; h < KH; ++h)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int j = 32 * h + 8 * (i >> 2) + 4 * half + (i & 3), key = key0 + j;
+            const bool sees = key <= pos && (g.window == 0 || key > pos - g.window || key < g.sinks) && hole[st][j] == 0.f;
+            sc[h][i] = sees ? sc[h][i] : -INFINITY;
+          }
+      }
+#pragma unroll
+      for (int h = 0; h < KH; ++h)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[h][i]);
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * scale2;
+      if (__ballot(mx > m + kSlack)) {
+        const float mn = mx > m + kSlack ? mx : m;
+        const float f = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= f;
+        le *= f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[d] *= f;
+      }
+      const float ref = (m == -INFINITY ? 0.f : m) - kShift<KV>;
+#pragma unroll
+      for (int h = 0; h < KH; ++h)
+#pragma unroll
+        for (int kg = 0; kg < 2; ++kg) {
+          u32x4 pb[NP];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            // f32: a product of its own, so that the reference's own key has weight 1
+            const float s0 = sc[h][8 * kg + 2 * i], s1 = sc[h][8 * kg + 2 * i + 1];
+            const float w0 = __builtin_amdgcn_exp2f(NP > 1 ? times(s0, scale2) - ref : fmaf(s0, scale2, -ref)),
+                        w1 = __builtin_amdgcn_exp2f(NP > 1 ? times(s1, scale2) - ref : fmaf(s1, scale2, -ref));
+            le += w0 + w1;
+            uint32_t w[NP];
+            split2<KV, NP>(w0, w1, w);
+            if constexpr (NP == 1) l = add2<KV>(w[0], l);
+#pragma unroll
+            for (int k = 0; k < NP; ++k) pb[k][i] = w[k];
+          }
+          // O^T: the head's values x 32 packed rows
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            const uint8_t* src = &vbuf[st][(32 * h + 16 * kg) * DP * 2 + vbase + (((4 * d + vunit) ^ vswz) << 4)];
+            typedef short s16x4 __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) s16x4* lds4;
+            const s16x4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uintptr_t)lds_at(src)),
+                        a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uintptr_t)lds_at(src + 8 * DP * 2));
+            const uint2 b0 = __builtin_bit_cast(uint2, a0), b1 = __builtin_bit_cast(uint2, a1);
+            const u32x4 va = {b0.x, b0.y, b1.x, b1.y};
+#pragma unroll
+            for (int k = NP - 1; k >= 0; --k) o[d] = mfma32<KV>(va, pb[k], o[d]);
+          }
+        }
+    }
+    if (t + 1 < tiles) settle(st ^ 1);
+  }
+  if (!active) return;
+
+  l += __shfl_xor(l, 32, 64);
+  le += __shfl_xor(le, 32, 64);
+  if constexpr (NP > 1) l = le;
+  float z = 0.f;
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) z = fmaf(o[d][i], 0.f, z);
+  uint64_t again = __ballot(z != 0.f && p < packed);   // 0 times an infinity or a NaN
+  again |= again >> 32;
+  const bool mine = (again >> c32) & 1;
+  const long long at = ((long long)split * g.kv.n_rows + row) * g.n_q + head;
+  if (p < packed && !mine) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T* out = (T*)g.out + row * g.ldo + (long long)head * D;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int e = 32 * d + 8 * i + 4 * half;
+        if (e >= D) continue;
+        const f32x4 v = {o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+        if (joined) {
+          *(f32x4*)(g.part_o + at * D + e) = v;
+        } else if (g.out_vec) {
+          typedef T vec_t __attribute__((ext_vector_type(4)));
+          *(vec_t*)(out + e) = vec_t{(T)(v[0] * inv), (T)(v[1] * inv), (T)(v[2] * inv), (T)(v[3] * inv)};
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) out[e + k] = (T)(v[k] * inv);
+        }
+      }
+    if (half == 0) {
+      if (joined) *(f32x4*)(g.part_ml + 4 * at) = f32x4{m, l, le, 0.f};
+      else if (g.lse) g.lse[(long long)row * g.n_q + head] = lse_of<KV>(m, le);
+    }
+  }
+  // rows that need care, one at a time
+  for (uint32_t left = (uint32_t)again; left; left &= left - 1) {
+    const int pr = pw + __builtin_ctz(left), orow = sq.first + pr / g.group, oh = kvh * g.group + pr % g.group;
+    float os[DP / 64], ms, ls;
+    slow_row<KV, DP, T>(g, s, sq, sp, u0, u1, kvh, pr, g.scale2, os, &ms, &ls);
+    const long long to = ((long long)split * g.kv.n_rows + orow) * g.n_q + oh;
+    const float inv = ls == 0.f ? 0.f : 1.f / ls;
+#pragma unroll
+    for (int i = 0; i < DP / 64; ++i) {
+      const int e = lane + 64 * i;
+      if (e >= D) continue;
+      if (joined) g.part_o[to * D + e] = scaled(os[i], exp2f(kShift<KV>));
+      else ((T*)g.out)[orow * g.ldo + (long long)oh * D + e] = (T)scaled(os[i], inv);
+    }
+    if (lane == 0) {
+      const float c = exp2f(kShift<KV>);   // the chunks' sums have it
+      if (joined) *(f32x4*)(g.part_ml + 4 * to) = f32x4{ms, ls * c, ls * c, 0.f};
+      else if (g.lse) g.lse[(long long)orow * g.n_q + oh] = lse_of<KV>(ms, ls * c);
+    }
+  }
+}
+
 // Joins the chunks of tiles that have several: one wave for a row's head.
 template <int KV, class T>
 __global__ __launch_bounds__(256) void k_attn_join(KvAttnArgs g, long long unit0) {
@@ -524,9 +928,11 @@ __global__ __launch_bounds__(256) void k_attn_join(KvAttnArgs g, long long unit0
   const int s = kv_seq_of(g.kv, row);
   if (s < 0) return;
   const KvSeq sq = kv_seq(g.kv, s);
-  const int tile_rows = kKvFewTile;
-  const int p0 = ((row - sq.first) * g.group + head % g.group) / tile_rows * tile_rows;
-  const Span sp = kv_span(g, sq, p0 / g.group, min((p0 + tile_rows - 1) / g.group, sq.rows - 1));
+  const bool few = sq.rows * g.group <= g.few_rows;
+  const int tile = few ? kKvFewTile : kKvManyTile;
+  const int p0 = ((row - sq.first) * g.group + head % g.group) / tile * tile;
+  const int t0 = p0 / g.group, t1 = min((p0 + tile - 1) / g.group, sq.rows - 1);
+  const Span sp = few ? kv_span<32>(g, sq, t0, t1) : kv_span<64>(g, sq, t0, t1);
   const int n = kv_splits(g, sp);
   if (n < 2) return;
   const long long step = (long long)g.kv.n_rows * g.n_q;
@@ -562,15 +968,26 @@ __global__ __launch_bounds__(256) void k_attn_join(KvAttnArgs g, long long unit0
 }
 
 template <int KV, int DP, class T>
-int attn_launch(const KvAttnArgs& g, hipStream_t s) {
+int attn_launch(const KvAttnArgs& g, int max_rows, hipStream_t s) {
   // launches of fewer than 2^24 blocks: a grid holds fewer than 2^32 threads
-  const long long slots = (long long)g.kv.n_rows * g.group / kKvFewTile + g.kv.n_seqs;
   const long long each = (long long)g.kv.n_kv * g.splits;
   const long long most = std::max(1ll, ((1ll << 24) - 1) / each);
-  for (long long at = 0; at < slots; at += most) {
-    hipLaunchKernelGGL((k_attn_few<KV, DP, T>), dim3((unsigned)(std::min(most, slots - at) * each)), dim3(256), 0, s, g, (int)at);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return (int)e;
+  if (g.few_rows > 0) {
+    const long long slots = (long long)g.kv.n_rows * g.group / kKvFewTile + g.kv.n_seqs;
+    for (long long at = 0; at < slots; at += most) {
+      hipLaunchKernelGGL((k_attn_few<KV, DP, T>), dim3((unsigned)(std::min(most, slots - at) * each)), dim3(256), 0, s, g, (int)at);
+      const hipError_t e = hipGetLastError();
+      if (e != hipSuccess) return (int)e;
+    }
+  }
+  if (g.few_rows < 0x7fffffff) {
+    const long long slots = (long long)g.kv.n_rows * g.group / kKvManyTile + g.kv.n_seqs;
+    for (long long at = 0; at < slots; at += most) {
+      const int n = (int)std::min(most, slots - at);
+      hipLaunchKernelGGL((k_attn_many<KV, DP, T>), dim3((unsigned)(n * each)), dim3(256), 0, s, g, (int)at, n);
+      const hipError_t e = hipGetLastError();
+      if (e != hipSuccess) return (int)e;
+    }
   }
   if (g.splits == 1) return 0;
   const long long units = (long long)g.kv.n_rows * g.n_q;
@@ -582,17 +999,17 @@ int attn_launch(const KvAttnArgs& g, hipStream_t s) {
   return 0;
 }
 template <int KV, class T>
-int attn_dim(const KvAttnArgs& g, hipStream_t s) {
-  if (g.kv.dim <= 64) return attn_launch<KV, 64, T>(g, s);
-  if (g.kv.dim <= 128) return attn_launch<KV, 128, T>(g, s);
-  return attn_launch<KV, 256, T>(g, s);
+int attn_dim(const KvAttnArgs& g, int max_rows, hipStream_t s) {
+  if (g.kv.dim <= 64) return attn_launch<KV, 64, T>(g, max_rows, s);
+  if (g.kv.dim <= 128) return attn_launch<KV, 128, T>(g, max_rows, s);
+  return attn_launch<KV, 256, T>(g, max_rows, s);
 }
 template <int KV>
-int attn_type(int elem, const KvAttnArgs& g, hipStream_t s) {
+int attn_type(int elem, const KvAttnArgs& g, int max_rows, hipStream_t s) {
   switch (elem) {
-    case ELEM_F32: return attn_dim<KV, float>(g, s);
-    case ELEM_F16: return attn_dim<KV, _Float16>(g, s);
-    case ELEM_BF16: return attn_dim<KV, __bf16>(g, s);
+    case ELEM_F32: return attn_dim<KV, float>(g, max_rows, s);
+    case ELEM_F16: return attn_dim<KV, _Float16>(g, max_rows, s);
+    case ELEM_BF16: return attn_dim<KV, __bf16>(g, max_rows, s);
   }
   return (int)hipErrorInvalidValue;
 }
@@ -601,13 +1018,21 @@ int attn_type(int elem, const KvAttnArgs& g, hipStream_t s) {
 
 KvAttnPlan kv_attn_plan(int n_seqs, int n_rows, int max_rows, int max_len, int n_kv, int group, int dim, int window, int sinks) {
   KvAttnPlan p{};
-  p.few_rows = 0x7fffffff;
+  constexpr int FEW = 64;   // packed rows of a sequence that k_attn_few takes
+  const bool few = (long long)max_rows * group <= FEW;
+  p.few_rows = few ? 0x7fffffff : FEW;
+  const int tile = few ? kKvFewTile : kKvManyTile;
   long long most = max_len;   // keys that a tile's rows see at most
-  if (window > 0) most = std::min(most, (long long)window + kKvFewTile) + ((long long)std::min(sinks, max_len) + 31) / 32 * 32;
-  most = std::max(most, 1ll);
-  const long long tiles = ((long long)n_rows * group / kKvFewTile + n_seqs) * n_kv;
-  long long chunk = (most * tiles / 4096 + kKvChunk) / kKvChunk * kKvChunk;
-  chunk = std::max(chunk, most <= 2048 ? 128ll : 512ll);
+  if (window > 0) most = std::min(most, (long long)window + tile) + ((long long)std::min(sinks, max_len) + 63) / 64 * 64;
+  const long long tiles = ((long long)n_rows * group / tile + n_seqs) * n_kv;
+  long long chunk;
+  if (few) {
+    chunk = (most * tiles / 4096 + kKvChunk) / kKvChunk * kKvChunk;
+    chunk = std::max(chunk, most <= 2048 ? 128ll : 512ll);
+  } else {
+    chunk = (most * tiles / 1024 + kKvChunk) / kKvChunk * kKvChunk;
+    chunk = std::max(chunk, 512ll);
+  }
   p.chunk = (int)std::min(chunk, (most + kKvChunk - 1) / kKvChunk * kKvChunk);
   p.splits = (int)((most + p.chunk - 1) / p.chunk);
   return p;
@@ -615,9 +1040,9 @@ KvAttnPlan kv_attn_plan(int n_seqs, int n_rows, int max_rows, int max_len, int n
 
 int launch_kv_attention(int kv_type, int elem, const KvAttnArgs& g, int max_rows, void* stream) {
   switch (kv_type) {
-    case KV_BF16: return attn_type<KV_BF16>(elem, g, (hipStream_t)stream);
-    case KV_F16: return attn_dim<KV_F16, _Float16>(g, (hipStream_t)stream);
-    case KV_E4M3: return attn_type<KV_E4M3>(elem, g, (hipStream_t)stream);
+    case KV_BF16: return attn_type<KV_BF16>(elem, g, max_rows, (hipStream_t)stream);
+    case KV_F16: return attn_dim<KV_F16, _Float16>(g, max_rows, (hipStream_t)stream);
+    case KV_E4M3: return attn_type<KV_E4M3>(elem, g, max_rows, (hipStream_t)stream);
   }
   return (int)hipErrorInvalidValue;
 }

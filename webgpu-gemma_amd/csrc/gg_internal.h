@@ -672,7 +672,7 @@ struct KvAttnArgs {
   float scale2;          // softmax scale times log2(e)
   int n_q, group;        // query heads, and those of a K/V head
   int window, sinks;     // window 0: none
-  bool q_vec;            // q rows aligned to 16 bytes
+  bool q_vec, out_vec;   // q rows aligned to 16 bytes, those of out to four values
   int few_rows;          // sequences of at most this many rows (times group) go to k_attn_few
   int chunk;             // keys of a block, a multiple of kKvChunk
   int splits;            // blocks that share a tile at most
@@ -680,6 +680,7 @@ struct KvAttnArgs {
 };
 constexpr int kKvChunk = 128;       // keys of the smallest chunk: 32 for each of four waves
 constexpr int kKvFewTile = 16;      // packed rows (row, head of the group) of a block of k_attn_few
+constexpr int kKvManyTile = 128;    // and of k_attn_many
 struct KvAttnPlan {
   int few_rows, chunk, splits;
 };

@@ -2099,6 +2099,7 @@ int gg_kv_attention(const gg_kv_pages* pages, const gg_kv_seqs* seqs, const void
   a.window = window;
   a.sinks = sinks;
   a.q_vec = aligned_to(q, 16) && ldq * (int64_t)elem_size(e) % 16 == 0;
+  a.out_vec = aligned_to(out, 4 * elem_size(e)) && ldo % 4 == 0;
   a.few_rows = p.few_rows;
   a.chunk = p.chunk;
   a.splits = p.splits;
