@@ -110,11 +110,12 @@ __device__ __forceinline__ Span kv_span(const KvAttnArgs& g, const KvSeq& sq, in
 }
 __device__ __forceinline__ int kv_splits(const KvAttnArgs& g, const Span& s) { return max(1, (s.n + g.chunk - 1) / g.chunk); }
 
-// The slots of a sequence's tiles: consecutive from floor(first row group / tile) + s
-// on, enough for tiles of whole sequences, so that a slot's sequence is found
-// by search and no list of tiles is made.
+// The first slot of a sequence's tiles. A sequence of n packed rows behind r others
+// has floor((r + n + (tile - 1) (s + 1)) / tile) - floor((r + (tile - 1) s) / tile) of
+// them, at least ceil(n / tile), so that a slot's sequence is found by search
+// and no list of tiles is made.
 __device__ __forceinline__ long long tile_slot(const KvAttnArgs& g, int s, int tile) {
-  return (long long)min(max(g.kv.row_start[s], 0), g.kv.n_rows) * g.group / tile + s;
+  return ((long long)min(max(g.kv.row_start[s], 0), g.kv.n_rows) * g.group + (long long)(tile - 1) * s) / tile;
 }
 
 // ln of a sum of weights relative to m (log2 units).
@@ -153,10 +154,12 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attn_few(KvAttnArgs 
   const int c16 = lane & 15, quad = lane >> 4, D = g.kv.dim;
   const int split = blockIdx.x % g.splits, hs = blockIdx.x / g.splits;
   const int kvh = hs % g.kv.n_kv, slot = slot0 + hs / g.kv.n_kv;
-  const int s = last_at_most(g.kv.n_seqs, [&](int i) { return tile_slot(g, i, kKvFewTile) <= slot; });
+  // beside k_attn_many only short sequences count, of a few tiles each
+  const bool all = g.few_rows == 0x7fffffff;
+  const int s = all ? last_at_most(g.kv.n_seqs, [&](int i) { return tile_slot(g, i, kKvFewTile) <= slot; }) : slot / kKvFewTiles;
   if (s < 0) return;
   const KvSeq sq = kv_seq(g.kv, s);
-  const long long tile_l = slot - tile_slot(g, s, kKvFewTile);
+  const long long tile_l = all ? slot - tile_slot(g, s, kKvFewTile) : slot % kKvFewTiles;
   const int packed = sq.rows * g.group;
   if (tile_l < 0 || tile_l * kKvFewTile >= packed || packed > g.few_rows) return;
   const int p0 = (int)tile_l * kKvFewTile;
@@ -518,10 +521,12 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attn_few(KvAttnArgs 
 // ---------------------------------------------------------------------------
 // Many rows: a block takes 128 packed rows of a K/V head, 32 a wave, and a chunk
 // of keys, 64 (heads above 128: 32) at a time. The waves share K and V through
-// LDS, two tiles of each: while one is used the next arrives by DMA, 16-byte
-// units of a row at places that a row's lowest bits permute, so that neither
-// the reads of K (a row a lane) nor those of V (transposed by the read, four
-// rows to 16 lanes) meet in a bank. 8-bit rows pass through registers and lie in
+// LDS, two tiles of each: while one is used the next arrives by DMA, 1 KB of
+// whole rows a copy, in the order of memory (16-byte units of a row at permuted
+// places, the usual way to keep reads from meeting in a bank, take the copies
+// twice as long here), at places such that neither the reads of K (a row a
+// lane) nor those of V (transposed by the read, four rows to 16 lanes) meet in a
+// bank. 8-bit rows pass through registers and lie in
 // LDS as bf16. One barrier a tile.
 // ---------------------------------------------------------------------------
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -538,7 +543,7 @@ __device__ __forceinline__ float add2(uint32_t w, float c) {
   typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
   typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
   if constexpr (KV == KV_F16) return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), f16x2{1, 1}, c, false);
-  else return value_lo<KV>(w) + (value_hi<KV>(w) + c);
+  else return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, 0x3f803f80u), c, false);
 }
 // A product that is rounded before what follows.
 __device__ __forceinline__ float times(float a, float b) {
@@ -621,13 +626,19 @@ __device__ void slow_row(const KvAttnArgs& g, int s, const KvSeq& sq, const Span
 }
 
 template <int KV, int DP, class T>
-__global__ __launch_bounds__(256, (kParts<KV, T> > 1 ? 1 : 2)) void k_attn_many(KvAttnArgs g, int slot0, int slots) {
-  constexpr int NP = kParts<KV, T>, KT = DP <= 128 ? 64 : 32, UN = DP / 8, RPI = 64 / UN, IPW = KT / RPI / 4;
+__global__ __launch_bounds__(256, (kParts<KV, T> > 1 || DP > 128 ? 1 : 2)) void k_attn_many(KvAttnArgs g, int slot0, int slots) {
+  constexpr int NP = kParts<KV, T>, KT = DP == 256 && NP > 1 ? 32 : 64, UN = DP / 8, RPI = 64 / UN, IPW = KT / RPI / 4;
   constexpr int KH = KT / 32, DT = DP / 32, CH = DP / 16, ES = KV == KV_E4M3 ? 1 : 2;
-  constexpr int KMASK = UN < 16 ? UN - 1 : 15, VMASK = UN < 16 ? 3 : 7;
-  __shared__ __align__(1024) uint8_t kbuf[2][KT * DP * 2], vbuf[2][KT * DP * 2];
+  // In LDS a copy's RPI rows are 1024 bytes, and some more to the next one: 16
+  // for K, 32 for V. Scores take the keys of a tile in an order in which
+  // neighbouring lanes read neighbouring copies: row m of 32 is key
+  // RPI (m % NI) + m / NI.
+  constexpr int NI = 32 / RPI, RB = DP * 2, KP = 1024 + 16, VP = 1024 + 32;
+  __shared__ __align__(16) uint8_t kbuf[2][KT / RPI * KP], vbuf[2][KT / RPI * VP];
   __shared__ __align__(16) float hole[2][KT];   // -inf where a key has no place
   __shared__ __align__(16) int holes[2][4];     // whether a wave's keys have any
+  __shared__ __align__(16) long long row_off[2][KT];   // bytes from the pool's start to a row, -1: none
+  __shared__ __align__(16) long long row_scale[2][KV == KV_E4M3 ? KT : 1];
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c32 = lane & 31, half = lane >> 5, D = g.kv.dim;
   // Blocks with one value of blockIdx % 8 share an XCD and its L2: they take a
@@ -688,51 +699,55 @@ __global__ __launch_bounds__(256, (kParts<KV, T> > 1 ? 1 : 2)) void k_attn_many(
     }
   }
 
-  // This lane's rows of a tile: (wv IPW + i) RPI + lane / UN, unit lane % UN of each in LDS.
+  // A wave copies RW rows of a tile; lane l's part of copy i is unit l % UN (in
+  // LDS) of row (wv IPW + i) RPI + l / UN. Where the rows lie is found by a lane
+  // each and handed over in LDS. Page ids are asked for a tile ahead and looked
+  // at when its rows are fetched: waiting for one sooner would wait for the
+  // copies before it too, and so would any branch or spill between the copies.
+  constexpr int RW = KT / 4;
   const int urow = lane / UN, unit16 = lane % UN;
-  long long off[IPW];
-  auto places = [&](int u) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < IPW; ++i) {
-      const int x = u + (wv * IPW + i) * RPI + urow, key = x < sp.a ? x : sp.lo + x - sp.a;
-      KvPlace at{};
-      const bool ok = x < u1 && (x >= sp.a || x < sp.sink) && kv_place(g.kv, s, key, &at);
-      off[i] = ok ? kv_offset(g.kv, at, kvh) : -1;
+  const int tiles = (u1 - u0 + KT - 1) / KT;
+  int page = 0;
+  auto key_of = [&](int u) __attribute__((always_inline)) { return u < sp.a ? u : sp.lo + u - sp.a; };
+  auto ask = [&](int t) __attribute__((always_inline)) {
+    const int key = min(max(key_of(u0 + t * KT + wv * RW + lane % RW), 0), g.kv.places - 1);
+    page = g.kv.table[(long long)s * g.kv.table_ld + (int)g.kv.page_div((uint32_t)key)];
+  };
+  auto rows = [&](int t) __attribute__((always_inline)) {
+    const int st = t & 1, r = wv * RW + lane % RW, x = u0 + t * KT + r, key = key_of(x);
+    const bool ok = x < u1 && (x >= sp.a || x < sp.sink) && (uint32_t)page < (uint32_t)g.kv.n_pages;
+    const KvPlace at{ok ? page : 0, ok ? key - (int)g.kv.page_div((uint32_t)key) * g.kv.page_size : 0};
+    const long long off = kv_offset(g.kv, at, kvh) * ES;
+    if (lane < RW) {
+      row_off[st][r] = ok ? off : -1;
+      hole[st][r] = ok ? 0.f : -INFINITY;
+      if constexpr (KV == KV_E4M3) row_scale[st][r] = ok ? kv_scale_at(g.kv, at, kvh) : -1;
     }
+    const int any = __ballot(!ok) != 0;
+    if (lane == 0) holes[st][wv] = any;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   };
   uint2 kreg[KV == KV_E4M3 ? IPW : 1], vreg[KV == KV_E4M3 ? IPW : 1];
   float kscale[KV == KV_E4M3 ? IPW : 1], vscale[KV == KV_E4M3 ? IPW : 1];
-  // Sends for a tile: into LDS stage st, or (8 bits) into registers.
-  auto fetch = [&](int u, int st) __attribute__((always_inline)) {
-    bool none = false;
-#pragma unroll
-    for (int i = 0; i < IPW; ++i) {
-      const int r = (wv * IPW + i) * RPI + urow;
-      const int ku = unit16 ^ (r & KMASK), vu = unit16 ^ ((r & VMASK) << 1);
-      const bool ok = off[i] >= 0;
-      none |= !ok;
-      if constexpr (KV == KV_E4M3) {
-        const uint8_t* kz = ok && 8 * ku < D ? (const uint8_t*)g.kv.k + off[i] + 8 * ku : kv_zeros;
-        const uint8_t* vz = ok && 8 * vu < D ? (const uint8_t*)g.kv.v + off[i] + 8 * vu : kv_zeros;
-        kreg[i] = *(const uint2*)kz;
-        vreg[i] = *(const uint2*)vz;
-        const int x = u + r, key = x < sp.a ? x : sp.lo + x - sp.a;
-        KvPlace at{};
-        kscale[i] = vscale[i] = 1.f;
-        if (ok && kv_place(g.kv, s, key, &at)) {
-          kscale[i] = g.kv.k_scale[kv_scale_at(g.kv, at, kvh)];
-          vscale[i] = g.kv.v_scale[kv_scale_at(g.kv, at, kvh)];
-        }
-      } else {
-        const void* kz = ok && 8 * ku < D ? (const void*)((const uint8_t*)g.kv.k + (off[i] + 8 * ku) * ES) : (const void*)kv_zeros;
-        const void* vz = ok && 8 * vu < D ? (const void*)((const uint8_t*)g.kv.v + (off[i] + 8 * vu) * ES) : (const void*)kv_zeros;
-        dma16(kz, lds_at(&kbuf[st][(wv * IPW + i) * 1024]));
-        dma16(vz, lds_at(&vbuf[st][(wv * IPW + i) * 1024]));
-      }
-      if (unit16 == 0) hole[st][r] = ok ? 0.f : -INFINITY;
+  // Sends for copy i of K or V of tile t: into its LDS stage, or (8 bits) into registers.
+  auto fetch1 = [&](auto is_k, int t, int i) __attribute__((always_inline)) {
+    const int st = t & 1, r = (wv * IPW + i) * RPI + urow;
+    const long long off = row_off[st][r];
+    const bool ok = off >= 0 && 8 * unit16 < D;
+    const uint64_t at = (uint64_t)(uintptr_t)(is_k ? g.kv.k : g.kv.v) + (uint64_t)off + (uint32_t)(8 * ES * unit16);
+    const uint8_t* src = (const uint8_t*)(uintptr_t)(ok ? at : (uint64_t)(uintptr_t)kv_zeros);
+    if constexpr (KV == KV_E4M3) {
+      (is_k ? kreg : vreg)[i] = *(const uint2*)src;
+      const long long sc = row_scale[st][r];
+      const float f = (is_k ? g.kv.k_scale : g.kv.v_scale)[max(sc, 0ll)];
+      (is_k ? kscale : vscale)[i] = sc >= 0 ? f : 1.f;
+    } else {
+      dma16(src, is_k ? lds_at(&kbuf[st][(wv * IPW + i) * KP]) : lds_at(&vbuf[st][(wv * IPW + i) * VP]));
     }
-    const int any = __ballot(none) != 0;
-    if (lane == 0) holes[st][wv] = any;
+  };
+  auto fetch = [&](auto is_k, int t) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < IPW; ++i) fetch1(is_k, t, i);
   };
   auto bf16x8_of = [&](uint2 w, float sc) __attribute__((always_inline)) {
     u32x4 r;
@@ -742,120 +757,200 @@ __global__ __launch_bounds__(256, (kParts<KV, T> > 1 ? 1 : 2)) void k_attn_many(
     r.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, sc, true));
     return sc == sc ? r : u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
   };
-  auto settle = [&](int st) __attribute__((always_inline)) {
+  auto settle = [&](auto is_k, int t) __attribute__((always_inline)) {
     if constexpr (KV == KV_E4M3) {
 #pragma unroll
-      for (int i = 0; i < IPW; ++i) {
-        *(u32x4*)&kbuf[st][(wv * IPW + i) * 1024 + 16 * lane] = bf16x8_of(kreg[i], kscale[i]);
-        *(u32x4*)&vbuf[st][(wv * IPW + i) * 1024 + 16 * lane] = bf16x8_of(vreg[i], vscale[i]);
-      }
+      for (int i = 0; i < IPW; ++i)
+        *(u32x4*)(is_k ? &kbuf[t & 1][(wv * IPW + i) * KP + 16 * lane] : &vbuf[t & 1][(wv * IPW + i) * VP + 16 * lane]) =
+            bf16x8_of((is_k ? kreg : vreg)[i], (is_k ? kscale : vscale)[i]);
     }
   };
+  constexpr std::true_type K{}, yes{};
+  constexpr std::false_type V{}, no{};
 
-  f32x16 o[DT];
+  f32x16 o[DT], sc[KH];
+  u32x4 pb[2 * KH][NP];
 #pragma unroll
   for (int t = 0; t < DT; ++t)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
   float m = -INFINITY, l = 0.f, le = 0.f;
-  const int kswz = c32 & KMASK;
-  const int g16 = lane >> 4, vr = 4 * (g16 >> 1) + ((lane & 15) >> 2), vswz = (vr & VMASK) << 1;
-  const int vunit = 2 * (g16 & 1) + ((lane & 3) >> 1), vbase = vr * DP * 2 + 8 * (lane & 1);
+  const int kbase = c32 % NI * KP + c32 / NI * RB + 16 * half;
+  // V's lanes: four rows of 16 values to 16 lanes, those of the second half of a wave four rows on
+  const int vm = 4 * half + ((lane & 15) >> 2), vbase = vm % NI * VP + vm / NI * RB + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+  constexpr int V8 = 8 % NI * VP + 8 / NI * RB, V16 = 16 % NI * VP + 16 / NI * RB;   // rows m + 8, m + 16
 
-  const int tiles = (u1 - u0 + KT - 1) / KT;
-  if (tiles > 0) {
-    places(u0);
-    fetch(u0, 0);
-    settle(0);
-    if (tiles > 1) places(u0 + KT);
-  }
-  for (int t = 0; t < tiles; ++t) {
-    const int st = t & 1, u = u0 + t * KT;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wave's copies of tile t
-    __syncthreads();                                   // and everybody's; the other stage is free
-    if (t + 1 < tiles) {
-      fetch(u + KT, st ^ 1);
-      if (t + 2 < tiles) places(u + 2 * KT);
-    }
-    const int key0 = u < sp.a ? u : sp.lo + u - sp.a, key1 = key0 + KT - 1;
-    const bool out_of_sight = !active || key0 > pos_max || (g.window > 0 && key1 <= pos_min - g.window && key0 >= g.sinks);
-    if (!out_of_sight) {
-      const int4 hs = *(const int4*)holes[st];
-      const bool some = (hs.x | hs.y | hs.z | hs.w) != 0;
-      const bool masked = key1 > pos_min || (g.window > 0 && !(key0 > pos_max - g.window || key1 < g.sinks)) || some;
-      // S^T: KT keys x 32 packed rows
-      f32x16 sc[KH];
+  // Scores of tile t (QK) into sc, and (EX) the weights of what sc held before into
+  // pb, each in the other's shadow, in the order written here: a slot is a read
+  // of K four slots ahead, the matrix instructions of one operand, a share of the
+  // weights and now and then a copy of V's next tile: sent in one go the copies
+  // would hold the wave up until their addresses are through.
+  constexpr int AHEAD = 4;
+  auto scores = [&](auto QK, auto EX, int t) __attribute__((always_inline)) {
+    constexpr int N = KH * CH, PAIRS = KH * 8;
+    f32x16 nx[KH];
+    const float ref = (m == -INFINITY ? 0.f : m) - kShift<KV>;
+    const uint8_t* kst = kbuf[t & 1];
+    u32x4 ka[N];
+    auto read = [&](int c) __attribute__((always_inline)) {
+      ka[c] = *(const u32x4*)&kst[kbase + c / CH * NI * KP + 32 * (c % CH)];
+    };
+    auto pair = [&](int e) __attribute__((always_inline)) {   // scores 2e and 2e + 1
+      const int h = e / 8, i = e % 8;
+      // f32: a product of its own, so that the reference's own key has weight 1
+      const float s0 = sc[h][2 * i], s1 = sc[h][2 * i + 1];
+      const float w0 = __builtin_amdgcn_exp2f(NP > 1 ? times(s0, scale2) - ref : fmaf(s0, scale2, -ref)),
+                  w1 = __builtin_amdgcn_exp2f(NP > 1 ? times(s1, scale2) - ref : fmaf(s1, scale2, -ref));
+      le += w0 + w1;
+      uint32_t w[NP];
+      split2<KV, NP>(w0, w1, w);
+      if constexpr (NP == 1) l = add2<KV>(w[0], l);
 #pragma unroll
-      for (int h = 0; h < KH; ++h) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) sc[h][i] = 0.f;
-#pragma unroll
-        for (int c = 0; c < CH; ++c) {
-          const u32x4 ka = *(const u32x4*)&kbuf[st][(32 * h + c32) * DP * 2 + (((2 * c + half) ^ kswz) << 4)];
-#pragma unroll
-          for (int k = NP - 1; k >= 0; --k) sc[h] = mfma32<KV>(ka, qb[k][c], sc[h]);
-        }
+      for (int k = 0; k < NP; ++k) {
+        asm volatile("" : "+v"(w[k]));   // here, not where it is used
+        pb[e / 4][k][e % 4] = w[k];
       }
-      float mx = -INFINITY;
-      if (masked) {
+    };
+    if constexpr (QK) {
 #pragma unroll
-        for (int h = 0; h < KH; ++h)
+      for (int h = 0; h < KH; ++h)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int j = 32 * h + 8 * (i >> 2) + 4 * half + (i & 3), key = key0 + j;
-            const bool sees = key <= pos && (g.window == 0 || key > pos - g.window || key < g.sinks) && hole[st][j] == 0.f;
-            sc[h][i] = sees ? sc[h][i] : -INFINITY;
+        for (int i = 0; i < 16; ++i) nx[h][i] = 0.f;
+#pragma unroll
+      for (int c = 0; c < AHEAD; ++c) read(c);
+#pragma unroll
+      for (int c = 0; c < N; ++c) {
+        if (c + AHEAD < N) read(c + AHEAD);
+#pragma unroll
+        for (int k = NP - 1; k >= 0; --k) nx[c / CH] = mfma32<KV>(ka[c], qb[k][c % CH], nx[c / CH]);
+        if constexpr (EX) {
+#pragma unroll
+          for (int e = c * PAIRS / N; e < (c + 1) * PAIRS / N; ++e) pair(e);
+          if constexpr (KV != KV_E4M3) {
+            if (c % (N / IPW) == 0) fetch1(V, t, c / (N / IPW));
           }
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
+#pragma unroll
+      for (int h = 0; h < KH; ++h) sc[h] = nx[h];
+    } else {
+#pragma unroll
+      for (int e = 0; e < PAIRS; ++e) pair(e);
+    }
+  };
+  // What a row does not see gets -inf; then the largest score.
+  int4 hs;   // whether tile t + 1 has keys without a place
+  auto mask = [&](int t) __attribute__((always_inline)) {
+    const int st = t & 1, key0 = key_of(u0 + t * KT), key1 = key0 + KT - 1;
+    if (key1 > pos_min || (g.window > 0 && !(key0 > pos_max - g.window || key1 < g.sinks)) || (hs.x | hs.y | hs.z | hs.w) != 0) {
+#pragma unroll
+      for (int h = 0; h < KH; ++h)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int m = 8 * (i >> 2) + 4 * half + (i & 3), j = 32 * h + RPI * (m % NI) + m / NI, key = key0 + j;
+          const bool sees = key <= pos && (g.window == 0 || key > pos - g.window || key < g.sinks) && hole[st][j] == 0.f;
+          sc[h][i] = sees ? sc[h][i] : -INFINITY;
+        }
+    }
+  };
+  // O^T += V^T P^T of tile t; MX: the largest of the scores in sc meanwhile, and the
+  // copies of K two tiles on.
+  float mx = -INFINITY;
+  auto products = [&](auto PV, auto MX, int t) __attribute__((always_inline)) {
+    const uint8_t* vst = vbuf[t & 1];
+    if constexpr (MX) mx = -INFINITY;
+    if constexpr (PV) {
+      constexpr int N = 2 * KH * DT;
+      u32x4 va[N];
+      auto read = [&](int c) __attribute__((always_inline)) {
+        const uint8_t* src = &vst[vbase + c / DT / 2 * NI * VP + c / DT % 2 * V16 + 64 * (c % DT)];
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) s16x4* lds4;
+        const s16x4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uintptr_t)lds_at(src)),
+                    a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uintptr_t)lds_at(src + V8));
+        const uint2 b0 = __builtin_bit_cast(uint2, a0), b1 = __builtin_bit_cast(uint2, a1);
+        va[c] = u32x4{b0.x, b0.y, b1.x, b1.y};
+      };
+#pragma unroll
+      for (int c = 0; c < AHEAD; ++c) read(c);
+#pragma unroll
+      for (int c = 0; c < N; ++c) {
+        if (c + AHEAD < N) read(c + AHEAD);
+#pragma unroll
+        for (int k = NP - 1; k >= 0; --k) o[c % DT] = mfma32<KV>(va[c], pb[c / DT][k], o[c % DT]);
+        if constexpr (MX) {   // two scores a slot
+#pragma unroll
+          for (int e = c * KH * 8 / N; e < (c + 1) * KH * 8 / N; ++e)
+            mx = fmaxf(fmaxf(mx, sc[e / 8][2 * (e % 8)]), sc[e / 8][2 * (e % 8) + 1]);
+          if constexpr (KV != KV_E4M3) {
+            if (c % (N / IPW) == 0) fetch1(K, t + 2, c / (N / IPW));
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else if constexpr (MX) {
 #pragma unroll
       for (int h = 0; h < KH; ++h)
 #pragma unroll
         for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[h][i]);
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * scale2;
-      if (__ballot(mx > m + kSlack)) {
-        const float mn = mx > m + kSlack ? mx : m;
-        const float f = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-        m = mn;
-        l *= f;
-        le *= f;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) o[d] *= f;
-      }
-      const float ref = (m == -INFINITY ? 0.f : m) - kShift<KV>;
-#pragma unroll
-      for (int h = 0; h < KH; ++h)
-#pragma unroll
-        for (int kg = 0; kg < 2; ++kg) {
-          u32x4 pb[NP];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            // f32: a product of its own, so that the reference's own key has weight 1
-            const float s0 = sc[h][8 * kg + 2 * i], s1 = sc[h][8 * kg + 2 * i + 1];
-            const float w0 = __builtin_amdgcn_exp2f(NP > 1 ? times(s0, scale2) - ref : fmaf(s0, scale2, -ref)),
-                        w1 = __builtin_amdgcn_exp2f(NP > 1 ? times(s1, scale2) - ref : fmaf(s1, scale2, -ref));
-            le += w0 + w1;
-            uint32_t w[NP];
-            split2<KV, NP>(w0, w1, w);
-            if constexpr (NP == 1) l = add2<KV>(w[0], l);
-#pragma unroll
-            for (int k = 0; k < NP; ++k) pb[k][i] = w[k];
-          }
-          // O^T: the head's values x 32 packed rows
-#pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            const uint8_t* src = &vbuf[st][(32 * h + 16 * kg) * DP * 2 + vbase + (((4 * d + vunit) ^ vswz) << 4)];
-            typedef short s16x4 __attribute__((ext_vector_type(4)));
-            typedef __attribute__((address_space(3))) s16x4* lds4;
-            const s16x4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uintptr_t)lds_at(src)),
-                        a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uintptr_t)lds_at(src + 8 * DP * 2));
-            const uint2 b0 = __builtin_bit_cast(uint2, a0), b1 = __builtin_bit_cast(uint2, a1);
-            const u32x4 va = {b0.x, b0.y, b1.x, b1.y};
-#pragma unroll
-            for (int k = NP - 1; k >= 0; --k) o[d] = mfma32<KV>(va, pb[k], o[d]);
-          }
-        }
     }
-    if (t + 1 < tiles) settle(st ^ 1);
+    if constexpr (MX) mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * scale2;
+  };
+  auto rescale = [&]() __attribute__((always_inline)) {
+    if (__ballot(mx > m + kSlack)) {
+      const float mn = mx > m + kSlack ? mx : m;
+      const float f = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l *= f;
+      le *= f;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[d] *= f;
+    }
+  };
+
+  // K runs a tile ahead of V: while tile t's weights are made, the scores of
+  // tile t + 1 are; the stage that a copy fills was last read before the barrier.
+  // Tiles that a wave's rows do not see are taken all the same, masked: the
+  // others would be waited for. K of tiles behind the last is read as zeros.
+  if (tiles > 0) {
+    ask(0);
+    rows(0);
+    ask(1);
+    fetch(K, 0);
+    fetch(V, 0);
+    settle(K, 0);
+    settle(V, 0);
+    rows(1);
+    ask(2);
+    fetch(K, 1);
+    settle(K, 1);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    hs = *(const int4*)holes[0];
+    scores(yes, no, 0);
+    mask(0);
+    products(no, yes, 0);
+    rescale();
+    for (int t = 0; t + 1 < tiles; ++t) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wave's copies of K t + 1 and V t
+      __syncthreads();                                   // and everybody's
+      hs = *(const int4*)holes[(t + 1) & 1];
+      if constexpr (KV == KV_E4M3) fetch(V, t + 1);
+      rows(t + 2);
+      ask(t + 3);
+      if constexpr (KV == KV_E4M3) fetch(K, t + 2);
+      scores(yes, yes, t + 1);
+      mask(t + 1);
+      products(yes, yes, t);
+      rescale();
+      settle(V, t + 1);
+      settle(K, t + 2);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    scores(no, yes, tiles - 1);
+    products(yes, no, tiles - 1);
   }
   if (!active) return;
 
@@ -967,13 +1062,18 @@ __global__ __launch_bounds__(256) void k_attn_join(KvAttnArgs g, long long unit0
   if (lane == 0 && g.lse) g.lse[unit] = lse_of<KV>(top, exact);
 }
 
+long long slots_of(const KvAttnArgs& g, int tile) {
+  return ((long long)g.kv.n_rows * g.group + (long long)(tile - 1) * g.kv.n_seqs) / tile;
+}
+
 template <int KV, int DP, class T>
 int attn_launch(const KvAttnArgs& g, int max_rows, hipStream_t s) {
   // launches of fewer than 2^24 blocks: a grid holds fewer than 2^32 threads
   const long long each = (long long)g.kv.n_kv * g.splits;
   const long long most = std::max(1ll, ((1ll << 24) - 1) / each);
   if (g.few_rows > 0) {
-    const long long slots = (long long)g.kv.n_rows * g.group / kKvFewTile + g.kv.n_seqs;
+    const long long slots = g.few_rows == 0x7fffffff ? slots_of(g, kKvFewTile)
+                                                     : (long long)g.kv.n_seqs * kKvFewTiles;
     for (long long at = 0; at < slots; at += most) {
       hipLaunchKernelGGL((k_attn_few<KV, DP, T>), dim3((unsigned)(std::min(most, slots - at) * each)), dim3(256), 0, s, g, (int)at);
       const hipError_t e = hipGetLastError();
@@ -981,7 +1081,7 @@ int attn_launch(const KvAttnArgs& g, int max_rows, hipStream_t s) {
     }
   }
   if (g.few_rows < 0x7fffffff) {
-    const long long slots = (long long)g.kv.n_rows * g.group / kKvManyTile + g.kv.n_seqs;
+    const long long slots = slots_of(g, kKvManyTile);
     for (long long at = 0; at < slots; at += most) {
       const int n = (int)std::min(most, slots - at);
       hipLaunchKernelGGL((k_attn_many<KV, DP, T>), dim3((unsigned)(n * each)), dim3(256), 0, s, g, (int)at, n);
@@ -1018,9 +1118,11 @@ int attn_type(int elem, const KvAttnArgs& g, int max_rows, hipStream_t s) {
 
 KvAttnPlan kv_attn_plan(int n_seqs, int n_rows, int max_rows, int max_len, int n_kv, int group, int dim, int window, int sinks) {
   KvAttnPlan p{};
-  constexpr int FEW = 64;   // packed rows of a sequence that k_attn_few takes
+  constexpr int FEW = kKvFewTiles * kKvFewTile;
   const bool few = (long long)max_rows * group <= FEW;
-  p.few_rows = few ? 0x7fffffff : FEW;
+  // Only long ones: k_attn_many alone, a launch less (5 us); what is short among
+  // them it can do too.
+  p.few_rows = few ? 0x7fffffff : (long long)n_rows * group >= 512ll * n_seqs ? 0 : FEW;
   const int tile = few ? kKvFewTile : kKvManyTile;
   long long most = max_len;   // keys that a tile's rows see at most
   if (window > 0) most = std::min(most, (long long)window + tile) + ((long long)std::min(sinks, max_len) + 63) / 64 * 64;
@@ -1030,8 +1132,20 @@ KvAttnPlan kv_attn_plan(int n_seqs, int n_rows, int max_rows, int max_len, int n
     chunk = (most * tiles / 4096 + kKvChunk) / kKvChunk * kKvChunk;
     chunk = std::max(chunk, most <= 2048 ? 128ll : 512ll);
   } else {
-    chunk = (most * tiles / 1024 + kKvChunk) / kKvChunk * kKvChunk;
-    chunk = std::max(chunk, 512ll);
+    // whole rounds of the CUs: a block's start and end cost about 200 keys, a
+    // chunk's sums are written and read once more
+    const long long real = ((long long)n_rows * group + tile - 1) / tile * n_kv;
+    double best = 1e300;
+    chunk = most;
+    for (long long c = 1; c <= 64 && c * 256 <= most; ++c) {
+      const long long len = ((most + c - 1) / c + kKvChunk - 1) / kKvChunk * kKvChunk;
+      const double rounds = (double)((real * c + 255) / 256);
+      const double cost = rounds * (len + 200.0) * dim / 256 + (c > 1 ? 100.0 + 0.06 * c * n_rows * group * n_kv * dim / 32768 : 0.0);
+      if (cost < best) {
+        best = cost;
+        chunk = len;
+      }
+    }
   }
   p.chunk = (int)std::min(chunk, (most + kKvChunk - 1) / kKvChunk * kKvChunk);
   p.splits = (int)((most + p.chunk - 1) / p.chunk);

@@ -680,6 +680,7 @@ struct KvAttnArgs {
 };
 constexpr int kKvChunk = 128;       // keys of the smallest chunk: 32 for each of four waves
 constexpr int kKvFewTile = 16;      // packed rows (row, head of the group) of a block of k_attn_few
+constexpr int kKvFewTiles = 4;      // tiles of a sequence that k_attn_few takes where others go to k_attn_many
 constexpr int kKvManyTile = 128;    // and of k_attn_many
 struct KvAttnPlan {
   int few_rows, chunk, splits;
