@@ -16,6 +16,7 @@
 #include "gg_kv_device.h"
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 namespace gg {
@@ -114,8 +115,9 @@ __device__ __forceinline__ int kv_splits(const KvAttnArgs& g, const Span& s) { r
 // has floor((r + n + (tile - 1) (s + 1)) / tile) - floor((r + (tile - 1) s) / tile) of
 // them, at least ceil(n / tile), so that a slot's sequence is found by search
 // and no list of tiles is made.
-__device__ __forceinline__ long long tile_slot(const KvAttnArgs& g, int s, int tile) {
-  return ((long long)min(max(g.kv.row_start[s], 0), g.kv.n_rows) * g.group + (long long)(tile - 1) * s) / tile;
+template <int TILE>
+__device__ __forceinline__ long long tile_slot(const KvAttnArgs& g, int row, int s) {
+  return ((long long)row * g.group + (long long)(TILE - 1) * s) / TILE;
 }
 
 // ln of a sum of weights relative to m (log2 units).
@@ -142,24 +144,43 @@ __device__ __forceinline__ bool odd_value(uint32_t h) {
 // when this one's is used up, V likewise.
 // ---------------------------------------------------------------------------
 template <int KV, int DP, class T>
-__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attn_few(KvAttnArgs g, int slot0) {
+__global__ __launch_bounds__(256, (DP <= 128 || (KV == KV_E4M3 && kParts<KV, T> == 1) ? 2 : 1)) void k_attn_few(KvAttnArgs g, int slot0, int slots) {
   constexpr int NP = kParts<KV, T>, KC = DP / 32, VD = DP / 16, OP = DP + 4;
   constexpr int ES = KV == KV_E4M3 ? 1 : 2;                 // bytes of an element in the pages
-  constexpr int KW = 2 * ES, VW = VD * ES / 4;              // dwords a lane loads of a K chunk, of a V row
+  constexpr int KL = KV == KV_E4M3 ? KC / 2 : KC, VW = VD * ES / 4;   // 16-byte loads of a K row, dwords of a V row
   __shared__ __align__(16) float o_all[4][kKvFewTile][OP];
   __shared__ float m_all[4][kKvFewTile], l_all[4][kKvFewTile], e_all[4][kKvFewTile];
   __shared__ __align__(16) long long key_off[4][32];        // where a step's rows lie, -1: nowhere
   __shared__ __align__(16) float k_sc[4][32], v_sc[4][32];
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c16 = lane & 15, quad = lane >> 4, D = g.kv.dim;
-  const int split = blockIdx.x % g.splits, hs = blockIdx.x / g.splits;
-  const int kvh = hs % g.kv.n_kv, slot = slot0 + hs / g.kv.n_kv;
+  // Heads fastest. With many tiles the chunks of one lie next to each other, and
+  // a place further round for each: the eight XCDs take blocks in turn, and
+  // without the turn one of them may get all of the last chunks, which few
+  // sequences have (61 tokens at up to 8192, 8 chunks, 8 heads: 295 us, 229 so, 252
+  // with the chunks slowest). With few tiles the chunks are slowest, so that the
+  // last blocks are short ones (3 tokens at up to 131072, 8 heads: 155 us, 191 the other way).
+  const int each = g.splits * g.kv.n_kv;
+  int split, kvh, slot;
+  if ((long long)slots * g.kv.n_kv >= 128) {
+    const int tile = (int)(blockIdx.x / each), r = (int)((blockIdx.x % each + (uint32_t)tile) % each);
+    kvh = r % g.kv.n_kv;
+    split = r / g.kv.n_kv;
+    slot = slot0 + tile;
+  } else {
+    const int r = (int)(blockIdx.x / g.kv.n_kv);
+    kvh = (int)(blockIdx.x % g.kv.n_kv);
+    split = r / slots;
+    slot = slot0 + r % slots;
+  }
   // beside k_attn_many only short sequences count, of a few tiles each
   const bool all = g.few_rows == 0x7fffffff;
-  const int s = all ? last_at_most(g.kv.n_seqs, [&](int i) { return tile_slot(g, i, kKvFewTile) <= slot; }) : slot / kKvFewTiles;
+  KvSeq sq;
+  int s = slot / kKvFewTiles;
+  if (all) s = kv_find(g.kv, slot, [&](int r, int i) { return tile_slot<kKvFewTile>(g, r, i); }, &sq);
+  else sq = kv_seq(g.kv, s);
   if (s < 0) return;
-  const KvSeq sq = kv_seq(g.kv, s);
-  const long long tile_l = all ? slot - tile_slot(g, s, kKvFewTile) : slot % kKvFewTiles;
+  const long long tile_l = all ? slot - tile_slot<kKvFewTile>(g, sq.first, s) : slot % kKvFewTiles;
   const int packed = sq.rows * g.group;
   if (tile_l < 0 || tile_l * kKvFewTile >= packed || packed > g.few_rows) return;
   const int p0 = (int)tile_l * kKvFewTile;
@@ -171,12 +192,14 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attn_few(KvAttnArgs 
   // this lane's packed row: its query as operand columns, its position
   const int p = p0 + c16, row = sq.first + p / g.group, head = kvh * g.group + p % g.group;
   const int pos = p < packed ? sq.len - sq.rows + p / g.group : -1;
+  const int pos_min = sq.len - sq.rows + p0 / g.group, pos_max = sq.len - sq.rows + min((p0 + kKvFewTile - 1) / g.group, sq.rows - 1);
   u32x4 qb[NP][KC];
   {
     const T* q = (const T*)g.q + (p < packed ? row * g.ldq + (long long)head * D : 0);
 #pragma unroll
     for (int c = 0; c < KC; ++c) {
-      const int d = 32 * c + 8 * quad;
+      // a lane's values of a chunk; with 8 bits those of two chunks lie together in K
+      const int d = KV == KV_E4M3 ? 64 * (c / 2) + 16 * quad + 8 * (c % 2) : 32 * c + 8 * quad;
       float f[8] = {};
       if (p < packed && d < D) {
         if (g.q_vec) {
@@ -207,45 +230,51 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attn_few(KvAttnArgs 
 #pragma unroll
   for (int t = 0; t < VD; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f, le = 0.f;   // le: of the weights before they are rounded, for lse
-  typedef uint32_t kw_t __attribute__((ext_vector_type(KW)));
   typedef uint32_t vw_t __attribute__((ext_vector_type(VW > 4 ? 4 : VW)));
   constexpr int VN = VW > 4 ? VW / 4 : 1;
-  kw_t kr[2][KC];
+  u32x4 kr[2][KL];
   vw_t vr[8][VN];
-  long long voff[8];
 
-  // The places of a step's keys, one a lane, into LDS.
+  // The page of a step's keys, one a lane, is asked for a step before its places
+  // are worked out and handed over in LDS; so are 8-bit rows' scales.
+  int page = 0;
+  float sk = 0.f, sv = 0.f;
+  const int key_lane = lane & 31;
+  auto ask = [&](int u) __attribute__((always_inline)) {
+    const int x = u + key_lane, key = min(max(x < sp.a ? x : sp.lo + x - sp.a, 0), g.kv.places - 1);
+    page = g.kv.table[(long long)s * g.kv.table_ld + (int)g.kv.page_div((uint32_t)key)];
+  };
+  uint32_t live = 0;   // bit i: key i of the step has a place; others are read from row 0
   auto places = [&](int u) __attribute__((always_inline)) {
-    if (lane < 32) {
-      const int x = u + lane, key = x < sp.a ? x : sp.lo + x - sp.a;
-      KvPlace at{};
-      const bool ok = x < u1 && (x >= sp.a || x < sp.sink) && kv_place(g.kv, s, key, &at);
-      key_off[wv][lane] = ok ? kv_offset(g.kv, at, kvh) : -1;
-      if constexpr (KV == KV_E4M3) {
-        k_sc[wv][lane] = ok ? g.kv.k_scale[kv_scale_at(g.kv, at, kvh)] : 0.f;
-        v_sc[wv][lane] = ok ? g.kv.v_scale[kv_scale_at(g.kv, at, kvh)] : 0.f;
-      }
+    const int x = u + key_lane, key = x < sp.a ? x : sp.lo + x - sp.a;
+    const bool ok = x < u1 && (x >= sp.a || x < sp.sink) && (uint32_t)page < (uint32_t)g.kv.n_pages;
+    const KvPlace at{ok ? page : 0, ok ? key - (int)g.kv.page_div((uint32_t)key) * g.kv.page_size : 0};
+    if (lane < 32) key_off[wv][lane] = kv_offset(g.kv, at, kvh) * ES;
+    live = (uint32_t)__ballot(ok);
+    if constexpr (KV == KV_E4M3) {
+      sk = g.kv.k_scale[kv_scale_at(g.kv, at, kvh)];
+      sv = g.kv.v_scale[kv_scale_at(g.kv, at, kvh)];
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   };
+  const int dk = 16 / ES * quad, dv = VD * c16;
+  const uint8_t* k_lane = (const uint8_t*)g.kv.k + dk * ES;
+  const uint8_t* v_lane = (const uint8_t*)g.kv.v + (dv < D ? dv : 0) * ES;
   auto load_k = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const long long off = max(key_off[wv][16 * h + c16], 0ll);
-      const uint8_t* r = (const uint8_t*)g.kv.k + off * ES;
+      const uint8_t* r = k_lane + key_off[wv][16 * h + c16];
 #pragma unroll
-      for (int c = 0; c < KC; ++c) {
-        const int d = 32 * c + 8 * quad;
-        kr[h][c] = *(const kw_t*)(r + (d < D ? d : 0) * ES);   // past D the query is 0
+      for (int c = 0; c < KL; ++c) {
+        const int d = 64 / ES * c;   // past D the query is 0
+        kr[h][c] = *(const u32x4*)(r + (d + dk < D ? d * ES : -dk * ES));
       }
     }
   };
   auto load_v = [&]() __attribute__((always_inline)) {
-    const int d = VD * c16;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      voff[j] = key_off[wv][4 * quad + (j & 3) + 16 * (j >> 2)];
-      const uint8_t* r = (const uint8_t*)g.kv.v + (max(voff[j], 0ll) + (d < D ? d : 0)) * ES;
+      const uint8_t* r = v_lane + key_off[wv][4 * quad + (j & 3) + 16 * (j >> 2)];
 #pragma unroll
       for (int n = 0; n < VN; ++n) vr[j][n] = ((const vw_t*)r)[n];
     }
@@ -257,24 +286,32 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attn_few(KvAttnArgs 
   int u = u0 + 32 * wv;
   float ks[8], vs[8];
   if (u < u1) {
+    ask(u);
     places(u);
+    ask(u + 128);
     load_k();
     if constexpr (!careful) load_v();
   }
   for (; u < u1; u += 128) {
     if constexpr (KV == KV_E4M3) {
+      if (lane < 32) {
+        k_sc[wv][lane] = sk;
+        v_sc[wv][lane] = sv;
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         ks[j] = k_sc[wv][4 * quad + (j & 3) + 16 * (j >> 2)];
         vs[j] = v_sc[wv][4 * quad + (j & 3) + 16 * (j >> 2)];
       }
     }
-    bool here[8], miss = false;
+    // this lane's keys are 4 quad + j and, from j = 4 on, 12 more
+    const uint32_t mine = __builtin_amdgcn_readfirstlane(live) >> (4 * quad);
+    const bool miss = __builtin_amdgcn_readfirstlane(live) != 0xffffffffu;
+    long long voff[8];
+    if constexpr (careful) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if constexpr (careful) voff[j] = key_off[wv][4 * quad + (j & 3) + 16 * (j >> 2)];
-      here[j] = voff[j] >= 0;
-      miss |= !here[j];
+      for (int j = 0; j < 8; ++j) voff[j] = key_off[wv][4 * quad + (j & 3) + 16 * (j >> 2)];
     }
     // S^T: 32 keys x 16 packed rows
     f32x4 sc[2];
@@ -286,10 +323,11 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attn_few(KvAttnArgs 
         u32x4 ka;
         if constexpr (KV == KV_E4M3) {
           typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-          const bf16x2 a0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(kr[h][c][0], 1.f, false),
-                       a1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(kr[h][c][0], 1.f, true),
-                       a2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(kr[h][c][1], 1.f, false),
-                       a3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(kr[h][c][1], 1.f, true);
+          const uint32_t k0 = kr[h][c / 2][2 * (c % 2)], k1 = kr[h][c / 2][2 * (c % 2) + 1];
+          const bf16x2 a0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(k0, 1.f, false),
+                       a1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(k0, 1.f, true),
+                       a2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(k1, 1.f, false),
+                       a3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(k1, 1.f, true);
           ka = u32x4{__builtin_bit_cast(uint32_t, a0), __builtin_bit_cast(uint32_t, a1), __builtin_bit_cast(uint32_t, a2),
                      __builtin_bit_cast(uint32_t, a3)};
         } else {
@@ -302,6 +340,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attn_few(KvAttnArgs 
     const int next = u + 128;
     if (next < u1) {
       places(next);
+      ask(next + 128);
       load_k();
     }
     // scores in log2 units; what the row does not see is -inf
@@ -309,14 +348,23 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attn_few(KvAttnArgs 
     float x[8], mx = -INFINITY;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int key = key0 + 4 * quad + (j & 3) + 16 * (j >> 2);
-      const bool sees = key <= pos && (g.window == 0 || key > pos - g.window || key < g.sinks);
-      float t = sc[j >> 2][j & 3] * g.scale2;
-      if constexpr (KV == KV_E4M3) t *= ks[j];
-      x[j] = here[j] && sees ? t : -INFINITY;
-      here[j] = here[j] && sees;
-      mx = fmaxf(mx, x[j]);
+      x[j] = sc[j >> 2][j & 3] * g.scale2;
+      if constexpr (KV == KV_E4M3) x[j] *= ks[j];
     }
+    // most steps are seen whole by all rows
+    const bool whole = !miss && key0 + 31 <= pos_min && (g.window == 0 || key0 > pos_max - g.window || key0 + 31 < g.sinks);
+    uint32_t here = ~0u;   // bit j: the row sees key j
+    if (!whole) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int i = (j & 3) + 16 * (j >> 2), key = key0 + 4 * quad + i;
+        const bool sees = ((mine >> i) & 1) && key <= pos && (g.window == 0 || key > pos - g.window || key < g.sinks);
+        x[j] = sees ? x[j] : -INFINITY;
+        here = sees ? here : here & ~(1u << j);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) mx = fmaxf(mx, x[j]);
     mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
     mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
     float f = 1.f;
@@ -348,37 +396,31 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attn_few(KvAttnArgs 
       }
       l += w0 + w1;
       if constexpr (KV == KV_E4M3) {
-        w0 = here[2 * i] ? w0 * vs[2 * i] : 0.f;
-        w1 = here[2 * i + 1] ? w1 * vs[2 * i + 1] : 0.f;
+        w0 *= vs[2 * i];
+        w1 *= vs[2 * i + 1];
+        if (!whole) {   // a hidden row's scale may be a NaN
+          w0 = (here >> (2 * i)) & 1 ? w0 : 0.f;
+          w1 = (here >> (2 * i + 1)) & 1 ? w1 : 0.f;
+        }
       }
       if constexpr (NP > 1 || KV == KV_E4M3) split2<KV, NP>(w0, w1, w);
 #pragma unroll
       for (int k = 0; k < NP; ++k) pb[k][i] = w[k];
     }
     // V of keys that are not there counts as 0: what lies there may be a NaN
-    if (!careful && __ballot(miss)) {
+    if (!careful && miss) {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
 #pragma unroll
-        for (int n = 0; n < VN; ++n) vr[j][n] = voff[j] >= 0 ? vr[j][n] : (vw_t)0;
+        for (int n = 0; n < VN; ++n) vr[j][n] = (mine >> ((j & 3) + 16 * (j >> 2))) & 1 ? vr[j][n] : (vw_t)0;
     }
-    // 16-bit rows of V: dword i of key j holds values 2i and 2i + 1
-    auto v_word = [&](int j, int i) __attribute__((always_inline)) -> uint32_t {
-      if constexpr (KV == KV_E4M3) {
-        const uint32_t w = vr[j][(i / 2) / 4][(i / 2) % 4];
-        return i % 2 ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, true))
-                     : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, false));
-      } else {
-        return vr[j][i / 4][i % 4];
-      }
-    };
     if constexpr (careful) {
       // sums in LDS, one value of a head at a time: the finite values as ever, then
       // the infinities of either sign among the keys that the row sees (a NaN is both)
       constexpr uint32_t ONE = KV == KV_F16 ? 0x3c00u : 0x3f80u, MANT = KV == KV_F16 ? 0x3ffu : 0x7fu;
       u32x4 seen;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) seen[i] = (here[2 * i] ? ONE : 0u) | (here[2 * i + 1] ? ONE << 16 : 0u);
+      for (int i = 0; i < 4; ++i) seen[i] = ((here >> (2 * i)) & 1 ? ONE : 0u) | ((here >> (2 * i + 1)) & 1 ? ONE << 16 : 0u);
 #pragma unroll 1
       for (int t = 0; t < VD; ++t) {
         const int d = VD * c16 + t;
@@ -389,8 +431,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attn_few(KvAttnArgs 
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             uint32_t h = 0;
-            if (voff[2 * i + e] >= 0 && d < D) {
-              const uint8_t* r = (const uint8_t*)g.kv.v + (voff[2 * i + e] + d) * ES;
+            if (((mine >> (((2 * i + e) & 3) + 16 * ((2 * i + e) >> 2))) & 1) && d < D) {
+              const uint8_t* r = (const uint8_t*)g.kv.v + voff[2 * i + e] + d * ES;
               if constexpr (KV == KV_E4M3)
                 h = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)*r, 1.f, false)) & 0xffffu;
               else
@@ -421,19 +463,40 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attn_few(KvAttnArgs 
         }
       }
     } else {
+      if constexpr (KV == KV_E4M3) {
+        // bytes of two keys side by side, then converted: four values of a head
 #pragma unroll
-      for (int t = 0; t < VD; t += 2) {
-        u32x4 lo, hi;
+        for (int t = 0; t < VD; t += 4) {
+          u32x4 va[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t w0 = v_word(2 * i, t / 2), w1 = v_word(2 * i + 1, t / 2);
-          lo[i] = lower2(w0, w1);
-          hi[i] = upper2(w0, w1);
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t w0 = vr[2 * i][t / 16][t / 4 % 4], w1 = vr[2 * i + 1][t / 16][t / 4 % 4];
+            const uint32_t lo = __builtin_amdgcn_perm(w1, w0, 0x05010400u), hi = __builtin_amdgcn_perm(w1, w0, 0x07030602u);
+            va[0][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false));
+            va[1][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true));
+            va[2][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false));
+            va[3][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true));
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int k = NP - 1; k >= 0; --k) o[t + e] = mfma16<KV>(va[e], pb[k], o[t + e]);
         }
+      } else {
 #pragma unroll
-        for (int k = NP - 1; k >= 0; --k) {
-          o[t] = mfma16<KV>(lo, pb[k], o[t]);
-          o[t + 1] = mfma16<KV>(hi, pb[k], o[t + 1]);
+        for (int t = 0; t < VD; t += 2) {
+          u32x4 lo, hi;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t w0 = vr[2 * i][t / 8][t / 2 % 4], w1 = vr[2 * i + 1][t / 8][t / 2 % 4];
+            lo[i] = lower2(w0, w1);
+            hi[i] = upper2(w0, w1);
+          }
+#pragma unroll
+          for (int k = NP - 1; k >= 0; --k) {
+            o[t] = mfma16<KV>(lo, pb[k], o[t]);
+            o[t + 1] = mfma16<KV>(hi, pb[k], o[t + 1]);
+          }
         }
       }
     }
@@ -647,10 +710,10 @@ __global__ __launch_bounds__(256, (kParts<KV, T> > 1 || DP > 128 ? 1 : 2)) void 
   const int unit = xcd * (G >> 3) + min(xcd, G & 7) + (blockIdx.x >> 3);
   const int slot = slot0 + unit % slots, ks_ = unit / slots;
   const int split = ks_ % g.splits, kvh = ks_ / g.splits;
-  const int s = last_at_most(g.kv.n_seqs, [&](int i) { return tile_slot(g, i, kKvManyTile) <= slot; });
+  KvSeq sq;
+  const int s = kv_find(g.kv, slot, [&](int r, int i) { return tile_slot<kKvManyTile>(g, r, i); }, &sq);
   if (s < 0) return;
-  const KvSeq sq = kv_seq(g.kv, s);
-  const long long tile_l = slot - tile_slot(g, s, kKvManyTile);
+  const long long tile_l = slot - tile_slot<kKvManyTile>(g, sq.first, s);
   const int packed = sq.rows * g.group;
   if (tile_l < 0 || tile_l * kKvManyTile >= packed || packed <= g.few_rows) return;
   const int p0 = (int)tile_l * kKvManyTile;
@@ -1013,53 +1076,103 @@ __global__ __launch_bounds__(256, (kParts<KV, T> > 1 || DP > 128 ? 1 : 2)) void 
   }
 }
 
-// Joins the chunks of tiles that have several: one wave for a row's head.
-template <int KV, class T>
+// Joins the chunks of tiles that have several: W waves for a row's head, L lanes
+// to a chunk's sums (four values each), so that 64 W / L chunks are read at once.
+template <int KV, class T, int W, int L>
 __global__ __launch_bounds__(256) void k_attn_join(KvAttnArgs g, long long unit0) {
-  const int lane = threadIdx.x & 63;
-  const long long unit = unit0 + (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (unit >= (long long)g.kv.n_rows * g.n_q) return;
-  const int row = (int)(unit / g.n_q), head = (int)(unit % g.n_q), D = g.kv.dim;
-  const int s = kv_seq_of(g.kv, row);
-  if (s < 0) return;
-  const KvSeq sq = kv_seq(g.kv, s);
-  const bool few = sq.rows * g.group <= g.few_rows;
-  const int tile = few ? kKvFewTile : kKvManyTile;
-  const int p0 = ((row - sq.first) * g.group + head % g.group) / tile * tile;
-  const int t0 = p0 / g.group, t1 = min((p0 + tile - 1) / g.group, sq.rows - 1);
-  const Span sp = few ? kv_span<32>(g, sq, t0, t1) : kv_span<64>(g, sq, t0, t1);
-  const int n = kv_splits(g, sp);
-  if (n < 2) return;
-  const long long step = (long long)g.kv.n_rows * g.n_q;
-  float top = -INFINITY;
-  for (int i = lane; i < n; i += 64) top = fmaxf(top, g.part_ml[4 * (unit + i * step)]);
-  top = wave_max(top);
-  float sum = 0.f, exact = 0.f;
-  for (int i = lane; i < n; i += 64) {
-    const f32x4 ml = *(const f32x4*)(g.part_ml + 4 * (unit + i * step));
-    const float f = ml.x == top ? 1.f : __builtin_amdgcn_exp2f(ml.x - top);
-    sum += f * ml.y;
-    exact += f * ml.z;
+  constexpr int N = W * 64 / L, PER = 4 / W;
+  __shared__ __align__(16) float sums[W > 1 ? W : 1][W > 1 ? 4 * L : 4];
+  __shared__ f32x4 stats[4];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  const long long unit = unit0 + (long long)blockIdx.x * PER + wv / W;
+  const int me = wv % W * (64 / L) + lane / L, d = 4 * (lane % L);   // this lane's chunks me, me + N, ..
+  const bool there = unit < (long long)g.kv.n_rows * g.n_q;
+  const int row = (int)(there ? unit / g.n_q : 0), head = (int)(there ? unit % g.n_q : 0), D = g.kv.dim;
+  KvSeq sq;
+  const int s = kv_seq_of(g.kv, row, &sq);
+  int n = 0;
+  if (there && s >= 0) {
+    const bool few = sq.rows * g.group <= g.few_rows;
+    const int tile = few ? kKvFewTile : kKvManyTile;
+    const int p0 = ((row - sq.first) * g.group + head % g.group) / tile * tile;
+    const int t0 = p0 / g.group, t1 = min((p0 + tile - 1) / g.group, sq.rows - 1);
+    n = kv_splits(g, few ? kv_span<32>(g, sq, t0, t1) : kv_span<64>(g, sq, t0, t1));
   }
-  sum = wave_sum(sum);
-  exact = wave_sum(exact);
-  const int d = 4 * lane;
+  if (n < 2) return;   // W > 1: the same in all of the block
+  const long long step = (long long)g.kv.n_rows * g.n_q;
+  // with a running reference, as the chunks themselves
+  float top = -INFINITY, sum = 0.f, exact = 0.f;
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
-  if (d < D) {
 #pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-      const float m = g.part_ml[4 * (unit + i * step)];
-      const float f = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top);
-      const f32x4 part = *(const f32x4*)(g.part_o + (unit + i * step) * D + d);
+  for (int i = me; i < n; i += N) {
+    const f32x4 ml = *(const f32x4*)(g.part_ml + 4 * (unit + i * step));
+    const f32x4 part = d < D ? *(const f32x4*)(g.part_o + (unit + i * step) * D + d) : f32x4{0.f, 0.f, 0.f, 0.f};
+    const float m = fmaxf(top, ml.x), f = top == m ? 1.f : __builtin_amdgcn_exp2f(top - m), h = ml.x == m ? 1.f : __builtin_amdgcn_exp2f(ml.x - m);
+    sum = f * sum + h * ml.y;
+    exact = f * exact + h * ml.z;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] += scaled(part[k], f);
+    for (int k = 0; k < 4; ++k) v[k] = scaled(v[k], f) + scaled(part[k], h);
+    top = m;
+  }
+  float all = top;
+#pragma unroll
+  for (int o = L; o < 64; o <<= 1) all = fmaxf(all, __shfl_xor(all, o, 64));
+  if constexpr (W > 1) {
+    if (lane == 0) stats[wv].x = all;
+    __syncthreads();
+    all = fmaxf(fmaxf(stats[0].x, stats[1].x), fmaxf(stats[2].x, stats[3].x));
+    __syncthreads();
+  }
+  const float f = top == all ? 1.f : __builtin_amdgcn_exp2f(top - all);
+  sum *= f;
+  exact *= f;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) v[k] = scaled(v[k], f);
+#pragma unroll
+  for (int o = L; o < 64; o <<= 1) {
+    sum += __shfl_xor(sum, o, 64);
+    exact += __shfl_xor(exact, o, 64);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] += __shfl_xor(v[k], o, 64);
+  }
+  if constexpr (W > 1) {
+    if (lane == 0) stats[wv] = f32x4{0.f, sum, exact, 0.f};
+    if (lane < L) *(f32x4*)&sums[wv][d] = v;
+    __syncthreads();
+    if (wv > 0) return;
+    sum = exact = 0.f;
+    v = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      sum += stats[w].y;
+      exact += stats[w].z;
+      if (lane < L) v += *(const f32x4*)&sums[w][d];
     }
+  }
+  if (lane < L && d < D) {
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     T* out = (T*)g.out + row * g.ldo + (long long)head * D + d;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) out[i] = (T)(v[i] * inv);
+    for (int i = 0; i < 4; ++i) out[i] = (T)scaled(v[i], inv);
   }
-  if (lane == 0 && g.lse) g.lse[unit] = lse_of<KV>(top, exact);
+  if (lane == 0 && g.lse) g.lse[unit] = lse_of<KV>(all, exact);
+}
+
+template <int KV, class T, int W, int L>
+int join_launch(const KvAttnArgs& g, hipStream_t s) {
+  constexpr long long MOST = 1ll << 22, PER = 4 / W;   // blocks
+  const long long units = (long long)g.kv.n_rows * g.n_q;
+  for (long long at = 0; at < units; at += MOST * PER) {
+    hipLaunchKernelGGL((k_attn_join<KV, T, W, L>), dim3((unsigned)((std::min(units - at, MOST * PER) + PER - 1) / PER)), dim3(256), 0, s, g, at);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return (int)e;
+  }
+  return 0;
+}
+template <int KV, class T, int L>
+int join_waves(const KvAttnArgs& g, hipStream_t s) {
+  // four waves where a wave would take more than eight turns (48 rows of 256, 256 chunks: 46 us with one)
+  return g.splits > 8 * (64 / L) ? join_launch<KV, T, 4, L>(g, s) : join_launch<KV, T, 1, L>(g, s);
 }
 
 long long slots_of(const KvAttnArgs& g, int tile) {
@@ -1075,7 +1188,8 @@ int attn_launch(const KvAttnArgs& g, int max_rows, hipStream_t s) {
     const long long slots = g.few_rows == 0x7fffffff ? slots_of(g, kKvFewTile)
                                                      : (long long)g.kv.n_seqs * kKvFewTiles;
     for (long long at = 0; at < slots; at += most) {
-      hipLaunchKernelGGL((k_attn_few<KV, DP, T>), dim3((unsigned)(std::min(most, slots - at) * each)), dim3(256), 0, s, g, (int)at);
+      const int n = (int)std::min(most, slots - at);
+      hipLaunchKernelGGL((k_attn_few<KV, DP, T>), dim3((unsigned)(n * each)), dim3(256), 0, s, g, (int)at, n);
       const hipError_t e = hipGetLastError();
       if (e != hipSuccess) return (int)e;
     }
@@ -1090,13 +1204,7 @@ int attn_launch(const KvAttnArgs& g, int max_rows, hipStream_t s) {
     }
   }
   if (g.splits == 1) return 0;
-  const long long units = (long long)g.kv.n_rows * g.n_q;
-  for (long long at = 0; at < units; at += 1ll << 25) {
-    hipLaunchKernelGGL((k_attn_join<KV, T>), dim3((unsigned)((std::min(units - at, 1ll << 25) + 3) / 4)), dim3(256), 0, s, g, at);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return (int)e;
-  }
-  return 0;
+  return g.kv.dim <= 64 ? join_waves<KV, T, 16>(g, s) : g.kv.dim <= 128 ? join_waves<KV, T, 32>(g, s) : join_waves<KV, T, 64>(g, s);
 }
 template <int KV, class T>
 int attn_dim(const KvAttnArgs& g, int max_rows, hipStream_t s) {
@@ -1116,7 +1224,18 @@ int attn_type(int elem, const KvAttnArgs& g, int max_rows, hipStream_t s) {
 
 }  // namespace
 
-KvAttnPlan kv_attn_plan(int n_seqs, int n_rows, int max_rows, int max_len, int n_kv, int group, int dim, int window, int sinks) {
+// The chunk length is taken from estimates of a call's time, in us, over the
+// numbers of chunks; lengths are taken to be spread between 0 and max_len.
+// k_attn_few: a block starts and ends in 5 us and takes 128 keys in 1.2, or as long as
+// 5 TB/s need for what all resident blocks read; a join takes 3 and 0.15 a chunk.
+// Measured at the two sides of the choice: 16 drafts of 12 packed rows at 4096
+// positions, heads of 128: 5 chunks 39 us, 3 46, 8 48; 61 tokens at 8192: 8
+// chunks 231, 4 330, 2 276; 3 tokens at 131072, 8-bit heads of 256: 21 chunks 155,
+// 64 165, 256 193.
+// k_attn_many: whole rounds of the CUs; a block's start and end cost about 200
+// keys, a chunk's sums are written and read once more.
+KvAttnPlan kv_attn_plan(int n_seqs, int n_rows, int max_rows, int max_len, int n_kv, int group, int dim, int window, int sinks,
+                        int key_bytes, bool two) {
   KvAttnPlan p{};
   constexpr int FEW = kKvFewTiles * kKvFewTile;
   const bool few = (long long)max_rows * group <= FEW;
@@ -1126,25 +1245,27 @@ KvAttnPlan kv_attn_plan(int n_seqs, int n_rows, int max_rows, int max_len, int n
   const int tile = few ? kKvFewTile : kKvManyTile;
   long long most = max_len;   // keys that a tile's rows see at most
   if (window > 0) most = std::min(most, (long long)window + tile) + ((long long)std::min(sinks, max_len) + 63) / 64 * 64;
-  const long long tiles = ((long long)n_rows * group / tile + n_seqs) * n_kv;
-  long long chunk;
-  if (few) {
-    chunk = (most * tiles / 4096 + kKvChunk) / kKvChunk * kKvChunk;
-    chunk = std::max(chunk, most <= 2048 ? 128ll : 512ll);
-  } else {
-    // whole rounds of the CUs: a block's start and end cost about 200 keys, a
-    // chunk's sums are written and read once more
-    const long long real = ((long long)n_rows * group + tile - 1) / tile * n_kv;
-    double best = 1e300;
-    chunk = most;
-    for (long long c = 1; c <= 64 && c * 256 <= most; ++c) {
-      const long long len = ((most + c - 1) / c + kKvChunk - 1) / kKvChunk * kKvChunk;
-      const double rounds = (double)((real * c + 255) / 256);
-      const double cost = rounds * (len + 200.0) * dim / 256 + (c > 1 ? 100.0 + 0.06 * c * n_rows * group * n_kv * dim / 32768 : 0.0);
-      if (cost < best) {
-        best = cost;
-        chunk = len;
-      }
+  const long long packed = (long long)n_rows * group, of_seq = (packed + n_seqs - 1) / n_seqs;
+  const double tiles = (double)n_seqs * (double)((of_seq + tile - 1) / tile) * n_kv;
+  const double share = window > 0 ? 1.0 : 0.5 + 0.5 / n_seqs, cus = two ? 512 : 256;
+  double best = 1e300;
+  long long chunk = most;
+  for (long long c = 1; c <= 256 && (c - 1) * kKvChunk < most; ++c) {
+    const long long len = ((most + c - 1) / c + kKvChunk - 1) / kKvChunk * kKvChunk;
+    double cost;
+    if (few) {
+      const double blocks = tiles * (most * share / len + (n_seqs > 1 ? 0.5 : 0.0));
+      const double rounds = std::max(1.0, blocks / 256 + (n_seqs > 1 ? 0.4 : 0.0));
+      cost = rounds * (5.0 + len / 128 * std::max(1.2, 128.0 * key_bytes / 5e6 * std::min(blocks, 256.0))) + (c > 1 ? 3.0 + 0.1 * c : 0.0);
+    } else {
+      if (c > 64) break;
+      const double real = std::max(1.0, (double)((packed + tile - 1) / tile * n_kv));
+      cost = std::ceil(real * c / 256) * (len + 200.0) * dim / 256 +
+             (c > 1 ? 100.0 + 0.06 * c * n_rows * group * n_kv * dim / 32768 : 0.0);
+    }
+    if (cost < best) {
+      best = cost;
+      chunk = len;
     }
   }
   p.chunk = (int)std::min(chunk, (most + kKvChunk - 1) / kKvChunk * kKvChunk);

@@ -685,7 +685,9 @@ constexpr int kKvManyTile = 128;    // and of k_attn_many
 struct KvAttnPlan {
   int few_rows, chunk, splits;
 };
-KvAttnPlan kv_attn_plan(int n_seqs, int n_rows, int max_rows, int max_len, int n_kv, int group, int dim, int window, int sinks);
+// key_bytes: of a key and its value; two: whether two blocks of k_attn_few share a CU.
+KvAttnPlan kv_attn_plan(int n_seqs, int n_rows, int max_rows, int max_len, int n_kv, int group, int dim, int window, int sinks,
+                        int key_bytes, bool two);
 int launch_kv_attention(int kv_type, int elem, const KvAttnArgs& a, int max_rows, void* stream);
 
 // ---- verification of drafted tokens (gg_verify.hip) ----------------------------

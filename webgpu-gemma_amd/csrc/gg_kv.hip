@@ -83,9 +83,9 @@ __global__ __launch_bounds__(256) void k_kv_store(KvStoreArgs a) {
     load4(source(group) + j, a.vec, lo);
     load4(source(group) + half + j, a.vec, hi);
   }
-  const int s = kv_seq_of(a.kv, row);
+  KvSeq sq;
+  const int s = kv_seq_of(a.kv, row, &sq);
   if (s < 0) return;   // the same in all of the block
-  const KvSeq sq = kv_seq(a.kv, s);
   const int pos = sq.len - sq.rows + (row - sq.first);
   KvPlace at{};
   const bool placed = pos >= 0 && pos < a.kv.places && kv_place(a.kv, s, pos, &at);
@@ -183,9 +183,9 @@ __global__ __launch_bounds__(256) void k_kv_store(KvStoreArgs a) {
 template <int KV, class T>
 __global__ __launch_bounds__(256) void k_kv_load(KvLoadArgs a) {
   const int row = a.row0 + blockIdx.x, D = a.kv.dim, per = D / 8, units = 2 * a.kv.n_kv * per;
-  const int s = kv_seq_of(a.kv, row);
+  KvSeq sq;
+  const int s = kv_seq_of(a.kv, row, &sq);
   if (s < 0) return;
-  const KvSeq sq = kv_seq(a.kv, s);
   const int pos = sq.len - sq.rows + (row - sq.first);
   KvPlace at{};
   const bool placed = pos >= 0 && pos < a.kv.places && kv_place(a.kv, s, pos, &at);

@@ -2011,7 +2011,7 @@ bool attn_shape_ok(const gg_kv_pages* p, const gg_kv_seqs* s, int32_t n_q_heads,
 }
 KvAttnPlan attn_plan(const gg_kv_pages* p, const gg_kv_seqs* s, int32_t n_q_heads, int32_t window, int32_t sinks) {
   return kv_attn_plan(s->n_seqs, s->n_rows, s->max_rows, s->max_len, p->n_kv_heads, n_q_heads / p->n_kv_heads, p->head_dim, window,
-                      sinks);
+                      sinks, 2 * p->head_dim * (p->type == GG_TYPE_E4M3 ? 1 : 2), p->head_dim <= 128 || p->type == GG_TYPE_E4M3);
 }
 
 }  // namespace
