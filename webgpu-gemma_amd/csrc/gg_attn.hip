@@ -689,7 +689,7 @@ __device__ void slow_row(const KvAttnArgs& g, int s, const KvSeq& sq, const Span
 }
 
 template <int KV, int DP, class T>
-__global__ __launch_bounds__(256, (kParts<KV, T> > 1 || DP > 128 ? 1 : 2)) void k_attn_many(KvAttnArgs g, int slot0, int slots) {
+__global__ __launch_bounds__(256, (kParts<KV, T> > 1 || DP > 128 || (DP == 128 && KV == KV_E4M3) ? 1 : 2)) void k_attn_many(KvAttnArgs g, int slot0, int slots) {
   constexpr int NP = kParts<KV, T>, KT = DP == 256 && NP > 1 ? 32 : 64, UN = DP / 8, RPI = 64 / UN, IPW = KT / RPI / 4;
   constexpr int KH = KT / 32, DT = DP / 32, CH = DP / 16, ES = KV == KV_E4M3 ? 1 : 2;
   // In LDS a copy's RPI rows are 1024 bytes, and some more to the next one: 16

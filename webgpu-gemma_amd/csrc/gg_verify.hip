@@ -28,14 +28,74 @@ __device__ __forceinline__ uint64_t logit_key(float z, int i) {
   const uint32_t b = __float_as_uint(z + 0.0f);   // -0 counts as 0
   return ((uint64_t)(b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u)) << 32) | (0xffffffffu - (uint32_t)i);
 }
-__device__ __forceinline__ uint64_t shfl_xor64(uint64_t x, int o) {
-  return ((uint64_t)(uint32_t)__shfl_xor((int)(x >> 32), o, 64) << 32) | (uint32_t)__shfl_xor((int)x, o, 64);
+// Wave reductions of 64-bit values on the DPP network, a few cycles a step where
+// shuffles through LDS take over a hundred: lanes without a source read 0.
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ uint64_t dpp64(uint64_t x) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(x >> 32), CTRL, ROWS, 0xf, false);
+  return ((uint64_t)hi << 32) | lo;
 }
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ double dpp_f64(double x) {
+  return __builtin_bit_cast(double, dpp64<CTRL, ROWS>(__builtin_bit_cast(uint64_t, x)));
 }
+__device__ __forceinline__ uint64_t lane63(uint64_t x) {
+  return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), 63) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
+}
+// Inclusive sums in lane order: within rows of 16, then rows 0 and 2 into the next one, then the first two into the others.
+__device__ __forceinline__ double wave_scan(double x) {
+  x += dpp_f64<0x111>(x);
+  x += dpp_f64<0x112>(x);
+  x += dpp_f64<0x114>(x);
+  x += dpp_f64<0x118>(x);
+  x += dpp_f64<0x142, 0xa>(x);
+  x += dpp_f64<0x143, 0xc>(x);
+  return x;
+}
+__device__ __forceinline__ double wave_sum(double x) { return __builtin_bit_cast(double, lane63(__builtin_bit_cast(uint64_t, wave_scan(x)))); }
+__device__ __forceinline__ uint64_t wave_max64(uint64_t x) {
+  const auto up = [](uint64_t a, uint64_t b) { return a > b ? a : b; };
+  x = up(x, dpp64<0x111>(x));
+  x = up(x, dpp64<0x112>(x));
+  x = up(x, dpp64<0x114>(x));
+  x = up(x, dpp64<0x118>(x));
+  x = up(x, dpp64<0x142, 0xa>(x));
+  x = up(x, dpp64<0x143, 0xc>(x));
+  return lane63(x);
+}
+__device__ __forceinline__ float wave_top(float x) {
+  x = fmaxf(x, dpp_mov_ninf<0x111, 0xf>(x));
+  x = fmaxf(x, dpp_mov_ninf<0x112, 0xf>(x));
+  x = fmaxf(x, dpp_mov_ninf<0x114, 0xf>(x));
+  x = fmaxf(x, dpp_mov_ninf<0x118, 0xf>(x));
+  x = fmaxf(x, dpp_mov_ninf<0x142, 0xa>(x));
+  x = fmaxf(x, dpp_mov_ninf<0x143, 0xc>(x));
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
+}
+
+// 2^x for x of 0 or less, f64: 2^round(x) times the Taylor sum of e^r to r^11,
+// |r| <= ln(2) / 2, so that 0.347^12 / 12! = 6e-15 of it is left out; under 2^-1100
+// it is 0. Under half the instructions of exp(), which is what k_verify_sums is bound by
+// (two rows of 262144 for each of 48 sequences).
+__device__ __forceinline__ double exp2_below(double x) {
+  x = fmax(x, -1100.0);
+  const double n = rint(x), r = (x - n) * 0.69314718055994530942;
+  double p = 1.0 / 39916800;
+  p = fma(p, r, 1.0 / 3628800);
+  p = fma(p, r, 1.0 / 362880);
+  p = fma(p, r, 1.0 / 40320);
+  p = fma(p, r, 1.0 / 5040);
+  p = fma(p, r, 1.0 / 720);
+  p = fma(p, r, 1.0 / 120);
+  p = fma(p, r, 1.0 / 24);
+  p = fma(p, r, 1.0 / 6);
+  p = fma(p, r, 0.5);
+  p = fma(p, r, 1.0);
+  p = fma(p, r, 1.0);
+  return ldexp(p, (int)n);
+}
+constexpr double kLog2e64 = 1.44269504088896340736;
 
 // Temperature of a sequence; 0 (or what is none): greedy.
 __device__ __forceinline__ bool greedy(float t) { return !(t > 0.f); }
@@ -81,14 +141,17 @@ __global__ __launch_bounds__(256) void k_verify_stat(VerifyArgs a) {
     bad |= !(v[i] < INFINITY);
     m = fmaxf(m, v[i]);
   }
+  if (greedy(t)) {
 #pragma unroll
-  for (int i = EPT - 1; i >= 0; --i)
-    if (v[i] == m) best = logit_key(m, (int)(((long long)part * 256 * NV + (i / VE) * 256 + tid) * VE - shift) + i % VE);
+    for (int i = EPT - 1; i >= 0; --i)
+      if (v[i] == m) best = logit_key(m, (int)(((long long)part * 256 * NV + (i / VE) * 256 + tid) * VE - shift) + i % VE);
+    best = wave_max64(best);
+  }
   __shared__ float ms[4];
   __shared__ double ss[4];
   __shared__ uint64_t bs[4];
   __shared__ int bads[4];
-  const float wm = wave_max(m);
+  const float wm = wave_top(m);
   if (lane == 0) ms[tid >> 6] = wm;
   __syncthreads();
   m = fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3]));
@@ -97,11 +160,6 @@ __global__ __launch_bounds__(256) void k_verify_stat(VerifyArgs a) {
 #pragma unroll
   for (int i = 0; i < EPT; ++i) sum[i & 3] += __builtin_amdgcn_exp2f((v[i] - ref) * c);
   const double total = wave_sum((double)((sum[0] + sum[1]) + (sum[2] + sum[3])));
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const uint64_t x = shfl_xor64(best, o);
-    best = x > best ? x : best;
-  }
   const int any = __ballot(bad) != 0;
   if (lane == 0) {
     ss[tid >> 6] = total;
@@ -128,7 +186,7 @@ struct Row {
   uint64_t best;
   bool bad;
 };
-__device__ Row join_parts(const VerifyPart* p, int n, double heat) {
+__device__ __forceinline__ Row join_parts(const VerifyPart* p, int n, double c, bool greedy) {
   const int lane = threadIdx.x & 63;
   Row r{-INFINITY, 0.0, 0, false};
   int bad = 0;
@@ -137,14 +195,10 @@ __device__ Row join_parts(const VerifyPart* p, int n, double heat) {
     r.best = p[i].best > r.best ? p[i].best : r.best;
     bad |= p[i].bad;
   }
-  r.m = wave_max(r.m);
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const uint64_t x = shfl_xor64(r.best, o);
-    r.best = x > r.best ? x : r.best;
-  }
+  r.m = wave_top(r.m);
+  if (greedy) r.best = wave_max64(r.best);
   for (int i = lane; i < n; i += 64)
-    if (p[i].max > -INFINITY) r.sum += p[i].sum * exp(((double)p[i].max - r.m) / heat);
+    if (p[i].max > -INFINITY) r.sum += p[i].sum * exp2_below(((double)p[i].max - r.m) * c);
   r.sum = wave_sum(r.sum);
   r.bad = __ballot(bad) != 0 || r.m == -INFINITY;
   return r;
@@ -168,13 +222,13 @@ __device__ Decision decide(const VerifyArgs& a, int s, bool write) {
   d.end = (int)min(max((long long)a.row_start[s + 1], 0ll), a.rows);
   const float t = a.temperature[s];
   d.greedy = greedy(t);
-  const double heat = d.greedy ? 1.0 : (double)t;
+  const double heat = d.greedy ? 1.0 : (double)t, c = kLog2e64 / heat;
   d.stop.row = -1;
   for (int r0 = d.first; r0 < d.end; r0 += 4) {
     const int row = r0 + wv;
     if (row < d.end) {
       const bool last = row == d.end - 1;
-      const Row p = join_parts(a.part + (long long)row * a.parts, a.parts, heat);
+      const Row p = join_parts(a.part + (long long)row * a.parts, a.parts, c, d.greedy);
       const int id = last ? -1 : a.draft[row];
       const bool real = id >= 0 && id < a.n;
       VerifyStop st{row, 0, p.m, 0.f, p.sum, 0.0};
@@ -187,13 +241,13 @@ __device__ Decision decide(const VerifyArgs& a, int s, bool write) {
       } else {
         double q = 1.0;
         if (a.y && !last) {
-          const Row y = join_parts(a.part + (a.rows + (long long)row) * a.parts, a.parts, heat);
+          const Row y = join_parts(a.part + (a.rows + (long long)row) * a.parts, a.parts, c, false);
           bad |= y.bad;
           st.mq = y.m;
           st.sq = y.sum;
-          q = real ? exp(((double)(float)((const T*)a.y)[row * a.ldy + id] - y.m) / heat) / y.sum : 0.0;
+          q = real ? exp2_below(((double)(float)((const T*)a.y)[row * a.ldy + id] - y.m) * c) / y.sum : 0.0;
         }
-        const bool stands = real && !last && a.accept_u[row] * q < exp((z_id - p.m) / heat) / p.sum;
+        const bool stands = real && !last && a.accept_u[row] * q * p.sum < exp2_below((z_id - p.m) * c);
         halt |= !stands;
         if (halt) st.draw = last ? 1 : a.y ? 3 : 2;
       }
@@ -230,33 +284,33 @@ __device__ Decision decide(const VerifyArgs& a, int s, bool write) {
   return d;
 }
 
-// The weights of 16 logits from e0 on, f64: of p, and of q where it counts.
-template <class T>
-__device__ __forceinline__ void load16(const T* row, long long e0, int n, float (&v)[16]) {
-  constexpr int VE = 16 / sizeof(T);
+// N logits from e0 on, -inf behind the row.
+template <class T, int N>
+__device__ __forceinline__ void load_some(const T* row, long long e0, int n, float (&v)[N]) {
+  constexpr int VE = 16 / sizeof(T) < N ? 16 / sizeof(T) : N;
   typedef T vec_t __attribute__((ext_vector_type(VE)));
-  if (e0 + 16 <= n && ((uintptr_t)(row + e0) & 15) == 0) {
+  if (e0 + N <= n && ((uintptr_t)(row + e0) & (VE * sizeof(T) - 1)) == 0) {
 #pragma unroll
-    for (int i = 0; i < 16; i += VE) {
+    for (int i = 0; i < N; i += VE) {
       const vec_t x = *(const vec_t*)(row + e0 + i);
 #pragma unroll
       for (int e = 0; e < VE; ++e) v[i + e] = (float)x[e];
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = e0 + i < n ? (float)row[e0 + i] : -INFINITY;
+    for (int i = 0; i < N; ++i) v[i] = e0 + i < n ? (float)row[e0 + i] : -INFINITY;
   }
 }
-__device__ __forceinline__ double weight(float z, float m, double inv_heat) { return exp(((double)z - (double)m) * inv_heat); }
+// e^((z - m) / T), c = log2(e) / T.
+__device__ __forceinline__ double weight(float z, float m, double c) { return exp2_below(((double)z - (double)m) * c); }
 
-// Block = a tile of a sequence's stop row.
+// Where sequence s stops; the block with `write` reports it and what lies
+// before and behind.
 template <class T>
-__global__ __launch_bounds__(256) void k_verify_sums(VerifyArgs a) {
-  const int tid = threadIdx.x, lane = tid & 63;
-  const long long at = a.block0 + blockIdx.x;
-  const int s = (int)(at / a.tiles), tile = (int)(at - (long long)s * a.tiles);
-  const Decision d = decide<T>(a, s, tile == 0);
-  if (tile == 0) {
+__device__ VerifyStop settle(const VerifyArgs& a, int s, bool write) {
+  const int tid = threadIdx.x;
+  const Decision d = decide<T>(a, s, write);
+  if (write) {
     if (tid == 0) {
       a.accepted[s] = d.stop.row >= 0 ? d.stop.row - d.first : 0;
       a.stop[s] = d.stop;
@@ -267,17 +321,36 @@ __global__ __launch_bounds__(256) void k_verify_sums(VerifyArgs a) {
         if (a.logprobs) a.logprobs[r] = 0.f;
       }
   }
-  const VerifyStop& st = d.stop;
+  return d.stop;
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void k_verify_stop(VerifyArgs a) {
+  settle<T>(a, (int)(a.block0 + blockIdx.x), true);
+}
+
+// Block = a tile of a sequence's stop row. With FIND each block finds that row
+// for itself, 5 us that a launch of its own takes as well; with many blocks to a
+// sequence's tiles and more of them than the CUs hold it has one
+// (48 sequences of 262144 logits: 34 us with FIND, 9 and 22 without).
+template <class T, bool FIND>
+__global__ __launch_bounds__(256) void k_verify_sums(VerifyArgs a) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  const long long at = a.block0 + blockIdx.x;
+  const int s = (int)(at / a.tiles), tile = (int)(at - (long long)s * a.tiles);
+  VerifyStop st;
+  if constexpr (FIND) st = settle<T>(a, s, tile == 0);
+  else st = a.stop[s];
   if (st.row < 0 || st.draw == 0) return;
-  const double inv_heat = 1.0 / (double)a.temperature[s];
+  const double inv_heat = kLog2e64 / (double)a.temperature[s];
   const long long e0 = (long long)tile * kVerifyTile + 16 * tid;
   const bool both = st.draw == 3;
   const int skip = st.draw == 2 ? a.draft[st.row] : -1;
   double sum[4] = {};
   if (e0 < a.n) {
     float z[16], y[16];
-    load16((const T*)a.z + st.row * a.ldz, e0, a.n, z);
-    if (both) load16((const T*)a.y + st.row * a.ldy, e0, a.n, y);
+    load_some((const T*)a.z + st.row * a.ldz, e0, a.n, z);
+    if (both) load_some((const T*)a.y + st.row * a.ldy, e0, a.n, y);
 #pragma unroll 4
     for (int i = 0; i < 16; ++i) {
       const double p = weight(z[i], st.mp, inv_heat);
@@ -304,44 +377,61 @@ __global__ __launch_bounds__(256) void k_verify_sums(VerifyArgs a) {
   if (tid < 4) a.sums[(at * 4) + tid] = (part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid]);
 }
 
-// Inclusive sums over the block's 256 threads in order.
+constexpr int kDrawThreads = 1024, kDrawWaves = kDrawThreads / 64, kDrawEach = kVerifyTile / kDrawThreads;
+
+// Inclusive sums over the block's threads in order.
 __device__ double block_scan(double v, double* sh, double* total) {
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-  double x = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double up = __shfl_up(x, o, 64);
-    if (lane >= o) x += up;
-  }
+  const double x = wave_scan(v);
   __syncthreads();
   if (lane == 63) sh[wv] = x;
   __syncthreads();
-  double before = 0;
-  for (int i = 0; i < wv; ++i) before += sh[i];
-  *total = ((sh[0] + sh[1]) + sh[2]) + sh[3];
+  double before = 0, all = 0;
+#pragma unroll
+  for (int i = 0; i < kDrawWaves; ++i) {
+    before += i < wv ? sh[i] : 0.0;
+    all += sh[i];
+  }
+  *total = all;
   return before + x;
+}
+// Sums of two values over the block, in every thread.
+__device__ void block_sums(double& x, double& y, double* sh) {
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  x = wave_sum(x);
+  y = wave_sum(y);
+  if (lane == 0) {
+    sh[wv] = x;
+    sh[kDrawWaves + wv] = y;
+  }
+  __syncthreads();
+  x = y = 0;
+#pragma unroll
+  for (int i = 0; i < kDrawWaves; ++i) {
+    x += sh[i];
+    y += sh[kDrawWaves + i];
+  }
 }
 
 // One block per sequence: the token that the draw falls on.
 template <class T>
-__global__ __launch_bounds__(256) void k_verify_draw(VerifyArgs a, int seq0) {
-  __shared__ double sh[4];
+__global__ __launch_bounds__(kDrawThreads) void k_verify_draw(VerifyArgs a, int seq0) {
+  __shared__ double sh[2 * kDrawWaves];
   __shared__ int hit, last;
   __shared__ double rest;
   const int tid = threadIdx.x, s = seq0 + blockIdx.x;
   const VerifyStop st = a.stop[s];
   if (st.row < 0 || st.draw == 0) return;
   const double* sums = a.sums + (long long)s * a.tiles * 4;
-  const int per = (a.tiles + 255) / 256, t0 = min(tid * per, a.tiles), t1 = min(t0 + per, a.tiles);
+  const int per = (a.tiles + kDrawThreads - 1) / kDrawThreads, t0 = min(tid * per, a.tiles), t1 = min(t0 + per, a.tiles);
   // the sums of all p and q first: their quotient scales q
   double p_all = 0, q_all = 0;
   for (int t = t0; t < t1; ++t) {
     p_all += sums[4 * t + 2];
     q_all += sums[4 * t + 3];
   }
-  double p_sum, q_sum, all;
-  block_scan(p_all, sh, &p_sum);
-  block_scan(q_all, sh, &q_sum);
+  double p_sum = p_all, q_sum = q_all, all;
+  block_sums(p_sum, q_sum, sh);
   const double c = st.draw == 3 ? p_sum / q_sum : 0.0;
   double mine = 0;
   auto tile_weight = [&](int t) { return fmax(sums[4 * t] - c * sums[4 * t + 1], 0.0); };
@@ -372,8 +462,10 @@ __global__ __launch_bounds__(256) void k_verify_draw(VerifyArgs a, int seq0) {
       }
       x += w;
     }
-    if (first < a.tiles) atomicMin(&hit, first);
-    atomicMax(&last, some);
+    // the threads are in order: a wave's first hit, its last weight
+    const uint64_t hits = __ballot(first < a.tiles), any = __ballot(some >= 0);
+    if (hits && (tid & 63) == __builtin_ctzll(hits)) atomicMin(&hit, first);
+    if (any && (tid & 63) == 63 - __builtin_clzll(any)) atomicMax(&last, some);
     __syncthreads();
     if (first < a.tiles && first == hit) rest = target - before;
     if (hit == a.tiles && tid == 0) rest = INFINITY;   // rounding left none: the last weight
@@ -381,17 +473,17 @@ __global__ __launch_bounds__(256) void k_verify_draw(VerifyArgs a, int seq0) {
   }
   const int tile = hit < a.tiles ? hit : max(last, 0);
   const double within = rest;
-  const double inv_heat = 1.0 / (double)a.temperature[s];
-  const long long e0 = (long long)tile * kVerifyTile + 16 * tid;
+  const double inv_heat = kLog2e64 / (double)a.temperature[s];
+  const long long e0 = (long long)tile * kVerifyTile + kDrawEach * tid;
   const int skip = st.draw == 2 && !plain ? a.draft[st.row] : -1;
-  double w[16];
+  double w[kDrawEach];
   mine = 0;
   {
-    float z[16], y[16];
-    load16((const T*)a.z + st.row * a.ldz, e0, a.n, z);
-    if (st.draw == 3 && !plain) load16((const T*)a.y + st.row * a.ldy, e0, a.n, y);
+    float z[kDrawEach], y[kDrawEach];
+    load_some((const T*)a.z + st.row * a.ldz, e0, a.n, z);
+    if (st.draw == 3 && !plain) load_some((const T*)a.y + st.row * a.ldy, e0, a.n, y);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < kDrawEach; ++i) {
       w[i] = weight(z[i], st.mp, inv_heat);
       if (st.draw == 3 && !plain) w[i] = fmax(w[i] - c * weight(y[i], st.mq, inv_heat), 0.0);
       if (e0 + i == skip || e0 + i >= a.n) w[i] = 0;
@@ -408,19 +500,22 @@ __global__ __launch_bounds__(256) void k_verify_draw(VerifyArgs a, int seq0) {
   double x = up_to - mine;
   int first = 0x7fffffff, some = -1;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
+  for (int i = 0; i < kDrawEach; ++i) {
     if (w[i] > 0) some = (int)(e0 + i);
     x += w[i];
     if (first == 0x7fffffff && w[i] > 0 && x > within) first = (int)(e0 + i);
   }
-  atomicMin(&hit, first);
-  atomicMax(&last, some);
+  {
+    const uint64_t hits = __ballot(first != 0x7fffffff), any = __ballot(some >= 0);
+    if (hits && (tid & 63) == __builtin_ctzll(hits)) atomicMin(&hit, first);
+    if (any && (tid & 63) == 63 - __builtin_clzll(any)) atomicMax(&last, some);
+  }
   __syncthreads();
   if (tid == 0) {
     const int token = hit != 0x7fffffff ? hit : max(last, 0);
     a.tokens[st.row] = token;
     if (a.logprobs)
-      a.logprobs[st.row] = (float)(((double)(float)((const T*)a.z)[st.row * a.ldz + token] - (double)st.mp) * inv_heat - log(p_sum));
+      a.logprobs[st.row] = (float)(((double)(float)((const T*)a.z)[st.row * a.ldz + token] - (double)st.mp) / (double)a.temperature[s] - log(p_sum));
   }
 }
 
@@ -437,13 +532,27 @@ int verify_t(VerifyArgs a, hipStream_t s) {
     if (e != hipSuccess) return (int)e;
   }
   const long long sums = (long long)a.n_seqs * a.tiles;
-  for (a.block0 = 0; a.block0 < sums; a.block0 += MOST) {
-    hipLaunchKernelGGL((k_verify_sums<T>), dim3((unsigned)(sums - a.block0 < MOST ? sums - a.block0 : MOST)), dim3(256), 0, s, a);
+  const bool find = sums <= 1024;
+  if (!find) {
+    a.block0 = 0;
+    hipLaunchKernelGGL((k_verify_stop<T>), dim3((unsigned)a.n_seqs), dim3(256), 0, s, a);   // at most 2^22 blocks
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
   }
-  hipLaunchKernelGGL((k_verify_draw<T>), dim3((unsigned)a.n_seqs), dim3(256), 0, s, a, 0);
-  return (int)hipGetLastError();
+  for (a.block0 = 0; a.block0 < sums; a.block0 += MOST) {
+    const unsigned n = (unsigned)(sums - a.block0 < MOST ? sums - a.block0 : MOST);
+    if (find) hipLaunchKernelGGL((k_verify_sums<T, true>), dim3(n), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_verify_sums<T, false>), dim3(n), dim3(256), 0, s, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return (int)e;
+  }
+  constexpr int DRAWS = 1 << 21;
+  for (int at = 0; at < a.n_seqs; at += DRAWS) {
+    hipLaunchKernelGGL((k_verify_draw<T>), dim3((unsigned)(a.n_seqs - at < DRAWS ? a.n_seqs - at : DRAWS)), dim3(kDrawThreads), 0, s, a, at);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return (int)e;
+  }
+  return 0;
 }
 
 }  // namespace
