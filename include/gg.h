@@ -365,7 +365,8 @@ int gg_score_logits(const void* logits, uint32_t type, int64_t rows, int32_t n, 
  * type GG_TYPE_BF16, GG_TYPE_F16 or GG_TYPE_E4M3; head_dim a multiple of 16 up
  * to 256; k, v and the strides multiples of 16 bytes. E4M3 rows (sign, 4
  * exponent bits, 3 of mantissa, up to 448) stand for their values times one
- * f32 scale at k_scale / v_scale [page][place][head].
+ * f32 scale at k_scale / v_scale [page][place][head]: a power of two from 2^-126
+ * on, as gg_kv_store makes it, or a NaN.
  *
  * gg_kv_seqs names the sequences of a call. Rows row_start[s] up to
  * row_start[s + 1] of its operands are the last ones of the len[s] positions

@@ -356,3 +356,29 @@ def test_pool_past_32_bits(gpu):
         ref = torch.stack([vals[1124 - rows + i - 99:1124 - rows + i + 1].mean(0) for i in range(rows)])
         # equal weights of 1: sums of 100 values and one division, all in f32
         assert ((out.view(rows, n_kv, d) - ref).abs() <= ref * 110 * 2.0 ** -24 + LEAST["f32"]).all()
+
+
+@pytest.mark.parametrize("cache,x", [("bf16", "bf16"), ("e4m3", "f32"), ("f16", "f16")])
+@pytest.mark.parametrize("rows", [[1] * 70, [2] * 40 + [300] + [0] * 5 + [1] * 40 + [70, 17], [0] * 30 + [130] * 3 + [0] * 70 + [5]])
+def test_more_than_64_sequences(gpu, rows, cache, x):
+    """Sequences found by search; long and short ones and such without rows in one call."""
+    lengths = [n + 37 * i % 210 for i, n in enumerate(rows)]
+    say("sequences", len(rows), sum(rows), cache, x)
+    c = Case(rows, lengths, 4, 1, 64, 24, cache, x)
+    c.check(every=7)
+    c.check(window=50, sinks=3, every=13)
+
+
+def test_thousands_of_sequences(gpu):
+    rows = [i % 3 for i in range(4200)]
+    c = Case(rows, [max(n, 1) + i % 5 for i, n in enumerate(rows)], 1, 1, 16, 4, "bf16", "bf16")
+    c.check()
+
+
+@pytest.mark.parametrize("cache,x", KINDS)
+@pytest.mark.parametrize("dim", [48, 112, 208, 240])
+def test_odd_heads(gpu, dim, cache, x):
+    """Heads between the kernels' widths, groups that no tile divides by: few rows, many, and both."""
+    for rows in ([3, 1], [60, 8], [50, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1]):
+        say("heads of", dim, cache, x, rows)
+        Case(rows, [n + 333 for n in rows], 17, 1, dim, 10, cache, x).check(every=5)

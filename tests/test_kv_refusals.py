@@ -62,7 +62,7 @@ def test_load_refuses(change):
 
 
 @pytest.mark.parametrize("change", [dict(q=None), dict(out=None), dict(type=MX), dict(type=E4M3), dict(n_q_heads=0), dict(n_q_heads=3), dict(ldq=511),
-                                    dict(ldo=0), dict(scale=float("nan")), dict(scale=float("inf")), dict(window=-1), dict(sinks=-1),
+                                    dict(ldo=0), dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=3e38), dict(window=-1), dict(sinks=-1),
                                     dict(q=P + 1), dict(out=P + 1), dict(lse=P + 2), dict(pages_type=F16), dict(pages_type=F16, type=F32),
                                     dict(workspace=None, max_len=4096), dict(workspace=P + 8, max_len=4096),
                                     dict(n_rows=1 << 28, n_q_heads=8, ldq=1024, ldo=1024)])

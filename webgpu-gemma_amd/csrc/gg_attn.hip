@@ -589,8 +589,11 @@ __global__ __launch_bounds__(256, (DP <= 128 || (KV == KV_E4M3 && kParts<KV, T> 
 // places, the usual way to keep reads from meeting in a bank, take the copies
 // twice as long here), at places such that neither the reads of K (a row a
 // lane) nor those of V (transposed by the read, four rows to 16 lanes) meet in a
-// bank. 8-bit rows pass through registers and lie in
-// LDS as bf16. One barrier a tile.
+// bank. One barrier a tile. 8-bit rows go to a place of their wave's own, and from
+// there as bf16 into one stage, between two barriers a tile: that fits two blocks
+// a CU. (Two sequences of 2048 rows to 8192 positions, 16 heads of 128 on 4: 406 us; one
+// block a CU with two stages, a barrier a tile, 599; loads to registers, which
+// the compiler waits for too early, 989. bf16 pages take 307.)
 // ---------------------------------------------------------------------------
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 template <int KV>
@@ -620,10 +623,15 @@ __device__ __forceinline__ void dma16(const void* src, uint32_t dst) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(dst)), "v"(src)
                : "memory", "m0");
 }
+__device__ __forceinline__ void dma4(uint64_t src, uint32_t dst) {   // lane l's four bytes
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(__builtin_amdgcn_readfirstlane(dst)), "v"(src)
+               : "memory", "m0");
+}
 __device__ __forceinline__ uint32_t lds_at(const void* p) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)p; }
 
 // What a key without a place is read from.
 __device__ __attribute__((aligned(16))) const uint8_t kv_zeros[kKvMaxDim * 2] = {};
+__device__ const float kv_one = 1.f;
 
 // One packed row over [u0, u1) in plain f32, a value or four of the head a
 // lane: for rows whose sums are not finite, where an infinity or a NaN in V must
@@ -689,19 +697,24 @@ __device__ void slow_row(const KvAttnArgs& g, int s, const KvSeq& sq, const Span
 }
 
 template <int KV, int DP, class T>
-__global__ __launch_bounds__(256, (kParts<KV, T> > 1 || DP > 128 || (DP == 128 && KV == KV_E4M3) ? 1 : 2)) void k_attn_many(KvAttnArgs g, int slot0, int slots) {
-  constexpr int NP = kParts<KV, T>, KT = DP == 256 && NP > 1 ? 32 : 64, UN = DP / 8, RPI = 64 / UN, IPW = KT / RPI / 4;
+__global__ __launch_bounds__(256, (kParts<KV, T> > 1 || DP > 128 ? 1 : 2)) void k_attn_many(KvAttnArgs g, int slot0, int slots) {
+  constexpr int NP = kParts<KV, T>, KT = DP == 256 && (NP > 1 || KV == KV_E4M3) ? 32 : 64, UN = DP / 8, RPI = 64 / UN, IPW = KT / RPI / 4;
   constexpr int KH = KT / 32, DT = DP / 32, CH = DP / 16, ES = KV == KV_E4M3 ? 1 : 2;
   // In LDS a copy's RPI rows are 1024 bytes, and some more to the next one: 16
   // for K, 32 for V. Scores take the keys of a tile in an order in which
   // neighbouring lanes read neighbouring copies: row m of 32 is key
   // RPI (m % NI) + m / NI.
   constexpr int NI = 32 / RPI, RB = DP * 2, KP = 1024 + 16, VP = 1024 + 32;
-  __shared__ __align__(16) uint8_t kbuf[2][KT / RPI * KP], vbuf[2][KT / RPI * VP];
+  constexpr bool RAW = KV == KV_E4M3;
+  constexpr int STAGES = RAW ? 1 : 2, CP = RAW ? IPW / 2 : IPW;   // CP: copies of a wave, for K or V
+  __shared__ __align__(16) uint8_t kbuf[STAGES][KT / RPI * KP], vbuf[STAGES][KT / RPI * VP];
+  // 8-bit rows are copied as they are, each wave's to a place of its own, and
+  // converted from there into the one stage of K and of V.
+  __shared__ __align__(16) uint8_t kraw[RAW ? KT * DP : 16], vraw[RAW ? KT * DP : 16];
+  __shared__ __align__(16) float scales[RAW ? 2 : 1][2][4][RAW ? 64 : 4];
   __shared__ __align__(16) float hole[2][KT];   // -inf where a key has no place
   __shared__ __align__(16) int holes[2][4];     // whether a wave's keys have any
   __shared__ __align__(16) long long row_off[2][KT];   // bytes from the pool's start to a row, -1: none
-  __shared__ __align__(16) long long row_scale[2][KV == KV_E4M3 ? KT : 1];
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c32 = lane & 31, half = lane >> 5, D = g.kv.dim;
   // Blocks with one value of blockIdx % 8 share an XCD and its L2: they take a
@@ -768,7 +781,6 @@ __global__ __launch_bounds__(256, (kParts<KV, T> > 1 || DP > 128 || (DP == 128 &
   // at when its rows are fetched: waiting for one sooner would wait for the
   // copies before it too, and so would any branch or spill between the copies.
   constexpr int RW = KT / 4;
-  const int urow = lane / UN, unit16 = lane % UN;
   const int tiles = (u1 - u0 + KT - 1) / KT;
   int page = 0;
   auto key_of = [&](int u) __attribute__((always_inline)) { return u < sp.a ? u : sp.lo + u - sp.a; };
@@ -777,55 +789,57 @@ __global__ __launch_bounds__(256, (kParts<KV, T> > 1 || DP > 128 || (DP == 128 &
     page = g.kv.table[(long long)s * g.kv.table_ld + (int)g.kv.page_div((uint32_t)key)];
   };
   auto rows = [&](int t) __attribute__((always_inline)) {
-    const int st = t & 1, r = wv * RW + lane % RW, x = u0 + t * KT + r, key = key_of(x);
+    const int r = wv * RW + lane % RW, x = u0 + t * KT + r, key = key_of(x);
     const bool ok = x < u1 && (x >= sp.a || x < sp.sink) && (uint32_t)page < (uint32_t)g.kv.n_pages;
     const KvPlace at{ok ? page : 0, ok ? key - (int)g.kv.page_div((uint32_t)key) * g.kv.page_size : 0};
     const long long off = kv_offset(g.kv, at, kvh) * ES;
     if (lane < RW) {
-      row_off[st][r] = ok ? off : -1;
-      hole[st][r] = ok ? 0.f : -INFINITY;
-      if constexpr (KV == KV_E4M3) row_scale[st][r] = ok ? kv_scale_at(g.kv, at, kvh) : -1;
+      row_off[t & 1][r] = ok ? off : -1;
+      hole[t & 1][r] = ok ? 0.f : -INFINITY;
     }
     const int any = __ballot(!ok) != 0;
-    if (lane == 0) holes[st][wv] = any;
+    if (lane == 0) holes[t & 1][wv] = any;
+    if constexpr (KV == KV_E4M3) {
+      const long long i = kv_scale_at(g.kv, at, kvh);
+      dma4(ok ? (uint64_t)(uintptr_t)(g.kv.k_scale + i) : (uint64_t)(uintptr_t)&kv_one, lds_at(scales[t & 1][0][wv]));
+      dma4(ok ? (uint64_t)(uintptr_t)(g.kv.v_scale + i) : (uint64_t)(uintptr_t)&kv_one, lds_at(scales[t & 1][1][wv]));
+    }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   };
-  uint2 kreg[KV == KV_E4M3 ? IPW : 1], vreg[KV == KV_E4M3 ? IPW : 1];
-  float kscale[KV == KV_E4M3 ? IPW : 1], vscale[KV == KV_E4M3 ? IPW : 1];
-  // Sends for copy i of K or V of tile t: into its LDS stage, or (8 bits) into registers.
+  // Sends for copy i of K or V of tile t: into its LDS stage, or its wave's place for 8-bit rows.
+  constexpr int CU = 1024 / (DP * ES), CL = 64 / CU;   // rows of a copy, lanes to one
   auto fetch1 = [&](auto is_k, int t, int i) __attribute__((always_inline)) {
-    const int st = t & 1, r = (wv * IPW + i) * RPI + urow;
+    const int st = t & 1, r = wv * RW + i * CU + lane / CL, unit = lane % CL;
     const long long off = row_off[st][r];
-    const bool ok = off >= 0 && 8 * unit16 < D;
-    const uint64_t at = (uint64_t)(uintptr_t)(is_k ? g.kv.k : g.kv.v) + (uint64_t)off + (uint32_t)(8 * ES * unit16);
+    const bool ok = off >= 0 && 16 / ES * unit < D;
+    const uint64_t at = (uint64_t)(uintptr_t)(is_k ? g.kv.k : g.kv.v) + (uint64_t)off + (uint32_t)(16 * unit);
     const uint8_t* src = (const uint8_t*)(uintptr_t)(ok ? at : (uint64_t)(uintptr_t)kv_zeros);
-    if constexpr (KV == KV_E4M3) {
-      (is_k ? kreg : vreg)[i] = *(const uint2*)src;
-      const long long sc = row_scale[st][r];
-      const float f = (is_k ? g.kv.k_scale : g.kv.v_scale)[max(sc, 0ll)];
-      (is_k ? kscale : vscale)[i] = sc >= 0 ? f : 1.f;
-    } else {
-      dma16(src, is_k ? lds_at(&kbuf[st][(wv * IPW + i) * KP]) : lds_at(&vbuf[st][(wv * IPW + i) * VP]));
-    }
+    if constexpr (RAW) dma16(src, is_k ? lds_at(&kraw[(wv * CP + i) * 1024]) : lds_at(&vraw[(wv * CP + i) * 1024]));
+    else dma16(src, is_k ? lds_at(&kbuf[st % STAGES][(wv * IPW + i) * KP]) : lds_at(&vbuf[st % STAGES][(wv * IPW + i) * VP]));
   };
   auto fetch = [&](auto is_k, int t) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < IPW; ++i) fetch1(is_k, t, i);
+    for (int i = 0; i < CP; ++i) fetch1(is_k, t, i);
   };
-  auto bf16x8_of = [&](uint2 w, float sc) __attribute__((always_inline)) {
-    u32x4 r;
-    r.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, sc, false));
-    r.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, sc, true));
-    r.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, sc, false));
-    r.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, sc, true));
-    return sc == sc ? r : u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
-  };
+  // This wave's 8-bit rows of tile t, which have arrived, as bf16 into the stage.
   auto settle = [&](auto is_k, int t) __attribute__((always_inline)) {
     if constexpr (KV == KV_E4M3) {
 #pragma unroll
-      for (int i = 0; i < IPW; ++i)
-        *(u32x4*)(is_k ? &kbuf[t & 1][(wv * IPW + i) * KP + 16 * lane] : &vbuf[t & 1][(wv * IPW + i) * VP + 16 * lane]) =
-            bf16x8_of((is_k ? kreg : vreg)[i], (is_k ? kscale : vscale)[i]);
+      for (int i = 0; i < CP; ++i) {
+        const u32x4 w = *(const u32x4*)(is_k ? &kraw[(wv * CP + i) * 1024 + 16 * lane] : &vraw[(wv * CP + i) * 1024 + 16 * lane]);
+        const int rw = i * CU + lane / CL, r = wv * RW + rw;
+        const float sc = scales[t & 1][is_k ? 0 : 1][wv][rw];
+        u32x4 o[2];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          o[e / 2][2 * (e % 2)] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[e], sc, false));
+          o[e / 2][2 * (e % 2) + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[e], sc, true));
+        }
+        uint8_t* dst = is_k ? &kbuf[0][r / RPI * KP + r % RPI * RB + 32 * (lane % CL)] : &vbuf[0][r / RPI * VP + r % RPI * RB + 32 * (lane % CL)];
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          *(u32x4*)(dst + 16 * e) = sc == sc ? o[e] : u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
+      }
     }
   };
   constexpr std::true_type K{}, yes{};
@@ -853,7 +867,7 @@ __global__ __launch_bounds__(256, (kParts<KV, T> > 1 || DP > 128 || (DP == 128 &
     constexpr int N = KH * CH, PAIRS = KH * 8;
     f32x16 nx[KH];
     const float ref = (m == -INFINITY ? 0.f : m) - kShift<KV>;
-    const uint8_t* kst = kbuf[t & 1];
+    const uint8_t* kst = kbuf[t % STAGES];
     u32x4 ka[N];
     auto read = [&](int c) __attribute__((always_inline)) {
       ka[c] = *(const u32x4*)&kst[kbase + c / CH * NI * KP + 32 * (c % CH)];
@@ -889,9 +903,7 @@ __global__ __launch_bounds__(256, (kParts<KV, T> > 1 || DP > 128 || (DP == 128 &
         if constexpr (EX) {
 #pragma unroll
           for (int e = c * PAIRS / N; e < (c + 1) * PAIRS / N; ++e) pair(e);
-          if constexpr (KV != KV_E4M3) {
-            if (c % (N / IPW) == 0) fetch1(V, t, c / (N / IPW));
-          }
+          if (c % (N / CP) == 0) fetch1(V, t, c / (N / CP));
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -921,7 +933,7 @@ __global__ __launch_bounds__(256, (kParts<KV, T> > 1 || DP > 128 || (DP == 128 &
   // copies of K two tiles on.
   float mx = -INFINITY;
   auto products = [&](auto PV, auto MX, int t) __attribute__((always_inline)) {
-    const uint8_t* vst = vbuf[t & 1];
+    const uint8_t* vst = vbuf[t % STAGES];
     if constexpr (MX) mx = -INFINITY;
     if constexpr (PV) {
       constexpr int N = 2 * KH * DT;
@@ -946,9 +958,7 @@ __global__ __launch_bounds__(256, (kParts<KV, T> > 1 || DP > 128 || (DP == 128 &
 #pragma unroll
           for (int e = c * KH * 8 / N; e < (c + 1) * KH * 8 / N; ++e)
             mx = fmaxf(fmaxf(mx, sc[e / 8][2 * (e % 8)]), sc[e / 8][2 * (e % 8) + 1]);
-          if constexpr (KV != KV_E4M3) {
-            if (c % (N / IPW) == 0) fetch1(K, t + 2, c / (N / IPW));
-          }
+          if (c % (N / CP) == 0) fetch1(K, t + 2, c / (N / CP));
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -977,18 +987,22 @@ __global__ __launch_bounds__(256, (kParts<KV, T> > 1 || DP > 128 || (DP == 128 &
   // Tiles that a wave's rows do not see are taken all the same, masked: the
   // others would be waited for. K of tiles behind the last is read as zeros.
   if (tiles > 0) {
+    const auto wait = []() __attribute__((always_inline)) { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); };
     ask(0);
     rows(0);
     ask(1);
     fetch(K, 0);
     fetch(V, 0);
-    settle(K, 0);
-    settle(V, 0);
     rows(1);
     ask(2);
-    fetch(K, 1);
-    settle(K, 1);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if constexpr (RAW) {
+      wait();
+      settle(K, 0);
+      fetch(K, 1);
+    } else {
+      fetch(K, 1);
+      wait();
+    }
     __syncthreads();
     hs = *(const int4*)holes[0];
     scores(yes, no, 0);
@@ -996,21 +1010,24 @@ __global__ __launch_bounds__(256, (kParts<KV, T> > 1 || DP > 128 || (DP == 128 &
     products(no, yes, 0);
     rescale();
     for (int t = 0; t + 1 < tiles; ++t) {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wave's copies of K t + 1 and V t
-      __syncthreads();                                   // and everybody's
+      wait();            // this wave's copies of K t + 1 and V t
+      __syncthreads();   // and everybody's; nobody reads the tiles before them any more
       hs = *(const int4*)holes[(t + 1) & 1];
-      if constexpr (KV == KV_E4M3) fetch(V, t + 1);
+      settle(K, t + 1);
+      settle(V, t);
       rows(t + 2);
       ask(t + 3);
-      if constexpr (KV == KV_E4M3) fetch(K, t + 2);
+      if constexpr (RAW) __syncthreads();
       scores(yes, yes, t + 1);
       mask(t + 1);
       products(yes, yes, t);
       rescale();
-      settle(V, t + 1);
-      settle(K, t + 2);
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    wait();
+    if constexpr (RAW) {
+      __syncthreads();
+      settle(V, tiles - 1);
+    }
     __syncthreads();
     scores(no, yes, tiles - 1);
     products(yes, no, tiles - 1);
@@ -1180,7 +1197,7 @@ long long slots_of(const KvAttnArgs& g, int tile) {
 }
 
 template <int KV, int DP, class T>
-int attn_launch(const KvAttnArgs& g, int max_rows, hipStream_t s) {
+int attn_launch(const KvAttnArgs& g, hipStream_t s) {
   // launches of fewer than 2^24 blocks: a grid holds fewer than 2^32 threads
   const long long each = (long long)g.kv.n_kv * g.splits;
   const long long most = std::max(1ll, ((1ll << 24) - 1) / each);
@@ -1207,17 +1224,17 @@ int attn_launch(const KvAttnArgs& g, int max_rows, hipStream_t s) {
   return g.kv.dim <= 64 ? join_waves<KV, T, 16>(g, s) : g.kv.dim <= 128 ? join_waves<KV, T, 32>(g, s) : join_waves<KV, T, 64>(g, s);
 }
 template <int KV, class T>
-int attn_dim(const KvAttnArgs& g, int max_rows, hipStream_t s) {
-  if (g.kv.dim <= 64) return attn_launch<KV, 64, T>(g, max_rows, s);
-  if (g.kv.dim <= 128) return attn_launch<KV, 128, T>(g, max_rows, s);
-  return attn_launch<KV, 256, T>(g, max_rows, s);
+int attn_dim(const KvAttnArgs& g, hipStream_t s) {
+  if (g.kv.dim <= 64) return attn_launch<KV, 64, T>(g, s);
+  if (g.kv.dim <= 128) return attn_launch<KV, 128, T>(g, s);
+  return attn_launch<KV, 256, T>(g, s);
 }
 template <int KV>
-int attn_type(int elem, const KvAttnArgs& g, int max_rows, hipStream_t s) {
+int attn_type(int elem, const KvAttnArgs& g, hipStream_t s) {
   switch (elem) {
-    case ELEM_F32: return attn_dim<KV, float>(g, max_rows, s);
-    case ELEM_F16: return attn_dim<KV, _Float16>(g, max_rows, s);
-    case ELEM_BF16: return attn_dim<KV, __bf16>(g, max_rows, s);
+    case ELEM_F32: return attn_dim<KV, float>(g, s);
+    case ELEM_F16: return attn_dim<KV, _Float16>(g, s);
+    case ELEM_BF16: return attn_dim<KV, __bf16>(g, s);
   }
   return (int)hipErrorInvalidValue;
 }
@@ -1235,7 +1252,7 @@ int attn_type(int elem, const KvAttnArgs& g, int max_rows, hipStream_t s) {
 // k_attn_many: whole rounds of the CUs; a block's start and end cost about 200
 // keys, a chunk's sums are written and read once more.
 KvAttnPlan kv_attn_plan(int n_seqs, int n_rows, int max_rows, int max_len, int n_kv, int group, int dim, int window, int sinks,
-                        int key_bytes, bool two) {
+                        int key_bytes) {
   KvAttnPlan p{};
   constexpr int FEW = kKvFewTiles * kKvFewTile;
   const bool few = (long long)max_rows * group <= FEW;
@@ -1247,7 +1264,7 @@ KvAttnPlan kv_attn_plan(int n_seqs, int n_rows, int max_rows, int max_len, int n
   if (window > 0) most = std::min(most, (long long)window + tile) + ((long long)std::min(sinks, max_len) + 63) / 64 * 64;
   const long long packed = (long long)n_rows * group, of_seq = (packed + n_seqs - 1) / n_seqs;
   const double tiles = (double)n_seqs * (double)((of_seq + tile - 1) / tile) * n_kv;
-  const double share = window > 0 ? 1.0 : 0.5 + 0.5 / n_seqs, cus = two ? 512 : 256;
+  const double share = window > 0 ? 1.0 : 0.5 + 0.5 / n_seqs;
   double best = 1e300;
   long long chunk = most;
   for (long long c = 1; c <= 256 && (c - 1) * kKvChunk < most; ++c) {
@@ -1273,11 +1290,11 @@ KvAttnPlan kv_attn_plan(int n_seqs, int n_rows, int max_rows, int max_len, int n
   return p;
 }
 
-int launch_kv_attention(int kv_type, int elem, const KvAttnArgs& g, int max_rows, void* stream) {
+int launch_kv_attention(int kv_type, int elem, const KvAttnArgs& g, void* stream) {
   switch (kv_type) {
-    case KV_BF16: return attn_type<KV_BF16>(elem, g, max_rows, (hipStream_t)stream);
-    case KV_F16: return attn_dim<KV_F16, _Float16>(g, max_rows, (hipStream_t)stream);
-    case KV_E4M3: return attn_type<KV_E4M3>(elem, g, max_rows, (hipStream_t)stream);
+    case KV_BF16: return attn_type<KV_BF16>(elem, g, (hipStream_t)stream);
+    case KV_F16: return attn_dim<KV_F16, _Float16>(g, (hipStream_t)stream);
+    case KV_E4M3: return attn_type<KV_E4M3>(elem, g, (hipStream_t)stream);
   }
   return (int)hipErrorInvalidValue;
 }

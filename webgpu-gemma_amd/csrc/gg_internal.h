@@ -685,10 +685,10 @@ constexpr int kKvManyTile = 128;    // and of k_attn_many
 struct KvAttnPlan {
   int few_rows, chunk, splits;
 };
-// key_bytes: of a key and its value; two: whether two blocks of k_attn_few share a CU.
+// key_bytes: of a key and its value.
 KvAttnPlan kv_attn_plan(int n_seqs, int n_rows, int max_rows, int max_len, int n_kv, int group, int dim, int window, int sinks,
-                        int key_bytes, bool two);
-int launch_kv_attention(int kv_type, int elem, const KvAttnArgs& a, int max_rows, void* stream);
+                        int key_bytes);
+int launch_kv_attention(int kv_type, int elem, const KvAttnArgs& a, void* stream);
 
 // ---- verification of drafted tokens (gg_verify.hip) ----------------------------
 // What one block found in its part of a row of logits.

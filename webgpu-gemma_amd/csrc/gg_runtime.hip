@@ -2011,7 +2011,7 @@ bool attn_shape_ok(const gg_kv_pages* p, const gg_kv_seqs* s, int32_t n_q_heads,
 }
 KvAttnPlan attn_plan(const gg_kv_pages* p, const gg_kv_seqs* s, int32_t n_q_heads, int32_t window, int32_t sinks) {
   return kv_attn_plan(s->n_seqs, s->n_rows, s->max_rows, s->max_len, p->n_kv_heads, n_q_heads / p->n_kv_heads, p->head_dim, window,
-                      sinks, 2 * p->head_dim * (p->type == GG_TYPE_E4M3 ? 1 : 2), p->head_dim <= 128 || p->type == GG_TYPE_E4M3);
+                      sinks, 2 * p->head_dim * (p->type == GG_TYPE_E4M3 ? 1 : 2));
 }
 
 }  // namespace
@@ -2080,7 +2080,7 @@ int gg_kv_attention(const gg_kv_pages* pages, const gg_kv_seqs* seqs, const void
   KvAttnArgs a{};
   const int e = elem_of(type);
   if (!kv_args(pages, seqs, &a.kv) || !attn_shape_ok(pages, seqs, n_q_heads, window, sinks) || e < 0 || !q || !out ||
-      (pages->type == GG_TYPE_F16 && type != GG_TYPE_F16) || !std::isfinite(scale))
+      (pages->type == GG_TYPE_F16 && type != GG_TYPE_F16) || !std::isfinite(scale * 1.4426950408889634f))
     return GG_ERR_INVALID;
   const int64_t width = (int64_t)n_q_heads * a.kv.dim;
   if (ldq < width || ldo < width || !aligned_to(q, elem_size(e)) || !aligned_to(out, elem_size(e)) || !aligned_to(lse, 4) ||
@@ -2105,7 +2105,7 @@ int gg_kv_attention(const gg_kv_pages* pages, const gg_kv_seqs* seqs, const void
   a.splits = p.splits;
   a.part_o = (float*)workspace;
   a.part_ml = a.part_o + (size_t)p.splits * seqs->n_rows * n_q_heads * a.kv.dim;
-  return launch_kv_attention(kv_type_of(pages->type), e, a, seqs->max_rows, stream) ? GG_ERR_HIP : GG_OK;
+  return launch_kv_attention(kv_type_of(pages->type), e, a, stream) ? GG_ERR_HIP : GG_OK;
 }
 
 size_t gg_verify_drafts_workspace_size(int64_t rows, int32_t n_seqs, int32_t n) {
