@@ -109,7 +109,11 @@ __device__ __forceinline__ Span kv_span(const KvAttnArgs& g, const KvSeq& sq, in
   s.n = s.a + max(0, hi - s.lo);
   return s;
 }
-__device__ __forceinline__ int kv_splits(const KvAttnArgs& g, const Span& s) { return max(1, (s.n + g.chunk - 1) / g.chunk); }
+__device__ __forceinline__ int kv_splits(const KvAttnArgs& g, const Span& s) { return max(1, (int)g.by_chunk((uint32_t)(s.n + g.chunk - 1))); }
+
+// The row of a sequence, and the head of its group, that a packed row is.
+__device__ __forceinline__ int row_in(const KvAttnArgs& g, int p) { return (int)g.by_group((uint32_t)p); }
+__device__ __forceinline__ int head_in(const KvAttnArgs& g, int p) { return p - row_in(g, p) * g.group; }
 
 // The first slot of a sequence's tiles. A sequence of n packed rows behind r others
 // has floor((r + n + (tile - 1) (s + 1)) / tile) - floor((r + (tile - 1) s) / tile) of
@@ -141,7 +145,11 @@ __device__ __forceinline__ bool odd_value(uint32_t h) {
 // waves 32 keys at a time in turn. K and V go from memory to registers, K in
 // operand order as it lies, V in rows (16 lanes share one) and transposed by
 // byte permutes: no LDS, no barrier in the loop; the next step's K is asked for
-// when this one's is used up, V likewise.
+// when this one's is used up, V likewise. Memory bounds it: 61 tokens of 32 heads of 128
+// on 8 at up to 8192 positions 221 us and 7 more for the join, 5.4 TB/s; 3 tokens
+// at up to 131072, 8-bit heads of 256, 138 and 5 us, 5.3 TB/s. Of one token's 8 us
+// 1.3 go until the table is read, 2.8 until K and V are here, 2 for the two
+// products and the weights, 1 to add the waves' sums.
 // ---------------------------------------------------------------------------
 template <int KV, int DP, class T>
 __global__ __launch_bounds__(256, (DP <= 128 || (KV == KV_E4M3 && kParts<KV, T> == 1) ? 2 : 1)) void k_attn_few(KvAttnArgs g, int slot0, int slots) {
@@ -152,6 +160,7 @@ __global__ __launch_bounds__(256, (DP <= 128 || (KV == KV_E4M3 && kParts<KV, T> 
   __shared__ float m_all[4][kKvFewTile], l_all[4][kKvFewTile], e_all[4][kKvFewTile];
   __shared__ __align__(16) long long key_off[4][32];        // where a step's rows lie, -1: nowhere
   __shared__ __align__(16) float k_sc[4][32], v_sc[4][32];
+  __shared__ u32x4 q_all[NP][KC][64];
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c16 = lane & 15, quad = lane >> 4, D = g.kv.dim;
   // Heads fastest. With many tiles the chunks of one lie next to each other, and
@@ -184,48 +193,15 @@ __global__ __launch_bounds__(256, (DP <= 128 || (KV == KV_E4M3 && kParts<KV, T> 
   const int packed = sq.rows * g.group;
   if (tile_l < 0 || tile_l * kKvFewTile >= packed || packed > g.few_rows) return;
   const int p0 = (int)tile_l * kKvFewTile;
-  const Span sp = kv_span<32>(g, sq, p0 / g.group, min((p0 + kKvFewTile - 1) / g.group, sq.rows - 1));
+  const Span sp = kv_span<32>(g, sq, row_in(g, p0), min(row_in(g, p0 + kKvFewTile - 1), sq.rows - 1));
   const int u0 = split * g.chunk, u1 = min(sp.n, u0 + g.chunk);
   if (split > 0 && u0 >= sp.n) return;
-  const bool joined = kv_splits(g, sp) > 1;
+  const bool joined = sp.n > g.chunk;
 
-  // this lane's packed row: its query as operand columns, its position
-  const int p = p0 + c16, row = sq.first + p / g.group, head = kvh * g.group + p % g.group;
-  const int pos = p < packed ? sq.len - sq.rows + p / g.group : -1;
-  const int pos_min = sq.len - sq.rows + p0 / g.group, pos_max = sq.len - sq.rows + min((p0 + kKvFewTile - 1) / g.group, sq.rows - 1);
-  u32x4 qb[NP][KC];
-  {
-    const T* q = (const T*)g.q + (p < packed ? row * g.ldq + (long long)head * D : 0);
-#pragma unroll
-    for (int c = 0; c < KC; ++c) {
-      // a lane's values of a chunk; with 8 bits those of two chunks lie together in K
-      const int d = KV == KV_E4M3 ? 64 * (c / 2) + 16 * quad + 8 * (c % 2) : 32 * c + 8 * quad;
-      float f[8] = {};
-      if (p < packed && d < D) {
-        if (g.q_vec) {
-          constexpr int V = 16 / sizeof(T);
-          typedef T vec_t __attribute__((ext_vector_type(V)));
-#pragma unroll
-          for (int i = 0; i < 8; i += V) {
-            const vec_t t = *(const vec_t*)(q + d + i);
-#pragma unroll
-            for (int k = 0; k < V; ++k) f[i + k] = (float)t[k];
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] = (float)q[d + i];
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t w[NP];
-        split2<KV, NP>(f[2 * i], f[2 * i + 1], w);
-#pragma unroll
-        for (int k = 0; k < NP; ++k) qb[k][c][i] = w[k];
-      }
-    }
-  }
-
+  // this lane's packed row
+  const int p = p0 + c16;
+  const int pos = p < packed ? sq.len - sq.rows + row_in(g, p) : -1;
+  const int pos_min = sq.len - sq.rows + row_in(g, p0), pos_max = sq.len - sq.rows + min(row_in(g, p0 + kKvFewTile - 1), sq.rows - 1);
   f32x4 o[VD];
 #pragma unroll
   for (int t = 0; t < VD; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -280,19 +256,82 @@ __global__ __launch_bounds__(256, (DP <= 128 || (KV == KV_E4M3 && kParts<KV, T> 
     }
   };
 
+  // The first step's keys are asked for before the queries are made operands, of
+  // which each wave makes a share for all (one token at 2049 positions, heads of
+  // 256, both launches: 13.4 us where each wave made all of them first, 11.9 so).
+  const int first = u0 + 32 * wv;
+  ask(first);
+  constexpr int QN = KC < 4 ? 1 : KC / 4;   // chunks of a wave
+  typedef T q8_t __attribute__((ext_vector_type(8)));
+  q8_t q8[QN];
+  int q_at[QN];
+  const bool q_wave = wv * QN < KC;
+#pragma unroll
+  for (int i = 0; i < QN; ++i) {
+    const int c = q_wave ? wv * QN + i : 0;
+    // a lane's values of a chunk; with 8 bits those of two chunks lie together in K
+    q_at[i] = KV == KV_E4M3 ? 64 * (c / 2) + 16 * quad + 8 * (c % 2) : 32 * c + 8 * quad;
+    const int pr = min(p, packed - 1);
+    const T* q = (const T*)g.q + (sq.first + row_in(g, pr)) * g.ldq + (long long)(kvh * g.group + head_in(g, pr)) * D + (q_at[i] < D ? q_at[i] : 0);
+    if (g.q_vec) {
+      constexpr int V = 16 / sizeof(T);
+      typedef T vec_t __attribute__((ext_vector_type(V)));
+      if constexpr (V == 8) {
+        q8[i] = *(const vec_t*)q;
+      } else {
+        const vec_t lo = *(const vec_t*)q, hi = *(const vec_t*)(q + 4);
+        q8[i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) q8[i][k] = q[k];
+    }
+  }
+  // (by waves without keys too, which read row 0: loads in a branch would all be
+  // waited for behind it)
+  places(first);
+  ask(first + 128);
+  load_k();
+  load_v();
+  if (q_wave) {
+#pragma unroll
+    for (int i = 0; i < QN; ++i) {
+      const bool on = p < packed && q_at[i] < D;
+      u32x4 part[NP];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        uint32_t w[NP];
+        split2<KV, NP>(on ? (float)q8[i][2 * k] : 0.f, on ? (float)q8[i][2 * k + 1] : 0.f, w);
+#pragma unroll
+        for (int n = 0; n < NP; ++n) part[n][k] = w[n];
+      }
+#pragma unroll
+      for (int n = 0; n < NP; ++n) q_all[n][wv * QN + i][lane] = part[n];
+    }
+  }
+  // for LDS only: a full barrier, or an acquire fence, would wait for the loads
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  u32x4 qb[NP][KC];
+#pragma unroll
+  for (int n = 0; n < NP; ++n)
+#pragma unroll
+    for (int c = 0; c < KC; ++c) qb[n][c] = q_all[n][c][lane];
+
   // All of this wave's keys. `careful`: infinities and NaN of V reach the rows
   // that see their keys and no others.
   auto pass = [&](auto careful) __attribute__((always_inline)) {
-  int u = u0 + 32 * wv;
   float ks[8], vs[8];
-  if (u < u1) {
-    ask(u);
-    places(u);
-    ask(u + 128);
+  if (careful && first < u1) {
+    ask(first);
+    places(first);
+    ask(first + 128);
     load_k();
-    if constexpr (!careful) load_v();
   }
-  for (; u < u1; u += 128) {
+  // (left from the middle: a path around the last loads back to the start would
+  // make K wait for V there)
+  if (first < u1) for (int u = first;; u += 128) {
     if constexpr (KV == KV_E4M3) {
       if (lane < 32) {
         k_sc[wv][lane] = sk;
@@ -314,13 +353,16 @@ __global__ __launch_bounds__(256, (DP <= 128 || (KV == KV_E4M3 && kParts<KV, T> 
       for (int j = 0; j < 8; ++j) voff[j] = key_off[wv][4 * quad + (j & 3) + 16 * (j >> 2)];
     }
     // S^T: 32 keys x 16 packed rows
-    f32x4 sc[2];
+    // with several parts in two sums each, chains of half the length
+    constexpr int CHAINS = NP > 1 ? 2 : 1;
+    f32x4 sc[2], acc[CHAINS][2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      sc[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < CHAINS; ++i) acc[i][0] = acc[i][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int c = 0; c < KC; ++c) {
-        u32x4 ka;
+    for (int c = 0; c < KC; ++c) {
+      u32x4 ka[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
         if constexpr (KV == KV_E4M3) {
           typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
           const uint32_t k0 = kr[h][c / 2][2 * (c % 2)], k1 = kr[h][c / 2][2 * (c % 2) + 1];
@@ -328,14 +370,21 @@ __global__ __launch_bounds__(256, (DP <= 128 || (KV == KV_E4M3 && kParts<KV, T> 
                        a1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(k0, 1.f, true),
                        a2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(k1, 1.f, false),
                        a3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(k1, 1.f, true);
-          ka = u32x4{__builtin_bit_cast(uint32_t, a0), __builtin_bit_cast(uint32_t, a1), __builtin_bit_cast(uint32_t, a2),
-                     __builtin_bit_cast(uint32_t, a3)};
+          ka[h] = u32x4{__builtin_bit_cast(uint32_t, a0), __builtin_bit_cast(uint32_t, a1), __builtin_bit_cast(uint32_t, a2),
+                        __builtin_bit_cast(uint32_t, a3)};
         } else {
-          ka = kr[h][c];
+          ka[h] = kr[h][c];
         }
-#pragma unroll
-        for (int k = NP - 1; k >= 0; --k) sc[h] = mfma16<KV>(ka, qb[k][c], sc[h]);
       }
+#pragma unroll
+      for (int k = NP - 1; k >= 0; --k)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) acc[c % CHAINS][h] = mfma16<KV>(ka[h], qb[k][c], acc[c % CHAINS][h]);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      sc[h] = acc[0][h];
+      if constexpr (CHAINS > 1) sc[h] += acc[CHAINS - 1][h];
     }
     const int next = u + 128;
     if (next < u1) {
@@ -478,29 +527,35 @@ __global__ __launch_bounds__(256, (DP <= 128 || (KV == KV_E4M3 && kParts<KV, T> 
             va[3][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true));
           }
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
+          for (int k = NP - 1; k >= 0; --k)
 #pragma unroll
-            for (int k = NP - 1; k >= 0; --k) o[t + e] = mfma16<KV>(va[e], pb[k], o[t + e]);
+            for (int e = 0; e < 4; ++e) o[t + e] = mfma16<KV>(va[e], pb[k], o[t + e]);
         }
       } else {
+        constexpr int TS = NP > 1 ? 4 : 2;   // values at a time: sums that wait for each other lie TS instructions apart
 #pragma unroll
-        for (int t = 0; t < VD; t += 2) {
-          u32x4 lo, hi;
+        for (int t = 0; t < VD; t += TS) {
+          u32x4 va[TS];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t w0 = vr[2 * i][t / 8][t / 2 % 4], w1 = vr[2 * i + 1][t / 8][t / 2 % 4];
-            lo[i] = lower2(w0, w1);
-            hi[i] = upper2(w0, w1);
-          }
+          for (int e = 0; e < TS; e += 2)
 #pragma unroll
-          for (int k = NP - 1; k >= 0; --k) {
-            o[t] = mfma16<KV>(lo, pb[k], o[t]);
-            o[t + 1] = mfma16<KV>(hi, pb[k], o[t + 1]);
-          }
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t w0 = vr[2 * i][(t + e) / 8][(t + e) / 2 % 4], w1 = vr[2 * i + 1][(t + e) / 8][(t + e) / 2 % 4];
+              va[e][i] = lower2(w0, w1);
+              va[e + 1][i] = upper2(w0, w1);
+            }
+#pragma unroll
+          for (int k = NP - 1; k >= 0; --k)
+#pragma unroll
+            for (int e = 0; e < TS; ++e) o[t + e] = mfma16<KV>(va[e], pb[k], o[t + e]);
         }
       }
     }
-    if (!careful && next < u1) load_v();
+    if (next >= u1) {
+      asm volatile("");   // an exit of its own
+      break;
+    }
+    if (!careful) load_v();
   }
   };
   // A weight of 0, or a part of one, times an infinity or a NaN leaves a NaN, so
@@ -508,12 +563,12 @@ __global__ __launch_bounds__(256, (DP <= 128 || (KV == KV_E4M3 && kParts<KV, T> 
   pass(std::false_type{});
   bool again;
   {
-    float z = 0.f;
+    f32x4 z = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int t = 0; t < VD; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) z = fmaf(o[t][i], 0.f, z);
-    again = __ballot(z != 0.f) != 0;   // 0 times an infinity or a NaN
+      for (int i = 0; i < 4; ++i) z[i] = fmaf(o[t][i], 0.f, z[i]);
+    again = __ballot((z[0] + z[1]) + (z[2] + z[3]) != 0.f) != 0;   // 0 times an infinity or a NaN
   }
   if (again) {
     for (int e = lane; e < kKvFewTile * OP; e += 64) (&o_all[wv][0][0])[e] = 0.f;
@@ -565,8 +620,8 @@ __global__ __launch_bounds__(256, (DP <= 128 || (KV == KV_E4M3 && kParts<KV, T> 
     f32x4 v = *(const f32x4*)&o_all[0][r][d];
 #pragma unroll
     for (int w = 1; w < 4; ++w) v += *(const f32x4*)&o_all[w][r][d];
-    const long long orow = sq.first + pr / g.group;
-    const int oh = kvh * g.group + pr % g.group;
+    const long long orow = sq.first + row_in(g, pr);
+    const int oh = kvh * g.group + head_in(g, pr);
     if (joined) {
       const long long at = ((long long)split * g.kv.n_rows + orow) * g.n_q + oh;
       *(f32x4*)(g.part_o + at * D + d) = v;
@@ -640,8 +695,8 @@ template <int KV, int DP, class T>
 __device__ void slow_row(const KvAttnArgs& g, int s, const KvSeq& sq, const Span& sp, int u0, int u1, int kvh, int p, float scale2,
                          float (&o)[DP / 64], float* m_out, float* l_out) {
   constexpr int N = DP / 64;
-  const int lane = threadIdx.x & 63, D = g.kv.dim, row = sq.first + p / g.group, head = kvh * g.group + p % g.group;
-  const int pos = sq.len - sq.rows + p / g.group;
+  const int lane = threadIdx.x & 63, D = g.kv.dim, row = sq.first + row_in(g, p), head = kvh * g.group + head_in(g, p);
+  const int pos = sq.len - sq.rows + row_in(g, p);
   float q[N], m = -INFINITY, l = 0.f;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -730,15 +785,15 @@ __global__ __launch_bounds__(256, (kParts<KV, T> > 1 || DP > 128 ? 1 : 2)) void 
   const int packed = sq.rows * g.group;
   if (tile_l < 0 || tile_l * kKvManyTile >= packed || packed <= g.few_rows) return;
   const int p0 = (int)tile_l * kKvManyTile;
-  const Span sp = kv_span<64>(g, sq, p0 / g.group, min((p0 + kKvManyTile - 1) / g.group, sq.rows - 1));
+  const Span sp = kv_span<64>(g, sq, row_in(g, p0), min(row_in(g, p0 + kKvManyTile - 1), sq.rows - 1));
   const int u0 = split * g.chunk, u1 = min(sp.n, u0 + g.chunk);
   if (split > 0 && u0 >= sp.n) return;
-  const bool joined = kv_splits(g, sp) > 1;
+  const bool joined = sp.n > g.chunk;
   const int before = sq.len - sq.rows;
-  const int pw = p0 + 32 * wv, p = pw + c32, row = sq.first + p / g.group, head = kvh * g.group + p % g.group;
-  const int pos = p < packed ? before + p / g.group : -1;
+  const int pw = p0 + 32 * wv, p = pw + c32, row = sq.first + row_in(g, p), head = kvh * g.group + head_in(g, p);
+  const int pos = p < packed ? before + row_in(g, p) : -1;
   const bool active = pw < packed;   // this wave has rows
-  const int pos_min = before + pw / g.group, pos_max = before + min((pw + 31) / g.group, sq.rows - 1);
+  const int pos_min = before + row_in(g, pw), pos_max = before + min(row_in(g, pw + 31), sq.rows - 1);
 
   // queries as operand columns; a negative scale turns their signs, so that the
   // largest product is the largest score, and scale 0 takes them out
@@ -1073,7 +1128,7 @@ __global__ __launch_bounds__(256, (kParts<KV, T> > 1 || DP > 128 ? 1 : 2)) void 
   }
   // rows that need care, one at a time
   for (uint32_t left = (uint32_t)again; left; left &= left - 1) {
-    const int pr = pw + __builtin_ctz(left), orow = sq.first + pr / g.group, oh = kvh * g.group + pr % g.group;
+    const int pr = pw + __builtin_ctz(left), orow = sq.first + row_in(g, pr), oh = kvh * g.group + head_in(g, pr);
     float os[DP / 64], ms, ls;
     slow_row<KV, DP, T>(g, s, sq, sp, u0, u1, kvh, pr, g.scale2, os, &ms, &ls);
     const long long to = ((long long)split * g.kv.n_rows + orow) * g.n_q + oh;
@@ -1104,15 +1159,15 @@ __global__ __launch_bounds__(256) void k_attn_join(KvAttnArgs g, long long unit0
   const long long unit = unit0 + (long long)blockIdx.x * PER + wv / W;
   const int me = wv % W * (64 / L) + lane / L, d = 4 * (lane % L);   // this lane's chunks me, me + N, ..
   const bool there = unit < (long long)g.kv.n_rows * g.n_q;
-  const int row = (int)(there ? unit / g.n_q : 0), head = (int)(there ? unit % g.n_q : 0), D = g.kv.dim;
+  const int row = (int)g.by_heads((uint32_t)(there ? unit : 0)), head = there ? (int)unit - row * g.n_q : 0, D = g.kv.dim;
   KvSeq sq;
   const int s = kv_seq_of(g.kv, row, &sq);
   int n = 0;
   if (there && s >= 0) {
     const bool few = sq.rows * g.group <= g.few_rows;
     const int tile = few ? kKvFewTile : kKvManyTile;
-    const int p0 = ((row - sq.first) * g.group + head % g.group) / tile * tile;
-    const int t0 = p0 / g.group, t1 = min((p0 + tile - 1) / g.group, sq.rows - 1);
+    const int p0 = ((row - sq.first) * g.group + head_in(g, head)) & -tile;
+    const int t0 = row_in(g, p0), t1 = min(row_in(g, p0 + tile - 1), sq.rows - 1);
     n = kv_splits(g, few ? kv_span<32>(g, sq, t0, t1) : kv_span<64>(g, sq, t0, t1));
   }
   if (n < 2) return;   // W > 1: the same in all of the block

@@ -671,6 +671,7 @@ struct KvAttnArgs {
   float* lse;
   float scale2;          // softmax scale times log2(e)
   int n_q, group;        // query heads, and those of a K/V head
+  FastDiv by_group, by_heads, by_chunk;   // divisions by group, n_q, chunk
   int window, sinks;     // window 0: none
   bool q_vec, out_vec;   // q rows aligned to 16 bytes, those of out to four values
   int few_rows;          // sequences of at most this many rows (times group) go to k_attn_few

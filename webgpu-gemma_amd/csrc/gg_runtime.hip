@@ -2096,6 +2096,9 @@ int gg_kv_attention(const gg_kv_pages* pages, const gg_kv_seqs* seqs, const void
   a.scale2 = scale * 1.4426950408889634f;
   a.n_q = n_q_heads;
   a.group = n_q_heads / a.kv.n_kv;
+  a.by_group = fast_div((uint32_t)a.group);
+  a.by_heads = fast_div((uint32_t)n_q_heads);
+  a.by_chunk = fast_div((uint32_t)p.chunk);
   a.window = window;
   a.sinks = sinks;
   a.q_vec = aligned_to(q, 16) && ldq * (int64_t)elem_size(e) % 16 == 0;
