@@ -4,10 +4,12 @@
 //   y = x w / sqrt(mean x^2 + eps);  a = p theta^(-2j/D):
 //   (y_j, y_{j+D/2}) -> (y_j cos a - y_{j+D/2} sin a, y_{j+D/2} cos a + y_j sin a)
 //
-// All of it is f64, which has the rate of f32 here, and hidden behind the
-// memory: a stored value is the formula's, rounded once. In f32 a value next to
-// a border of the 8-bit format lands on its other side now and then, a whole
-// step of 2^-4 away, and the angle of position 10^6 is off by 2^-5.
+// All of it is f64: a stored value is the formula's, rounded once. In f32 a value
+// next to a border of the 8-bit format lands on its other side now and then, a
+// whole step of 2^-4 away, and the angle of position 10^6 is off by 2^-5.
+// 4380 rows of 48 heads of 128, bf16 to bf16 queries and 8-bit pages: 38 us, 98 MB at 2.6
+// TB/s, a block being a row's chain of sequence, angles (one wave's) and heads in
+// turn; v past the f64 and a shorter rounding took 40. Back into rows 9 us.
 #include "gg_kv_device.h"
 
 namespace gg {
