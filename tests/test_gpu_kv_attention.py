@@ -382,3 +382,21 @@ def test_odd_heads(gpu, dim, cache, x):
     for rows in ([3, 1], [60, 8], [50, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1]):
         say("heads of", dim, cache, x, rows)
         Case(rows, [n + 333 for n in rows], 17, 1, dim, 10, cache, x).check(every=5)
+
+
+@pytest.mark.parametrize("cache,x", KINDS)
+@pytest.mark.parametrize("rows", [4, 150])
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+def test_queries_that_are_not_finite(gpu, rows, cache, x, bad):
+    """One head of one row has a NaN or an infinity: no other row or head changes but within its bounds."""
+    say("query", bad, rows, cache, x)
+    c = Case([rows], [rows + 300], 3, 1, 64, 16, cache, x)
+    r = rows // 2
+    c.buf.view(-1, c.ld)[r, 5] = bad
+    out, lse = c.run()
+    for h in range(3):
+        keep = np.array([i for i in range(rows) if (i, h) != (r, 0)])
+        ro, rl, bo, bl = attention(c.q[keep, h], c.k[0][:, 0], c.v[0][:, 0], 300 + keep, np.float32(0.125).astype(np.float64), 0, 0, cache, x)
+        assert (np.abs(out[keep, h] - ro) <= bo).all() and (np.abs(lse[keep, h] - rl) <= bl).all()
+    if np.isnan(bad):
+        assert np.isnan(out[r, 0]).all() and np.isnan(lse[r, 0])
