@@ -435,7 +435,8 @@ int gg_kv_load(const gg_kv_pages* pages, const gg_kv_seqs* seqs, void* k_out, in
  * j > p - window or j < sinks:
  *   out = sum_j softmax_j(scale q.k_j) v_j
  *   lse = ln sum_j e^(scale q.k_j)          [n_rows][n_q_heads], may be NULL
- * A row that sees nothing has out 0 and lse -inf. What a row does not see has
+ * A row that sees nothing has out 0 and lse -inf, one that sees a score of +inf
+ * or NaN has NaN in both; a score of -inf has weight 0. What a row does not see has
  * no effect on it, infinities and NaN included. Products take every bit of f32
  * q; the weights keep 24 bits with f32, 16 with f16 on other than F16 pages,
  * else those of the pages' type; sums are f32. out overlaps neither q nor the

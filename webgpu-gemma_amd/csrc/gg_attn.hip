@@ -741,11 +741,13 @@ __device__ void slow_row(const KvAttnArgs& g, int s, const KvSeq& sq, const Span
 #pragma unroll
       for (int i = 0; i < N; ++i) o[i] = scaled(o[i], f);
     }
-    // a weight that rounds to 0 is none: an infinity counts
-    const float w = x == -INFINITY ? 0.f : fmaxf(__builtin_amdgcn_exp2f(x - (m == -INFINITY ? 0.f : m)), x != x ? NAN : 1e-38f);
-    l += x != x ? NAN : w;
+    // a NaN or +inf leaves nothing of the row: e^(s - m) is a NaN with either
+    const float w = x == -INFINITY ? 0.f : x < INFINITY ? __builtin_amdgcn_exp2f(x - m) : NAN;
+    l += w;
+    // a weight that only rounds to 0 is one for an infinity, whatever it is
+    const bool some = w == 0.f && x > -INFINITY;
 #pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = fmaf(x != x ? NAN : w, v[i], o[i]);
+    for (int i = 0; i < N; ++i) o[i] = fmaf(some && !(fabsf(v[i]) < INFINITY) ? 1.f : w, v[i], o[i]);
   }
   *m_out = m;
   *l_out = l;
