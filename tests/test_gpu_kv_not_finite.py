@@ -53,7 +53,7 @@ def compare(c, out, lse, rows, lengths, scale=0.125, every=1):
 
 
 @pytest.mark.parametrize("cache,x", INF_KINDS)
-@pytest.mark.parametrize("rows,lengths", [([140], [200])])
+@pytest.mark.parametrize("rows,lengths", [([4, 2], [70, 100]), ([140], [200])])
 @pytest.mark.parametrize("dim", [64, 80, 128, 256])
 @pytest.mark.parametrize("bad", [np.inf, -np.inf])
 def test_an_infinity_in_a_key(gpu, bad, dim, rows, lengths, cache, x):
@@ -71,7 +71,7 @@ def test_an_infinity_in_a_key(gpu, bad, dim, rows, lengths, cache, x):
 
 
 @pytest.mark.parametrize("cache,x", INF_KINDS)
-@pytest.mark.parametrize("rows", [[140]])
+@pytest.mark.parametrize("rows", [[3], [140]])
 def test_an_infinity_in_a_key_of_several_chunks(gpu, rows, cache, x):
     """Each chunk but one is finite; the join keeps what is left of the rows."""
     lengths = [12000]

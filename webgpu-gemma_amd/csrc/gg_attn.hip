@@ -133,11 +133,152 @@ __device__ __forceinline__ float lse_of(float m, float sum) {
 // A sum times a factor that is not 0 but may have become it: an infinity stays.
 __device__ __forceinline__ float scaled(float x, float f) { return fabsf(x) == INFINITY ? x : x * f; }
 
-// Whether a 16-bit value is an infinity or a NaN.
+// Infinities and NaN. A weight of 0, or a zero part of a query, times one of them
+// leaves a NaN, so whatever needs care shows in O, and no main loop looks for it.
+// Where a row's sums are not finite its wave or block goes over the keys again
+// without those whose K or V holds one, and careful_rows adds these keys, to the
+// rows that see them, as the formula has it.
+// Whether one of 16-byte units first, first + step, .. below n of a row of K or V is such a value.
 template <int KV>
-__device__ __forceinline__ bool odd_value(uint32_t h) {
-  constexpr uint32_t M = KV == KV_F16 ? 0x7c00u : 0x7f80u;
-  return (h & M) == M;
+__device__ __forceinline__ bool row_odd(const uint8_t* row, int first, int step, int n) {
+  uint32_t odd = 0;
+#pragma unroll 4
+  for (int i = first; i < n; i += step) {
+    const u32x4 w = *(const u32x4*)(row + 16 * i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (KV == KV_E4M3) {
+        odd |= ((w[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;   // a byte of 0x7f
+      } else {
+        constexpr uint32_t M = KV == KV_F16 ? 0x7c00u : 0x7f80u;
+        odd |= (uint32_t)((w[e] & M) == M) | (uint32_t)((w[e] & (M << 16)) == M << 16);
+      }
+    }
+  }
+  return odd != 0;
+}
+
+// R packed rows of a wave over those keys of [u0, u1), 64 at a time, in f32: for
+// the scores a lane has a key, for the sums values of the head. A row whose query
+// is not finite (lost) takes all keys here. Of an axis that waves share in strips
+// of W keys, STEP apart, the wave has the strips from u0 on.
+template <int KV, int DP, class T, int W, int STEP, int R>
+__device__ __forceinline__ void careful_rows(const KvAttnArgs& g, int s, const KvSeq& sq, const Span& sp, int u0, int u1, int kvh, const int (&p)[R],
+                                             float (&o)[R][DP / 64], float (&m)[R], float (&l)[R], bool (&lost)[R]) {
+  constexpr int N = DP / 64, ES = KV == KV_E4M3 ? 1 : 2;
+  const int lane = threadIdx.x & 63, D = g.kv.dim;
+  float q[R][N];
+  int pos[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int row = row_in(g, p[r]);
+    const T* src = (const T*)g.q + (sq.first + row) * g.ldq + (long long)(kvh * g.group + head_in(g, p[r])) * D;
+    pos[r] = sq.len - sq.rows + row;
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      q[r][i] = lane + 64 * i < D ? (float)src[lane + 64 * i] : 0.f;
+      odd |= !(fabsf(q[r][i]) < INFINITY);
+      o[r][i] = 0.f;
+    }
+    lost[r] = __ballot(odd) != 0;
+  }
+#pragma unroll 1
+  for (int base = u0; base < u1; base += 64 / W * STEP) {
+    const int u = base + lane / W * STEP + lane % W, key = u < sp.a ? u : sp.lo + u - sp.a;
+    KvPlace at{};
+    bool ok = u < u1 && (u >= sp.a || u < sp.sink);
+    if (ok) ok = kv_place(g.kv, s, key, &at);
+    if (!ok) at = KvPlace{0, 0};
+    const long long off = kv_offset(g.kv, at, kvh) * ES;
+    const uint8_t* kp = (const uint8_t*)g.kv.k + off;
+    float ks = 1.f, vs = 1.f;
+    if constexpr (KV == KV_E4M3) {
+      ks = g.kv.k_scale[kv_scale_at(g.kv, at, kvh)];
+      vs = g.kv.v_scale[kv_scale_at(g.kv, at, kvh)];
+    }
+    const bool odd = row_odd<KV>(kp, 0, 1, D * ES / 16) || row_odd<KV>((const uint8_t*)g.kv.v + off, 0, 1, D * ES / 16) || !(ks < INFINITY) ||
+                     !(vs < INFINITY);
+    bool sees[R], some = false;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      sees[r] = ok && (odd || lost[r]) && key <= pos[r] && (g.window == 0 || key > pos[r] - g.window || key < g.sinks);
+      some |= sees[r];
+    }
+    const uint64_t any = __ballot(some);
+    if (any == 0) continue;
+    // eight sums, each of every eighth product
+    float x[R][8];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[r][e] = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll 1
+      for (int d = 0; d < 64 && 64 * i + d < D; d += 8) {
+        float k[8];
+        if constexpr (KV == KV_E4M3) {
+          const uint2 w = *(const uint2*)(kp + 64 * i + d);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const uint32_t t = e < 4 ? w.x : w.y;
+            k[e] = e % 4 == 0 ? __builtin_amdgcn_cvt_f32_fp8(t, 0) : e % 4 == 1 ? __builtin_amdgcn_cvt_f32_fp8(t, 1)
+                   : e % 4 == 2 ? __builtin_amdgcn_cvt_f32_fp8(t, 2) : __builtin_amdgcn_cvt_f32_fp8(t, 3);
+          }
+        } else {
+          const u32x4 w = *(const u32x4*)(kp + 2 * (64 * i + d));
+#pragma unroll
+          for (int e = 0; e < 8; ++e) k[e] = e % 2 == 0 ? value_lo<KV>(w[e / 2]) : value_hi<KV>(w[e / 2]);
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            x[r][e] = fmaf(__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, q[r][i]), d + e)), k[e], x[r][e]);
+      }
+    float w[R];
+    uint64_t seen[R], slight[R];   // slight: a weight that only rounds to 0, which is one for an infinity
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float t = (((x[r][0] + x[r][1]) + (x[r][2] + x[r][3])) + ((x[r][4] + x[r][5]) + (x[r][6] + x[r][7]))) * g.scale2 * ks;
+      if (!sees[r]) t = -INFINITY;
+      const float top = fmaxf(m[r], gg::wave_max(t)), f = top == m[r] ? 1.f : __builtin_amdgcn_exp2f(m[r] - top);
+      m[r] = top;
+      // a NaN or +inf leaves nothing of the row: e^(s - m) is a NaN with either
+      w[r] = t == -INFINITY ? 0.f : t < INFINITY ? __builtin_amdgcn_exp2f(t - top) * (float)(1 << (int)kShift<KV>) : NAN;
+      l[r] = f * l[r] + gg::wave_sum(w[r]);
+#pragma unroll
+      for (int i = 0; i < N; ++i) o[r][i] = scaled(o[r][i], f);
+      seen[r] = __ballot(sees[r]);
+      slight[r] = __ballot(t > -INFINITY && w[r] == 0.f);
+    }
+#pragma unroll 1
+    for (uint64_t left = any; left; left &= left - 1) {
+      const int b = __builtin_ctzll(left);
+      const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)off, b), hi = (uint32_t)__builtin_amdgcn_readlane((int)(off >> 32), b);
+      const uint8_t* vp = (const uint8_t*)g.kv.v + (long long)(((uint64_t)hi << 32) | lo);
+      float v[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int d = lane + 64 * i < D ? lane + 64 * i : 0;
+        if constexpr (KV == KV_E4M3)
+          v[i] = __builtin_amdgcn_cvt_f32_fp8((uint32_t)vp[d], 0) * __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vs), b));
+        else
+          v[i] = value_lo<KV>((uint32_t)((const uint16_t*)vp)[d]);
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        if (((seen[r] >> b) & 1) == 0) continue;
+        const float wr = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w[r]), b));
+        const float wi = (slight[r] >> b) & 1 ? 1.f : wr;
+#pragma unroll
+        for (int i = 0; i < N; ++i) o[r][i] = fmaf(fabsf(v[i]) < INFINITY ? wr : wi, v[i], o[r][i]);
+      }
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -221,7 +362,7 @@ __global__ __launch_bounds__(256, (DP <= 128 || (KV == KV_E4M3 && kParts<KV, T> 
     page = g.kv.table[(long long)s * g.kv.table_ld + (int)g.kv.page_div((uint32_t)key)];
   };
   uint32_t live = 0;   // bit i: key i of the step has a place; others are read from row 0
-  auto places = [&](int u) __attribute__((always_inline)) {
+  auto places = [&](auto careful, int u) __attribute__((always_inline)) {
     const int x = u + key_lane, key = x < sp.a ? x : sp.lo + x - sp.a;
     const bool ok = x < u1 && (x >= sp.a || x < sp.sink) && (uint32_t)page < (uint32_t)g.kv.n_pages;
     const KvPlace at{ok ? page : 0, ok ? key - (int)g.kv.page_div((uint32_t)key) * g.kv.page_size : 0};
@@ -230,6 +371,12 @@ __global__ __launch_bounds__(256, (DP <= 128 || (KV == KV_E4M3 && kParts<KV, T> 
     if constexpr (KV == KV_E4M3) {
       sk = g.kv.k_scale[kv_scale_at(g.kv, at, kvh)];
       sv = g.kv.v_scale[kv_scale_at(g.kv, at, kvh)];
+    }
+    if constexpr (careful) {   // half of the lanes look at K, half at V
+      bool odd = row_odd<KV>((const uint8_t*)(lane < 32 ? g.kv.k : g.kv.v) + kv_offset(g.kv, at, kvh) * ES, 0, 1, D * ES / 16);
+      if constexpr (KV == KV_E4M3) odd |= !(sk < INFINITY) || !(sv < INFINITY);
+      const uint64_t b = __ballot(odd);
+      live &= ~(uint32_t)(b | (b >> 32));
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   };
@@ -289,7 +436,7 @@ __global__ __launch_bounds__(256, (DP <= 128 || (KV == KV_E4M3 && kParts<KV, T> 
   }
   // (by waves without keys too, which read row 0: loads in a branch would all be
   // waited for behind it)
-  places(first);
+  places(std::false_type{}, first);
   ask(first + 128);
   load_k();
   load_v();
@@ -319,15 +466,15 @@ __global__ __launch_bounds__(256, (DP <= 128 || (KV == KV_E4M3 && kParts<KV, T> 
 #pragma unroll
     for (int c = 0; c < KC; ++c) qb[n][c] = q_all[n][c][lane];
 
-  // All of this wave's keys. `careful`: infinities and NaN of V reach the rows
-  // that see their keys and no others.
+  // All of this wave's keys; `careful`: without those that careful_rows takes.
   auto pass = [&](auto careful) __attribute__((always_inline)) {
   float ks[8], vs[8];
   if (careful && first < u1) {
     ask(first);
-    places(first);
+    places(careful, first);
     ask(first + 128);
     load_k();
+    load_v();
   }
   // (left from the middle: a path around the last loads back to the start would
   // make K wait for V there)
@@ -347,11 +494,6 @@ __global__ __launch_bounds__(256, (DP <= 128 || (KV == KV_E4M3 && kParts<KV, T> 
     // this lane's keys are 4 quad + j and, from j = 4 on, 12 more
     const uint32_t mine = __builtin_amdgcn_readfirstlane(live) >> (4 * quad);
     const bool miss = __builtin_amdgcn_readfirstlane(live) != 0xffffffffu;
-    long long voff[8];
-    if constexpr (careful) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) voff[j] = key_off[wv][4 * quad + (j & 3) + 16 * (j >> 2)];
-    }
     // S^T: 32 keys x 16 packed rows
     // with several parts in two sums each, chains of half the length
     constexpr int CHAINS = NP > 1 ? 2 : 1;
@@ -388,7 +530,7 @@ __global__ __launch_bounds__(256, (DP <= 128 || (KV == KV_E4M3 && kParts<KV, T> 
     }
     const int next = u + 128;
     if (next < u1) {
-      places(next);
+      places(careful, next);
       ask(next + 128);
       load_k();
     }
@@ -417,16 +559,15 @@ __global__ __launch_bounds__(256, (DP <= 128 || (KV == KV_E4M3 && kParts<KV, T> 
     mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
     mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
     float f = 1.f;
-    if (__ballot(mx > m + kSlack)) {
-      const float mn = mx > m + kSlack ? mx : m;
+    constexpr float SLACK = careful ? 0.f : kSlack;   // large values: weights of 1 at most
+    if (__ballot(mx > m + SLACK)) {
+      const float mn = mx > m + SLACK ? mx : m;
       f = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
       m = mn;
       l *= f;
       le *= f;
-      if constexpr (!careful) {
 #pragma unroll
-        for (int t = 0; t < VD; ++t) o[t] *= f;
-      }
+      for (int t = 0; t < VD; ++t) o[t] *= f;
     }
     const float ref = (m == -INFINITY ? 0.f : m) - kShift<KV>;
     // weights, as the second product's operand
@@ -457,125 +598,115 @@ __global__ __launch_bounds__(256, (DP <= 128 || (KV == KV_E4M3 && kParts<KV, T> 
       for (int k = 0; k < NP; ++k) pb[k][i] = w[k];
     }
     // V of keys that are not there counts as 0: what lies there may be a NaN
-    if (!careful && miss) {
+    if (miss) {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
 #pragma unroll
         for (int n = 0; n < VN; ++n) vr[j][n] = (mine >> ((j & 3) + 16 * (j >> 2))) & 1 ? vr[j][n] : (vw_t)0;
     }
-    if constexpr (careful) {
-      // sums in LDS, one value of a head at a time: the finite values as ever, then
-      // the infinities of either sign among the keys that the row sees (a NaN is both)
-      constexpr uint32_t ONE = KV == KV_F16 ? 0x3c00u : 0x3f80u, MANT = KV == KV_F16 ? 0x3ffu : 0x7fu;
-      u32x4 seen;
+    if constexpr (KV == KV_E4M3) {
+      // bytes of two keys side by side, then converted: four values of a head
 #pragma unroll
-      for (int i = 0; i < 4; ++i) seen[i] = ((here >> (2 * i)) & 1 ? ONE : 0u) | ((here >> (2 * i + 1)) & 1 ? ONE << 16 : 0u);
-#pragma unroll 1
-      for (int t = 0; t < VD; ++t) {
-        const int d = VD * c16 + t;
-        u32x4 clean, up, down;
+      for (int t = 0; t < VD; t += 4) {
+        u32x4 va[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          uint32_t cl[2], pu[2], pd[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            uint32_t h = 0;
-            if (((mine >> (((2 * i + e) & 3) + 16 * ((2 * i + e) >> 2))) & 1) && d < D) {
-              const uint8_t* r = (const uint8_t*)g.kv.v + voff[2 * i + e] + d * ES;
-              if constexpr (KV == KV_E4M3)
-                h = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)*r, 1.f, false)) & 0xffffu;
-              else
-                h = *(const uint16_t*)r;
-            }
-            const bool is_odd = odd_value<KV>(h), nan = is_odd && (h & MANT);
-            cl[e] = is_odd ? 0u : h;
-            pu[e] = is_odd && (nan || !(h & 0x8000u)) ? ONE : 0u;
-            pd[e] = is_odd && (nan || (h & 0x8000u)) ? ONE : 0u;
-          }
-          clean[i] = cl[0] | (cl[1] << 16);
-          up[i] = pu[0] | (pu[1] << 16);
-          down[i] = pd[0] | (pd[1] << 16);
+          const uint32_t w0 = vr[2 * i][t / 16][t / 4 % 4], w1 = vr[2 * i + 1][t / 16][t / 4 % 4];
+          const uint32_t lo = __builtin_amdgcn_perm(w1, w0, 0x05010400u), hi = __builtin_amdgcn_perm(w1, w0, 0x07030602u);
+          va[0][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false));
+          va[1][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true));
+          va[2][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false));
+          va[3][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true));
         }
-        float* sum = &o_all[wv][c16][4 * VD * quad + t];
-        f32x4 c;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) c[i] = scaled(sum[VD * i], f);
+        for (int k = NP - 1; k >= 0; --k)
 #pragma unroll
-        for (int k = NP - 1; k >= 0; --k) c = mfma16<KV>(clean, pb[k], c);
-        const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-        const f32x4 nu = mfma16<KV>(up, seen, zero), nd = mfma16<KV>(down, seen, zero);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (nu[i] > 0.f) c[i] += INFINITY;
-          if (nd[i] > 0.f) c[i] -= INFINITY;
-          sum[VD * i] = c[i];
-        }
+          for (int e = 0; e < 4; ++e) o[t + e] = mfma16<KV>(va[e], pb[k], o[t + e]);
       }
     } else {
-      if constexpr (KV == KV_E4M3) {
-        // bytes of two keys side by side, then converted: four values of a head
+      constexpr int TS = NP > 1 ? 4 : 2;   // values at a time: sums that wait for each other lie TS instructions apart
 #pragma unroll
-        for (int t = 0; t < VD; t += 4) {
-          u32x4 va[4];
+      for (int t = 0; t < VD; t += TS) {
+        u32x4 va[TS];
+#pragma unroll
+        for (int e = 0; e < TS; e += 2)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const uint32_t w0 = vr[2 * i][t / 16][t / 4 % 4], w1 = vr[2 * i + 1][t / 16][t / 4 % 4];
-            const uint32_t lo = __builtin_amdgcn_perm(w1, w0, 0x05010400u), hi = __builtin_amdgcn_perm(w1, w0, 0x07030602u);
-            va[0][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false));
-            va[1][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true));
-            va[2][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false));
-            va[3][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true));
+            const uint32_t w0 = vr[2 * i][(t + e) / 8][(t + e) / 2 % 4], w1 = vr[2 * i + 1][(t + e) / 8][(t + e) / 2 % 4];
+            va[e][i] = lower2(w0, w1);
+            va[e + 1][i] = upper2(w0, w1);
           }
 #pragma unroll
-          for (int k = NP - 1; k >= 0; --k)
+        for (int k = NP - 1; k >= 0; --k)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[t + e] = mfma16<KV>(va[e], pb[k], o[t + e]);
-        }
-      } else {
-        constexpr int TS = NP > 1 ? 4 : 2;   // values at a time: sums that wait for each other lie TS instructions apart
-#pragma unroll
-        for (int t = 0; t < VD; t += TS) {
-          u32x4 va[TS];
-#pragma unroll
-          for (int e = 0; e < TS; e += 2)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t w0 = vr[2 * i][(t + e) / 8][(t + e) / 2 % 4], w1 = vr[2 * i + 1][(t + e) / 8][(t + e) / 2 % 4];
-              va[e][i] = lower2(w0, w1);
-              va[e + 1][i] = upper2(w0, w1);
-            }
-#pragma unroll
-          for (int k = NP - 1; k >= 0; --k)
-#pragma unroll
-            for (int e = 0; e < TS; ++e) o[t + e] = mfma16<KV>(va[e], pb[k], o[t + e]);
-        }
+          for (int e = 0; e < TS; ++e) o[t + e] = mfma16<KV>(va[e], pb[k], o[t + e]);
       }
     }
     if (next >= u1) {
       asm volatile("");   // an exit of its own
       break;
     }
-    if (!careful) load_v();
+    load_v();
   }
   };
-  // A weight of 0, or a part of one, times an infinity or a NaN leaves a NaN, so
-  // whatever needs care shows in O, and the main loop need not look at V.
   pass(std::false_type{});
-  bool again;
+  uint32_t again;   // rows whose sums are not finite
   {
     f32x4 z = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int t = 0; t < VD; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) z[i] = fmaf(o[t][i], 0.f, z[i]);
-    again = __ballot((z[0] + z[1]) + (z[2] + z[3]) != 0.f) != 0;   // 0 times an infinity or a NaN
+    uint64_t odd = __ballot((z[0] + z[1]) + (z[2] + z[3]) != 0.f && p < packed);   // 0 times an infinity or a NaN
+    odd |= odd >> 32;
+    again = (uint32_t)(odd | (odd >> 16)) & 0xffffu;
   }
-  if (again) {
-    for (int e = lane; e < kKvFewTile * OP; e += 64) (&o_all[wv][0][0])[e] = 0.f;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  // (expected not to be: in line this code costs a single token 0.4 us)
+  if (__builtin_expect(again != 0, 0)) {
+#pragma unroll
+    for (int t = 0; t < VD; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
     m = -INFINITY;
     l = le = 0.f;
     pass(std::true_type{});
+    // and the keys left out, four rows at a time, whose sums come through LDS
+    constexpr int R = 4, N = DP / 64;
+    float m2 = -INFINITY, l2 = 0.f;
+    bool drop = false;
+    for (uint32_t left = again; left;) {
+      int c[R], pr[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        c[r] = left ? __builtin_ctz(left) : c[0];
+        left &= left - 1;
+        pr[r] = p0 + c[r];
+      }
+      float os[R][N], ms[R], ls[R];
+      bool lost[R];
+      careful_rows<KV, DP, T, 32, 128, R>(g, s, sq, sp, first, u1, kvh, pr, os, ms, ls, lost);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) o_all[wv][c[r]][lane + 64 * i] = os[r][i];
+        if (c16 == c[r]) {
+          m2 = ms[r];
+          l2 = ls[r];
+          drop = lost[r];
+        }
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if ((again >> c16) & 1) {
+      if (drop) m = -INFINITY;
+      const float top = fmaxf(m, m2), f = drop ? 0.f : m == top ? 1.f : __builtin_amdgcn_exp2f(m - top),
+                  f2 = m2 == top ? 1.f : __builtin_amdgcn_exp2f(m2 - top);
+      m = top;
+      l = (drop ? 0.f : l * f) + (quad == 0 ? l2 * f2 : 0.f);
+      le = (drop ? 0.f : le * f) + (quad == 0 ? l2 * f2 : 0.f);
+#pragma unroll
+      for (int t = 0; t < VD; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[t][i] = (drop ? 0.f : o[t][i] * f) + scaled(o_all[wv][c16][4 * VD * quad + VD * i + t], f2);
+    }
   }
 
   // the four waves' parts; this lane has values 4 VD quad + VD i + t of its packed row
@@ -593,9 +724,11 @@ __global__ __launch_bounds__(256, (DP <= 128 || (KV == KV_E4M3 && kParts<KV, T> 
     const float top = fmaxf(fmaxf(m_all[0][c16], m_all[1][c16]), fmaxf(m_all[2][c16], m_all[3][c16]));
     const float f = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top);
     float* dst = &o_all[wv][c16][4 * VD * quad];
-    if (again) {
-#pragma unroll 1
-      for (int i = 0; i < 4 * VD; ++i) dst[i] = scaled(dst[i], f);
+    if (__builtin_expect(again != 0, 0)) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int t = 0; t < VD; ++t) dst[VD * i + t] = scaled(o[t][i], f);
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
