@@ -143,3 +143,58 @@ def test_nothing_but_nan(gpu, rows, cache, x):
     c.pool.table_dev.copy_(torch.from_numpy(c.pool.table))
     out, lse = c.run()
     assert (out == 0).all() and np.isneginf(lse).all()
+
+
+@pytest.mark.parametrize("rows,length,heads,dim", [([256], [4096], 4, 256), ([300, 40], [3000, 2500], 8, 128), ([1] * 16, [3000] * 16, 8, 128)])
+def test_one_nan_does_not_stop_a_call(gpu, rows, length, heads, dim):
+    """A NaN in V that all rows see: some ten times the call's time, not hundreds of times."""
+    c = Case(rows, length, heads, 1, dim, 64, "bf16", "bf16")
+    seqs, keep = seqs_of(c.pool, rows, length)
+    pages = c.pool.pages()
+    out = torch.empty(c.n, heads * dim, dtype=torch.bfloat16, device="cuda:0")
+    ws = torch.empty(max(capi.kv_attention_workspace_size(pages, seqs, heads), 16), dtype=torch.uint8, device="cuda:0")
+
+    def best():
+        times = []
+        for _ in range(6):
+            a, b = torch.cuda.Event(True), torch.cuda.Event(True)
+            a.record()
+            capi.kv_attention(pages, seqs, c.buf.data_ptr(), capi.GG_TYPE_BF16, c.ld, heads, dim ** -0.5, 0, 0, out.data_ptr(), heads * dim, None,
+                              ws.data_ptr(), stream())
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times)
+    clean = best()
+    for s in range(len(rows)):
+        c.pool.views()[1][c.pool.table[s, 0], 10, 0, 7] = np.nan
+    dirty = best()
+    say("one NaN", rows[0], length[0], clean, dirty)
+    assert torch.isnan(out.view(c.n, heads, dim)[:, :, 7]).all() and torch.isfinite(out.view(c.n, heads, dim)[:, :, 8]).all()
+    assert dirty < 40 * clean
+
+
+@pytest.mark.parametrize("cache,x", KINDS)
+@pytest.mark.parametrize("rows,length", [(6, 9000), (200, 9000)])
+def test_many_keys_that_are_not_finite(gpu, rows, length, cache, x):
+    """NaN, infinities and large finite values in V all along a long axis: each in a column of its own, the others as they are."""
+    c = Case([rows], [length], 2, 1, 64, 16, cache, x)
+    rng = np.random.default_rng(rows)
+    view = c.pool.views()[1]
+    cols = {3: 0x7f} if cache == "e4m3" else {3: np.nan, 20: np.inf, 41: -np.inf}
+    if cache == "e4m3":
+        # a NaN scale takes the whole row with it: only codes here
+        for p in rng.integers(0, length - rows, 40):
+            view[c.pool.table[0, p // 16], p % 16, 0, 3] = 0x7f
+    else:
+        for d, value in cols.items():
+            for p in rng.integers(0, length - rows, 40):
+                view[c.pool.table[0, p // 16], p % 16, 0, d] = value
+    out, lse = c.run()
+    good = ~np.isin(np.arange(64), list(cols))
+    for i in range(0, rows, 1 if rows < 100 else 17):
+        for h in range(2):
+            ro, rl, bo, bl = (t[0] for t in attention(c.q[i:i + 1, h], c.k[0][:, 0], c.v[0][:, 0], [length - rows + i], 0.125, 0, 0, cache, x))
+            assert (np.abs(out[i, h] - ro) <= bo)[good].all() and abs(lse[i, h] - rl) <= bl
+            assert np.isnan(out[i, h, 3])
+            assert cache == "e4m3" or out[i, h, 20] == np.inf and out[i, h, 41] == -np.inf

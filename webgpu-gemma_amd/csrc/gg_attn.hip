@@ -135,15 +135,15 @@ __device__ __forceinline__ float scaled(float x, float f) { return fabsf(x) == I
 
 // Infinities and NaN. A weight of 0, or a zero part of a query, times one of them
 // leaves a NaN, so whatever needs care shows in O, and no main loop looks for it.
-// Where a row's sums are not finite its wave or block goes over the keys again
-// without those whose K or V holds one, and careful_rows adds these keys, to the
-// rows that see them, as the formula has it.
-// Whether one of 16-byte units first, first + step, .. below n of a row of K or V is such a value.
+// A wave takes rows whose sums are not finite again with redo_rows: without the
+// keys whose K or V holds one, which careful_rows adds to the rows that see them,
+// as the formula has it.
+// Whether one of the n 16-byte units of a row of K or V holds one.
 template <int KV>
-__device__ __forceinline__ bool row_odd(const uint8_t* row, int first, int step, int n) {
+__device__ __forceinline__ bool row_odd(const uint8_t* row, int n) {
   uint32_t odd = 0;
 #pragma unroll 4
-  for (int i = first; i < n; i += step) {
+  for (int i = 0; i < n; ++i) {
     const u32x4 w = *(const u32x4*)(row + 16 * i);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -161,10 +161,11 @@ __device__ __forceinline__ bool row_odd(const uint8_t* row, int first, int step,
 // R packed rows of a wave over those keys of [u0, u1), 64 at a time, in f32: for
 // the scores a lane has a key, for the sums values of the head. A row whose query
 // is not finite (lost) takes all keys here. Of an axis that waves share in strips
-// of W keys, STEP apart, the wave has the strips from u0 on.
-template <int KV, int DP, class T, int W, int STEP, int R>
-__device__ __forceinline__ void careful_rows(const KvAttnArgs& g, int s, const KvSeq& sq, const Span& sp, int u0, int u1, int kvh, const int (&p)[R],
-                                             float (&o)[R][DP / 64], float (&m)[R], float (&l)[R], bool (&lost)[R]) {
+// of 32 keys, STEP apart, the wave has the strips from u0 on; strip i can hold such
+// a key only if bit i >> shift of marks is set.
+template <int KV, int DP, class T, int STEP, int R>
+__device__ __forceinline__ void careful_rows(const KvAttnArgs& g, int s, const KvSeq& sq, const Span& sp, int u0, int u1, int kvh, uint64_t marks,
+                                             int shift, const int (&p)[R], float (&o)[R][DP / 64], float (&m)[R], float (&l)[R], bool (&lost)[R]) {
   constexpr int N = DP / 64, ES = KV == KV_E4M3 ? 1 : 2;
   const int lane = threadIdx.x & 63, D = g.kv.dim;
   float q[R][N];
@@ -179,15 +180,17 @@ __device__ __forceinline__ void careful_rows(const KvAttnArgs& g, int s, const K
     bool odd = false;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      q[r][i] = lane + 64 * i < D ? (float)src[lane + 64 * i] : 0.f;
+      q[r][i] = (float)src[min(lane + 64 * i, D - 1)];
       odd |= !(fabsf(q[r][i]) < INFINITY);
       o[r][i] = 0.f;
     }
     lost[r] = __ballot(odd) != 0;
+    if (lost[r]) marks = ~0ull;
   }
 #pragma unroll 1
-  for (int base = u0; base < u1; base += 64 / W * STEP) {
-    const int u = base + lane / W * STEP + lane % W, key = u < sp.a ? u : sp.lo + u - sp.a;
+  for (int base = u0, i = 0; base < u1; base += 2 * STEP, i += 2) {
+    if (((marks >> (i >> shift) | marks >> min((i + 1) >> shift, 63)) & 1) == 0) continue;
+    const int u = base + lane / 32 * STEP + lane % 32, key = u < sp.a ? u : sp.lo + u - sp.a;
     KvPlace at{};
     bool ok = u < u1 && (u >= sp.a || u < sp.sink);
     if (ok) ok = kv_place(g.kv, s, key, &at);
@@ -199,7 +202,7 @@ __device__ __forceinline__ void careful_rows(const KvAttnArgs& g, int s, const K
       ks = g.kv.k_scale[kv_scale_at(g.kv, at, kvh)];
       vs = g.kv.v_scale[kv_scale_at(g.kv, at, kvh)];
     }
-    const bool odd = row_odd<KV>(kp, 0, 1, D * ES / 16) || row_odd<KV>((const uint8_t*)g.kv.v + off, 0, 1, D * ES / 16) || !(ks < INFINITY) ||
+    const bool odd = row_odd<KV>(kp, D * ES / 16) || row_odd<KV>((const uint8_t*)g.kv.v + off, D * ES / 16) || !(ks < INFINITY) ||
                      !(vs < INFINITY);
     bool sees[R], some = false;
 #pragma unroll
@@ -263,7 +266,7 @@ __device__ __forceinline__ void careful_rows(const KvAttnArgs& g, int s, const K
       float v[N];
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int d = lane + 64 * i < D ? lane + 64 * i : 0;
+        const int d = min(lane + 64 * i, D - 1);
         if constexpr (KV == KV_E4M3)
           v[i] = __builtin_amdgcn_cvt_f32_fp8((uint32_t)vp[d], 0) * __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vs), b));
         else
@@ -278,6 +281,208 @@ __device__ __forceinline__ void careful_rows(const KvAttnArgs& g, int s, const K
         for (int i = 0; i < N; ++i) o[r][i] = fmaf(fabsf(v[i]) < INFINITY ? wr : wi, v[i], o[r][i]);
       }
     }
+  }
+}
+
+// The 16 packed rows from p0 on, those of `which` for certain, over the strips of
+// 32 keys from u0 on, STEP apart: one wave, K and V straight from memory. Lane
+// (c, quad) gets values 16 t + 4 quad + i of packed row c, its m and its sums of
+// weights. buf: 4 DP floats of the wave's own. It shares nothing with the other waves: with one NaN that all rows see, 61 tokens of 32 heads of 128 on 8 at up to
+// 8192 positions take 368 us for 228, 2048 rows at 32768, 4 heads of 256 on 1, 4.3 ms for 0.33.
+template <int KV, int DP, class T, int STEP>
+__device__ __forceinline__ void redo_rows(const KvAttnArgs& g, int s, const KvSeq& sq, const Span& sp, int u0, int u1, int kvh, int p0, uint32_t which,
+                                          float* buf, f32x4 (&o)[DP / 16], float& m, float& l, float& le) {
+  constexpr int NP = kParts<KV, T>, KC = DP / 32, VD = DP / 16, ES = KV == KV_E4M3 ? 1 : 2;
+  const int lane = threadIdx.x & 63, c16 = lane & 15, quad = lane >> 4, D = g.kv.dim;
+  const int p = min(p0 + c16, sq.rows * g.group - 1), row = row_in(g, p), pos = sq.len - sq.rows + row;
+  const T* q = (const T*)g.q + (sq.first + row) * g.ldq + (long long)(kvh * g.group + head_in(g, p)) * D;
+  u32x4 qb[NP][KC];
+#pragma unroll
+  for (int c = 0; c < KC; ++c) {
+    const int d = min(32 * c + 8 * quad, D - 8);
+    const uint32_t on = 32 * c + 8 * quad < D ? ~0u : 0u;   // past D the query is 0
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t w[NP];
+      split2<KV, NP>((float)q[d + 2 * i], (float)q[d + 2 * i + 1], w);
+#pragma unroll
+      for (int n = 0; n < NP; ++n) qb[n][c][i] = w[n] & on;
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < VD; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  m = -INFINITY;
+  l = le = 0.f;
+  const auto of_lane = [](float x, int i) __attribute__((always_inline)) { return __shfl(x, i, 64); };
+  // whether one of two 16-bit values is an infinity or a NaN
+  const auto odd2 = [](uint32_t w) __attribute__((always_inline)) {
+    constexpr uint32_t M = KV == KV_F16 ? 0x7c00u : 0x7f80u;
+    return (uint32_t)((w & M) == M) | (uint32_t)((w & (M << 16)) == M << 16) << 1;
+  };
+  uint64_t marks = 0;
+  int shift = 0, strip = 0;
+  while (((u1 - u0) / STEP) >> shift > 63) ++shift;
+#pragma unroll 1
+  for (int u = u0; u < u1; u += STEP, ++strip) {
+    const int x = u + (lane & 31), mine = x < sp.a ? x : sp.lo + x - sp.a;
+    KvPlace at{};
+    bool ok = x < u1 && (x >= sp.a || x < sp.sink);
+    if (ok) ok = kv_place(g.kv, s, mine, &at);
+    if (!ok) at = KvPlace{0, 0};
+    const long long off = kv_offset(g.kv, at, kvh) * ES;
+    float sk = 1.f, sv = 1.f;
+    if constexpr (KV == KV_E4M3) {
+      sk = g.kv.k_scale[kv_scale_at(g.kv, at, kvh)];
+      sv = g.kv.v_scale[kv_scale_at(g.kv, at, kvh)];
+    }
+    const uint32_t placed = (uint32_t)__ballot(ok);
+    uint32_t odd = (uint32_t)__ballot(!(sk < INFINITY) || !(sv < INFINITY));   // keys that hold an infinity or a NaN
+    long long voff[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) voff[j] = __shfl(off, 4 * quad + (j & 3) + 16 * (j >> 2), 64);
+    u32x4 va[VD];
+    uint32_t v_odd[4] = {};
+#pragma unroll
+    for (int t = 0; t < VD; ++t) {
+      const int d = min(16 * t + c16, D - 1);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint8_t *r0 = (const uint8_t*)g.kv.v + voff[2 * i] + d * ES, *r1 = (const uint8_t*)g.kv.v + voff[2 * i + 1] + d * ES;
+        if constexpr (KV == KV_E4M3) va[t][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)*r0 | ((uint32_t)*r1 << 8), 1.f, false));
+        else va[t][i] = (uint32_t)*(const uint16_t*)r0 | ((uint32_t)*(const uint16_t*)r1 << 16);
+        v_odd[i] |= odd2(va[t][i]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint64_t b = __ballot((v_odd[j >> 1] >> (j & 1)) & 1);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) odd |= (uint32_t)(((b >> (16 * k)) & 0xffff) != 0) << (4 * k + (j & 3) + 16 * (j >> 2));
+    }
+    f32x4 sc[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint8_t* k = (const uint8_t*)g.kv.k + __shfl(off, c16 + 16 * h, 64);
+      uint32_t k_odd = 0;
+      sc[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < KC; ++c) {
+        const int d = min(32 * c + 8 * quad, D - 8);
+        u32x4 ka;
+        if constexpr (KV == KV_E4M3) {
+          const uint2 w = *(const uint2*)(k + d);
+          ka[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, 1.f, false));
+          ka[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, 1.f, true));
+          ka[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, 1.f, false));
+          ka[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, 1.f, true));
+        } else {
+          ka = *(const u32x4*)(k + 2 * d);
+        }
+        k_odd |= odd2(ka[0]) | odd2(ka[1]) | odd2(ka[2]) | odd2(ka[3]);
+#pragma unroll
+        for (int n = NP - 1; n >= 0; --n) sc[h] = mfma16<KV>(ka, qb[n][c], sc[h]);
+      }
+      uint64_t b = __ballot(k_odd != 0);
+      b |= b >> 32;
+      odd |= (uint32_t)((b | (b >> 16)) & 0xffff) << (16 * h);
+    }
+    const uint32_t live = placed & ~odd;
+    if (odd & placed) marks |= 1ull << (strip >> shift);
+    // this lane's keys are 4 quad + j and, from j = 4 on, 12 more
+    const int key0 = u < sp.a ? u : sp.lo + u - sp.a;
+    float y[8], mx = -INFINITY;
+    uint32_t there[4];   // of two values of V
+    uint32_t pb[NP][4];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int i = 4 * quad + (j & 3) + 16 * (j >> 2), key = key0 + i;
+      const bool sees = ((live >> i) & 1) && key <= pos && (g.window == 0 || key > pos - g.window || key < g.sinks);
+      float t = sc[j >> 2][j & 3] * g.scale2;
+      if constexpr (KV == KV_E4M3) t *= of_lane(sk, i);
+      y[j] = sees ? t : -INFINITY;
+      mx = fmaxf(mx, y[j]);
+      const uint32_t half = (live >> i) & 1 ? 0xffffu : 0u;
+      there[j >> 1] = j & 1 ? there[j >> 1] | (half << 16) : half;
+    }
+    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    // (no slack: with large values no weight is above 1)
+    const float top = fmaxf(m, mx), f = top == m ? 1.f : __builtin_amdgcn_exp2f(m - top), ref = (top == -INFINITY ? 0.f : top) - kShift<KV>;
+    m = top;
+    l *= f;
+    le *= f;
+#pragma unroll
+    for (int t = 0; t < VD; ++t) o[t] *= f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float w0 = __builtin_amdgcn_exp2f(y[2 * i] - ref), w1 = __builtin_amdgcn_exp2f(y[2 * i + 1] - ref);
+      uint32_t w[NP];
+      le += w0 + w1;
+      split2<KV, NP>(w0, w1, w);
+      if constexpr (NP == 1) {
+        w0 = value_lo<KV>(w[0]);
+        w1 = value_hi<KV>(w[0]);
+      }
+      l += w0 + w1;
+      if constexpr (KV == KV_E4M3) {
+        const int j = 4 * quad + (2 * i & 3) + 16 * (i >> 1);
+        const float s0 = of_lane(sv, j), s1 = of_lane(sv, j + 1);   // of hidden rows maybe a NaN
+        w0 = w0 == 0.f ? 0.f : w0 * s0;
+        w1 = w1 == 0.f ? 0.f : w1 * s1;
+        split2<KV, NP>(w0, w1, w);
+      }
+#pragma unroll
+      for (int n = 0; n < NP; ++n) pb[n][i] = w[n];
+    }
+#pragma unroll
+    for (int t = 0; t < VD; ++t) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) va[t][i] &= there[i];
+#pragma unroll
+      for (int n = NP - 1; n >= 0; --n) o[t] = mfma16<KV>(va[t], u32x4{pb[n][0], pb[n][1], pb[n][2], pb[n][3]}, o[t]);
+    }
+  }
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  le += __shfl_xor(le, 16, 64);
+  le += __shfl_xor(le, 32, 64);
+  // the keys left out, four rows at a time
+  constexpr int R = 4;
+#pragma unroll 1
+  for (uint32_t left = which; left;) {
+    int c[R], pr[R], r_of = -1;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      c[r] = left ? __builtin_ctz(left) : c[0];
+      r_of = left && c16 == c[r] ? r : r_of;
+      left &= left - 1;
+      pr[r] = p0 + c[r];
+    }
+    float os[R][DP / 64], ms[R], ls[R], m2 = 0.f, l2 = 0.f;
+    bool lost[R], drop = false;
+    careful_rows<KV, DP, T, STEP, R>(g, s, sq, sp, u0, u1, kvh, marks, shift, pr, os, ms, ls, lost);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+#pragma unroll
+      for (int i = 0; i < DP / 64; ++i) buf[r * DP + lane + 64 * i] = os[r][i];
+      m2 = r_of == r ? ms[r] : m2;
+      l2 = r_of == r ? ls[r] : l2;
+      drop = r_of == r ? lost[r] : drop;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (r_of >= 0) {
+      if (drop) m = -INFINITY;
+      const float top = fmaxf(m, m2), f = drop ? 0.f : m == top ? 1.f : __builtin_amdgcn_exp2f(m - top),
+                  f2 = m2 == top ? 1.f : __builtin_amdgcn_exp2f(m2 - top);
+      m = top;
+      l = (drop ? 0.f : l * f) + l2 * f2;
+      le = (drop ? 0.f : le * f) + l2 * f2;
+#pragma unroll
+      for (int t = 0; t < VD; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[t][i] = (drop ? 0.f : o[t][i] * f) + scaled(buf[r_of * DP + 16 * t + 4 * quad + i], f2);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
 }
 
@@ -362,7 +567,7 @@ __global__ __launch_bounds__(256, (DP <= 128 || (KV == KV_E4M3 && kParts<KV, T> 
     page = g.kv.table[(long long)s * g.kv.table_ld + (int)g.kv.page_div((uint32_t)key)];
   };
   uint32_t live = 0;   // bit i: key i of the step has a place; others are read from row 0
-  auto places = [&](auto careful, int u) __attribute__((always_inline)) {
+  auto places = [&](int u) __attribute__((always_inline)) {
     const int x = u + key_lane, key = x < sp.a ? x : sp.lo + x - sp.a;
     const bool ok = x < u1 && (x >= sp.a || x < sp.sink) && (uint32_t)page < (uint32_t)g.kv.n_pages;
     const KvPlace at{ok ? page : 0, ok ? key - (int)g.kv.page_div((uint32_t)key) * g.kv.page_size : 0};
@@ -371,12 +576,6 @@ __global__ __launch_bounds__(256, (DP <= 128 || (KV == KV_E4M3 && kParts<KV, T> 
     if constexpr (KV == KV_E4M3) {
       sk = g.kv.k_scale[kv_scale_at(g.kv, at, kvh)];
       sv = g.kv.v_scale[kv_scale_at(g.kv, at, kvh)];
-    }
-    if constexpr (careful) {   // half of the lanes look at K, half at V
-      bool odd = row_odd<KV>((const uint8_t*)(lane < 32 ? g.kv.k : g.kv.v) + kv_offset(g.kv, at, kvh) * ES, 0, 1, D * ES / 16);
-      if constexpr (KV == KV_E4M3) odd |= !(sk < INFINITY) || !(sv < INFINITY);
-      const uint64_t b = __ballot(odd);
-      live &= ~(uint32_t)(b | (b >> 32));
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   };
@@ -436,7 +635,7 @@ __global__ __launch_bounds__(256, (DP <= 128 || (KV == KV_E4M3 && kParts<KV, T> 
   }
   // (by waves without keys too, which read row 0: loads in a branch would all be
   // waited for behind it)
-  places(std::false_type{}, first);
+  places(first);
   ask(first + 128);
   load_k();
   load_v();
@@ -466,16 +665,10 @@ __global__ __launch_bounds__(256, (DP <= 128 || (KV == KV_E4M3 && kParts<KV, T> 
 #pragma unroll
     for (int c = 0; c < KC; ++c) qb[n][c] = q_all[n][c][lane];
 
-  // All of this wave's keys; `careful`: without those that careful_rows takes.
-  auto pass = [&](auto careful) __attribute__((always_inline)) {
+  // All of this wave's keys. (Not written in line: the weights are then compiled
+  // into blocks of their own, 3 tokens at up to 131072, 8-bit heads of 256, 145.6 us for 142.4.)
+  auto pass = [&]() __attribute__((always_inline)) {
   float ks[8], vs[8];
-  if (careful && first < u1) {
-    ask(first);
-    places(careful, first);
-    ask(first + 128);
-    load_k();
-    load_v();
-  }
   // (left from the middle: a path around the last loads back to the start would
   // make K wait for V there)
   if (first < u1) for (int u = first;; u += 128) {
@@ -530,7 +723,7 @@ __global__ __launch_bounds__(256, (DP <= 128 || (KV == KV_E4M3 && kParts<KV, T> 
     }
     const int next = u + 128;
     if (next < u1) {
-      places(careful, next);
+      places(next);
       ask(next + 128);
       load_k();
     }
@@ -559,9 +752,8 @@ __global__ __launch_bounds__(256, (DP <= 128 || (KV == KV_E4M3 && kParts<KV, T> 
     mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
     mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
     float f = 1.f;
-    constexpr float SLACK = careful ? 0.f : kSlack;   // large values: weights of 1 at most
-    if (__ballot(mx > m + SLACK)) {
-      const float mn = mx > m + SLACK ? mx : m;
+    if (__ballot(mx > m + kSlack)) {
+      const float mn = mx > m + kSlack ? mx : m;
       f = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
       m = mn;
       l *= f;
@@ -649,7 +841,7 @@ __global__ __launch_bounds__(256, (DP <= 128 || (KV == KV_E4M3 && kParts<KV, T> 
     load_v();
   }
   };
-  pass(std::false_type{});
+  pass();
   uint32_t again;   // rows whose sums are not finite
   {
     f32x4 z = {0.f, 0.f, 0.f, 0.f};
@@ -663,50 +855,14 @@ __global__ __launch_bounds__(256, (DP <= 128 || (KV == KV_E4M3 && kParts<KV, T> 
   }
   // (expected not to be: in line this code costs a single token 0.4 us)
   if (__builtin_expect(again != 0, 0)) {
+    f32x4 o2[VD];
+    float m2, l2, le2;
+    redo_rows<KV, DP, T, 128>(g, s, sq, sp, first, u1, kvh, p0, again, &o_all[wv][0][0], o2, m2, l2, le2);
+    m = m2;
+    l = quad == 0 ? l2 : 0.f;
+    le = quad == 0 ? le2 : 0.f;
 #pragma unroll
-    for (int t = 0; t < VD; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    m = -INFINITY;
-    l = le = 0.f;
-    pass(std::true_type{});
-    // and the keys left out, four rows at a time, whose sums come through LDS
-    constexpr int R = 4, N = DP / 64;
-    float m2 = -INFINITY, l2 = 0.f;
-    bool drop = false;
-    for (uint32_t left = again; left;) {
-      int c[R], pr[R];
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        c[r] = left ? __builtin_ctz(left) : c[0];
-        left &= left - 1;
-        pr[r] = p0 + c[r];
-      }
-      float os[R][N], ms[R], ls[R];
-      bool lost[R];
-      careful_rows<KV, DP, T, 32, 128, R>(g, s, sq, sp, first, u1, kvh, pr, os, ms, ls, lost);
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) o_all[wv][c[r]][lane + 64 * i] = os[r][i];
-        if (c16 == c[r]) {
-          m2 = ms[r];
-          l2 = ls[r];
-          drop = lost[r];
-        }
-      }
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    if ((again >> c16) & 1) {
-      if (drop) m = -INFINITY;
-      const float top = fmaxf(m, m2), f = drop ? 0.f : m == top ? 1.f : __builtin_amdgcn_exp2f(m - top),
-                  f2 = m2 == top ? 1.f : __builtin_amdgcn_exp2f(m2 - top);
-      m = top;
-      l = (drop ? 0.f : l * f) + (quad == 0 ? l2 * f2 : 0.f);
-      le = (drop ? 0.f : le * f) + (quad == 0 ? l2 * f2 : 0.f);
-#pragma unroll
-      for (int t = 0; t < VD; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[t][i] = (drop ? 0.f : o[t][i] * f) + scaled(o_all[wv][c16][4 * VD * quad + VD * i + t], f2);
-    }
+    for (int t = 0; t < VD; ++t) *(f32x4*)&o_all[wv][c16][16 * t + 4 * quad] = o2[t];
   }
 
   // the four waves' parts; this lane has values 4 VD quad + VD i + t of its packed row
@@ -724,11 +880,9 @@ __global__ __launch_bounds__(256, (DP <= 128 || (KV == KV_E4M3 && kParts<KV, T> 
     const float top = fmaxf(fmaxf(m_all[0][c16], m_all[1][c16]), fmaxf(m_all[2][c16], m_all[3][c16]));
     const float f = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top);
     float* dst = &o_all[wv][c16][4 * VD * quad];
-    if (__builtin_expect(again != 0, 0)) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int t = 0; t < VD; ++t) dst[VD * i + t] = scaled(o[t][i], f);
+    if (__builtin_expect(again != 0, 0)) {   // they lie there
+#pragma unroll 1
+      for (int i = 0; i < 4 * VD; ++i) dst[i] = scaled(dst[i], f);
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -821,69 +975,48 @@ __device__ __forceinline__ uint32_t lds_at(const void* p) { return (uint32_t)(ui
 __device__ __attribute__((aligned(16))) const uint8_t kv_zeros[kKvMaxDim * 2] = {};
 __device__ const float kv_one = 1.f;
 
-// One packed row over [u0, u1) in plain f32, a value or four of the head a
-// lane: for rows whose sums are not finite, where an infinity or a NaN in V must
-// reach the rows that see its key and no others.
+// The rows of a wave of k_attn_many whose sums are not finite, 16 at a time. A
+// call, and no reference among its arguments: in line its registers are taken from
+// the main loop (prompts of 32 heads of 128 79 us for 77.5, windowed f32 turns 70.4 for 67.7).
+// gp: the kernel's arguments where they lie.
+typedef __attribute__((address_space(3))) float lds_float;
 template <int KV, int DP, class T>
-__device__ void slow_row(const KvAttnArgs& g, int s, const KvSeq& sq, const Span& sp, int u0, int u1, int kvh, int p, float scale2,
-                         float (&o)[DP / 64], float* m_out, float* l_out) {
-  constexpr int N = DP / 64;
-  const int lane = threadIdx.x & 63, D = g.kv.dim, row = sq.first + row_in(g, p), head = kvh * g.group + head_in(g, p);
-  const int pos = sq.len - sq.rows + row_in(g, p);
-  float q[N], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int d = lane + 64 * i;
-    q[i] = d < D ? (float)((const T*)g.q)[row * g.ldq + (long long)head * D + d] : 0.f;
-    o[i] = 0.f;
-  }
+__device__ __attribute__((noinline)) void redo_many(const KvAttnArgs* gp, int s, int first, int rows, int len, int lo, int a, int sink, int n, int u0, int u1, int kvh,
+                                                    int split, int pw, uint32_t again, uint32_t lds) {
+  const auto uni = [](int x) __attribute__((always_inline)) { return __builtin_amdgcn_readfirstlane(x); };
+  const uint64_t at = (uint32_t)uni((int)(uint32_t)(uintptr_t)gp) | (uint64_t)(uint32_t)uni((int)((uintptr_t)gp >> 32)) << 32;
+  const KvAttnArgs& g = *(const KvAttnArgs*)(const __attribute__((address_space(4))) KvAttnArgs*)(uintptr_t)at;
+  const KvSeq sq{uni(first), uni(rows), uni(len)};
+  const Span sp{uni(lo), uni(a), uni(sink), uni(n)};
+  s = uni(s), u0 = uni(u0), u1 = uni(u1), kvh = uni(kvh), split = uni(split), pw = uni(pw), again = uni(again), lds = uni(lds);
+  const int lane = threadIdx.x & 63, D = g.kv.dim;
+  const bool joined = sp.n > g.chunk;
 #pragma unroll 1
-  for (int u = u0; u < u1; ++u) {
-    const int key = u < sp.a ? u : sp.lo + u - sp.a;
-    if ((u < sp.a && u >= sp.sink) || key > pos || (g.window > 0 && key <= pos - g.window && key >= g.sinks)) continue;
-    KvPlace at{};
-    if (!kv_place(g.kv, s, key, &at)) continue;
-    const long long off = kv_offset(g.kv, at, kvh);
-    float k[N], v[N], ks = 1.f, vs = 1.f;
-    if constexpr (KV == KV_E4M3) {
-      ks = g.kv.k_scale[kv_scale_at(g.kv, at, kvh)];
-      vs = g.kv.v_scale[kv_scale_at(g.kv, at, kvh)];
-    }
-    float x = 0.f;
+  for (int h = 0; h < 32; h += 16) {
+    const uint32_t which = (again >> h) & 0xffffu;
+    if (which == 0) continue;
+    f32x4 o2[DP / 16];
+    float m2, l2, le2;
+    redo_rows<KV, DP, T, 32>(g, s, sq, sp, u0, u1, kvh, pw + h, which, (float*)(lds_float*)(uintptr_t)lds, o2, m2, l2, le2);
+    const int c16 = lane & 15, quad = lane >> 4, p2 = pw + h + c16;
+    if (((which >> c16) & 1) == 0) continue;
+    const int orow = sq.first + row_in(g, p2), oh = kvh * g.group + head_in(g, p2);
+    const long long to = ((long long)split * g.kv.n_rows + orow) * g.n_q + oh;
+    const float inv = l2 == 0.f ? 0.f : 1.f / l2;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int d = lane + 64 * i;
-      k[i] = v[i] = 0.f;
-      if (d < D) {
-        if constexpr (KV == KV_E4M3) {
-          k[i] = ks * __builtin_amdgcn_cvt_f32_fp8((uint32_t)((const uint8_t*)g.kv.k)[off + d], 0);
-          v[i] = vs * __builtin_amdgcn_cvt_f32_fp8((uint32_t)((const uint8_t*)g.kv.v)[off + d], 0);
-        } else {
-          typedef typename std::conditional<KV == KV_BF16, __bf16, _Float16>::type C;
-          k[i] = (float)((const C*)g.kv.k)[off + d];
-          v[i] = (float)((const C*)g.kv.v)[off + d];
-        }
-      }
-      x = fmaf(q[i], k[i], x);
-    }
-    x = gg::wave_sum(x) * scale2;
-    if (x > m) {
-      const float f = __builtin_amdgcn_exp2f(m - x);
-      m = x;
-      l *= f;
+    for (int t = 0; t < DP / 16; ++t) {
+      if (16 * t >= D) continue;
+      const int e = 16 * t + 4 * quad;
+      if (joined) *(f32x4*)(g.part_o + to * D + e) = o2[t];
 #pragma unroll
-      for (int i = 0; i < N; ++i) o[i] = scaled(o[i], f);
+      for (int i = 0; i < 4; ++i)
+        if (!joined) ((T*)g.out)[orow * g.ldo + (long long)oh * D + e + i] = (T)(o2[t][i] * inv);
     }
-    // a NaN or +inf leaves nothing of the row: e^(s - m) is a NaN with either
-    const float w = x == -INFINITY ? 0.f : x < INFINITY ? __builtin_amdgcn_exp2f(x - m) : NAN;
-    l += w;
-    // a weight that only rounds to 0 is one for an infinity, whatever it is
-    const bool some = w == 0.f && x > -INFINITY;
-#pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = fmaf(some && !(fabsf(v[i]) < INFINITY) ? 1.f : w, v[i], o[i]);
+    if (quad == 0) {
+      if (joined) *(f32x4*)(g.part_ml + 4 * to) = f32x4{m2, l2, le2, 0.f};
+      else if (g.lse) g.lse[(long long)orow * g.n_q + oh] = lse_of<KV>(m2, le2);
+    }
   }
-  *m_out = m;
-  *l_out = l;
 }
 
 template <int KV, int DP, class T>
@@ -925,7 +1058,8 @@ __global__ __launch_bounds__(256, (kParts<KV, T> > 1 || DP > 128 ? 1 : 2)) void 
   if (split > 0 && u0 >= sp.n) return;
   const bool joined = sp.n > g.chunk;
   const int before = sq.len - sq.rows;
-  const int pw = p0 + 32 * wv, p = pw + c32, row = sq.first + row_in(g, p), head = kvh * g.group + head_in(g, p);
+  const int pw = p0 + 32 * wv;
+  int p = pw + c32;
   const int pos = p < packed ? before + row_in(g, p) : -1;
   const bool active = pw < packed;   // this wave has rows
   const int pos_min = before + row_in(g, pw), pos_max = before + min(row_in(g, pw + 31), sq.rows - 1);
@@ -935,7 +1069,7 @@ __global__ __launch_bounds__(256, (kParts<KV, T> > 1 || DP > 128 ? 1 : 2)) void 
   const float scale2 = g.scale2 == 0.f ? 1.f : fabsf(g.scale2), sign = g.scale2 > 0.f ? 1.f : g.scale2 < 0.f ? -1.f : 0.f;
   u32x4 qb[NP][CH];
   {
-    const T* q = (const T*)g.q + (p < packed ? row * g.ldq + (long long)head * D : 0);
+    const T* q = (const T*)g.q + (p < packed ? (sq.first + row_in(g, p)) * g.ldq + (long long)(kvh * g.group + head_in(g, p)) * D : 0);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int d = 16 * c + 8 * half;
@@ -1224,6 +1358,8 @@ __global__ __launch_bounds__(256, (kParts<KV, T> > 1 || DP > 128 ? 1 : 2)) void 
   }
   if (!active) return;
 
+  asm volatile("" : "+v"(p));   // what follows from it is worked out here: it need not be kept in the loop
+  const int row = sq.first + row_in(g, p), head = kvh * g.group + head_in(g, p);
   l += __shfl_xor(l, 32, 64);
   le += __shfl_xor(le, 32, 64);
   if constexpr (NP > 1) l = le;
@@ -1261,26 +1397,11 @@ __global__ __launch_bounds__(256, (kParts<KV, T> > 1 || DP > 128 ? 1 : 2)) void 
       else if (g.lse) g.lse[(long long)row * g.n_q + head] = lse_of<KV>(m, le);
     }
   }
-  // rows that need care, one at a time
-  for (uint32_t left = (uint32_t)again; left; left &= left - 1) {
-    const int pr = pw + __builtin_ctz(left), orow = sq.first + row_in(g, pr), oh = kvh * g.group + head_in(g, pr);
-    float os[DP / 64], ms, ls;
-    slow_row<KV, DP, T>(g, s, sq, sp, u0, u1, kvh, pr, g.scale2, os, &ms, &ls);
-    const long long to = ((long long)split * g.kv.n_rows + orow) * g.n_q + oh;
-    const float inv = ls == 0.f ? 0.f : 1.f / ls;
-#pragma unroll
-    for (int i = 0; i < DP / 64; ++i) {
-      const int e = lane + 64 * i;
-      if (e >= D) continue;
-      if (joined) g.part_o[to * D + e] = scaled(os[i], exp2f(kShift<KV>));
-      else ((T*)g.out)[orow * g.ldo + (long long)oh * D + e] = (T)scaled(os[i], inv);
-    }
-    if (lane == 0) {
-      const float c = exp2f(kShift<KV>);   // the chunks' sums have it
-      if (joined) *(f32x4*)(g.part_ml + 4 * to) = f32x4{ms, ls * c, ls * c, 0.f};
-      else if (g.lse) g.lse[(long long)orow * g.n_q + oh] = lse_of<KV>(ms, ls * c);
-    }
-  }
+  // the others; K's stages, which nobody reads any more, have a place for each wave
+  static_assert(sizeof(kbuf) >= 4 * 4 * DP * sizeof(float), "four rows for each of four waves");
+  if (__builtin_expect(again != 0, 0))
+    redo_many<KV, DP, T>((const KvAttnArgs*)__builtin_amdgcn_kernarg_segment_ptr(), s, sq.first, sq.rows, sq.len, sp.lo, sp.a, sp.sink, sp.n, u0, u1, kvh, split, pw, again,
+                         lds_at(&kbuf[0][0]) + wv * 16 * DP);
 }
 
 // Joins the chunks of tiles that have several: W waves for a row's head, L lanes
