@@ -464,7 +464,8 @@ int gg_kv_attention(const gg_kv_pages* pages, const gg_kv_seqs* seqs, const void
  *   draft from p: the least id whose sum of weights up to it exceeds
  *   draw_u[s] times the sum of all;
  * temperature 0: a draft stands while it is the largest logit's id (the lowest
- * among equals), and the token is that id. Random numbers in [0, 1).
+ * among equals), and the token is that id. Any temperature above 0, infinity
+ * too; one below 2^-126 counts as that. Random numbers in [0, 1).
  *   accepted[s]   drafts that stand
  *   tokens[rows]  they, the token behind them, then -1 up to the sequence's end
  *   logprobs[rows]  ln p of each of those tokens (temperature 0: of softmax z), 0 behind them; may be NULL

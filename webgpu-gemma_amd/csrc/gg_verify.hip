@@ -100,8 +100,10 @@ __device__ __forceinline__ double exp2_below(double x) {
 }
 constexpr double kLog2e64 = 1.44269504088896340736;
 
-// Temperature of a sequence; 0 (or what is none): greedy.
+// Temperature of a sequence; 0 (or what is none): greedy. Below 2^-126 its inverse
+// is no f32 number.
 __device__ __forceinline__ bool greedy(float t) { return !(t > 0.f); }
+__device__ __forceinline__ float heat_of(float t) { return greedy(t) ? 1.f : fmaxf(t, 0x1p-126f); }
 
 // One block: part blockIdx % parts of a row of z, or of y behind all of z's.
 template <class T, int EPT>
@@ -118,7 +120,10 @@ __global__ __launch_bounds__(256) void k_verify_stat(VerifyArgs a) {
   const int end = a.row_start[s + 1];
   const float t = a.temperature[s];
   if (row >= end || (draft && (row == end - 1 || greedy(t)))) return;   // no row of y
-  const float c = greedy(t) ? kLog2e : kLog2e / t;
+  // exponents (z - m) log2(e) / T as (z h - m h) c: from T = 2^64 on h keeps the
+  // difference of large logits, and c, in range (infinite T: 2^-126, which makes
+  // every finite logit's weight 1 and leaves -inf what it is)
+  const float heat = heat_of(t), h = heat >= 0x1p64f ? 0x1p-64f : 1.f, c = fmaxf(kLog2e / (heat * h), 0x1p-126f);
   const T* z = draft ? (const T*)a.y + row * a.ldy : (const T*)a.z + row * a.ldz;
   const int shift = (int)(((uintptr_t)z & 15) / sizeof(T));
   const T* z0 = z - shift;
@@ -161,7 +166,7 @@ __global__ __launch_bounds__(256) void k_verify_stat(VerifyArgs a) {
   const float ref = m == -INFINITY ? 0.f : m;
   float sum[4] = {};
 #pragma unroll
-  for (int i = 0; i < EPT; ++i) sum[i & 3] += __builtin_amdgcn_exp2f((v[i] - ref) * c);
+  for (int i = 0; i < EPT; ++i) sum[i & 3] += __builtin_amdgcn_exp2f(fmaf(v[i], h, -ref * h) * c);
   const double total = wave_sum((double)((sum[0] + sum[1]) + (sum[2] + sum[3])));
   const int any = __ballot(bad) != 0;
   if (lane == 0) {
@@ -225,7 +230,7 @@ __device__ Decision decide(const VerifyArgs& a, int s, bool write) {
   d.end = (int)min(max((long long)a.row_start[s + 1], 0ll), a.rows);
   const float t = a.temperature[s];
   d.greedy = greedy(t);
-  const double heat = d.greedy ? 1.0 : (double)t, c = kLog2e64 / heat;
+  const double heat = (double)heat_of(t), c = kLog2e64 / heat;
   d.stop.row = -1;
   for (int r0 = d.first; r0 < d.end; r0 += 4) {
     const int row = r0 + wv;
@@ -304,7 +309,8 @@ __device__ __forceinline__ void load_some(const T* row, long long e0, int n, flo
     for (int i = 0; i < N; ++i) v[i] = e0 + i < n ? (float)row[e0 + i] : -INFINITY;
   }
 }
-// e^((z - m) / T), c = log2(e) / T.
+// e^((z - m) / T), c = log2(e) / T. (With an infinite T a logit of -inf gives 0 times
+// infinity, a NaN, in whose place exp2_below's fmax takes its bound.)
 __device__ __forceinline__ double weight(float z, float m, double c) { return exp2_below(((double)z - (double)m) * c); }
 
 // Where sequence s stops; the block with `write` reports it and what lies
@@ -345,7 +351,7 @@ __global__ __launch_bounds__(256) void k_verify_sums(VerifyArgs a) {
   if constexpr (FIND) st = settle<T>(a, s, tile == 0);
   else st = a.stop[s];
   if (st.row < 0 || st.draw == 0) return;
-  const double inv_heat = kLog2e64 / (double)a.temperature[s];
+  const double inv_heat = kLog2e64 / (double)heat_of(a.temperature[s]);
   const long long e0 = (long long)tile * kVerifyTile + 16 * tid;
   const bool both = st.draw == 3;
   const int skip = st.draw == 2 ? a.draft[st.row] : -1;
@@ -476,7 +482,7 @@ __global__ __launch_bounds__(kDrawThreads) void k_verify_draw(VerifyArgs a, int 
   }
   const int tile = hit < a.tiles ? hit : max(last, 0);
   const double within = rest;
-  const double inv_heat = kLog2e64 / (double)a.temperature[s];
+  const double inv_heat = kLog2e64 / (double)heat_of(a.temperature[s]);
   const long long e0 = (long long)tile * kVerifyTile + kDrawEach * tid;
   const int skip = st.draw == 2 && !plain ? a.draft[st.row] : -1;
   double w[kDrawEach];
@@ -518,7 +524,7 @@ __global__ __launch_bounds__(kDrawThreads) void k_verify_draw(VerifyArgs a, int 
     const int token = hit != 0x7fffffff ? hit : max(last, 0);
     a.tokens[st.row] = token;
     if (a.logprobs)
-      a.logprobs[st.row] = (float)(((double)(float)((const T*)a.z)[st.row * a.ldz + token] - (double)st.mp) / (double)a.temperature[s] - log(p_sum));
+      a.logprobs[st.row] = (float)(((double)(float)((const T*)a.z)[st.row * a.ldz + token] - (double)st.mp) / (double)heat_of(a.temperature[s]) - log(p_sum));
   }
 }
 
