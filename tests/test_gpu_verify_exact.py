@@ -1,6 +1,8 @@
-"""Verification of drafted tokens at the ends of the range of temperatures."""
+"""Verification of drafted tokens where decisions are close: next to the border
+of acceptance, and at the ends of the range of temperatures."""
 import numpy as np
 import pytest
+import torch
 
 from gpu_util import say
 from kv_ref import verify
@@ -14,6 +16,32 @@ def soft(z, heat):
     with np.errstate(over="ignore"):
         w = np.where(np.isneginf(z), 0.0, np.exp((np.where(np.isneginf(z), 0.0, z) - z.max()) / heat))
     return w / w.sum()
+
+
+@pytest.mark.parametrize("with_y", [True, False])
+@pytest.mark.parametrize("n,seqs", [(1000, 40), (50257, 24), (262144, 8), (262144, 40)])
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+def test_drafts_next_to_the_border(gpu, name, n, seqs, with_y):
+    """u q(d) is p(d) but for one part in 10^10: f64 sums of some 10^5 weights are off by 10^-13 of it at most, f32 ones by 10^-7."""
+    say("border", name, n, seqs, with_y)
+    rng = np.random.default_rng(n + seqs)
+    z = rng.standard_normal((2 * seqs, n)) * 3
+    y = z + rng.standard_normal((2 * seqs, n))
+    z, y = (torch.from_numpy(t).to(dict(f32=torch.float32, bf16=torch.bfloat16)[name]).double().numpy() for t in (z, y))
+    heat = rng.choice([0.5, 1.0, 1.7], seqs).astype(np.float32)
+    draft, u = np.zeros(2 * seqs, int), np.zeros(2 * seqs)
+    stands = np.arange(seqs) % 2 == 0
+    for s in range(seqs):
+        p, q = soft(z[2 * s], float(heat[s])), soft(y[2 * s], float(heat[s]))
+        d = int(np.argmax(np.where(p < q, p, 0))) if with_y else int(rng.choice(n, p=p))
+        draft[2 * s] = d
+        u[2 * s] = p[d] / (q[d] if with_y else 1.0) * (1 - 1e-10 if stands[s] else 1 + 1e-10)
+    start = np.arange(0, 2 * seqs + 1, 2)
+    v = rng.random(seqs)
+    acc, tok, lp, _, _ = run(z, y if with_y else None, draft, start, heat, u, v, name)
+    assert np.array_equal(acc, stands.astype(int))
+    ra, rt, rl, margin = verify(z, y if with_y else None, draft, start, heat, u, v)
+    assert (margin > 1e-11).all() and np.array_equal(tok, rt)
 
 
 @pytest.mark.parametrize("with_y", [True, False])

@@ -716,7 +716,7 @@ struct VerifyArgs {
   int32_t *accepted, *tokens;
   float* logprobs;
   int parts;             // parts of a row
-  int per;               // 16-byte units of one, 256 threads each
+  double near;           // how far the first launch's sums may be off, relative
   VerifyPart* part;      // [z, y][rows][parts]
   int tiles;
   VerifyStop* stop;      // [n_seqs]
@@ -729,6 +729,14 @@ inline bool verify_short(long long rows, int n) { return rows * ((n + 256LL * kV
 inline int verify_parts(long long rows, int n) {
   const int tile = 256 * (verify_short(rows, n) ? kVerifyShort : kVerifyLong);
   return (int)(((long long)n + 7 + tile - 1) / tile);   // a row may begin up to 7 elements into its first 16 bytes
+}
+// How far a row's sum of f32 weights may be off, relative: an exponent of -x is off by
+// 2^-22 of it (four roundings), so its weight by 0.7 x 2^-22, and the mean of x over the weights is log2(n)
+// at most; 2^-23 for an exponential, 10 roundings of a sum of 32. With y a product of two sums is compared.
+inline double verify_near(int n, bool y) {
+  double bits = 0;
+  while ((1ll << (int)bits) < n) ++bits;
+  return (y ? 2 : 1) * (0.7 * bits + 4) / (1 << 22);
 }
 inline int verify_tiles(int n) { return (n + kVerifyTile - 1) / kVerifyTile; }
 int launch_verify(int elem, const VerifyArgs& a, void* stream);

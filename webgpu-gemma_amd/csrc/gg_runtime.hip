@@ -2146,6 +2146,7 @@ int gg_verify_drafts(const void* z, const void* y, uint32_t type, int64_t rows, 
   a.logprobs = logprobs;
   a.parts = verify_parts(rows, n);
   a.tiles = verify_tiles(n);
+  a.near = verify_near(n, y != nullptr);
   a.part = (VerifyPart*)workspace;
   a.sums = (double*)(a.part + 2 * (size_t)rows * a.parts);
   a.stop = (VerifyStop*)(a.sums + 4 * (size_t)n_seqs * a.tiles);

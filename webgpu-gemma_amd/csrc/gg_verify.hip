@@ -15,8 +15,12 @@
 //
 // The draw picks among borders that lie closer than f32 tells apart: with f32
 // sums one draw in a hundred over 262144 logits gives a neighbour of the
-// right token. So all that a draw compares is f64. Whether p exceeds q at a token is taken from
-// the sums of the first launch (2^-22 off): that changes the sum over them in the
+// right token. So all that a draw compares is f64. So is whether a draft stands: the
+// sums of the first launch say so but where u q(d) and p(d) lie closer than they
+// can be off (VerifyArgs::near, some 2^-18 of p(d)), and there, at one draft in 10^5,
+// both sums are taken again in f64 (0.4 ms for rows of 262144).
+// Whether p exceeds q at a token is taken from
+// the sums of the first launch: that changes the sum over them in the
 // second order only, and their scale is put right afterwards, since
 // sum (p - q) over a set = sum p - c sum q with any c.
 #include "gg_kv_device.h"
@@ -218,6 +222,42 @@ struct Decision {
   bool greedy;
 };
 
+// N logits from e0 on, -inf behind the row.
+template <class T, int N>
+__device__ __forceinline__ void load_some(const T* row, long long e0, int n, float (&v)[N]) {
+  constexpr int VE = 16 / sizeof(T) < N ? 16 / sizeof(T) : N;
+  typedef T vec_t __attribute__((ext_vector_type(VE)));
+  if (e0 + N <= n && ((uintptr_t)(row + e0) & (VE * sizeof(T) - 1)) == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += VE) {
+      const vec_t x = *(const vec_t*)(row + e0 + i);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) v[i + e] = (float)x[e];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = e0 + i < n ? (float)row[e0 + i] : -INFINITY;
+  }
+}
+// e^((z - m) / T), c = log2(e) / T. (With an infinite T a logit of -inf gives 0 times
+// infinity, a NaN, in whose place exp2_below's fmax takes its bound.)
+__device__ __forceinline__ double weight(float z, float m, double c) { return exp2_below(((double)z - (double)m) * c); }
+
+// The sum of a row's weights, every logit's in f64, by a wave.
+template <class T>
+__device__ __forceinline__ double row_sum(const T* row, int n, float m, double c) {
+  const int lane = threadIdx.x & 63;
+  double sum = 0;
+#pragma unroll 1
+  for (long long e0 = 8 * lane; e0 < n; e0 += 512) {
+    float z[8];
+    load_some(row, e0, n, z);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += weight(z[i], m, c);
+  }
+  return wave_sum(sum);
+}
+
 // Where sequence s stops: four rows at a time, one a wave, up to the first that
 // stops. The block with `write` also reports the rows before.
 template <class T>
@@ -236,7 +276,7 @@ __device__ Decision decide(const VerifyArgs& a, int s, bool write) {
     const int row = r0 + wv;
     if (row < d.end) {
       const bool last = row == d.end - 1;
-      const Row p = join_parts(a.part + (long long)row * a.parts, a.parts, c, d.greedy);
+      Row p = join_parts(a.part + (long long)row * a.parts, a.parts, c, d.greedy);
       const int id = last ? -1 : a.draft[row];
       const bool real = id >= 0 && id < a.n;
       VerifyStop st{row, 0, p.m, 0.f, p.sum, 0.0};
@@ -255,7 +295,18 @@ __device__ Decision decide(const VerifyArgs& a, int s, bool write) {
           st.sq = y.sum;
           q = real ? exp2_below(((double)(float)((const T*)a.y)[row * a.ldy + id] - y.m) * c) / y.sum : 0.0;
         }
-        const bool stands = real && !last && a.accept_u[row] * q * p.sum < exp2_below((z_id - p.m) * c);
+        const double u = real && !last ? a.accept_u[row] : 0.0, w = exp2_below((z_id - p.m) * c);
+        bool stands = real && !last && u * q * p.sum < w;
+        // closer than f32 exponentials tell: with both sums again
+        if (__builtin_expect(real && !last && !bad && w > 0.0 && fabs(u * q * p.sum - w) <= a.near * w, 0)) {
+          st.sp = p.sum = row_sum((const T*)a.z + row * a.ldz, a.n, p.m, c);
+          if (a.y) {
+            q *= st.sq;
+            st.sq = row_sum((const T*)a.y + row * a.ldy, a.n, st.mq, c);
+            q /= st.sq;
+          }
+          stands = u * q * p.sum < w;
+        }
         halt |= !stands;
         if (halt) st.draw = last ? 1 : a.y ? 3 : 2;
       }
@@ -291,27 +342,6 @@ __device__ Decision decide(const VerifyArgs& a, int s, bool write) {
   }
   return d;
 }
-
-// N logits from e0 on, -inf behind the row.
-template <class T, int N>
-__device__ __forceinline__ void load_some(const T* row, long long e0, int n, float (&v)[N]) {
-  constexpr int VE = 16 / sizeof(T) < N ? 16 / sizeof(T) : N;
-  typedef T vec_t __attribute__((ext_vector_type(VE)));
-  if (e0 + N <= n && ((uintptr_t)(row + e0) & (VE * sizeof(T) - 1)) == 0) {
-#pragma unroll
-    for (int i = 0; i < N; i += VE) {
-      const vec_t x = *(const vec_t*)(row + e0 + i);
-#pragma unroll
-      for (int e = 0; e < VE; ++e) v[i + e] = (float)x[e];
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = e0 + i < n ? (float)row[e0 + i] : -INFINITY;
-  }
-}
-// e^((z - m) / T), c = log2(e) / T. (With an infinite T a logit of -inf gives 0 times
-// infinity, a NaN, in whose place exp2_below's fmax takes its bound.)
-__device__ __forceinline__ double weight(float z, float m, double c) { return exp2_below(((double)z - (double)m) * c); }
 
 // Where sequence s stops; the block with `write` reports it and what lies
 // before and behind.
