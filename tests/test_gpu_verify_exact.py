@@ -1,5 +1,6 @@
 """Verification of drafted tokens where decisions are close: next to the border
-of acceptance, and at the ends of the range of temperatures."""
+of acceptance, draws from a draft model's row next to the target's, and the
+ends of the range of temperatures."""
 import numpy as np
 import pytest
 import torch
@@ -42,6 +43,78 @@ def test_drafts_next_to_the_border(gpu, name, n, seqs, with_y):
     assert np.array_equal(acc, stands.astype(int))
     ra, rt, rl, margin = verify(z, y if with_y else None, draft, start, heat, u, v)
     assert (margin > 1e-11).all() and np.array_equal(tok, rt)
+
+
+@pytest.mark.parametrize("n", [4096, 50000, 262144])
+def test_a_draft_model_next_to_the_target(gpu, n):
+    """The target is the draft model's row but for two tokens: d's probability is gone and a rises by a part of it. All others then
+    have p above q by the rest, some 10^-9 of their own: less than f32 sums tell, and half of what the draw is from."""
+    seqs = 64
+    rng = np.random.default_rng(n)
+    y = (rng.standard_normal((2 * seqs, n))).astype(np.float32)
+    z = y.copy()
+    d, a = n // 3, n // 2
+    for s in range(seqs):
+        r = 2 * s
+        w = np.exp(y[r].astype(np.float64) - y[r].max())
+        small = 2.0 ** -28 * w.sum()
+        y[r, d] = np.float32(np.log(2 * small) + y[r].max())
+        z[r] = y[r]
+        z[r, d] = -np.inf
+        z[r, a] = np.float32(np.log(np.exp(np.float64(y[r, a]) - y[r].max()) + small) + y[r].max())
+    draft = np.full(2 * seqs, d)
+    start = np.arange(0, 2 * seqs + 1, 2)
+    u, v, heat = np.full(2 * seqs, 0.5), (np.arange(seqs) + 0.5) / seqs, np.ones(seqs, np.float32)
+    z64, y64 = z.astype(np.float64), y.astype(np.float64)
+    p, q = soft(z64[0], 1.0), soft(y64[0], 1.0)
+    rest = np.maximum(p - q, 0)
+    assert 0.2 < rest[a] / rest.sum() < 0.8 and (rest > 0).sum() > n // 2     # that is what the inputs are
+    acc, tok, lp, _, _ = run(z64, y64, draft, start, heat, u, v)
+    ra, rt, rl, margin = verify(z64, y64, draft, start, heat, u, v)
+    assert (acc == 0).all()
+    # p - q is 2^-28 of either, in f64 off by 2^-50 of them: borders within 10^-6 of the whole may fall either way
+    clear = margin > 1e-6
+    say("next to the target", n, int(clear.sum()))
+    for s in range(seqs):
+        res = np.maximum(soft(z64[2 * s], 1.0) - soft(y64[2 * s], 1.0), 0)
+        c = np.cumsum(res)
+        lo, hi = (int(np.searchsorted(c, (v[s] + e) * c[-1], side="right")) for e in (-1e-6, 1e-6))
+        assert lo <= tok[2 * s] <= hi and res[tok[2 * s]] > 0, (s, tok[2 * s], rt[2 * s], lo, hi)
+        assert tok[2 * s + 1] == -1
+
+
+@pytest.mark.parametrize("heat", [1.0, 0.7])
+@pytest.mark.parametrize("n", [7, 37, 500, 5000, 70000])
+def test_a_draft_model_that_differs_by_roundings(gpu, n, heat):
+    """y is z but for the last bits of some logits, and the draft has no probability under either: p - q is some 2^-24 of them, about what
+    f32 sums are off by, and which tokens have any of it is decided by that."""
+    say("roundings", n, heat)
+    seqs = 64
+    rng = np.random.default_rng(n)
+    z = (rng.standard_normal((2 * seqs, n)) * 2).astype(np.float32)
+    if n > 7:
+        z[:, rng.random(n) < 0.3] = -np.inf
+    z[:, 0] = -np.inf
+    z[:, n - 1] = 0.5
+    y = z.copy()
+    change = rng.random(y.shape) < 0.4
+    y[change] = np.nextafter(y[change], np.where(rng.random(change.sum()) < 0.5, np.float32(10), np.float32(-10)))
+    y[:, 0] = -np.inf
+    y[:, n - 1] = np.nextafter(np.float32(0.5), np.float32(1))
+    start = np.arange(0, 2 * seqs + 1, 2)
+    T = float(np.float32(heat))
+    v = rng.random(seqs)
+    z64, y64 = z.astype(np.float64), y.astype(np.float64)
+    acc, tok, lp, _, _ = run(z64, y64, np.zeros(2 * seqs, int), start, np.full(seqs, T), np.full(2 * seqs, 0.5), v)
+    assert (acc == 0).all()
+    for s in range(seqs):
+        r, t = 2 * s, tok[2 * s]
+        assert np.isfinite(z[r, t]) and np.isfinite(lp[r])
+        res = np.maximum(soft(z64[r], T) - soft(y64[r], T), 0)
+        c = np.cumsum(res)
+        # f64 leaves 2^-50 of p and q: 2^-22 of what is left, in all of its tokens at once
+        lo, hi = (int(np.searchsorted(c, (v[s] + e) * c[-1], side="right")) for e in (-2e-6, 2e-6))
+        assert lo <= t <= min(hi, n - 1) and res[t] > 0, (s, t, lo, hi, res[t] / c[-1])
 
 
 @pytest.mark.parametrize("with_y", [True, False])

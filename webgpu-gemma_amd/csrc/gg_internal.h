@@ -706,6 +706,7 @@ struct VerifyStop {
   double sp, sq;         // sums, as the parts give them
 };
 constexpr int kVerifyTile = 4096;   // logits of a block of the 64-bit sums
+constexpr int kVerifySums = 5;      // of a tile: p and q where p is the larger, all p, all q, p where f32 sums cannot tell which is
 struct VerifyArgs {
   const void *z, *y;
   long long ldz, ldy, rows;
@@ -720,7 +721,7 @@ struct VerifyArgs {
   VerifyPart* part;      // [z, y][rows][parts]
   int tiles;
   VerifyStop* stop;      // [n_seqs]
-  double* sums;          // [n_seqs][tiles][4]: p, q where p is the larger; p, q
+  double* sums;          // [n_seqs][tiles][kVerifySums]
   long long block0;
 };
 // 32 logits a thread, or 8 where that leaves CUs without work.

@@ -2113,7 +2113,7 @@ int gg_kv_attention(const gg_kv_pages* pages, const gg_kv_seqs* seqs, const void
 
 size_t gg_verify_drafts_workspace_size(int64_t rows, int32_t n_seqs, int32_t n) {
   if (rows <= 0 || rows > (1LL << 30) || !count_ok(n) || n_seqs <= 0 || n_seqs > (1 << 22)) return 0;
-  return (size_t)rows * 2 * verify_parts(rows, n) * sizeof(VerifyPart) + (size_t)n_seqs * verify_tiles(n) * 32 +
+  return (size_t)rows * 2 * verify_parts(rows, n) * sizeof(VerifyPart) + (size_t)n_seqs * verify_tiles(n) * kVerifySums * sizeof(double) +
          (size_t)n_seqs * sizeof(VerifyStop);
 }
 
@@ -2149,7 +2149,7 @@ int gg_verify_drafts(const void* z, const void* y, uint32_t type, int64_t rows, 
   a.near = verify_near(n, y != nullptr);
   a.part = (VerifyPart*)workspace;
   a.sums = (double*)(a.part + 2 * (size_t)rows * a.parts);
-  a.stop = (VerifyStop*)(a.sums + 4 * (size_t)n_seqs * a.tiles);
+  a.stop = (VerifyStop*)(a.sums + kVerifySums * (size_t)n_seqs * a.tiles);
   return launch_verify(e, a, stream) ? GG_ERR_HIP : GG_OK;
 }
 

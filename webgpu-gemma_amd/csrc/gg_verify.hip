@@ -11,7 +11,7 @@
 // k_verify_draw finds the tile and the token that the draw falls on.
 // Measured, 262144 logits: one sequence, 5 rows of f32: 3.8, 8.0 and 7.0 us, each little
 // more than its chain of reads and reductions; 48 sequences, 7 rows each of both
-// models, bf16: 36.7 us (4.9 TB/s), 8.9, 21.6 (exponentials in f64) and 8.3.
+// models, bf16: 36.8 us (4.9 TB/s), 9.1, 22.6 (exponentials in f64) and 9.0.
 //
 // The draw picks among borders that lie closer than f32 tells apart: with f32
 // sums one draw in a hundred over 262144 logits gives a neighbour of the
@@ -22,7 +22,9 @@
 // Whether p exceeds q at a token is taken from
 // the sums of the first launch: that changes the sum over them in the
 // second order only, and their scale is put right afterwards, since
-// sum (p - q) over a set = sum p - c sum q with any c.
+// sum (p - q) over a set = sum p - c sum q with any c. Where p and q lie so close
+// together that it changes more than 2^-34 of it, k_verify_draw takes the
+// tiles concerned again (0.1 ms for rows of 262144).
 #include "gg_kv_device.h"
 
 namespace gg {
@@ -385,7 +387,11 @@ __global__ __launch_bounds__(256) void k_verify_sums(VerifyArgs a) {
   const long long e0 = (long long)tile * kVerifyTile + 16 * tid;
   const bool both = st.draw == 3;
   const int skip = st.draw == 2 ? a.draft[st.row] : -1;
-  double sum[4] = {};
+  double sum[kVerifySums] = {};
+  // two numbers no further apart than a.near have upper halves, 20 bits of the
+  // mantissa, no further apart than this
+  const uint32_t near = (uint32_t)(a.near * (1 << 21)) + 2;
+  bool close = false;
   if (e0 < a.n) {
     float z[16], y[16];
     load_some((const T*)a.z + st.row * a.ldz, e0, a.n, z);
@@ -397,23 +403,27 @@ __global__ __launch_bounds__(256) void k_verify_sums(VerifyArgs a) {
       if (both) {
         const double q = weight(y[i], st.mq, inv_heat);
         sum[3] += q;
-        if (p * st.sq > q * st.sp) {
+        const double ps = p * st.sq, qs = q * st.sp;
+        if (ps > qs) {
           sum[0] += p;
           sum[1] += q;
         }
+        close |= (uint32_t)(__double2hiint(ps) - __double2hiint(qs) + near) <= 2 * near;
       } else if (e0 + i != skip) {
         sum[0] += p;
       }
     }
   }
-  __shared__ double part[4][4];
+  if (close) sum[4] = sum[2];   // all of a thread's p
+  __shared__ double part[4][kVerifySums];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const double x = wave_sum(sum[k]);
+  for (int k = 0; k < kVerifySums; ++k) {
+    if (k % 2 == 1 && !both) continue;   // no q
+    const double x = k == 4 && __ballot(close) == 0 ? 0.0 : wave_sum(sum[k]);
     if (lane == 0) part[tid >> 6][k] = x;
   }
   __syncthreads();
-  if (tid < 4) a.sums[(at * 4) + tid] = (part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid]);
+  if (tid < kVerifySums && (both || tid % 2 == 0)) a.sums[at * kVerifySums + tid] = (part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid]);
 }
 
 constexpr int kDrawThreads = 1024, kDrawWaves = kDrawThreads / 64, kDrawEach = kVerifyTile / kDrawThreads;
@@ -434,48 +444,86 @@ __device__ double block_scan(double v, double* sh, double* total) {
   *total = all;
   return before + x;
 }
-// Sums of two values over the block, in every thread.
-__device__ void block_sums(double& x, double& y, double* sh) {
+// Sums of N values over the block, in every thread. sh: N * kDrawWaves.
+template <int N>
+__device__ void block_sums(double (&x)[N], double* sh) {
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-  x = wave_sum(x);
-  y = wave_sum(y);
-  if (lane == 0) {
-    sh[wv] = x;
-    sh[kDrawWaves + wv] = y;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const double t = k == 2 && __ballot(x[k] != 0.0) == 0 ? 0.0 : wave_sum(x[k]);   // most often 0
+    if (lane == 0) sh[k * kDrawWaves + wv] = t;
   }
   __syncthreads();
-  x = y = 0;
 #pragma unroll
-  for (int i = 0; i < kDrawWaves; ++i) {
-    x += sh[i];
-    y += sh[kDrawWaves + i];
+  for (int k = 0; k < N; ++k) {
+    x[k] = 0;
+#pragma unroll
+    for (int i = 0; i < kDrawWaves; ++i) x[k] += sh[k * kDrawWaves + i];
   }
 }
 
 // One block per sequence: the token that the draw falls on.
 template <class T>
 __global__ __launch_bounds__(kDrawThreads) void k_verify_draw(VerifyArgs a, int seq0) {
-  __shared__ double sh[2 * kDrawWaves];
-  __shared__ int hit, last;
+  __shared__ double sh[3 * kDrawWaves];
+  __shared__ int hit, last, last_p;
   __shared__ double rest;
   const int tid = threadIdx.x, s = seq0 + blockIdx.x;
   const VerifyStop st = a.stop[s];
   if (st.row < 0 || st.draw == 0) return;
-  const double* sums = a.sums + (long long)s * a.tiles * 4;
+  double* sums = a.sums + (long long)s * a.tiles * kVerifySums;
+  const double inv_heat = kLog2e64 / (double)heat_of(a.temperature[s]);
   const int per = (a.tiles + kDrawThreads - 1) / kDrawThreads, t0 = min(tid * per, a.tiles), t1 = min(t0 + per, a.tiles);
   // the sums of all p and q first: their quotient scales q
-  double p_all = 0, q_all = 0;
-  for (int t = t0; t < t1; ++t) {
-    p_all += sums[4 * t + 2];
-    q_all += sums[4 * t + 3];
+  const bool both = st.draw == 3;
+  double p_all = 0, p_sum, c = 0, close = 0;
+  for (int t = t0; t < t1; ++t) p_all += sums[kVerifySums * t + 2];
+  if (both) {
+    double totals[3] = {p_all, 0, 0};
+    for (int t = t0; t < t1; ++t) {
+      totals[1] += sums[kVerifySums * t + 3];
+      totals[2] += sums[kVerifySums * t + 4];
+    }
+    block_sums(totals, sh);
+    p_sum = totals[0];
+    c = p_sum / totals[1];
+    close = totals[2];
+  } else {
+    double totals[1] = {p_all};
+    block_sums(totals, sh);
+    p_sum = totals[0];
   }
-  double p_sum = p_all, q_sum = q_all, all;
-  block_sums(p_sum, q_sum, sh);
-  const double c = st.draw == 3 ? p_sum / q_sum : 0.0;
-  double mine = 0;
-  auto tile_weight = [&](int t) { return fmax(sums[4 * t] - c * sums[4 * t + 1], 0.0); };
+  double mine = 0, all;
+  auto tile_weight = [&](int t) { return both ? fmax(sums[kVerifySums * t] - c * sums[kVerifySums * t + 1], 0.0) : sums[kVerifySums * t]; };
   for (int t = t0; t < t1; ++t) mine += tile_weight(t);
   double up_to = block_scan(mine, sh, &all);
+  if (both) {
+    // tokens with p / q between the first launch's quotient and c are on the wrong
+    // side: they lie within `near` of it, and each is off by this much of p at most
+    const double off = fabs(c * st.sq - st.sp);   // times sp
+    if (off * close > 0x1p-34 * all * st.sp) {   // a draft model next to the target: these tiles again
+      for (int t = 0; t < a.tiles; ++t) {
+        if (sums[kVerifySums * t + 4] == 0.0) continue;
+        const long long e0 = (long long)t * kVerifyTile + kDrawEach * tid;
+        float z[kDrawEach], y[kDrawEach];
+        load_some((const T*)a.z + st.row * a.ldz, e0, a.n, z);
+        load_some((const T*)a.y + st.row * a.ldy, e0, a.n, y);
+        double w[1] = {};
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kDrawEach; ++i) w[0] += fmax(weight(z[i], st.mp, inv_heat) - c * weight(y[i], st.mq, inv_heat), 0.0);
+        block_sums(w, sh);
+        if (tid == 0) {
+          sums[kVerifySums * t] = w[0];
+          sums[kVerifySums * t + 1] = 0;
+        }
+      }
+      __syncthreads();
+      mine = 0;
+      for (int t = t0; t < t1; ++t) mine += tile_weight(t);
+      up_to = block_scan(mine, sh, &all);
+    }
+  }
   const bool plain = st.draw == 1 || !(all > 0.0);   // nothing left: from p
   if (plain) {
     mine = p_all;
@@ -493,7 +541,7 @@ __global__ __launch_bounds__(kDrawThreads) void k_verify_draw(VerifyArgs a, int 
     int first = a.tiles, some = -1;
     double before = 0;
     for (int t = t0; t < t1; ++t) {
-      const double w = plain ? sums[4 * t + 2] : tile_weight(t);
+      const double w = plain ? sums[kVerifySums * t + 2] : tile_weight(t);
       if (w > 0) some = t;
       if (first == a.tiles && w > 0 && x + w > target) {
         first = t;
@@ -512,19 +560,20 @@ __global__ __launch_bounds__(kDrawThreads) void k_verify_draw(VerifyArgs a, int 
   }
   const int tile = hit < a.tiles ? hit : max(last, 0);
   const double within = rest;
-  const double inv_heat = kLog2e64 / (double)heat_of(a.temperature[s]);
   const long long e0 = (long long)tile * kVerifyTile + kDrawEach * tid;
   const int skip = st.draw == 2 && !plain ? a.draft[st.row] : -1;
   double w[kDrawEach];
   mine = 0;
+  int some_p = -1;   // the last id that p has any of
   {
     float z[kDrawEach], y[kDrawEach];
     load_some((const T*)a.z + st.row * a.ldz, e0, a.n, z);
-    if (st.draw == 3 && !plain) load_some((const T*)a.y + st.row * a.ldy, e0, a.n, y);
+    if (both && !plain) load_some((const T*)a.y + st.row * a.ldy, e0, a.n, y);
 #pragma unroll
     for (int i = 0; i < kDrawEach; ++i) {
       w[i] = weight(z[i], st.mp, inv_heat);
-      if (st.draw == 3 && !plain) w[i] = fmax(w[i] - c * weight(y[i], st.mq, inv_heat), 0.0);
+      if (w[i] > 0) some_p = (int)(e0 + i);
+      if (both && !plain) w[i] = fmax(w[i] - c * weight(y[i], st.mq, inv_heat), 0.0);
       if (e0 + i == skip || e0 + i >= a.n) w[i] = 0;
       mine += w[i];
     }
@@ -533,7 +582,7 @@ __global__ __launch_bounds__(kDrawThreads) void k_verify_draw(VerifyArgs a, int 
   up_to = block_scan(mine, sh, &all);
   if (tid == 0) {
     hit = 0x7fffffff;
-    last = -1;
+    last = last_p = -1;
   }
   __syncthreads();
   double x = up_to - mine;
@@ -550,8 +599,13 @@ __global__ __launch_bounds__(kDrawThreads) void k_verify_draw(VerifyArgs a, int 
     if (any && (tid & 63) == 63 - __builtin_clzll(any)) atomicMax(&last, some);
   }
   __syncthreads();
+  if (__builtin_expect(hit == 0x7fffffff && last < 0, 0)) {
+    // the tile's weight was the rounding of p - c q over tokens that have none: the last one that p has any of
+    if (some_p >= 0) atomicMax(&last_p, some_p);
+    __syncthreads();
+  }
   if (tid == 0) {
-    const int token = hit != 0x7fffffff ? hit : max(last, 0);
+    const int token = hit != 0x7fffffff ? hit : last >= 0 ? last : max(last_p, 0);
     a.tokens[st.row] = token;
     if (a.logprobs)
       a.logprobs[st.row] = (float)(((double)(float)((const T*)a.z)[st.row * a.ldz + token] - (double)st.mp) / (double)heat_of(a.temperature[s]) - log(p_sum));
