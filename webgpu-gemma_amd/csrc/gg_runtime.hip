@@ -2005,6 +2005,10 @@ bool kv_args(const gg_kv_pages* p, const gg_kv_seqs* s, KvArgs* a) {
   return true;
 }
 
+bool overlap(const void* a, const void* b, size_t bytes) {   // ranges of one length
+  return (uintptr_t)a < (uintptr_t)b + bytes && (uintptr_t)b < (uintptr_t)a + bytes;
+}
+
 bool attn_shape_ok(const gg_kv_pages* p, const gg_kv_seqs* s, int32_t n_q_heads, int32_t window, int32_t sinks) {
   return kv_shape_ok(p, s) && n_q_heads > 0 && n_q_heads <= (1 << 16) && n_q_heads % p->n_kv_heads == 0 &&
          (int64_t)s->n_rows * n_q_heads <= (1LL << 30) && window >= 0 && sinks >= 0 && window <= (1 << 30) && sinks <= (1 << 30);
@@ -2126,7 +2130,7 @@ int gg_verify_drafts(const void* z, const void* y, uint32_t type, int64_t rows, 
       !temperature || !accept_u || !draw_u || !accepted || !tokens || !workspace || !aligned_to(z, elem_size(e)) ||
       !aligned_to(y, elem_size(e)) || !aligned_to(draft, 4) || !aligned_to(row_start, 4) || !aligned_to(temperature, 4) ||
       !aligned_to(accept_u, 8) || !aligned_to(draw_u, 8) || !aligned_to(accepted, 4) || !aligned_to(tokens, 4) ||
-      !aligned_to(logprobs, 4) || !aligned_to(workspace, 16) || !stream_here(stream))
+      !aligned_to(logprobs, 4) || !aligned_to(workspace, 16) || overlap(draft, tokens, (size_t)rows * 4) || !stream_here(stream))
     return GG_ERR_INVALID;
   VerifyArgs a{};
   a.z = z;
