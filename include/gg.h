@@ -376,8 +376,9 @@ int gg_score_logits(const void* logits, uint32_t type, int64_t rows, int32_t n, 
  * max_len or the table have no place: nothing is stored there or seen.
  * row_start ascends from 0 or more to n_rows or less; rows outside are left alone. The device
  * reads the arrays, so a captured call follows them; the counts and bounds in
- * the structure are the host's: max_rows a bound of a sequence's rows that only
- * chooses kernels, max_len one of len (lengths above it count as max_len). */
+ * the structure are the host's: max_rows a bound of a sequence's rows, which
+ * chooses kernels and with them the workspace's size but no result (a wrong one
+ * costs time), max_len one of len (lengths above it count as max_len). */
 typedef struct gg_kv_pages {
   void* k;
   void* v;
@@ -440,7 +441,16 @@ int gg_kv_load(const gg_kv_pages* pages, const gg_kv_seqs* seqs, void* k_out, in
  * no effect on it, infinities and NaN included. Products take every bit of f32
  * q; the weights keep 24 bits with f32, 16 with f16 on other than F16 pages,
  * else those of the pages' type; sums are f32. out overlaps neither q nor the
- * pages. */
+ * pages.
+ * workspace: that many device bytes, 16-byte aligned (NULL where it is 0), as for
+ * gg_mxfp4_linear. The size belongs to these very structures and arguments, and
+ * does not grow with them alone: with few rows the axis is cut into more
+ * chunks, so that a call of fewer rows, another max_rows or max_len may need
+ * more than a larger one, whose size may even be 0. A caller that keeps one
+ * buffer asks for every call (the size function works on the host alone), or
+ * takes the largest over the calls it will make; none needs more than 256 (or, with
+ * max_rows times the heads of a group above 64, 64) times
+ * n_rows * n_q_heads * (head_dim + 4) * 4 bytes. */
 size_t gg_kv_attention_workspace_size(const gg_kv_pages* pages, const gg_kv_seqs* seqs, int32_t n_q_heads, int32_t window,
                                       int32_t sinks);
 int gg_kv_attention(const gg_kv_pages* pages, const gg_kv_seqs* seqs, const void* q, uint32_t type, int64_t ldq,

@@ -474,6 +474,7 @@ def kv_load(pages: GGKvPages, seqs: GGKvSeqs, k_out_ptr: int | None, ldk: int, v
 
 
 def kv_attention_workspace_size(pages: GGKvPages, seqs: GGKvSeqs, n_q_heads: int, window: int = 0, sinks: int = 0) -> int:
+    """Of a call with these structures; one of fewer rows may need more."""
     return int(lib().gg_kv_attention_workspace_size(ctypes.byref(pages), ctypes.byref(seqs), n_q_heads, window, sinks))
 
 
