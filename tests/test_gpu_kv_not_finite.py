@@ -198,3 +198,24 @@ def test_many_keys_that_are_not_finite(gpu, rows, length, cache, x):
             assert (np.abs(out[i, h] - ro) <= bo)[good].all() and abs(lse[i, h] - rl) <= bl
             assert np.isnan(out[i, h, 3])
             assert cache == "e4m3" or out[i, h, 20] == np.inf and out[i, h, 41] == -np.inf
+
+
+@pytest.mark.parametrize("cache,x", KINDS)
+@pytest.mark.parametrize("rows,length", [(5, 400), (5, 9000), (140, 500), (140, 9000)])
+@pytest.mark.parametrize("dim", [48, 144, 192, 240, 256])
+def test_every_part_of_a_head(gpu, dim, rows, length, cache, x):
+    """NaN in V in the first, the middle and the last values of heads of all widths, for rows from the middle of the chunk on."""
+    c = Case([rows], [length], 3, 1, dim, 16, cache, x)
+    p = length - rows // 2
+    cols = [0, dim // 2 - 1, dim // 2, dim - 1]
+    row = c.pool.views()[1][c.pool.table[0, p // 16], p % 16, 0]
+    row[cols] = 0x7f if cache == "e4m3" else np.nan
+    out, lse = c.run()
+    good = ~np.isin(np.arange(dim), cols)
+    scale = np.float64(np.float32(dim ** -0.5))
+    for i in range(0, rows, 1 if rows < 100 else 13):
+        pos = length - rows + i
+        for h in range(3):
+            ro, rl, bo, bl = (t[0] for t in attention(c.q[i:i + 1, h], c.k[0][:, 0], c.v[0][:, 0], [pos], scale, 0, 0, cache, x))
+            assert (np.abs(out[i, h] - ro) <= bo)[good | (pos < p)].all() and abs(lse[i, h] - rl) <= bl
+            assert (np.isnan(out[i, h][cols]) == (pos >= p)).all()

@@ -136,8 +136,8 @@ __device__ __forceinline__ float scaled(float x, float f) { return fabsf(x) == I
 // Infinities and NaN. A weight of 0, or a zero part of a query, times one of them
 // leaves a NaN, so whatever needs care shows in O, and no main loop looks for it.
 // A wave takes rows whose sums are not finite again with redo_rows: without the
-// keys whose K or V holds one, which careful_rows adds to the rows that see them,
-// as the formula has it.
+// keys whose K holds one, and with zeros in the place of those in V. careful_rows
+// adds both, to the rows that see them, as the formula has it.
 // Whether one of the n 16-byte units of a row of K or V holds one.
 template <int KV>
 __device__ __forceinline__ bool row_odd(const uint8_t* row, int n) {
@@ -158,15 +158,18 @@ __device__ __forceinline__ bool row_odd(const uint8_t* row, int n) {
   return odd != 0;
 }
 
-// R packed rows of a wave over those keys of [u0, u1), 64 at a time, in f32: for
-// the scores a lane has a key, for the sums values of the head. A row whose query
-// is not finite (lost) takes all keys here. Of an axis that waves share in strips
-// of 32 keys, STEP apart, the wave has the strips from u0 on; strip i can hold such
-// a key only if bit i >> shift of marks is set.
-template <int KV, int DP, class T, int STEP, int R>
+// R packed rows of a wave over the keys of [u0, u1) with such values, 64 at a time, in
+// f32: for the scores a lane has a key, for the sums values of the head. Where K
+// holds one the key is taken whole; of other keys the infinities and NaN of V alone, which
+// have a weight above 0 whatever it is. A row whose query is not finite (lost) takes
+// all keys whole, and here only. The sums are those of values d0 to d0 + DW - 1. Of an axis that waves share in strips of 32 keys,
+// STEP apart, the wave has the strips from u0 on; strip i can hold such a key only
+// if bit i >> shift of marks is set.
+template <int KV, int DP, int DW, class T, int STEP, int R>
 __device__ __forceinline__ void careful_rows(const KvAttnArgs& g, int s, const KvSeq& sq, const Span& sp, int u0, int u1, int kvh, uint64_t marks,
-                                             int shift, const int (&p)[R], float (&o)[R][DP / 64], float (&m)[R], float (&l)[R], bool (&lost)[R]) {
-  constexpr int N = DP / 64, ES = KV == KV_E4M3 ? 1 : 2;
+                                             int shift, int d0, const int (&p)[R], float (&o)[R][DW / 64], float (&m)[R], float (&l)[R],
+                                             bool (&lost)[R]) {
+  constexpr int N = DP / 64, NV = DW / 64, ES = KV == KV_E4M3 ? 1 : 2;
   const int lane = threadIdx.x & 63, D = g.kv.dim;
   float q[R][N];
   int pos[R];
@@ -182,8 +185,9 @@ __device__ __forceinline__ void careful_rows(const KvAttnArgs& g, int s, const K
     for (int i = 0; i < N; ++i) {
       q[r][i] = (float)src[min(lane + 64 * i, D - 1)];
       odd |= !(fabsf(q[r][i]) < INFINITY);
-      o[r][i] = 0.f;
     }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) o[r][i] = 0.f;
     lost[r] = __ballot(odd) != 0;
     if (lost[r]) marks = ~0ull;
   }
@@ -202,12 +206,11 @@ __device__ __forceinline__ void careful_rows(const KvAttnArgs& g, int s, const K
       ks = g.kv.k_scale[kv_scale_at(g.kv, at, kvh)];
       vs = g.kv.v_scale[kv_scale_at(g.kv, at, kvh)];
     }
-    const bool odd = row_odd<KV>(kp, D * ES / 16) || row_odd<KV>((const uint8_t*)g.kv.v + off, D * ES / 16) || !(ks < INFINITY) ||
-                     !(vs < INFINITY);
+    const bool k_odd = row_odd<KV>(kp, D * ES / 16) || !(ks < INFINITY), v_odd = row_odd<KV>((const uint8_t*)g.kv.v + off, D * ES / 16) || !(vs < INFINITY);
     bool sees[R], some = false;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      sees[r] = ok && (odd || lost[r]) && key <= pos[r] && (g.window == 0 || key > pos[r] - g.window || key < g.sinks);
+      sees[r] = ok && (k_odd || v_odd || lost[r]) && key <= pos[r] && (g.window == 0 || key > pos[r] - g.window || key < g.sinks);
       some |= sees[r];
     }
     const uint64_t any = __ballot(some);
@@ -243,30 +246,31 @@ __device__ __forceinline__ void careful_rows(const KvAttnArgs& g, int s, const K
             x[r][e] = fmaf(__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, q[r][i]), d + e)), k[e], x[r][e]);
       }
     float w[R];
-    uint64_t seen[R], slight[R];   // slight: a weight that only rounds to 0, which is one for an infinity
+    uint64_t seen[R], slight[R];   // slight: a weight that is 0 here, but one for an infinity
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       float t = (((x[r][0] + x[r][1]) + (x[r][2] + x[r][3])) + ((x[r][4] + x[r][5]) + (x[r][6] + x[r][7]))) * g.scale2 * ks;
-      if (!sees[r]) t = -INFINITY;
+      const bool whole = k_odd || lost[r];
+      if (!sees[r] || !whole) t = -INFINITY;
       const float top = fmaxf(m[r], gg::wave_max(t)), f = top == m[r] ? 1.f : __builtin_amdgcn_exp2f(m[r] - top);
       m[r] = top;
       // a NaN or +inf leaves nothing of the row: e^(s - m) is a NaN with either
       w[r] = t == -INFINITY ? 0.f : t < INFINITY ? __builtin_amdgcn_exp2f(t - top) * (float)(1 << (int)kShift<KV>) : NAN;
       l[r] = f * l[r] + gg::wave_sum(w[r]);
 #pragma unroll
-      for (int i = 0; i < N; ++i) o[r][i] = scaled(o[r][i], f);
+      for (int i = 0; i < NV; ++i) o[r][i] = scaled(o[r][i], f);
       seen[r] = __ballot(sees[r]);
-      slight[r] = __ballot(t > -INFINITY && w[r] == 0.f);
+      slight[r] = __ballot(sees[r] && (!whole || (t > -INFINITY && w[r] == 0.f)));
     }
 #pragma unroll 1
     for (uint64_t left = any; left; left &= left - 1) {
       const int b = __builtin_ctzll(left);
       const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)off, b), hi = (uint32_t)__builtin_amdgcn_readlane((int)(off >> 32), b);
       const uint8_t* vp = (const uint8_t*)g.kv.v + (long long)(((uint64_t)hi << 32) | lo);
-      float v[N];
+      float v[NV];
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int d = min(lane + 64 * i, D - 1);
+      for (int i = 0; i < NV; ++i) {
+        const int d = min(d0 + lane + 64 * i, D - 1);
         if constexpr (KV == KV_E4M3)
           v[i] = __builtin_amdgcn_cvt_f32_fp8((uint32_t)vp[d], 0) * __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vs), b));
         else
@@ -278,27 +282,31 @@ __device__ __forceinline__ void careful_rows(const KvAttnArgs& g, int s, const K
         const float wr = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w[r]), b));
         const float wi = (slight[r] >> b) & 1 ? 1.f : wr;
 #pragma unroll
-        for (int i = 0; i < N; ++i) o[r][i] = fmaf(fabsf(v[i]) < INFINITY ? wr : wi, v[i], o[r][i]);
+        for (int i = 0; i < NV; ++i) o[r][i] = fmaf(fabsf(v[i]) < INFINITY ? wr : wi, v[i], o[r][i]);
       }
     }
   }
 }
 
 // The 16 packed rows from p0 on, those of `which` for certain, over the strips of
-// 32 keys from u0 on, STEP apart: one wave, K and V straight from memory. Lane
-// (c, quad) gets values 16 t + 4 quad + i of packed row c, its m and its sums of
-// weights. buf: 4 DP floats of the wave's own. It shares nothing with the other waves: with one NaN that all rows see, 61 tokens of 32 heads of 128 on 8 at up to
-// 8192 positions take 368 us for 228, 2048 rows at 32768, 4 heads of 256 on 1, 4.3 ms for 0.33.
-template <int KV, int DP, class T, int STEP>
+// 32 keys from u0 on, STEP apart, values d0 to d0 + DW - 1 of them: one wave, K and V
+// straight from memory. Lane (c, quad) gets values d0 + 16 t + 4 quad + i of packed
+// row c, its m and its sums of weights. buf: four rows of DW floats, ld apart, of the
+// wave's own. The registers that a call of it saves are scratch memory, of 8192
+// waves for each hardware queue in use: with 128 values at a time 0.19 GB, with all 256
+// 0.45, and 0.87 with queries and V held too (windowed f32 turns; 64 at a time
+// 0.08, but twice the time). It shares nothing with the other waves: with one NaN that
+// all rows see, 61 tokens of 32 heads of 128 on 8 at up to 8192 positions take 323 us
+// for 228, 2048 rows at 32768, 4 heads of 256 on 1, 6.1 ms for 0.33.
+constexpr int kRedoDims = 128;
+template <int KV, int DP, class T, int STEP, int DW = DP < kRedoDims ? DP : kRedoDims>
 __device__ __forceinline__ void redo_rows(const KvAttnArgs& g, int s, const KvSeq& sq, const Span& sp, int u0, int u1, int kvh, int p0, uint32_t which,
-                                          float* buf, f32x4 (&o)[DP / 16], float& m, float& l, float& le) {
-  constexpr int NP = kParts<KV, T>, KC = DP / 32, VD = DP / 16, ES = KV == KV_E4M3 ? 1 : 2;
+                                          int d0, float* buf, int ld, f32x4 (&o)[DW / 16], float& m, float& l, float& le) {
+  constexpr int NP = kParts<KV, T>, KC = DP / 32, VD = DW / 16, ES = KV == KV_E4M3 ? 1 : 2;
   const int lane = threadIdx.x & 63, c16 = lane & 15, quad = lane >> 4, D = g.kv.dim;
   const int p = min(p0 + c16, sq.rows * g.group - 1), row = row_in(g, p), pos = sq.len - sq.rows + row;
   const T* q = (const T*)g.q + (sq.first + row) * g.ldq + (long long)(kvh * g.group + head_in(g, p)) * D;
-  u32x4 qb[NP][KC];
-#pragma unroll
-  for (int c = 0; c < KC; ++c) {
+  const auto query = [&](int c, u32x4 (&qb)[NP]) __attribute__((always_inline)) {
     const int d = min(32 * c + 8 * quad, D - 8);
     const uint32_t on = 32 * c + 8 * quad < D ? ~0u : 0u;   // past D the query is 0
 #pragma unroll
@@ -306,9 +314,9 @@ __device__ __forceinline__ void redo_rows(const KvAttnArgs& g, int s, const KvSe
       uint32_t w[NP];
       split2<KV, NP>((float)q[d + 2 * i], (float)q[d + 2 * i + 1], w);
 #pragma unroll
-      for (int n = 0; n < NP; ++n) qb[n][c][i] = w[n] & on;
+      for (int n = 0; n < NP; ++n) qb[n][i] = w[n] & on;
     }
-  }
+  };
 #pragma unroll
   for (int t = 0; t < VD; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
   m = -INFINITY;
@@ -336,62 +344,50 @@ __device__ __forceinline__ void redo_rows(const KvAttnArgs& g, int s, const KvSe
       sv = g.kv.v_scale[kv_scale_at(g.kv, at, kvh)];
     }
     const uint32_t placed = (uint32_t)__ballot(ok);
-    uint32_t odd = (uint32_t)__ballot(!(sk < INFINITY) || !(sv < INFINITY));   // keys that hold an infinity or a NaN
-    long long voff[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) voff[j] = __shfl(off, 4 * quad + (j & 3) + 16 * (j >> 2), 64);
-    u32x4 va[VD];
-    uint32_t v_odd[4] = {};
-#pragma unroll
-    for (int t = 0; t < VD; ++t) {
-      const int d = min(16 * t + c16, D - 1);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint8_t *r0 = (const uint8_t*)g.kv.v + voff[2 * i] + d * ES, *r1 = (const uint8_t*)g.kv.v + voff[2 * i + 1] + d * ES;
-        if constexpr (KV == KV_E4M3) va[t][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)*r0 | ((uint32_t)*r1 << 8), 1.f, false));
-        else va[t][i] = (uint32_t)*(const uint16_t*)r0 | ((uint32_t)*(const uint16_t*)r1 << 16);
-        v_odd[i] |= odd2(va[t][i]);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint64_t b = __ballot((v_odd[j >> 1] >> (j & 1)) & 1);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) odd |= (uint32_t)(((b >> (16 * k)) & 0xffff) != 0) << (4 * k + (j & 3) + 16 * (j >> 2));
-    }
+    uint32_t odd = (uint32_t)__ballot(!(sk < INFINITY));   // keys whose K holds an infinity or a NaN
+    bool mark = !(sv < INFINITY);
     f32x4 sc[2];
+    uint32_t k_odd[2] = {};
+    const uint8_t* kp[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const uint8_t* k = (const uint8_t*)g.kv.k + __shfl(off, c16 + 16 * h, 64);
-      uint32_t k_odd = 0;
       sc[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+      kp[h] = (const uint8_t*)g.kv.k + __shfl(off, c16 + 16 * h, 64);
+    }
+    // the queries' parts are made again each time, for their registers
+#pragma unroll 2
+    for (int c = 0; c < KC; ++c) {
+      const int d = min(32 * c + 8 * quad, D - 8);
+      u32x4 qb[NP];
+      query(c, qb);
 #pragma unroll
-      for (int c = 0; c < KC; ++c) {
-        const int d = min(32 * c + 8 * quad, D - 8);
+      for (int h = 0; h < 2; ++h) {
         u32x4 ka;
         if constexpr (KV == KV_E4M3) {
-          const uint2 w = *(const uint2*)(k + d);
+          const uint2 w = *(const uint2*)(kp[h] + d);
           ka[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, 1.f, false));
           ka[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, 1.f, true));
           ka[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, 1.f, false));
           ka[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, 1.f, true));
         } else {
-          ka = *(const u32x4*)(k + 2 * d);
+          ka = *(const u32x4*)(kp[h] + 2 * d);
         }
-        k_odd |= odd2(ka[0]) | odd2(ka[1]) | odd2(ka[2]) | odd2(ka[3]);
+        k_odd[h] |= odd2(ka[0]) | odd2(ka[1]) | odd2(ka[2]) | odd2(ka[3]);
 #pragma unroll
-        for (int n = NP - 1; n >= 0; --n) sc[h] = mfma16<KV>(ka, qb[n][c], sc[h]);
+        for (int n = NP - 1; n >= 0; --n) sc[h] = mfma16<KV>(ka, qb[n], sc[h]);
       }
-      uint64_t b = __ballot(k_odd != 0);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint64_t b = __ballot(k_odd[h] != 0);
       b |= b >> 32;
       odd |= (uint32_t)((b | (b >> 16)) & 0xffff) << (16 * h);
     }
     const uint32_t live = placed & ~odd;
-    if (odd & placed) marks |= 1ull << (strip >> shift);
+    mark |= (odd & placed) != 0;
     // this lane's keys are 4 quad + j and, from j = 4 on, 12 more
     const int key0 = u < sp.a ? u : sp.lo + u - sp.a;
     float y[8], mx = -INFINITY;
-    uint32_t there[4];   // of two values of V
     uint32_t pb[NP][4];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -401,8 +397,6 @@ __device__ __forceinline__ void redo_rows(const KvAttnArgs& g, int s, const KvSe
       if constexpr (KV == KV_E4M3) t *= of_lane(sk, i);
       y[j] = sees ? t : -INFINITY;
       mx = fmaxf(mx, y[j]);
-      const uint32_t half = (live >> i) & 1 ? 0xffffu : 0u;
-      there[j >> 1] = j & 1 ? there[j >> 1] | (half << 16) : half;
     }
     mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
     mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
@@ -426,21 +420,34 @@ __device__ __forceinline__ void redo_rows(const KvAttnArgs& g, int s, const KvSe
       l += w0 + w1;
       if constexpr (KV == KV_E4M3) {
         const int j = 4 * quad + (2 * i & 3) + 16 * (i >> 1);
-        const float s0 = of_lane(sv, j), s1 = of_lane(sv, j + 1);   // of hidden rows maybe a NaN
-        w0 = w0 == 0.f ? 0.f : w0 * s0;
-        w1 = w1 == 0.f ? 0.f : w1 * s1;
+        const float s0 = of_lane(sv, j), s1 = of_lane(sv, j + 1);
+        w0 = s0 < INFINITY ? w0 * s0 : 0.f;
+        w1 = s1 < INFINITY ? w1 * s1 : 0.f;
         split2<KV, NP>(w0, w1, w);
       }
 #pragma unroll
       for (int n = 0; n < NP; ++n) pb[n][i] = w[n];
     }
+    const uint8_t* vp[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) vp[j] = (const uint8_t*)g.kv.v + __shfl(off, 4 * quad + (j & 3) + 16 * (j >> 2), 64) + min(c16, D - 1) * ES;
 #pragma unroll
     for (int t = 0; t < VD; ++t) {
+      const int d = min(d0 + 16 * t, D - 16) * ES;   // what lies past D is nobody's
+      u32x4 va;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) va[t][i] &= there[i];
+      for (int i = 0; i < 4; ++i) {
+        const uint8_t *r0 = vp[2 * i] + d, *r1 = vp[2 * i + 1] + d;
+        if constexpr (KV == KV_E4M3) va[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)*r0 | ((uint32_t)*r1 << 8), 1.f, false));
+        else va[i] = (uint32_t)*(const uint16_t*)r0 | ((uint32_t)*(const uint16_t*)r1 << 16);
+        const uint32_t no = odd2(va[i]);
+        mark |= no != 0;
+        va[i] &= (no & 1 ? 0u : 0xffffu) | (no & 2 ? 0u : 0xffff0000u);
+      }
 #pragma unroll
-      for (int n = NP - 1; n >= 0; --n) o[t] = mfma16<KV>(va[t], u32x4{pb[n][0], pb[n][1], pb[n][2], pb[n][3]}, o[t]);
+      for (int n = NP - 1; n >= 0; --n) o[t] = mfma16<KV>(va, u32x4{pb[n][0], pb[n][1], pb[n][2], pb[n][3]}, o[t]);
     }
+    if (__ballot(mark) != 0) marks |= 1ull << (strip >> shift);
   }
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
@@ -458,13 +465,13 @@ __device__ __forceinline__ void redo_rows(const KvAttnArgs& g, int s, const KvSe
       left &= left - 1;
       pr[r] = p0 + c[r];
     }
-    float os[R][DP / 64], ms[R], ls[R], m2 = 0.f, l2 = 0.f;
+    float os[R][DW / 64], ms[R], ls[R], m2 = 0.f, l2 = 0.f;
     bool lost[R], drop = false;
-    careful_rows<KV, DP, T, STEP, R>(g, s, sq, sp, u0, u1, kvh, marks, shift, pr, os, ms, ls, lost);
+    careful_rows<KV, DP, DW, T, STEP, R>(g, s, sq, sp, u0, u1, kvh, marks, shift, d0, pr, os, ms, ls, lost);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
 #pragma unroll
-      for (int i = 0; i < DP / 64; ++i) buf[r * DP + lane + 64 * i] = os[r][i];
+      for (int i = 0; i < DW / 64; ++i) buf[r * ld + lane + 64 * i] = os[r][i];
       m2 = r_of == r ? ms[r] : m2;
       l2 = r_of == r ? ls[r] : l2;
       drop = r_of == r ? lost[r] : drop;
@@ -480,7 +487,7 @@ __device__ __forceinline__ void redo_rows(const KvAttnArgs& g, int s, const KvSe
 #pragma unroll
       for (int t = 0; t < VD; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[t][i] = (drop ? 0.f : o[t][i] * f) + scaled(buf[r_of * DP + 16 * t + 4 * quad + i], f2);
+        for (int i = 0; i < 4; ++i) o[t][i] = (drop ? 0.f : o[t][i] * f) + scaled(buf[r_of * ld + 16 * t + 4 * quad + i], f2);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
@@ -855,14 +862,18 @@ __global__ __launch_bounds__(256, (DP <= 128 || (KV == KV_E4M3 && kParts<KV, T> 
   }
   // (expected not to be: in line this code costs a single token 0.4 us)
   if (__builtin_expect(again != 0, 0)) {
-    f32x4 o2[VD];
+    constexpr int DW = DP < kRedoDims ? DP : kRedoDims;
     float m2, l2, le2;
-    redo_rows<KV, DP, T, 128>(g, s, sq, sp, first, u1, kvh, p0, again, &o_all[wv][0][0], o2, m2, l2, le2);
+#pragma unroll 1
+    for (int d0 = 0; d0 < DP; d0 += DW) {
+      f32x4 o2[DW / 16];
+      redo_rows<KV, DP, T, 128>(g, s, sq, sp, first, u1, kvh, p0, again, d0, &o_all[wv][0][d0], OP, o2, m2, l2, le2);
+#pragma unroll
+      for (int t = 0; t < DW / 16; ++t) *(f32x4*)&o_all[wv][c16][d0 + 16 * t + 4 * quad] = o2[t];
+    }
     m = m2;
     l = quad == 0 ? l2 : 0.f;
     le = quad == 0 ? le2 : 0.f;
-#pragma unroll
-    for (int t = 0; t < VD; ++t) *(f32x4*)&o_all[wv][c16][16 * t + 4 * quad] = o2[t];
   }
 
   // the four waves' parts; this lane has values 4 VD quad + VD i + t of its packed row
@@ -995,26 +1006,30 @@ __device__ __attribute__((noinline)) void redo_many(const KvAttnArgs* gp, int s,
   for (int h = 0; h < 32; h += 16) {
     const uint32_t which = (again >> h) & 0xffffu;
     if (which == 0) continue;
-    f32x4 o2[DP / 16];
-    float m2, l2, le2;
-    redo_rows<KV, DP, T, 32>(g, s, sq, sp, u0, u1, kvh, pw + h, which, (float*)(lds_float*)(uintptr_t)lds, o2, m2, l2, le2);
+    constexpr int DW = DP < kRedoDims ? DP : kRedoDims;
     const int c16 = lane & 15, quad = lane >> 4, p2 = pw + h + c16;
-    if (((which >> c16) & 1) == 0) continue;
-    const int orow = sq.first + row_in(g, p2), oh = kvh * g.group + head_in(g, p2);
-    const long long to = ((long long)split * g.kv.n_rows + orow) * g.n_q + oh;
-    const float inv = l2 == 0.f ? 0.f : 1.f / l2;
+#pragma unroll 1
+    for (int d0 = 0; d0 < D; d0 += DW) {
+      f32x4 o2[DW / 16];
+      float m2, l2, le2;
+      redo_rows<KV, DP, T, 32>(g, s, sq, sp, u0, u1, kvh, pw + h, which, d0, (float*)(lds_float*)(uintptr_t)lds, DW, o2, m2, l2, le2);
+      if (((which >> c16) & 1) == 0) continue;
+      const int orow = sq.first + row_in(g, p2), oh = kvh * g.group + head_in(g, p2);
+      const long long to = ((long long)split * g.kv.n_rows + orow) * g.n_q + oh;
+      const float inv = l2 == 0.f ? 0.f : 1.f / l2;
 #pragma unroll
-    for (int t = 0; t < DP / 16; ++t) {
-      if (16 * t >= D) continue;
-      const int e = 16 * t + 4 * quad;
-      if (joined) *(f32x4*)(g.part_o + to * D + e) = o2[t];
+      for (int t = 0; t < DW / 16; ++t) {
+        const int e = d0 + 16 * t + 4 * quad;
+        if (d0 + 16 * t >= D) continue;
+        if (joined) *(f32x4*)(g.part_o + to * D + e) = o2[t];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (!joined) ((T*)g.out)[orow * g.ldo + (long long)oh * D + e + i] = (T)(o2[t][i] * inv);
-    }
-    if (quad == 0) {
-      if (joined) *(f32x4*)(g.part_ml + 4 * to) = f32x4{m2, l2, le2, 0.f};
-      else if (g.lse) g.lse[(long long)orow * g.n_q + oh] = lse_of<KV>(m2, le2);
+        for (int i = 0; i < 4; ++i)
+          if (!joined) ((T*)g.out)[orow * g.ldo + (long long)oh * D + e + i] = (T)(o2[t][i] * inv);
+      }
+      if (quad == 0 && d0 == 0) {
+        if (joined) *(f32x4*)(g.part_ml + 4 * to) = f32x4{m2, l2, le2, 0.f};
+        else if (g.lse) g.lse[(long long)orow * g.n_q + oh] = lse_of<KV>(m2, le2);
+      }
     }
   }
 }
