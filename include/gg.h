@@ -484,11 +484,10 @@ int gg_kv_attention(const gg_kv_pages* pages, const gg_kv_seqs* seqs, const void
  * to it. A row that is reached and has a NaN or +inf, or nothing above -inf, in z
  * or (before its last row, at a temperature above 0) y ends its sequence: token
  * -1, log probability NaN. A sequence without rows: accepted 0. rows and n from 1
- * to 2^30, n_seqs from 1 to 2^22. What decides a token is summed in 64 bits, and
- * the sum of max(p - q, 0) known to 2^-34 of it; a log probability is off by 2^-17 at
- * most besides its rounding. Outputs overlap no input (tokens over draft is
- * refused). Same rules for pointers, streams and the workspace as
- * gg_mxfp4_linear. */
+ * to 2^30, n_seqs from 1 to 2^22. What decides a token is summed in 64 bits; a
+ * log probability is off by 2^-17 at most besides its rounding. Outputs overlap
+ * no input (tokens over draft is refused). Same rules for pointers, streams and
+ * the workspace as gg_mxfp4_linear. */
 size_t gg_verify_drafts_workspace_size(int64_t rows, int32_t n_seqs, int32_t n);
 int gg_verify_drafts(const void* z, const void* y, uint32_t type, int64_t rows, int32_t n, int64_t ldz, int64_t ldy,
                      const int32_t* draft, const int32_t* row_start, int32_t n_seqs, const float* temperature,

@@ -497,7 +497,8 @@ __device__ __forceinline__ void redo_rows(const KvAttnArgs& g, int s, const KvSe
 // Few rows: a block takes 16 packed rows of a K/V head and a chunk of keys, its
 // waves 32 keys at a time in turn. K and V go from memory to registers, K in
 // operand order as it lies, V in rows (16 lanes share one) and transposed by
-// byte permutes: no LDS, no barrier in the loop; the next step's K is asked for
+// byte permutes: no barrier in the loop, and through LDS only where a step's rows lie
+// and 8-bit rows' scales; the next step's K is asked for
 // when this one's is used up, V likewise. Memory bounds it: 61 tokens of 32 heads of 128
 // on 8 at up to 8192 positions 221 us and 7 more for the join, 5.4 TB/s; 3 tokens
 // at up to 131072, 8-bit heads of 256, 138 and 5 us, 5.3 TB/s. Of one token's 8 us
@@ -936,17 +937,19 @@ __global__ __launch_bounds__(256, (DP <= 128 || (KV == KV_E4M3 && kParts<KV, T> 
 
 // ---------------------------------------------------------------------------
 // Many rows: a block takes 128 packed rows of a K/V head, 32 a wave, and a chunk
-// of keys, 64 (heads above 128: 32) at a time. The waves share K and V through
+// of keys, 64 at a time (32 with heads above 128 where rows are f32, or f16 on
+// other than f16 pages, or pages 8-bit). The waves share K and V through
 // LDS, two tiles of each: while one is used the next arrives by DMA, 1 KB of
 // whole rows a copy, in the order of memory (16-byte units of a row at permuted
 // places, the usual way to keep reads from meeting in a bank, take the copies
 // twice as long here), at places such that neither the reads of K (a row a
 // lane) nor those of V (transposed by the read, four rows to 16 lanes) meet in a
 // bank. One barrier a tile. 8-bit rows go to a place of their wave's own, and from
-// there as bf16 into one stage, between two barriers a tile: that fits two blocks
-// a CU. (Two sequences of 2048 rows to 8192 positions, 16 heads of 128 on 4: 406 us; one
+// there as bf16 into one stage, between two barriers a tile: with bf16 rows and heads
+// up to 128 that fits two blocks a CU, with 13 registers in scratch memory. (Two
+// sequences of 2048 rows to 8192 positions, 16 heads of 128 on 4: 400 us; one
 // block a CU with two stages, a barrier a tile, 599; loads to registers, which
-// the compiler waits for too early, 989. bf16 pages take 307.)
+// the compiler waits for too early, 989. bf16 pages take 319.)
 // ---------------------------------------------------------------------------
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 template <int KV>
@@ -1570,20 +1573,26 @@ int attn_type(int elem, const KvAttnArgs& g, hipStream_t s) {
 // The chunk length is taken from estimates of a call's time, in us, over the
 // numbers of chunks; lengths are taken to be spread between 0 and max_len.
 // k_attn_few: a block starts and ends in 5 us and takes 128 keys in 1.2, or as long as
-// 5 TB/s need for what all resident blocks read; a join takes 3 and 0.15 a chunk.
-// Measured at the two sides of the choice: 16 drafts of 12 packed rows at 4096
-// positions, heads of 128: 5 chunks 39 us, 3 46, 8 48; 61 tokens at 8192: 8
-// chunks 231, 4 330, 2 276; 3 tokens at 131072, 8-bit heads of 256: 21 chunks 155,
-// 64 165, 256 193.
+// 5 TB/s need for what all resident blocks read; a join takes 3 and 0.1 a chunk.
 // k_attn_many: whole rounds of the CUs; a block's start and end cost about 200
 // keys, a chunk's sums are written and read once more.
+// Measured at the two sides of the choice, us, on three sets of inputs in turn,
+// which no cache holds together: 16 times 6 drafts to 4096 positions, 16 heads of 128 on 8, the estimate's
+// 7 chunks 50, 1 62, 2 70, 3 52, 5 47.5, 8 48; 61 tokens to 8192, its 8 229, 2 257, 4 233,
+// 12 229; 3 tokens to 131072, 8-bit heads of 256, its 18 142, 16 147, 24 210, 64 151,
+// 256 174; 2048 rows at 32768, 4 heads of 256 on 1, its 4 329, 3 431, 5 528, 8 356;
+// windowed f32 turns, its 2 67.5, 1 80, 3 95.
 KvAttnPlan kv_attn_plan(int n_seqs, int n_rows, int max_rows, int max_len, int n_kv, int group, int dim, int window, int sinks,
                         int key_bytes) {
   KvAttnPlan p{};
   constexpr int FEW = kKvFewTiles * kKvFewTile;
   const bool few = (long long)max_rows * group <= FEW;
-  // Only long ones: k_attn_many alone, a launch less (5 us); what is short among
-  // them it can do too.
+  // Long ones: k_attn_many alone, a launch less; what is short among them it can do
+  // too. A prompt beside single tokens at up to 8192 positions, us with k_attn_many
+  // alone / both, 4 heads of 256 on 1 and 32 of 128 on 8: 4096 rows and 31 tokens
+  // 245 / 265 and 386 / 391, 8192 and 31 465 / 522 and 901 / 960; below the border 256 and 31
+  // 77 / 69 and 176 / 163. Near it neither is always the better: 2048 and 31 150 / 158 and
+  // 248 / 259, 300 and 1 28 / 40 but 58 / 41.
   p.few_rows = few ? 0x7fffffff : (long long)n_rows * group >= 512ll * n_seqs ? 0 : FEW;
   const int tile = few ? kKvFewTile : kKvManyTile;
   long long most = max_len;   // keys that a tile's rows see at most

@@ -706,7 +706,7 @@ struct VerifyStop {
   double sp, sq;         // sums, as the parts give them
 };
 constexpr int kVerifyTile = 4096;   // logits of a block of the 64-bit sums
-constexpr int kVerifySums = 5;      // of a tile: p and q where p is the larger, all p, all q, p where f32 sums cannot tell which is
+constexpr int kVerifySums = 5;      // of a tile: p and q where p is the larger, all p, all q; how near a token comes to the border
 struct VerifyArgs {
   const void *z, *y;
   long long ldz, ldy, rows;

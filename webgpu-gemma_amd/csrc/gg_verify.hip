@@ -11,7 +11,7 @@
 // k_verify_draw finds the tile and the token that the draw falls on.
 // Measured, 262144 logits: one sequence, 5 rows of f32: 3.8, 8.0 and 7.0 us, each little
 // more than its chain of reads and reductions; 48 sequences, 7 rows each of both
-// models, bf16: 36.8 us (4.9 TB/s), 9.1, 22.6 (exponentials in f64) and 9.0.
+// models, bf16: 37.1 us (4.9 TB/s), 9.0, 22.2 (exponentials in f64) and 9.1.
 //
 // The draw picks among borders that lie closer than f32 tells apart: with f32
 // sums one draw in a hundred over 262144 logits gives a neighbour of the
@@ -22,9 +22,9 @@
 // Whether p exceeds q at a token is taken from
 // the sums of the first launch: that changes the sum over them in the
 // second order only, and their scale is put right afterwards, since
-// sum (p - q) over a set = sum p - c sum q with any c. Where p and q lie so close
-// together that it changes more than 2^-34 of it, k_verify_draw takes the
-// tiles concerned again (0.15 ms for rows of 262144).
+// sum (p - q) over a set = sum p - c sum q with any c. Tiles with a token that the exact c
+// puts on the other side are taken again by k_verify_draw, 2 us each (all of them with a draft
+// model next to the target: 0.15 ms for rows of 262144).
 #include "gg_kv_device.h"
 
 namespace gg {
@@ -387,11 +387,10 @@ __global__ __launch_bounds__(256) void k_verify_sums(VerifyArgs a) {
   const long long e0 = (long long)tile * kVerifyTile + 16 * tid;
   const bool both = st.draw == 3;
   const int skip = st.draw == 2 ? a.draft[st.row] : -1;
-  double sum[kVerifySums] = {};
+  double sum[kVerifySums - 1] = {}, border = 1.0;
   // two numbers no further apart than a.near have upper halves, 20 bits of the
   // mantissa, no further apart than this
   const uint32_t near = (uint32_t)(a.near * (1 << 21)) + 2;
-  bool close = false;
   if (e0 < a.n) {
     float z[16], y[16];
     load_some((const T*)a.z + st.row * a.ldz, e0, a.n, z);
@@ -408,22 +407,26 @@ __global__ __launch_bounds__(256) void k_verify_sums(VerifyArgs a) {
           sum[0] += p;
           sum[1] += q;
         }
-        close |= (uint32_t)(__double2hiint(ps) - __double2hiint(qs) + near) <= 2 * near;
+        // (0 / 0, where both are 0, is passed over by fmin)
+        if ((uint32_t)(__double2hiint(ps) - __double2hiint(qs) + near) <= 2 * near) border = fmin(border, fabs(ps - qs) / ps);
       } else if (e0 + i != skip) {
         sum[0] += p;
       }
     }
   }
-  if (close) sum[4] = sum[2];   // all of a thread's p
   __shared__ double part[4][kVerifySums];
 #pragma unroll
-  for (int k = 0; k < kVerifySums; ++k) {
+  for (int k = 0; k < kVerifySums - 1; ++k) {
     if (k % 2 == 1 && !both) continue;   // no q
-    const double x = k == 4 && __ballot(close) == 0 ? 0.0 : wave_sum(sum[k]);
+    const double x = wave_sum(sum[k]);
     if (lane == 0) part[tid >> 6][k] = x;
   }
+  // positive f64 numbers are in the order of their bits
+  const double least = __ballot(border < 1.0) == 0 ? 1.0 : __builtin_bit_cast(double, ~wave_max64(~__builtin_bit_cast(uint64_t, border)));
+  if (lane == 0) part[tid >> 6][kVerifySums - 1] = least;
   __syncthreads();
-  if (tid < kVerifySums && (both || tid % 2 == 0)) a.sums[at * kVerifySums + tid] = (part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid]);
+  if (tid < kVerifySums - 1 && (both || tid % 2 == 0)) a.sums[at * kVerifySums + tid] = (part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid]);
+  if (tid == kVerifySums - 1) a.sums[at * kVerifySums + tid] = fmin(fmin(part[0][tid], part[1][tid]), fmin(part[2][tid], part[3][tid]));
 }
 
 constexpr int kDrawThreads = 1024, kDrawWaves = kDrawThreads / 64, kDrawEach = kVerifyTile / kDrawThreads;
@@ -450,7 +453,7 @@ __device__ void block_sums(double (&x)[N], double* sh) {
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
 #pragma unroll
   for (int k = 0; k < N; ++k) {
-    const double t = k == 2 && __ballot(x[k] != 0.0) == 0 ? 0.0 : wave_sum(x[k]);   // most often 0
+    const double t = wave_sum(x[k]);
     if (lane == 0) sh[k * kDrawWaves + wv] = t;
   }
   __syncthreads();
@@ -465,7 +468,7 @@ __device__ void block_sums(double (&x)[N], double* sh) {
 // One block per sequence: the token that the draw falls on.
 template <class T>
 __global__ __launch_bounds__(kDrawThreads) void k_verify_draw(VerifyArgs a, int seq0) {
-  __shared__ double sh[3 * kDrawWaves];
+  __shared__ double sh[2 * kDrawWaves];
   __shared__ int hit, last, last_p;
   __shared__ double rest;
   const int tid = threadIdx.x, s = seq0 + blockIdx.x;
@@ -476,34 +479,24 @@ __global__ __launch_bounds__(kDrawThreads) void k_verify_draw(VerifyArgs a, int 
   const int per = (a.tiles + kDrawThreads - 1) / kDrawThreads, t0 = min(tid * per, a.tiles), t1 = min(t0 + per, a.tiles);
   // the sums of all p and q first: their quotient scales q
   const bool both = st.draw == 3;
-  double p_all = 0, p_sum, c = 0, close = 0;
-  for (int t = t0; t < t1; ++t) p_all += sums[kVerifySums * t + 2];
-  if (both) {
-    double totals[3] = {p_all, 0, 0};
-    for (int t = t0; t < t1; ++t) {
-      totals[1] += sums[kVerifySums * t + 3];
-      totals[2] += sums[kVerifySums * t + 4];
-    }
-    block_sums(totals, sh);
-    p_sum = totals[0];
-    c = p_sum / totals[1];
-    close = totals[2];
-  } else {
-    double totals[1] = {p_all};
-    block_sums(totals, sh);
-    p_sum = totals[0];
+  double p_all = 0, totals[2] = {}, c = 0;
+  for (int t = t0; t < t1; ++t) {
+    p_all += sums[kVerifySums * t + 2];
+    if (both) totals[1] += sums[kVerifySums * t + 3];
   }
-  double mine = 0, all;
-  auto tile_weight = [&](int t) { return both ? fmax(sums[kVerifySums * t] - c * sums[kVerifySums * t + 1], 0.0) : sums[kVerifySums * t]; };
-  for (int t = t0; t < t1; ++t) mine += tile_weight(t);
-  double up_to = block_scan(mine, sh, &all);
+  totals[0] = p_all;
+  block_sums(totals, sh);
+  const double p_sum = totals[0];
   if (both) {
+    c = p_sum / totals[1];
     // tokens with p / q between the first launch's quotient and c are on the wrong
-    // side: they lie within `near` of it, and each is off by this much of p at most
-    const double off = fabs(c * st.sq - st.sp);   // times sp
-    if (off * close > 0x1p-34 * all * st.sp) {   // a draft model next to the target: these tiles again
+    // side: tiles with one that near are summed again
+    const double off = 1.0001 * fabs(c * st.sq - st.sp) + 0x1p-45 * st.sp;   // relative to sp; roundings, c for sp / sq
+    bool again = false;
+    for (int t = t0; t < t1; ++t) again |= sums[kVerifySums * t + 4] * st.sp <= off;
+    if (__syncthreads_or(again)) {
       for (int t = 0; t < a.tiles; ++t) {
-        if (sums[kVerifySums * t + 4] == 0.0) continue;
+        if (!(sums[kVerifySums * t + 4] * st.sp <= off)) continue;
         const long long e0 = (long long)t * kVerifyTile + kDrawEach * tid;
         float z[kDrawEach], y[kDrawEach];
         load_some((const T*)a.z + st.row * a.ldz, e0, a.n, z);
@@ -519,11 +512,12 @@ __global__ __launch_bounds__(kDrawThreads) void k_verify_draw(VerifyArgs a, int 
         }
       }
       __syncthreads();
-      mine = 0;
-      for (int t = t0; t < t1; ++t) mine += tile_weight(t);
-      up_to = block_scan(mine, sh, &all);
     }
   }
+  double mine = 0, all;
+  auto tile_weight = [&](int t) { return both ? fmax(sums[kVerifySums * t] - c * sums[kVerifySums * t + 1], 0.0) : sums[kVerifySums * t]; };
+  for (int t = t0; t < t1; ++t) mine += tile_weight(t);
+  double up_to = block_scan(mine, sh, &all);
   const bool plain = st.draw == 1 || !(all > 0.0);   // nothing left: from p
   if (plain) {
     mine = p_all;
