@@ -414,8 +414,9 @@ typedef struct gg_kv_seqs {
  * rotation). q goes to q_out (rows ldqo apart), k and v to their places; a row
  * without a place goes nowhere but to q_out, where its position counts all the
  * same. q may be NULL, with n_q_heads 0.
- * All between reading and storing is 64-bit: each stored value is the formula's, rounded once to nearest
- * (even). An E4M3 row's scale is the least power of two from 2^-126 on that
+ * All between reading and storing is 64-bit, an angle at position p within
+ * 2^-51 p: each stored value is the formula's, rounded once to nearest (even).
+ * An E4M3 row's scale is the least power of two from 2^-126 on that
  * holds its largest magnitude within 448; a row with an infinity or a NaN gets
  * the scale NaN. Two rows of a call must not have the same place. */
 int gg_kv_store(const gg_kv_pages* pages, const gg_kv_seqs* seqs, uint32_t type, const void* q, int64_t ldq, const void* k,
